@@ -36,6 +36,11 @@ struct EntryPoints {
     decltype(&dg_m_grouped_fp8_gemm_nt_contiguous_swiglu) contiguous_swiglu;
     decltype(&dg_m_grouped_fp8_gemm_nt_masked_swiglu) masked_swiglu;
     decltype(&dg_moe_combine) combine;
+    decltype(&dg_m_grouped_bf16_gemm_nt_ragged) ragged_nt;
+    decltype(&dg_m_grouped_bf16_gemm_nn_ragged) ragged_nn;
+    decltype(&dg_k_grouped_bf16_gemm_tn_ragged) ragged_tn;
+    decltype(&dg_moe_swiglu_checkpoint) swiglu_checkpoint;
+    decltype(&dg_moe_swiglu_backward) swiglu_backward;
 } g_entry{};
 
 struct TypeMismatch : std::runtime_error {
@@ -149,7 +154,7 @@ PyObject* guarded(Py_ssize_t nargs, Py_ssize_t want, F&& f) {
     return nullptr;
 }
 
-// init(addresses of the entry points, in EntryPoints' order)
+// init(addresses of the entry points up to combine, in EntryPoints' order)
 PyObject* init(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded(n, 11, [&] {
         auto set = [&](auto& entry, int i) { entry = reinterpret_cast<std::decay_t<decltype(entry)>>(pointer<void>(a[i])); };
@@ -157,6 +162,16 @@ PyObject* init(PyObject*, PyObject* const* a, Py_ssize_t n) {
         set(g_entry.contiguous, 3), set(g_entry.masked, 4), set(g_entry.cast, 5), set(g_entry.dispatch, 6);
         set(g_entry.swiglu, 7), set(g_entry.contiguous_swiglu, 8), set(g_entry.masked_swiglu, 9);
         set(g_entry.combine, 10);
+        return 0;
+    });
+}
+
+// init_bf16(addresses of the entry points after combine)
+PyObject* init_bf16(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded(n, 5, [&] {
+        auto set = [&](auto& entry, int i) { entry = reinterpret_cast<std::decay_t<decltype(entry)>>(pointer<void>(a[i])); };
+        set(g_entry.ragged_nt, 0), set(g_entry.ragged_nn, 1), set(g_entry.ragged_tn, 2);
+        set(g_entry.swiglu_checkpoint, 3), set(g_entry.swiglu_backward, 4);
         return 0;
     });
 }
@@ -266,6 +281,42 @@ PyObject* combine(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
+// m_grouped_ragged(nn, a, b, d, group_ends, alignment, stream)
+PyObject* m_grouped_ragged(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded(n, 7, [&] {
+        const auto entry = integer(a[0]) ? g_entry.ragged_nn : g_entry.ragged_nt;
+        const Arg ta(a[1]), tb(a[2]), d(a[3]), ends(a[4]);
+        return call(entry, ta.get(), tb.get(), d.get(), ends.get(), (int32_t)integer(a[5]), pointer<void>(a[6]));
+    });
+}
+
+// k_grouped_ragged(a, b, b_sf | None, d, group_ends, c | None, alignment, stream)
+PyObject* k_grouped_ragged(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded(n, 8, [&] {
+        const Arg ta(a[0]), tb(a[1]), sf(a[2], true), d(a[3]), ends(a[4]), c(a[5], true);
+        return call(g_entry.ragged_tn, ta.get(), tb.get(), sf.get(), d.get(), ends.get(), c.get(), (int32_t)integer(a[6]),
+                    pointer<void>(a[7]));
+    });
+}
+
+// swiglu_checkpoint(x, row_weights | None, row_layout | None, clamp, h, q, sf, stream)
+PyObject* swiglu_checkpoint(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded(n, 8, [&] {
+        const Arg x(a[0]), w(a[1], true), layout(a[2], true), h(a[4]), q(a[5]), sf(a[6]);
+        return call(g_entry.swiglu_checkpoint, x.get(), w.get(), layout.get(), real(a[3]), h.get(), q.get(), sf.get(),
+                    pointer<void>(a[7]));
+    });
+}
+
+// swiglu_backward(dh, q, sf, row_weights | None, row_layout | None, clamp, dx, h, d_row_weights | None, stream)
+PyObject* swiglu_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded(n, 10, [&] {
+        const Arg dh(a[0]), q(a[1]), sf(a[2]), w(a[3], true), layout(a[4], true), dx(a[6]), h(a[7]), dw(a[8], true);
+        return call(g_entry.swiglu_backward, dh.get(), q.get(), sf.get(), w.get(), layout.get(), real(a[5]), dx.get(),
+                    h.get(), dw.get(), pointer<void>(a[9]));
+    });
+}
+
 template <PyObject* (*F)(PyObject*, PyObject* const*, Py_ssize_t)>
 PyMethodDef method(const char* name) {
     return {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(F)), METH_FASTCALL, nullptr};
@@ -275,6 +326,10 @@ PyMethodDef g_methods[] = {method<init>("init"),     method<gemm_nt>("gemm_nt"),
                            method<masked>("masked"), method<cast>("cast"),       method<dispatch>("dispatch"),
                            method<swiglu>("swiglu"), method<contiguous_swiglu>("contiguous_swiglu"),
                            method<masked_swiglu>("masked_swiglu"),               method<combine>("combine"),
+                           method<init_bf16>("init_bf16"), method<m_grouped_ragged>("m_grouped_ragged"),
+                           method<k_grouped_ragged>("k_grouped_ragged"),
+                           method<swiglu_checkpoint>("swiglu_checkpoint"),
+                           method<swiglu_backward>("swiglu_backward"),
                            {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_dgbind", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};

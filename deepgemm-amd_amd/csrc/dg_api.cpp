@@ -1531,6 +1531,242 @@ void k_grouped_impl(const dg_tensor* a_, const dg_tensor* sfa_, const dg_tensor*
     launch_1d1d(true, args, stream, m, n, sum_k, g);
 }
 
+// ---------------------------------------------------------------- BF16 expert products, SwiGLU checkpoints
+
+// Every given tensor is on one device, which is made current for the launch (a null
+// stream, and a stream's kernels, belong to the current device) and set back after it.
+class OnDevice {
+public:
+    explicit OnDevice(int device) {
+        DG_HIP_CHECK(hipGetDevice(&before_));
+        if (before_ != device) {
+            DG_HIP_CHECK(hipSetDevice(device));
+            changed_ = true;
+        }
+    }
+    ~OnDevice() {
+        if (changed_) (void)hipSetDevice(before_);
+    }
+    OnDevice(const OnDevice&) = delete;
+    OnDevice& operator=(const OnDevice&) = delete;
+
+private:
+    int before_ = 0;
+    bool changed_ = false;
+};
+
+int one_device(std::initializer_list<const dg_tensor*> tensors) {
+    int device = -1;
+    for (const dg_tensor* t : tensors) {
+        if (t == nullptr) continue;
+        DG_CHECK(t->device >= 0);
+        if (device < 0) device = t->device;
+        DG_CHECK(t->device == device);   // all operands on one device
+    }
+    return device;
+}
+
+void check_sizes(const View& t) {
+    for (int i = 0; i < t.dim(); ++i) DG_CHECK(t.size(i) >= 0 && t.size(i) < ((int64_t)1 << 30));
+}
+
+// Matrices of the ragged products: unit stride along the last dimension, rows apart by at
+// least their length (outputs: so that no two elements share memory). The kernels' tile
+// offsets are 32-bit: 256 rows of at most kRaggedMaxPitch elements.
+constexpr int64_t kRaggedMaxPitch = (int64_t)1 << 22;
+void check_ragged_matrix(const View& t, int dims) {
+    check_shape(t, dims);
+    check_sizes(t);
+    DG_CHECK(t.size(-1) <= 1 || t.stride(-1) == 1);
+    DG_CHECK(t.size(-2) <= 1 || (t.stride(-2) >= t.size(-1) && t.stride(-2) <= kRaggedMaxPitch));
+    DG_CHECK(t.size(-1) <= kRaggedMaxPitch);
+    if (dims == 3 && t.size(0) > 1) DG_CHECK(t.stride(0) >= (t.size(1) > 0 ? (t.size(1) - 1) * t.stride(1) + t.size(2) : 0));
+}
+
+bool has_elements(const View& t) {
+    for (int i = 0; i < t.dim(); ++i)
+        if (t.size(i) == 0) return false;
+    return true;
+}
+
+void check_group_ends(const View& t, int64_t groups, int32_t alignment) {
+    DG_CHECK(t.dim() == 1 && t.dtype() == DG_I32 && t.on_device() && contiguous_view(t));
+    DG_CHECK(t.size(0) == groups);
+    DG_CHECK(alignment > 0 && alignment <= (1 << 20));
+}
+
+void ragged_config(const char* kind, const RaggedGemmArgs& a) {
+    char buf[160];
+    std::snprintf(buf, sizeof(buf), "%s rows=%d m=%d n=%d k=%d groups=%d", kind, a.rows, a.m, a.n, a.k, a.groups);
+    t_last_config = buf;
+}
+
+void m_grouped_ragged_impl(RaggedKind kind, const dg_tensor* a_, const dg_tensor* b_, const dg_tensor* d_,
+                           const dg_tensor* ends_, int32_t alignment, hipStream_t stream) {
+    const View a = view(a_, "a"), b = view(b_, "b"), d = view(d_, "d"), ends = view(ends_, "group_ends");
+    check_ragged_matrix(a, 2);
+    check_ragged_matrix(b, 3);
+    check_ragged_matrix(d, 2);
+    DG_CHECK(a.dtype() == DG_BF16 && b.dtype() == DG_BF16);
+    DG_CHECK(d.dtype() == DG_BF16 || d.dtype() == DG_F32);
+    const int64_t rows = a.size(0), k = a.size(1), groups = b.size(0), n = b.size(kind == kRaggedNT ? 1 : 2);
+    DG_CHECK(b.size(kind == kRaggedNT ? 2 : 1) == k);
+    DG_CHECK(d.size(0) == rows && d.size(1) == n);
+    DG_CHECK(k % 8 == 0);
+    check_group_ends(ends, groups, alignment);
+    if (has_elements(a)) check_vector_alignment(a, "a");
+    if (has_elements(b)) check_vector_alignment(b, "b");
+    const int device = one_device({a_, b_, d_, ends_});
+    if (rows == 0 || n == 0 || groups == 0) return;
+    RaggedGemmArgs p{};
+    p.a = static_cast<const uint16_t*>(a.data()), p.lda = a.stride(0);
+    p.b = b.data(), p.ldb = b.stride(1), p.b_gs = b.stride(0);
+    p.d = const_cast<void*>(d.data()), p.ldd = d.stride(0);
+    p.ends = static_cast<const int32_t*>(ends.data());
+    p.rows = (int32_t)rows, p.n = (int32_t)n, p.k = (int32_t)k, p.groups = (int32_t)groups, p.alignment = alignment;
+    p.out_f32 = d.dtype() == DG_F32;
+    const OnDevice on(device);
+    launch_ragged_gemm(kind, p, stream);
+    ragged_config(kind == kRaggedNT ? "bf16_ragged_nt" : "bf16_ragged_nn", p);
+}
+
+void k_grouped_ragged_impl(const dg_tensor* a_, const dg_tensor* b_, const dg_tensor* b_sf_, const dg_tensor* d_,
+                           const dg_tensor* ends_, const dg_tensor* c_, int32_t alignment, hipStream_t stream) {
+    const View a = view(a_, "a"), b = view(b_, "b"), d = view(d_, "d"), ends = view(ends_, "group_ends");
+    check_ragged_matrix(a, 2);
+    check_ragged_matrix(b, 2);
+    check_ragged_matrix(d, 3);
+    DG_CHECK(a.dtype() == DG_BF16);
+    DG_CHECK(b.dtype() == (b_sf_ ? DG_E4M3 : DG_BF16));
+    DG_CHECK(d.dtype() == DG_BF16 || d.dtype() == DG_F32);
+    const int64_t rows = a.size(0), m = a.size(1), n = b.size(1), groups = d.size(0);
+    DG_CHECK(b.size(0) == rows);
+    DG_CHECK(d.size(1) == m && d.size(2) == n);
+    check_group_ends(ends, groups, alignment);
+    if (has_elements(a)) check_vector_alignment(a, "a");
+    RaggedGemmArgs p{};
+    if (b_sf_) {
+        const View sf = view(b_sf_, "b_sf");
+        DG_CHECK(sf.dim() == 2 && sf.dtype() == DG_F32 && sf.on_device());
+        DG_CHECK(sf.size(0) == rows && sf.size(1) == ceil_div(n, (int64_t)128));
+        if (has_elements(b))
+            DG_CHECK(reinterpret_cast<uintptr_t>(b.data()) % 8 == 0 && (rows <= 1 || b.stride(0) % 8 == 0));
+        p.b_sf = static_cast<const float*>(sf.data()), p.sf_sr = sf.stride(0), p.sf_sc = sf.stride(1);
+    } else if (has_elements(b)) {
+        check_vector_alignment(b, "b");
+    }
+    if (c_) {
+        const View c = view(c_, "c");
+        check_ragged_matrix(c, 3);
+        DG_CHECK(c.dtype() == d.dtype());
+        for (int i = 0; i < 3; ++i) DG_CHECK(c.size(i) == d.size(i));
+        if (c.data() == d.data())   // accumulation in place: the same elements
+            for (int i = 0; i < 3; ++i) DG_CHECK(c.size(i) <= 1 || c.stride(i) == d.stride(i));
+        p.c = c.data(), p.ldc = c.stride(1), p.c_gs = c.stride(0);
+    }
+    const int device = one_device({a_, b_, b_sf_, d_, ends_, c_});
+    if (m == 0 || n == 0 || groups == 0) return;
+    p.a = static_cast<const uint16_t*>(a.data()), p.lda = a.stride(0);
+    p.b = b.data(), p.ldb = b.stride(0);
+    p.d = const_cast<void*>(d.data()), p.ldd = d.stride(1), p.d_gs = d.stride(0);
+    p.ends = static_cast<const int32_t*>(ends.data());
+    p.rows = (int32_t)rows, p.m = (int32_t)m, p.n = (int32_t)n, p.groups = (int32_t)groups, p.alignment = alignment;
+    p.out_f32 = d.dtype() == DG_F32;
+    const OnDevice on(device);
+    launch_ragged_gemm(kRaggedTN, p, stream);
+    ragged_config(b_sf_ ? "bf16_ragged_tn b=e4m3" : "bf16_ragged_tn", p);
+}
+
+const float* row_weights_of(const dg_tensor* w_, int64_t m) {
+    if (!w_) return nullptr;
+    const View w = view(w_, "row_weights");
+    DG_CHECK(w.dim() == 1 && w.dtype() == DG_F32 && w.on_device() && w.size(0) == m && contiguous_view(w));
+    return static_cast<const float*>(w.data());
+}
+
+const int32_t* row_layout_of(const dg_tensor* l_, int64_t m) {
+    if (!l_) return nullptr;
+    const View l = view(l_, "row_layout");
+    DG_CHECK(l.dim() == 1 && l.dtype() == DG_I32 && l.on_device() && l.size(0) == m && contiguous_view(l));
+    return static_cast<const int32_t*>(l.data());
+}
+
+// A BF16 matrix [m, n] whose rows are read or written in 16-byte vectors.
+View bf16_rows(const dg_tensor* t_, const char* name, int64_t m, int64_t n) {
+    const View t = view(t_, name);
+    DG_CHECK(t.dim() == 2 && t.dtype() == DG_BF16 && t.on_device());
+    DG_CHECK(t.size(0) == m && t.size(1) == n);
+    DG_CHECK((n <= 1 || t.stride(1) == 1) && (m <= 1 || t.stride(0) >= n));
+    if (has_elements(t)) check_vector_alignment(t, name);
+    return t;
+}
+
+// The checkpoint (q, sf) of SwiGLU's input: e4m3 [m, 2n] in rows of whole 8-byte pieces,
+// f32 [m, 2 ceil(n / 128)].
+void check_swiglu_checkpoint(const View& q, const View& sf, int64_t m, int64_t n) {
+    DG_CHECK(q.dim() == 2 && q.dtype() == DG_E4M3 && q.on_device());
+    DG_CHECK(q.size(0) == m && q.size(1) == 2 * n && (n == 0 || q.stride(1) == 1) && (m <= 1 || q.stride(0) >= 2 * n));
+    DG_CHECK(reinterpret_cast<uintptr_t>(q.data()) % 8 == 0 && (m <= 1 || q.stride(0) % 8 == 0));
+    DG_CHECK(sf.dim() == 2 && sf.dtype() == DG_F32 && sf.on_device());
+    DG_CHECK(sf.size(0) == m && sf.size(1) == 2 * ceil_div(n, (int64_t)128));
+}
+
+void swiglu_checkpoint_impl(const dg_tensor* x_, const dg_tensor* w_, const dg_tensor* rl_, float clamp,
+                            const dg_tensor* h_, const dg_tensor* q_, const dg_tensor* sf_, hipStream_t stream) {
+    const View x0 = view(x_, "x");
+    DG_CHECK(x0.dim() == 2 && x0.size(1) % 16 == 0);   // each half in whole 16-byte pieces
+    check_sizes(x0);
+    const int64_t m = x0.size(0), n = x0.size(1) / 2;
+    const View x = bf16_rows(x_, "x", m, 2 * n), h = bf16_rows(h_, "h", m, n), q = view(q_, "q"), sf = view(sf_, "sf");
+    check_swiglu_checkpoint(q, sf, m, n);
+    SwigluCheckpointArgs p{};
+    p.row_weight = row_weights_of(w_, m), p.row_layout = row_layout_of(rl_, m);
+    const int device = one_device({x_, w_, rl_, h_, q_, sf_});
+    if (m == 0 || n == 0) return;
+    p.x = static_cast<const uint16_t*>(x.data()), p.ldx = x.stride(0);
+    p.clamp = clamp;
+    p.h = static_cast<uint16_t*>(const_cast<void*>(h.data())), p.ldh = h.stride(0);
+    p.q = static_cast<uint8_t*>(const_cast<void*>(q.data())), p.ldq = q.stride(0);
+    p.sf = static_cast<float*>(const_cast<void*>(sf.data())), p.sf_sm = sf.stride(0), p.sf_sk = sf.stride(1);
+    p.m = (int32_t)m, p.n = (int32_t)n;
+    const OnDevice on(device);
+    launch_swiglu_checkpoint(p, stream);
+    char buf[96];
+    std::snprintf(buf, sizeof(buf), "moe_swiglu_checkpoint m=%lld n=%lld", (long long)m, (long long)n);
+    t_last_config = buf;
+}
+
+void swiglu_backward_impl(const dg_tensor* dh_, const dg_tensor* q_, const dg_tensor* sf_, const dg_tensor* w_,
+                          const dg_tensor* rl_, float clamp, const dg_tensor* dx_, const dg_tensor* h_,
+                          const dg_tensor* dw_, hipStream_t stream) {
+    const View dh0 = view(dh_, "dh");
+    DG_CHECK(dh0.dim() == 2 && dh0.size(1) % 8 == 0);
+    check_sizes(dh0);
+    const int64_t m = dh0.size(0), n = dh0.size(1);
+    DG_CHECK(2 * n < ((int64_t)1 << 30));
+    const View dh = bf16_rows(dh_, "dh", m, n), dx = bf16_rows(dx_, "dx", m, 2 * n), h = bf16_rows(h_, "h", m, n);
+    const View q = view(q_, "q"), sf = view(sf_, "sf");
+    check_swiglu_checkpoint(q, sf, m, n);
+    SwigluBackwardArgs p{};
+    p.row_weight = row_weights_of(w_, m), p.row_layout = row_layout_of(rl_, m);
+    p.dw = const_cast<float*>(row_weights_of(dw_, m));
+    DG_CHECK((dw_ == nullptr) || (w_ != nullptr));   // a gradient of weights that were not given
+    const int device = one_device({dh_, q_, sf_, w_, rl_, dx_, h_, dw_});
+    if (m == 0) return;
+    p.dh = static_cast<const uint16_t*>(dh.data()), p.lddh = dh.stride(0);
+    p.q = static_cast<const uint8_t*>(q.data()), p.ldq = q.stride(0);
+    p.sf = static_cast<const float*>(sf.data()), p.sf_sm = sf.stride(0), p.sf_sk = sf.stride(1);
+    p.clamp = clamp;
+    p.dx = static_cast<uint16_t*>(const_cast<void*>(dx.data())), p.lddx = dx.stride(0);
+    p.h = static_cast<uint16_t*>(const_cast<void*>(h.data())), p.ldh = h.stride(0);
+    p.m = (int32_t)m, p.n = (int32_t)n;
+    const OnDevice on(device);
+    launch_swiglu_backward(p, stream);
+    char buf[96];
+    std::snprintf(buf, sizeof(buf), "moe_swiglu_backward m=%lld n=%lld", (long long)m, (long long)n);
+    t_last_config = buf;
+}
+
 }  // namespace
 }  // namespace dgm
 
@@ -1727,6 +1963,44 @@ int dg_moe_swiglu_apply_weight_to_fp8(const dg_tensor* x, const dg_tensor* row_w
 int dg_moe_combine(const dg_tensor* y, const dg_tensor* pos, const dg_tensor* topk_weights, const dg_tensor* out,
                    void* stream) {
     return guarded([&] { moe_combine_impl(y, pos, topk_weights, out, static_cast<hipStream_t>(stream)); });
+}
+
+int dg_m_grouped_bf16_gemm_nt_ragged(const dg_tensor* a, const dg_tensor* b, const dg_tensor* d,
+                                     const dg_tensor* group_ends, int32_t alignment, void* stream) {
+    return guarded([&] {
+        m_grouped_ragged_impl(kRaggedNT, a, b, d, group_ends, alignment, static_cast<hipStream_t>(stream));
+    });
+}
+
+int dg_m_grouped_bf16_gemm_nn_ragged(const dg_tensor* a, const dg_tensor* b, const dg_tensor* d,
+                                     const dg_tensor* group_ends, int32_t alignment, void* stream) {
+    return guarded([&] {
+        m_grouped_ragged_impl(kRaggedNN, a, b, d, group_ends, alignment, static_cast<hipStream_t>(stream));
+    });
+}
+
+int dg_k_grouped_bf16_gemm_tn_ragged(const dg_tensor* a, const dg_tensor* b, const dg_tensor* b_sf, const dg_tensor* d,
+                                     const dg_tensor* group_ends, const dg_tensor* c, int32_t alignment, void* stream) {
+    return guarded([&] {
+        k_grouped_ragged_impl(a, b, b_sf, d, group_ends, c, alignment, static_cast<hipStream_t>(stream));
+    });
+}
+
+int dg_moe_swiglu_checkpoint(const dg_tensor* x, const dg_tensor* row_weights, const dg_tensor* row_layout,
+                             float clamp_value, const dg_tensor* h, const dg_tensor* q, const dg_tensor* sf,
+                             void* stream) {
+    return guarded([&] {
+        swiglu_checkpoint_impl(x, row_weights, row_layout, clamp_value, h, q, sf, static_cast<hipStream_t>(stream));
+    });
+}
+
+int dg_moe_swiglu_backward(const dg_tensor* dh, const dg_tensor* q, const dg_tensor* sf, const dg_tensor* row_weights,
+                           const dg_tensor* row_layout, float clamp_value, const dg_tensor* dx, const dg_tensor* h,
+                           const dg_tensor* d_row_weights, void* stream) {
+    return guarded([&] {
+        swiglu_backward_impl(dh, q, sf, row_weights, row_layout, clamp_value, dx, h, d_row_weights,
+                             static_cast<hipStream_t>(stream));
+    });
 }
 
 int dg_set_num_sms(int32_t num_sms) {

@@ -316,6 +316,50 @@ struct CombineArgs {
 };
 void launch_moe_combine(const CombineArgs& args, hipStream_t stream);
 
+// BF16 products over ragged row segments (dg_gemm_bf16.hip). Strides in elements.
+enum RaggedKind : int { kRaggedNT = 0, kRaggedNN = 1, kRaggedTN = 2 };
+struct RaggedGemmArgs {
+    const uint16_t* a;         // NT, NN: bf16 [rows, k]; TN: bf16 [rows, m]
+    const void* b;             // NT: bf16 [groups, n, k]; NN: bf16 [groups, k, n]; TN: [rows, n], bf16 or e4m3
+    const float* b_sf;         // TN: f32 [rows, ceil(n / 128)] of an e4m3 b, or null
+    void* d;                   // NT, NN: [rows, n]; TN: [groups, m, n]; bf16 or f32
+    const void* c;             // TN: d's type and shape, or null
+    const int32_t* ends;       // [groups]
+    int32_t rows, m, n, k, groups, alignment, out_f32;
+    int64_t lda, ldb, ldd, ldc, b_gs, d_gs, c_gs, sf_sr, sf_sc;
+};
+void launch_ragged_gemm(RaggedKind kind, const RaggedGemmArgs& args, hipStream_t stream);
+
+// SwiGLU with an 8-bit checkpoint, and its backward pass (dg_swiglu_grad.hip). n: columns
+// of h; gate columns [0, n), up columns [n, 2n) of x, q and dx; scales of the gate half
+// first, ceil(n / 128) for each half.
+struct SwigluCheckpointArgs {
+    const uint16_t* x;         // bf16 [m, 2n]
+    const float* row_weight;   // [m] or null
+    const int32_t* row_layout; // [m] or null: rows with a negative entry count as zeros
+    float clamp;               // <= 0: none
+    uint16_t* h;               // bf16 [m, n]
+    uint8_t* q;                // e4m3 [m, 2n]
+    float* sf;
+    int64_t ldx, ldh, ldq, sf_sm, sf_sk;
+    int32_t m, n;
+};
+void launch_swiglu_checkpoint(const SwigluCheckpointArgs& args, hipStream_t stream);
+struct SwigluBackwardArgs {
+    const uint16_t* dh;        // bf16 [m, n]
+    const uint8_t* q;          // e4m3 [m, 2n]
+    const float* sf;
+    const float* row_weight;
+    const int32_t* row_layout;
+    float clamp;
+    uint16_t* dx;              // bf16 [m, 2n]
+    uint16_t* h;               // bf16 [m, n]
+    float* dw;                 // [m] or null
+    int64_t lddh, ldq, sf_sm, sf_sk, lddx, ldh;
+    int32_t m, n;
+};
+void launch_swiglu_backward(const SwigluBackwardArgs& args, hipStream_t stream);
+
 // D <- C (or zeros when c is null), used by the K == 0 early return.
 void launch_fill_or_copy(void* d, const void* c, int32_t rows, int32_t cols, int32_t groups,
                          int64_t ldd, int64_t d_gs, int64_t ldc, int64_t c_gs, int elem_bytes,

@@ -595,3 +595,69 @@ def per_token_cast_to_fp8_mn_major(x: torch.Tensor, use_ue8m0: bool,
     sf = torch.empty_strided((m, groups), (1, am), dtype=torch.float32, device=x.device)
     _check(_bind.cast(x, q, sf, int(gran_k), int(bool(use_ue8m0)), _raw_stream_of(x)))
     return q, sf
+
+
+# ------------------------------------------------------------------ BF16 expert products and SwiGLU checkpoints
+
+def m_grouped_bf16_gemm_nt_ragged(a: torch.Tensor, b: torch.Tensor, d: torch.Tensor, group_ends: torch.Tensor,
+                                  alignment: int = 1) -> None:
+    """D[r] = A[r] @ B[g(r)].T over ragged row segments: a bf16 [M, K], b bf16 [G, N, K],
+    d bf16 or float32 [M, N]. group_ends (int32 [G] on the device, not decreasing): group
+    g owns rows [align(group_ends[g - 1], alignment), group_ends[g]), of any number; with
+    alignment 1 the segments lie back to back, with moe_dispatch's alignment they are its
+    psum layout. Rows of no group are left untouched. K a multiple of 8; rows of a and b
+    start at multiples of 16 bytes, those of d anywhere."""
+    _check(_bind.m_grouped_ragged(0, a, b, d, group_ends, int(alignment), _raw_stream_of(d)))
+
+
+def m_grouped_bf16_gemm_nn_ragged(a: torch.Tensor, b: torch.Tensor, d: torch.Tensor, group_ends: torch.Tensor,
+                                  alignment: int = 1) -> None:
+    """D[r] = A[r] @ B[g(r)], b bf16 [G, K, N]: the gradient of the NT form's input, with
+    the forward weight as it lies (K = its output columns). Otherwise as the NT form."""
+    _check(_bind.m_grouped_ragged(1, a, b, d, group_ends, int(alignment), _raw_stream_of(d)))
+
+
+def k_grouped_bf16_gemm_tn_ragged(a: torch.Tensor, b, d: torch.Tensor, group_ends: torch.Tensor,
+                                  c: Optional[torch.Tensor] = None, alignment: int = 1) -> None:
+    """D[g] = C[g] + A_g.T @ B_g over the rows of each group (group_ends as in the NT form):
+    the gradient of its weight, with a = the gradient of its output [R, M] and b = its input
+    [R, N], in BF16 or as an 8-bit checkpoint (e4m3 [R, N], float32 [R, ceil(N / 128)]) such
+    as per_token_cast_to_fp8(x, use_ue8m0=True) or moe_dispatch gives (values are rounded to
+    BF16 after their scale: exact where it is a power of two). d bf16 or float32 [G, M, N];
+    c None (zeros) or like d, also d itself. Groups without rows get c."""
+    b_t, b_sf = _pair(b, 'b') if isinstance(b, (tuple, list)) else (b, None)
+    _check(_bind.k_grouped_ragged(a, b_t, b_sf, d, group_ends, c, int(alignment), _raw_stream_of(d)))
+
+
+def moe_swiglu_checkpoint(x: torch.Tensor, row_weights: Optional[torch.Tensor] = None,
+                          row_layout: Optional[torch.Tensor] = None, clamp_value: Optional[float] = None
+                          ) -> Tuple[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
+    """bf16 [M, 2I] (gate | up) -> (h bf16 [M, I] = silu(gate) * up * w, checkpoint), the
+    checkpoint being x in 8 bits for moe_swiglu_backward: (e4m3 [M, 2I], float32
+    [M, 2 ceil(I / 128)]) with power-of-two scales, each half as per_token_cast_to_fp8(half,
+    use_ue8m0=True). One HBM pass. row_layout (m_indices): rows with a negative entry count
+    as zeros. clamp_value: up within [-c, c] and gate at most c in h (x is kept unclamped)."""
+    m, i2 = x.shape
+    h = torch.empty((m, i2 // 2), dtype=torch.bfloat16, device=x.device)
+    q = torch.empty((m, i2), dtype=torch.float8_e4m3fn, device=x.device)
+    sf = torch.empty((m, 2 * ((i2 // 2 + 127) // 128)), dtype=torch.float32, device=x.device)
+    _check(_bind.swiglu_checkpoint(x, row_weights, row_layout, float(clamp_value or 0.0), h, q, sf, _raw_stream_of(x)))
+    return h, (q, sf)
+
+
+def moe_swiglu_backward(dh: torch.Tensor, checkpoint: Tuple[torch.Tensor, torch.Tensor],
+                        row_weights: Optional[torch.Tensor] = None, row_layout: Optional[torch.Tensor] = None,
+                        clamp_value: Optional[float] = None
+                        ) -> Tuple[torch.Tensor, torch.Tensor, Optional[torch.Tensor]]:
+    """Backward pass of moe_swiglu_checkpoint, at the gate and up values its checkpoint
+    holds: dh bf16 [M, I] -> (dx bf16 [M, 2I], h bf16 [M, I] recomputed for the weight
+    gradient of the product after it, float32 [M] gradient of row_weights or None without
+    them). The other arguments as in the forward pass."""
+    q, sf = _pair(checkpoint, 'checkpoint')
+    m, i = dh.shape
+    dx = torch.empty((m, 2 * i), dtype=torch.bfloat16, device=dh.device)
+    h = torch.empty((m, i), dtype=torch.bfloat16, device=dh.device)
+    dw = torch.empty((m,), dtype=torch.float32, device=dh.device) if row_weights is not None else None
+    _check(_bind.swiglu_backward(dh, q, sf, row_weights, row_layout, float(clamp_value or 0.0), dx, h, dw,
+                                 _raw_stream_of(dh)))
+    return dx, h, dw

@@ -95,6 +95,11 @@ SIGNATURES = {
     'dg_m_grouped_fp8_gemm_nt_masked_swiglu': (_I, [_T, _T, _T, _T, _T, _I, _T, ctypes.c_float, _T, _T, _V]),
     'dg_k_grouped_fp8_gemm_nt_contiguous': (_I, [_T, _T, _T, _T, _T, _P(_I), _I, _T, _T, _P(_I), _I, _V]),
     'dg_k_grouped_fp8_gemm_tn_contiguous': (_I, [_T, _T, _T, _T, _T, _P(_I), _I, _T, _T, _P(_I), _I, _V]),
+    'dg_m_grouped_bf16_gemm_nt_ragged': (_I, [_T, _T, _T, _T, _I, _V]),
+    'dg_m_grouped_bf16_gemm_nn_ragged': (_I, [_T, _T, _T, _T, _I, _V]),
+    'dg_k_grouped_bf16_gemm_tn_ragged': (_I, [_T, _T, _T, _T, _T, _T, _I, _V]),
+    'dg_moe_swiglu_checkpoint': (_I, [_T, _T, _T, ctypes.c_float, _T, _T, _T, _V]),
+    'dg_moe_swiglu_backward': (_I, [_T, _T, _T, _T, _T, ctypes.c_float, _T, _T, _T, _V]),
     'dg_set_num_sms': (_I, [_I]),
     'dg_get_num_sms': (_I, [_P(_I)]),
     'dg_set_mk_alignment_for_contiguous_layout': (_I, [_I]),
@@ -128,12 +133,17 @@ def _load_bind():
     except ImportError as e:
         raise ImportError(f'deep_gemm._dgbind is not built ({e}); run `python -c "import __graft_entry__ as g; '
                           f'g.build()"` from the repository root') from e
-    _dgbind.init(*[ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in
-                   ('dg_fp8_fp4_gemm_nt', 'dg_fp8_fp4_gemm_nt_ws', 'dg_fp8_gemm_nt_workspace_size',
+    def addresses(*names):
+        return [ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in names]
+    _dgbind.init(*addresses(
+                    'dg_fp8_fp4_gemm_nt', 'dg_fp8_fp4_gemm_nt_ws', 'dg_fp8_gemm_nt_workspace_size',
                     'dg_m_grouped_fp8_fp4_gemm_nt_contiguous', 'dg_m_grouped_fp8_fp4_gemm_nt_masked',
                     'dg_per_token_cast_to_fp8', 'dg_moe_dispatch', 'dg_moe_swiglu_apply_weight_to_fp8',
                     'dg_m_grouped_fp8_gemm_nt_contiguous_swiglu', 'dg_m_grouped_fp8_gemm_nt_masked_swiglu',
-                    'dg_moe_combine')])
+                    'dg_moe_combine'))
+    _dgbind.init_bf16(*addresses('dg_m_grouped_bf16_gemm_nt_ragged', 'dg_m_grouped_bf16_gemm_nn_ragged',
+                                 'dg_k_grouped_bf16_gemm_tn_ragged', 'dg_moe_swiglu_checkpoint',
+                                 'dg_moe_swiglu_backward'))
     return _dgbind
 
 

@@ -394,6 +394,68 @@ int dg_m_grouped_fp8_gemm_nt_masked_swiglu(const dg_tensor* a, const dg_tensor* 
 int dg_moe_combine(const dg_tensor* y, const dg_tensor* pos, const dg_tensor* topk_weights, const dg_tensor* out,
                    void* stream);
 
+/* ---------------------------------------------------------------- BF16 expert products */
+
+/* Training and BF16 serving of an MoE layer's experts: products over ragged row segments,
+ * without padding rows or host-side group sizes. `group_ends` (int32 [G], on the device,
+ * not decreasing) holds the end of each group's rows: group g owns rows
+ * [align(group_ends[g-1], alignment), group_ends[g]) (group 0 from row 0). alignment 1:
+ * segments back to back; dg_moe_dispatch's psum layout with the alignment it was made
+ * with otherwise. Groups may be empty. Ends past the rows that exist are cut off there.
+ * The reference's BF16 grouped GEMMs (csrc/apis/gemm.hpp) take segments padded to the MK
+ * alignment and K-group sizes on the host. */
+
+/* Forward: d[r] = a[r] @ b[g(r)]^T. Rows outside every group are left as they were.
+ *   a  bf16 [M, K], b bf16 [G, N, K], unit stride along K, K % 8 == 0, 16-byte rows
+ *   d  bf16 or fp32 [M, N], unit stride along N, any row pitch from N on
+ * Row pitches of at most 2^22 elements. */
+int dg_m_grouped_bf16_gemm_nt_ragged(const dg_tensor* a, const dg_tensor* b, const dg_tensor* d,
+                                     const dg_tensor* group_ends, int32_t alignment, void* stream);
+
+/* Gradient of the input: d[r] = a[r] @ b[g(r)], b bf16 [G, K, N] with unit stride along N
+ * (the forward weight as it lies: its rows are this product's K). Otherwise as the NT form. */
+int dg_m_grouped_bf16_gemm_nn_ragged(const dg_tensor* a, const dg_tensor* b, const dg_tensor* d,
+                                     const dg_tensor* group_ends, int32_t alignment, void* stream);
+
+/* Gradient of the weights: d[g] = c[g] + a_g^T @ b_g over the rows of group g.
+ *   a     bf16 [R, M], unit stride along M, 16-byte rows
+ *   b     bf16 [R, N] likewise (b_sf NULL), or an 8-bit checkpoint: e4m3 [R, N] in 8-byte
+ *         rows with b_sf f32 [R, ceil(N/128)] (any strides), the 1 x 128 scales of
+ *         dg_per_token_cast_to_fp8 or dg_moe_dispatch; a value is bf16(code * scale), exact
+ *         where the scale is a power of two (use_ue8m0)
+ *   d     bf16 or fp32 [G, M, N], unit stride along N
+ *   c     NULL (zeros), or d's type and shape; may be d (accumulation in place)
+ * A group without rows gets c. Sums in FP32. */
+int dg_k_grouped_bf16_gemm_tn_ragged(const dg_tensor* a, const dg_tensor* b, const dg_tensor* b_sf, const dg_tensor* d,
+                                     const dg_tensor* group_ends, const dg_tensor* c, int32_t alignment, void* stream);
+
+/* SwiGLU x routing weight in BF16, leaving its input in 8 bits for the backward pass:
+ * h = silu(gate) * up * w, gate = x[:, :I], up = x[:, I:], in FP32, rounded once.
+ *   x            bf16 [M, 2I], I % 8 == 0, 16-byte rows
+ *   row_weights  f32 [M] or NULL (w = 1)
+ *   row_layout   int32 [M] or NULL: rows with a negative entry count as zeros
+ *   clamp_value  > 0: up clamped to [-c, c] and gate to <= c in h; <= 0: no clamp
+ *   h            bf16 [M, I], 16-byte rows
+ *   q            e4m3 [M, 2I] in 8-byte rows, the codes of x (not clamped)
+ *   sf           f32 [M, 2 ceil(I/128)], any strides: power-of-two scales of 128 columns,
+ *                of the gate half first; each half as dg_per_token_cast_to_fp8 (gran_k 128,
+ *                use_ue8m0) gives it */
+int dg_moe_swiglu_checkpoint(const dg_tensor* x, const dg_tensor* row_weights, const dg_tensor* row_layout,
+                             float clamp_value, const dg_tensor* h, const dg_tensor* q, const dg_tensor* sf,
+                             void* stream);
+
+/* Its backward pass, at the gate and up values that the checkpoint holds (code * scale),
+ * with s = 1 / (1 + exp(-gate)):
+ *   dx = [dh w up s (1 + gate (1 - s)) | dh w gate s]   bf16 [M, 2I]; zero where the
+ *        clamp held the value (gate > c, |up| > c)
+ *   h  = gate s up w, recomputed for the next product's weight gradient   bf16 [M, I]
+ *   d_row_weights = sum over the row of dh gate s up   f32 [M], or NULL (needs row_weights)
+ * dh bf16 [M, I]; the other arguments as above. Rows with a negative row_layout entry give
+ * zeros. The row sums are taken in a fixed order. */
+int dg_moe_swiglu_backward(const dg_tensor* dh, const dg_tensor* q, const dg_tensor* sf, const dg_tensor* row_weights,
+                           const dg_tensor* row_layout, float clamp_value, const dg_tensor* dx, const dg_tensor* h,
+                           const dg_tensor* d_row_weights, void* stream);
+
 /* ---------------------------------------------------------------- knobs */
 
 /* Replace set_num_sms / get_num_sms (csrc/apis/config.hpp:15-20,
