@@ -39,6 +39,7 @@ struct EntryPoints {
     decltype(&dg_m_grouped_bf16_gemm_nt_ragged) ragged_nt;
     decltype(&dg_m_grouped_bf16_gemm_nn_ragged) ragged_nn;
     decltype(&dg_k_grouped_bf16_gemm_tn_ragged) ragged_tn;
+    decltype(&dg_bf16_gemm_ragged_workspace_size) ragged_workspace_size;
     decltype(&dg_moe_swiglu_checkpoint) swiglu_checkpoint;
     decltype(&dg_moe_swiglu_backward) swiglu_backward;
 } g_entry{};
@@ -168,10 +169,11 @@ PyObject* init(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 // init_bf16(addresses of the entry points after combine)
 PyObject* init_bf16(PyObject*, PyObject* const* a, Py_ssize_t n) {
-    return guarded(n, 5, [&] {
+    return guarded(n, 6, [&] {
         auto set = [&](auto& entry, int i) { entry = reinterpret_cast<std::decay_t<decltype(entry)>>(pointer<void>(a[i])); };
         set(g_entry.ragged_nt, 0), set(g_entry.ragged_nn, 1), set(g_entry.ragged_tn, 2);
-        set(g_entry.swiglu_checkpoint, 3), set(g_entry.swiglu_backward, 4);
+        set(g_entry.ragged_workspace_size, 3);
+        set(g_entry.swiglu_checkpoint, 4), set(g_entry.swiglu_backward, 5);
         return 0;
     });
 }
@@ -281,12 +283,31 @@ PyObject* combine(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
+// The workspace of a ragged product, from torch's caching allocator on the output's device
+// and current stream (it goes back there once the launches are queued); undefined if none.
+struct Workspace {
+    at::Tensor tensor;
+    Arg arg;
+    Workspace(int form, const at::Tensor& out, int64_t rows, int64_t m, int64_t n, int64_t k, int64_t groups) {
+        const int64_t bytes = out.is_cuda() ? g_entry.ragged_workspace_size(form, rows, m, n, k, (int32_t)groups) : 0;
+        if (bytes <= 0) return;   // (-1: sizes that the call itself refuses)
+        tensor = unlocked([&] { return at::empty({bytes}, out.options().dtype(at::kByte)); });
+        arg.fill(tensor);
+        arg.given = true;
+    }
+};
+
 // m_grouped_ragged(nn, a, b, d, group_ends, alignment, stream)
 PyObject* m_grouped_ragged(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded(n, 7, [&] {
-        const auto entry = integer(a[0]) ? g_entry.ragged_nn : g_entry.ragged_nt;
+        const bool nn = integer(a[0]) != 0;
+        const auto entry = nn ? g_entry.ragged_nn : g_entry.ragged_nt;
         const Arg ta(a[1]), tb(a[2]), d(a[3]), ends(a[4]);
-        return call(entry, ta.get(), tb.get(), d.get(), ends.get(), (int32_t)integer(a[5]), pointer<void>(a[6]));
+        const int32_t alignment = (int32_t)integer(a[5]);
+        void* stream = pointer<void>(a[6]);
+        const bool fits = ta.d.ndim == 2 && tb.d.ndim == 3;
+        const Workspace ws(nn, tensor(a[3]), fits ? ta.d.sizes[0] : 0, 0, tb.d.sizes[nn ? 2 : 1], ta.d.sizes[1], tb.d.sizes[0]);
+        return call(entry, ta.get(), tb.get(), d.get(), ends.get(), alignment, ws.arg.get(), stream);
     });
 }
 
@@ -294,8 +315,12 @@ PyObject* m_grouped_ragged(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyObject* k_grouped_ragged(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded(n, 8, [&] {
         const Arg ta(a[0]), tb(a[1]), sf(a[2], true), d(a[3]), ends(a[4]), c(a[5], true);
-        return call(g_entry.ragged_tn, ta.get(), tb.get(), sf.get(), d.get(), ends.get(), c.get(), (int32_t)integer(a[6]),
-                    pointer<void>(a[7]));
+        const int32_t alignment = (int32_t)integer(a[6]);
+        void* stream = pointer<void>(a[7]);
+        const bool fits = ta.d.ndim == 2 && tb.d.ndim == 2 && d.d.ndim == 3;
+        const Workspace ws(2, tensor(a[3]), ta.d.sizes[0], ta.d.sizes[1], fits ? tb.d.sizes[1] : 0, 0, d.d.sizes[0]);
+        return call(g_entry.ragged_tn, ta.get(), tb.get(), sf.get(), d.get(), ends.get(), c.get(), alignment, ws.arg.get(),
+                    stream);
     });
 }
 

@@ -86,6 +86,7 @@ TileConfig choose_tinym(int64_t m, int64_t n, int64_t k, int cus) {
 std::atomic<int> g_num_sms{0};                 // 0: query the device
 std::atomic<int> g_mk_alignment{kDefaultMKAlignment};
 std::atomic<int> g_tile_variant{0}, g_tile_m{0}, g_tile_n{0};   // variant 0: heuristic
+std::atomic<int> g_ragged_block{0}, g_ragged_splits{0};         // variant 13: the ragged BF16 products'
 
 template <typename F>
 int guarded(F&& f) {
@@ -1583,6 +1584,9 @@ void check_ragged_matrix(const View& t, int dims) {
     if (dims == 3 && t.size(0) > 1) DG_CHECK(t.stride(0) >= (t.size(1) > 0 ? (t.size(1) - 1) * t.stride(1) + t.size(2) : 0));
 }
 
+// Row pitch of a matrix: of a single row (whose stride says nothing) its length.
+int64_t row_pitch(const View& t) { return t.size(-2) > 1 ? t.stride(-2) : align_up(t.size(-1), 8); }
+
 bool has_elements(const View& t) {
     for (int i = 0; i < t.dim(); ++i)
         if (t.size(i) == 0) return false;
@@ -1595,14 +1599,34 @@ void check_group_ends(const View& t, int64_t groups, int32_t alignment) {
     DG_CHECK(alignment > 0 && alignment <= (1 << 20));
 }
 
-void ragged_config(const char* kind, const RaggedGemmArgs& a) {
+RaggedPlan ragged_plan(RaggedKind kind, const RaggedGemmArgs& a) {
+    return plan_ragged_gemm(kind, a, num_sms_now(), g_ragged_block.load(), g_ragged_splits.load());
+}
+
+// Plans and launches a call; without a workspace, or with one too small, the reduced axis
+// stays whole.
+void run_ragged(const char* name, RaggedKind kind, const RaggedGemmArgs& a, const dg_tensor* ws_, hipStream_t stream) {
+    RaggedPlan plan = ragged_plan(kind, a);
+    float* ws = nullptr;
+    if (plan.splits > 1) {
+        if (ws_ != nullptr) {
+            const View w = view(ws_, "workspace");
+            DG_CHECK(w.on_device() && w.dim() == 1 && contiguous_view(w));
+            DG_CHECK(reinterpret_cast<uintptr_t>(w.data()) % 16 == 0);
+            if (w.size(0) * elem_size(w.dtype()) >= plan.workspace_bytes)
+                ws = static_cast<float*>(const_cast<void*>(w.data()));
+        }
+        if (ws == nullptr) plan.splits = 1, plan.workspace_bytes = 0;
+    }
+    launch_ragged_gemm(kind, a, plan, ws, num_sms_now(), stream);
     char buf[160];
-    std::snprintf(buf, sizeof(buf), "%s rows=%d m=%d n=%d k=%d groups=%d", kind, a.rows, a.m, a.n, a.k, a.groups);
+    std::snprintf(buf, sizeof(buf), "%s block=%d splits=%d rows=%d m=%d n=%d k=%d groups=%d", name, plan.block, plan.splits,
+                  a.rows, a.m, a.n, a.k, a.groups);
     t_last_config = buf;
 }
 
 void m_grouped_ragged_impl(RaggedKind kind, const dg_tensor* a_, const dg_tensor* b_, const dg_tensor* d_,
-                           const dg_tensor* ends_, int32_t alignment, hipStream_t stream) {
+                           const dg_tensor* ends_, int32_t alignment, const dg_tensor* ws_, hipStream_t stream) {
     const View a = view(a_, "a"), b = view(b_, "b"), d = view(d_, "d"), ends = view(ends_, "group_ends");
     check_ragged_matrix(a, 2);
     check_ragged_matrix(b, 3);
@@ -1616,22 +1640,22 @@ void m_grouped_ragged_impl(RaggedKind kind, const dg_tensor* a_, const dg_tensor
     check_group_ends(ends, groups, alignment);
     if (has_elements(a)) check_vector_alignment(a, "a");
     if (has_elements(b)) check_vector_alignment(b, "b");
-    const int device = one_device({a_, b_, d_, ends_});
+    const int device = one_device({a_, b_, d_, ends_, ws_});
     if (rows == 0 || n == 0 || groups == 0) return;
     RaggedGemmArgs p{};
-    p.a = static_cast<const uint16_t*>(a.data()), p.lda = a.stride(0);
-    p.b = b.data(), p.ldb = b.stride(1), p.b_gs = b.stride(0);
+    p.a = static_cast<const uint16_t*>(a.data()), p.lda = row_pitch(a);
+    p.b = b.data(), p.ldb = row_pitch(b), p.b_gs = b.stride(0);
     p.d = const_cast<void*>(d.data()), p.ldd = d.stride(0);
     p.ends = static_cast<const int32_t*>(ends.data());
     p.rows = (int32_t)rows, p.n = (int32_t)n, p.k = (int32_t)k, p.groups = (int32_t)groups, p.alignment = alignment;
     p.out_f32 = d.dtype() == DG_F32;
     const OnDevice on(device);
-    launch_ragged_gemm(kind, p, stream);
-    ragged_config(kind == kRaggedNT ? "bf16_ragged_nt" : "bf16_ragged_nn", p);
+    run_ragged(kind == kRaggedNT ? "bf16_ragged_nt" : "bf16_ragged_nn", kind, p, ws_, stream);
 }
 
 void k_grouped_ragged_impl(const dg_tensor* a_, const dg_tensor* b_, const dg_tensor* b_sf_, const dg_tensor* d_,
-                           const dg_tensor* ends_, const dg_tensor* c_, int32_t alignment, hipStream_t stream) {
+                           const dg_tensor* ends_, const dg_tensor* c_, int32_t alignment, const dg_tensor* ws_,
+                           hipStream_t stream) {
     const View a = view(a_, "a"), b = view(b_, "b"), d = view(d_, "d"), ends = view(ends_, "group_ends");
     check_ragged_matrix(a, 2);
     check_ragged_matrix(b, 2);
@@ -1664,17 +1688,16 @@ void k_grouped_ragged_impl(const dg_tensor* a_, const dg_tensor* b_, const dg_te
             for (int i = 0; i < 3; ++i) DG_CHECK(c.size(i) <= 1 || c.stride(i) == d.stride(i));
         p.c = c.data(), p.ldc = c.stride(1), p.c_gs = c.stride(0);
     }
-    const int device = one_device({a_, b_, b_sf_, d_, ends_, c_});
+    const int device = one_device({a_, b_, b_sf_, d_, ends_, c_, ws_});
     if (m == 0 || n == 0 || groups == 0) return;
-    p.a = static_cast<const uint16_t*>(a.data()), p.lda = a.stride(0);
-    p.b = b.data(), p.ldb = b.stride(0);
+    p.a = static_cast<const uint16_t*>(a.data()), p.lda = row_pitch(a);
+    p.b = b.data(), p.ldb = row_pitch(b);
     p.d = const_cast<void*>(d.data()), p.ldd = d.stride(1), p.d_gs = d.stride(0);
     p.ends = static_cast<const int32_t*>(ends.data());
     p.rows = (int32_t)rows, p.m = (int32_t)m, p.n = (int32_t)n, p.groups = (int32_t)groups, p.alignment = alignment;
     p.out_f32 = d.dtype() == DG_F32;
     const OnDevice on(device);
-    launch_ragged_gemm(kRaggedTN, p, stream);
-    ragged_config(b_sf_ ? "bf16_ragged_tn b=e4m3" : "bf16_ragged_tn", p);
+    run_ragged(b_sf_ ? "bf16_ragged_tn b=e4m3" : "bf16_ragged_tn", kRaggedTN, p, ws_, stream);
 }
 
 const float* row_weights_of(const dg_tensor* w_, int64_t m) {
@@ -1785,6 +1808,7 @@ int dg_init(void) {
         g_tile_variant = 0;
         g_tile_m = 0;
         g_tile_n = 0;
+        g_ragged_block = 0, g_ragged_splits = 0;
     });
 }
 
@@ -1965,24 +1989,40 @@ int dg_moe_combine(const dg_tensor* y, const dg_tensor* pos, const dg_tensor* to
     return guarded([&] { moe_combine_impl(y, pos, topk_weights, out, static_cast<hipStream_t>(stream)); });
 }
 
+int64_t dg_bf16_gemm_ragged_workspace_size(int32_t form, int64_t rows, int64_t m, int64_t n, int64_t k, int32_t groups) {
+    int64_t bytes = -1;
+    guarded([&] {
+        DG_CHECK(form >= 0 && form <= 2);
+        for (int64_t v : {rows, m, n, k, (int64_t)groups}) DG_CHECK(v >= 0 && v < ((int64_t)1 << 30));
+        RaggedGemmArgs a{};
+        a.rows = (int32_t)rows, a.m = (int32_t)m, a.n = (int32_t)n, a.k = (int32_t)k, a.groups = groups;
+        const bool nothing = n == 0 || groups == 0 || (form == 2 ? m == 0 : rows == 0);
+        bytes = nothing ? 0 : ragged_plan((RaggedKind)form, a).workspace_bytes;
+    });
+    return bytes;
+}
+
 int dg_m_grouped_bf16_gemm_nt_ragged(const dg_tensor* a, const dg_tensor* b, const dg_tensor* d,
-                                     const dg_tensor* group_ends, int32_t alignment, void* stream) {
+                                     const dg_tensor* group_ends, int32_t alignment, const dg_tensor* workspace,
+                                     void* stream) {
     return guarded([&] {
-        m_grouped_ragged_impl(kRaggedNT, a, b, d, group_ends, alignment, static_cast<hipStream_t>(stream));
+        m_grouped_ragged_impl(kRaggedNT, a, b, d, group_ends, alignment, workspace, static_cast<hipStream_t>(stream));
     });
 }
 
 int dg_m_grouped_bf16_gemm_nn_ragged(const dg_tensor* a, const dg_tensor* b, const dg_tensor* d,
-                                     const dg_tensor* group_ends, int32_t alignment, void* stream) {
+                                     const dg_tensor* group_ends, int32_t alignment, const dg_tensor* workspace,
+                                     void* stream) {
     return guarded([&] {
-        m_grouped_ragged_impl(kRaggedNN, a, b, d, group_ends, alignment, static_cast<hipStream_t>(stream));
+        m_grouped_ragged_impl(kRaggedNN, a, b, d, group_ends, alignment, workspace, static_cast<hipStream_t>(stream));
     });
 }
 
 int dg_k_grouped_bf16_gemm_tn_ragged(const dg_tensor* a, const dg_tensor* b, const dg_tensor* b_sf, const dg_tensor* d,
-                                     const dg_tensor* group_ends, const dg_tensor* c, int32_t alignment, void* stream) {
+                                     const dg_tensor* group_ends, const dg_tensor* c, int32_t alignment,
+                                     const dg_tensor* workspace, void* stream) {
     return guarded([&] {
-        k_grouped_ragged_impl(a, b, b_sf, d, group_ends, c, alignment, static_cast<hipStream_t>(stream));
+        k_grouped_ragged_impl(a, b, b_sf, d, group_ends, c, alignment, workspace, static_cast<hipStream_t>(stream));
     });
 }
 
@@ -2037,6 +2077,13 @@ int dg_set_tile_override(int32_t variant, int32_t block_m, int32_t block_n) {
     return guarded([&] {
         if (variant == 0) {
             g_tile_variant = 0, g_tile_m = 0, g_tile_n = 0;
+            g_ragged_block = 0, g_ragged_splits = 0;
+            return;
+        }
+        if (variant == 13) {
+            if ((block_m != 128 && block_m != 256) || block_n < 0 || block_n > (block_m == 128 ? 32 : 0))
+                DG_UNSUPPORTED("tile shape not compiled");
+            g_ragged_block = block_m, g_ragged_splits = block_n;
             return;
         }
         const bool ok = variant == 1   ? fp8_1d2d_tile_supported(block_m, block_n)

@@ -13,9 +13,11 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 
 #include "dg_internal.hpp"
 #include "dg_kernel_common.hpp"
+#include "dg_lds_dma.hpp"
 
 namespace dgm {
 namespace {
@@ -24,6 +26,20 @@ using namespace dev;
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
+// Two values rounded to BF16 by one v_cvt_pk_bf16_f32.
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{lo, hi}, bf16x2));
+}
+
+// Tiles of a launch: row and column blocks (NT, NN: row blocks at most; of 256 for quarters),
+// CUs, pieces of the reduced axis (blockIdx.y), and whether D and C take 16-byte accesses.
+struct RaggedLaunch {
+    int row_blocks, col_blocks, slots, splits, vec;
+};
+constexpr int kRasterBlocks = 8;   // row blocks of a raster band
+
 // Rows [start, end) of group g, inside the `rows` that exist whatever group_ends holds.
 __device__ __forceinline__ void group_rows(const int32_t* ends, int g, int rows, int alignment, int& start, int& end) {
     const int prev = g > 0 ? min(max(ends[g - 1], 0), rows) : 0;
@@ -31,139 +47,691 @@ __device__ __forceinline__ void group_rows(const int32_t* ends, int g, int rows,
     end = max(start, min(ends[g], rows));
 }
 
-// The row block `blk` (of BM rows each) of the launch's blocks, groups in order: its group,
-// first row and the group's end; false past the last one. A wave looks at 64 groups at a
-// time: every lane counts one group's blocks, a prefix sum over the lanes places them.
-template <int BM>
-__device__ __forceinline__ bool find_block(const int32_t* ends, int groups, int rows, int alignment, int64_t blk, int& g,
-                                           int& m0, int& row_end) {
+// A launch of 256 x 256 tiles whose last round (a tile per CU) would be at most 58% full
+// leaves that round's tiles to a second launch, as four 128 x 128 quarters each: two
+// workgroups of those fit a CU, so 150 tiles' quarters take 1.2 rounds of 512, about 0.65
+// of a 256 x 256 round (PART 1 and 2; 0 is a launch by itself). Both launches work it
+// out alike, from the tiles that there are. 8 experts, 16384 x 4096 x 7168 (NT, 1088
+// tiles, 4.25 rounds): see launch_ragged_gemm.
+__device__ __forceinline__ int tail_tiles(int tiles, int slots) {
+    const int rest = tiles % slots;
+    return rest * 128 <= slots * 75 ? rest : 0;
+}
+
+// What a workgroup computes: rows [m0, m_end) of D and columns from n0, for group g,
+// reduced over [k0, k_end).
+struct RaggedTile {
+    int g, m0, m_end, n0, k0, k_end;
+};
+
+// Item `i` of the `tiles` items of a list (PART 2: a quarter of one of its last tiles):
+// the tile, or -1.
+template <int PART>
+__device__ __forceinline__ int list_tile(int i, int tiles, int slots, int& quarter) {
+    const int full = PART == 0 ? tiles : tiles - tail_tiles(tiles, slots);
+    quarter = 0;
+    if constexpr (PART == 2) {
+        quarter = i & 3;
+        i = full + (i >> 2);
+        return i < tiles ? i : -1;
+    }
+    return i < full ? i : -1;
+}
+
+// NT, NN: row blocks of BM rows, groups in order; a wave looks at 64 groups at a time, every
+// lane counting one group's blocks, a prefix sum over the lanes placing them. Each XCD
+// gets a contiguous part of the tiles that there are (the grid is an upper bound:
+// group_ends is on the device).
+template <int BM, int BN, int PART>
+__device__ __forceinline__ bool locate_rows(const RaggedGemmArgs& p, const RaggedLaunch& l, RaggedTile& t) {
     const int lane = threadIdx.x & 63;
-    int64_t base = 0;
-    for (int g0 = 0; g0 < groups; g0 += 64) {
-        int start = 0, end = 0;
-        if (g0 + lane < groups) group_rows(ends, g0 + lane, rows, alignment, start, end);
-        const int mine = (end - start + BM - 1) / BM;
-        int incl = mine;
+    int start = 0, end = 0, mine = 0, incl = 0;
+    auto count = [&](int g0) {   // blocks of groups [g0, g0 + 64): this lane's, and up to it
+        start = end = 0;
+        if (g0 + lane < p.groups) group_rows(p.ends, g0 + lane, p.rows, p.alignment, start, end);
+        mine = (end - start + BM - 1) / BM;
+        incl = mine;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
             const int v = __shfl_up(incl, o);
             incl += lane >= o ? v : 0;
         }
-        const int total = __shfl(incl, 63);
-        if (blk < base + total) {
-            const int at = __ffsll((unsigned long long)__ballot(base + incl > blk)) - 1;
-            g = g0 + at;
-            m0 = __shfl(start, at) + (int)(blk - base - __shfl(incl - mine, at)) * BM;
-            row_end = __shfl(end, at);
-            return true;
+        return __builtin_amdgcn_readlane(incl, 63);
+    };
+    int total = 0;   // (decreasing ends could count more than the launch holds)
+    for (int g0 = 0; g0 < p.groups; g0 += 64) total = min(total + count(g0), l.row_blocks);
+    const int tiles = total * l.col_blocks;
+    const int full = PART == 0 ? tiles : tiles - tail_tiles(tiles, l.slots);
+    const int items = PART == 2 ? (tiles - full) * 4 : full;
+    if ((int)blockIdx.x >= items) return false;
+    int quarter;
+    const int lt = list_tile<PART>(xcd_remap(blockIdx.x, items), tiles, l.slots, quarter);
+    const int block = lt / l.col_blocks;
+    int base = 0;
+    for (int g0 = 0; g0 < p.groups; g0 += 64) {
+        const int here = p.groups <= 64 ? total : count(g0);
+        if (block < base + here) {
+            const int at = __ffsll((unsigned long long)__ballot(base + incl > block)) - 1;
+            const int blocks = __builtin_amdgcn_readlane(mine, at);
+            const int first = base + __builtin_amdgcn_readlane(incl, at) - blocks;
+            int mb, nb;
+            raster_tile(lt - first * l.col_blocks, blocks, l.col_blocks, kRasterBlocks, mb, nb);
+            t.g = g0 + at;
+            t.m0 = __builtin_amdgcn_readlane(start, at) + mb * BM + (quarter >> 1) * (BM / 2);
+            t.m_end = __builtin_amdgcn_readlane(end, at);
+            t.n0 = nb * BN + (quarter & 1) * (BN / 2);
+            t.k0 = 0, t.k_end = p.k;
+            return t.m0 < t.m_end && t.n0 < p.n;
         }
-        base += total;
+        base += here;
     }
     return false;
 }
 
-constexpr int kBM = 128, kBN = 128, kBK = 32, kPitch = kBK + 8;
-
-__device__ __forceinline__ uint16_t load_b(const RaggedGemmArgs& p, int64_t row, int col, const uint16_t* b) {
-    if (!p.b_sf) return b[row * p.ldb + col];
-    const uint8_t q = reinterpret_cast<const uint8_t*>(b)[row * p.ldb + col];
-    const float v = __builtin_amdgcn_cvt_f32_fp8(q, 0) * p.b_sf[row * p.sf_sr + (int64_t)(col >> 7) * p.sf_sc];
-    return bf16_bits(v);
+// Group at place q of the groups from the longest to the shortest (up to 64 groups; in
+// their own order otherwise), so that the last tiles of a launch are the short ones.
+__device__ __forceinline__ int group_by_length(const RaggedGemmArgs& p, int q) {
+    if (p.groups > 64) return q;
+    const int lane = threadIdx.x & 63;
+    int start = 0, end = -1;
+    if (lane < p.groups) group_rows(p.ends, lane, p.rows, p.alignment, start, end);
+    const int size = end - start;
+    int place = 0;
+    for (int j = 0; j < p.groups; ++j) {
+        const int other = __builtin_amdgcn_readlane(size, j);
+        place += other > size || (other == size && j < lane);
+    }
+    return __ffsll((unsigned long long)__ballot(place == q && lane < p.groups)) - 1;
 }
 
-template <int KIND>
-__global__ void __launch_bounds__(256) ragged_gemm_kernel(const RaggedGemmArgs p, const int nb) {
-    __shared__ __attribute__((aligned(16))) uint16_t s_a[kBM * kPitch], s_b[kBN * kPitch];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    int g, m0, m_end, k0 = 0, k_end = p.k;   // output rows [m0, m_end), reduced over [k0, k_end)
-    const int64_t blk = blockIdx.x / nb;
-    const int n0 = (int)(blockIdx.x % nb) * kBN;
-    if constexpr (KIND == kRaggedTN) {
-        const int mb = (p.m + kBM - 1) / kBM;
-        g = (int)(blk / mb);
-        m0 = (int)(blk % mb) * kBM;
-        m_end = p.m;
-        group_rows(p.ends, g, p.rows, p.alignment, k0, k_end);
-    } else {
-        if (!find_block<kBM>(p.ends, p.groups, p.rows, p.alignment, blk, g, m0, m_end)) return;
+// TN: every group has the same tiles. Every XCD takes an eighth of each group's, group
+// after group, so that groups of different lengths weigh on all of them alike (groups
+// of few tiles: tiles dealt out one by one).
+template <int BM, int BN, int PART>
+__device__ __forceinline__ bool locate_outputs(const RaggedGemmArgs& p, const RaggedLaunch& l, RaggedTile& t) {
+    const int per = l.row_blocks * l.col_blocks;
+    const bool eighths = per % 8 == 0 || per >= 64;
+    int lo = 0, mine = per, i = blockIdx.x, slots = l.slots;
+    if (eighths) {
+        const int x = blockIdx.x & 7;
+        lo = (int)((int64_t)x * per / 8);
+        mine = (int)((int64_t)(x + 1) * per / 8) - lo;
+        i = blockIdx.x >> 3;
+        slots = max(l.slots / 8, 1);
     }
-    const uint16_t* b = static_cast<const uint16_t*>(p.b) + (KIND == kRaggedTN ? 0 : (int64_t)g * p.b_gs);
+    int quarter;
+    const int at = list_tile<PART>(i, mine * p.groups, slots, quarter);
+    if (at < 0) return false;
+    const int q = at / mine;
+    int mb, nb;
+    raster_tile(lo + at - q * mine, l.row_blocks, l.col_blocks, kRasterBlocks, mb, nb);
+    t.g = group_by_length(p, q);
+    t.m0 = mb * BM + (quarter >> 1) * (BM / 2), t.n0 = nb * BN + (quarter & 1) * (BN / 2);
+    t.m_end = p.m;
+    group_rows(p.ends, t.g, p.rows, p.alignment, t.k0, t.k_end);
+    return t.m0 < p.m && t.n0 < p.n;
+}
 
-    f32x16 acc[2][2];
+// ---------------------------------------------------------------- tiles
+//
+// One workgroup per BM x BN tile of D, 64 reduced elements a step, two steps in LDS.
+// Operands go straight to LDS by buffer loads (16 bytes a lane) whose descriptor ends at
+// the last valid byte: rows past the group's, columns past N and reduced elements past the
+// end arrive as zeros, in both operands, and nothing is read there. So there are no edge
+// variants, and steps past the end may be issued freely (they read nothing).
+//
+// An operand whose reduced dimension is contiguous ("K-major": A of NT and NN, B of NT)
+// holds 64 reduced elements of a row in 128 bytes, 16-byte chunk c of row r at c ^ g(r); a
+// matrix instruction's fragment (row lane & 31, 8 reduced elements) is one 16-byte read.
+// The others ("MN-major": B of NN, both of TN) hold one reduced row of BM or BN columns
+// after another; their fragments are read by ds_read_b64_tr_b16, which hands 16 lanes a
+// transposed 4 x 16 block: 4 reduced rows of 32 bytes each. The 32-byte units of a row are
+// permuted (column unit 2a + b of reduced row k at b * 4 + (a & 3 ^ k & 3) + (a >> 2) * 8)
+// so that the four rows of a block, and the two blocks side by side, lie in distinct banks.
+//
+// The hand-off to the next step (wait for its loads, barrier, issue the loads of the step
+// after it into the freed half of LDS) comes before the last 32-row slice of a step's
+// matrix instructions, with the next step's fragments read under them.
+
+__device__ __forceinline__ int swz_g(int r) { return ((r >> 1) ^ ((r & 1) << 2)) & 7; }
+
+// 16 bytes a lane from `rsrc` at byte voff (zeros past its end) to lds + 16 * lane. Inline
+// asm: the compiler would wait for every load in flight before each LDS read.
+__device__ __forceinline__ void dma16_buffer(const i32x4& rsrc, uint32_t voff, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voff), "s"(rsrc)
+                 : "memory", "m0");
+}
+
+// Buffer descriptor of `bytes` bytes (a multiple of 4 is read, dword by dword) from `base`.
+__device__ __forceinline__ i32x4 descriptor(const void* base, int bytes) {
+    const uint64_t a = reinterpret_cast<uint64_t>(base);
+    return i32x4{__builtin_amdgcn_readfirstlane((int)(uint32_t)a), __builtin_amdgcn_readfirstlane((int)((uint32_t)(a >> 32) & 0xFFFFu)),
+                 __builtin_amdgcn_readfirstlane(bytes), 0x00020000};
+}
+
+// No offset of a valid byte: past the end of every descriptor here.
+constexpr uint32_t kPastEnd = 0x80000000u;
+
+// One operand of a tile: where its steps come from. ROWS: BM or BN; KMAJOR as above.
+constexpr int BK = 64;
+
+template <int ROWS, int KMAJOR, int NW>
+struct Operand {
+    static constexpr int kInstr = ROWS * BK / (512 * NW);   // wave loads (1 KB) of a step for each wave
+    static_assert(kInstr * 512 * NW == ROWS * BK && (KMAJOR || ROWS == 128 || ROWS == 256), "whole wave loads");
+
+    const uint8_t* base;   // the tile's first element of the step to be issued next
+    int64_t pitch;         // bytes
+    int rows;              // valid rows (KMAJOR) or columns of the tile
+    int left;              // reduced elements from there on
+    uint32_t vlane;        // this lane's offset in a wave load
+    int chunk;             // KMAJOR: first reduced element of this lane's chunk
+
+    __device__ __forceinline__ void init(const uint16_t* at, int64_t ld, int valid, int reduced, int wave, int lane) {
+        base = reinterpret_cast<const uint8_t*>(at);
+        pitch = ld * 2;
+        rows = valid;
+        left = reduced;
+        if constexpr (KMAJOR) {
+            const int rs = lane / (BK / 8);
+            // (NW is even, so a wave's 8-row pieces share a parity)
+            chunk = ((lane & 7) ^ swz_g((wave & 1) * 8 + rs)) * 8;
+            vlane = (uint32_t)(rs * (int)pitch) + chunk * 2;
+        } else {
+            constexpr int LPR = ROWS / 8;   // lanes per reduced row
+            const int k = lane / LPR + (ROWS == 256 ? (wave & 1) * 2 : 0);   // its two low bits
+            const int slot = lane % LPR, pu = slot >> 1;
+            const int a = ((pu & 3) ^ (k & 3)) | (pu >> 3) << 2, b = (pu >> 2) & 1;
+            const int col = (2 * a + b) * 16 + (slot & 1) * 8;
+            vlane = col < valid ? (uint32_t)(lane / LPR * (int)pitch) + col * 2 : kPastEnd;
+        }
+    }
+    // The next step to lds (this operand's part of a stage).
+    __device__ __forceinline__ void issue(uint32_t lds, int wave) {
+        constexpr int PER = 512 / (KMAJOR ? BK : ROWS);   // rows of a wave load
+        // (without branches, which would split the loop's instruction sequence; nothing
+        // left: every lane past the end, or no bytes, as a row is no longer than the pitch)
+        const int n = min(max(left, 0), BK);
+        const int bytes = KMAJOR ? (rows - 1) * (int)pitch + n * 2 : max((n - 1) * (int)pitch + ((rows * 2 + 3) & ~3), 0);
+        const uint32_t v = !KMAJOR || chunk < left ? vlane : kPastEnd;
+        const i32x4 rsrc = descriptor(base, bytes);
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < kInstr; ++i) {
+            const int seg = i * NW + wave;
+            dma16_buffer(rsrc, v + (uint32_t)(seg * PER * (int)pitch), lds + seg * 1024);
+        }
+        base += KMAJOR ? (int64_t)BK * 2 : BK * pitch;
+        left -= BK;
+    }
+};
+
+// Fragment reads of a 32-row slab: off[] for slab 0 of the wave, see above.
+template <int ROWS, int KMAJOR, int SLABS>
+struct Fragments {
+    uint32_t off[KMAJOR ? BK / 16 : SLABS];
+    __device__ __forceinline__ void init(int first_row, int lane) {
+        if constexpr (KMAJOR) {
+            const int r = lane & 31;
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+            for (int ks = 0; ks < BK / 16; ++ks)
+                off[ks] = (first_row + r) * (BK * 2) + (((2 * ks + (lane >> 5)) ^ swz_g(r)) << 4);
+        } else {
+            const int i = lane & 15, a = first_row >> 5;
+#pragma unroll
+            for (int s = 0; s < SLABS; ++s)
+                off[s] = ((lane >> 5) * 8 + (i >> 2)) * (ROWS * 2) + ((lane >> 4) & 1) * 128 +
+                         ((((a + s) & 3) ^ (i >> 2)) << 5) + ((a + s) >> 2) * 256 + (i & 3) * 8;
+        }
+    }
+    __device__ __forceinline__ bf16x8 read(const uint8_t* tile, int slab, int ks) const {
+        if constexpr (KMAJOR) {
+            return *reinterpret_cast<const bf16x8*>(tile + off[ks] + slab * 32 * (BK * 2));
+        } else {
+            typedef short s16x4 __attribute__((ext_vector_type(4)));
+            typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+            const uint8_t* at = tile + off[slab] + ks * 16 * (ROWS * 2);
+            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at);
+            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 4 * (ROWS * 2)));
+            return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+        }
+    }
+};
+
+// An 8-bit B of TN: 64 reduced rows of BN codes through registers (32 codes of one row, so
+// one scale, per thread), to BF16, into the MN-major layout.
+template <int BN, int NT>
+struct CodeOperand {
+    static constexpr int TPR = BN / 32;   // threads per reduced row
+    static_assert(NT == TPR * BK, "32 codes per thread");
+    const uint8_t* base;
+    const float* sf;
+    int64_t pitch, sf_pitch;
+    int left, row;
+    int pieces;          // valid 8-code pieces of this thread (columns)
+    uint32_t to[4];      // where its 8-column pieces go
+    uint2 raw[4];
+    float scale;
+
+    __device__ __forceinline__ void init(const RaggedGemmArgs& p, int k0, int reduced, int n0, int tid) {
+        row = tid / TPR;
+        const int col = tid % TPR * 32;
+        pitch = p.ldb, sf_pitch = p.sf_sr;
+        base = static_cast<const uint8_t*>(p.b) + (int64_t)(k0 + row) * pitch + n0 + col;
+        const int valid = p.n - n0 - col;   // columns from there on
+        pieces = min(max((valid + 7) / 8, 0), 4);
+        sf = p.b_sf + (int64_t)(k0 + row) * sf_pitch + (int64_t)min((n0 + col) >> 7, (p.n - 1) >> 7) * p.sf_sc;
+        left = reduced;
+        const int a = col >> 5;
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            to[q] = row * (BN * 2) + (q >> 1) * 128 + (((a & 3) ^ (row & 3)) << 5) + (a >> 2) * 256 + (q & 1) * 16;
+    }
+    __device__ __forceinline__ void load() {
+        const bool in = row < left;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) raw[q] = in && q < pieces ? *reinterpret_cast<const uint2*>(base + q * 8) : uint2{0u, 0u};
+        scale = in ? *sf : 0.f;
+        base += BK * pitch, sf += BK * sf_pitch, left -= BK;
+    }
+    __device__ __forceinline__ void store(uint8_t* tile) const {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            uint32_t w[4];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int c = (int)(h ? raw[q].y : raw[q].x);
+                const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(c, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(c, true);
+                w[2 * h] = pack2(lo[0] * scale, lo[1] * scale);
+                w[2 * h + 1] = pack2(hi[0] * scale, hi[1] * scale);
+            }
+            *reinterpret_cast<uint4*>(tile + to[q]) = uint4{w[0], w[1], w[2], w[3]};
+        }
+    }
+};
+
+// One wave's WM x WN sums to D (+ C), 32 rows at a time through its own part of LDS
+// (32 rows of WN floats), so that a store covers whole 128-byte pieces of rows. C's values
+// of the next 32 rows are loaded ahead of the ones in hand: their latency would otherwise
+// come once for every 8 rows.
+template <int SM, int SN>
+__device__ __forceinline__ void store_wave_tile(const RaggedGemmArgs& p, const f32x16 (&acc)[SM][SN], uint8_t* buf, int g,
+                                                int r0, int row_end, int c0, int lane, bool vec) {
+    constexpr int WN = SN * 32;
+    constexpr int LPR = WN / 8;          // lanes per row, 8 columns each
+    constexpr int RPT = 64 / LPR, T = 32 / RPT;   // rows of one access, accesses of 32 rows
+    constexpr int kRowBytes = WN * 4;
+    constexpr int kSwz = WN >= 64 ? 2 : 1;
+    const int lrow = lane & 31, lhalf = lane >> 5;
+    const int my_row = lane / LPR, c = c0 + lane % LPR * 8;
+    const bool whole = vec && c + 8 <= p.n;
+    const int64_t d_off = (int64_t)blockIdx.y * p.d_split + (int64_t)g * p.d_gs + c, c_off = (int64_t)g * p.c_gs + c;
+    f32x4 cv[2][T][2];   // C's values (BF16: packed in the first of each pair)
+    auto load_c = [&](int i, int b) {
+#pragma unroll
+        for (int t = 0; t < T; ++t) {
+            const int r = r0 + i * 32 + t * RPT + my_row;
+            if (r >= row_end || !whole) continue;
+            const int64_t from = c_off + (int64_t)r * p.ldc;
+            if (p.out_f32) {
+                const f32x4* at = reinterpret_cast<const f32x4*>(static_cast<const float*>(p.c) + from);
+                cv[b][t][0] = at[0], cv[b][t][1] = at[1];
+            } else {
+                cv[b][t][0] = *reinterpret_cast<const f32x4*>(static_cast<const uint16_t*>(p.c) + from);
+            }
+        }
+    };
+    if (p.c) load_c(0, 0);
+#pragma unroll
+    for (int i = 0; i < SM; ++i) {
+        if (r0 + i * 32 >= row_end) break;   // wave-uniform
+        if (p.c && i + 1 < SM) load_c(i + 1, (i + 1) & 1);
+        // 16-byte unit u (4 columns) of row r at u ^ (r & 7) * 2: 16 rows on distinct banks
+#pragma unroll
+        for (int j = 0; j < SN; ++j)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int u = j * 8 + 2 * q + lhalf;
+                const f32x4 v{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+                *reinterpret_cast<f32x4*>(buf + lrow * kRowBytes + ((u ^ ((lrow & 7) * kSwz)) & (WN / 4 - 1)) * 16) = v;
+            }
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int t = 0; t < T; ++t) {
+            const int lr = t * RPT + my_row, cu = lane % LPR, sw = (lr & 7) * kSwz;
+            const f32x4 x0 = *reinterpret_cast<const f32x4*>(buf + lr * kRowBytes + (((2 * cu) ^ sw) & (WN / 4 - 1)) * 16);
+            const f32x4 x1 = *reinterpret_cast<const f32x4*>(buf + lr * kRowBytes + (((2 * cu + 1) ^ sw) & (WN / 4 - 1)) * 16);
+            float v[8] = {x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]};
+            const int r = r0 + i * 32 + lr;
+            if (r >= row_end || c >= p.n) continue;
+            const int64_t to = d_off + (int64_t)r * p.ldd, from = c_off + (int64_t)r * p.ldc;
+            if (p.out_f32) {
+                float* d = static_cast<float*>(p.d) + to;
+                if (whole) {
+                    if (p.c) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) v[e] += cv[i & 1][t][e >> 2][e & 3];
+                    }
+                    __builtin_nontemporal_store(f32x4{v[0], v[1], v[2], v[3]}, reinterpret_cast<f32x4*>(d));
+                    __builtin_nontemporal_store(f32x4{v[4], v[5], v[6], v[7]}, reinterpret_cast<f32x4*>(d + 4));
+                } else {
+                    const float* cc = static_cast<const float*>(p.c) + from;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (c + e < p.n) d[e] = p.c ? v[e] + cc[e] : v[e];
+                }
+            } else {
+                uint16_t* d = static_cast<uint16_t*>(p.d) + to;
+                if (whole) {
+                    if (p.c) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const uint32_t w = __float_as_uint(cv[i & 1][t][0][e >> 1]);
+                            v[e] += __uint_as_float(e & 1 ? w & 0xFFFF0000u : w << 16);
+                        }
+                    }
+                    *reinterpret_cast<uint4*>(d) =
+                        uint4{pack2(v[0], v[1]), pack2(v[2], v[3]), pack2(v[4], v[5]), pack2(v[6], v[7])};
+                } else {
+                    const uint16_t* cc = static_cast<const uint16_t*>(p.c) + from;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (c + e < p.n) d[e] = bf16_bits(p.c ? v[e] + bf16_to_f32(cc[e]) : v[e]);
+                }
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+// PART 2: 128 x 128 tiles, quarters of 256 x 256 ones.
+template <int KIND, int BM, int BN, int WGM, int WGN, int PART, int EIGHT>
+__global__ void __launch_bounds__(WGM * WGN * 64, WGM * WGN == 4 ? 2 : 1)
+ragged_tile_kernel(const RaggedGemmArgs p, const RaggedLaunch l) {
+    constexpr int NW = WGM * WGN, NT = NW * 64;
+    constexpr int WM = BM / WGM, WN = BN / WGN, SM = WM / 32, SN = WN / 32;
+    constexpr int A_KMAJOR = KIND != kRaggedTN, B_KMAJOR = KIND == kRaggedNT;
+    constexpr int KS = BK / 16;
+    constexpr int A_STEP = BM * BK * 2, B_STEP = BN * BK * 2;   // bytes of a step
+    constexpr int B_AT = 3 * A_STEP;
+    static_assert(SM % 2 == 0, "A fragments alternate between two buffers");
+    static_assert(NW * 32 * WN * 4 <= 3 * A_STEP + 2 * B_STEP, "the epilogue's rows fit");
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[3 * A_STEP + 2 * B_STEP];
+
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wm = wave / WGN, wn = wave % WGN;
+
+    constexpr int LIST_BM = PART == 2 ? 2 * BM : BM, LIST_BN = PART == 2 ? 2 * BN : BN;
+    RaggedTile t{};
+    if constexpr (KIND == kRaggedTN) {
+        if (!locate_outputs<LIST_BM, LIST_BN, PART>(p, l, t)) return;
+    } else {
+        if (!locate_rows<LIST_BM, LIST_BN, PART>(p, l, t)) return;
+    }
+    const int g = t.g, m0 = t.m0, n0 = t.n0, m_end = t.m_end;
+    // this workgroup's piece of the reduced axis, in whole steps (none: it writes zeros)
+    const int piece = ((t.k_end - t.k0 + BK - 1) / BK + l.splits - 1) / l.splits * BK;
+    const int k0 = min(t.k0 + (int)blockIdx.y * piece, t.k_end);
+    const int reduced = min(piece, t.k_end - k0);
+    const uint16_t* b = static_cast<const uint16_t*>(p.b);
+
+    Operand<BM, A_KMAJOR, NW> oa;
+    Operand<BN, B_KMAJOR, NW> ob;
+    CodeOperand<EIGHT ? BN : 256, EIGHT ? NT : 512> oc;
+    if constexpr (A_KMAJOR)
+        oa.init(p.a + (int64_t)m0 * p.lda + k0, p.lda, min(BM, m_end - m0), reduced, wave, lane);
+    else
+        oa.init(p.a + (int64_t)k0 * p.lda + m0, p.lda, min(BM, p.m - m0), reduced, wave, lane);
+    if constexpr (EIGHT)
+        oc.init(p, k0, reduced, n0, tid);
+    else if constexpr (KIND == kRaggedNT)
+        ob.init(b + (int64_t)g * p.b_gs + (int64_t)n0 * p.ldb + k0, p.ldb, min(BN, p.n - n0), reduced, wave, lane);
+    else if constexpr (KIND == kRaggedNN)
+        ob.init(b + (int64_t)g * p.b_gs + (int64_t)k0 * p.ldb + n0, p.ldb, min(BN, p.n - n0), reduced, wave, lane);
+    else
+        ob.init(b + (int64_t)k0 * p.ldb + n0, p.ldb, min(BN, p.n - n0), reduced, wave, lane);
+
+    f32x16 acc[SM][SN];
+#pragma unroll
+    for (int i = 0; i < SM; ++i)
+#pragma unroll
+        for (int j = 0; j < SN; ++j)
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-    const int wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
-    for (int kk = k0; kk < k_end; kk += kBK) {
-        __syncthreads();
-        for (int i = tid; i < kBM * kBK; i += 256) {
-            const int r = KIND == kRaggedTN ? i % kBM : i / kBK, k = KIND == kRaggedTN ? i / kBM : i % kBK;
-            const bool in = m0 + r < m_end && kk + k < k_end;
-            s_a[r * kPitch + k] =
-                !in ? (uint16_t)0
-                    : KIND == kRaggedTN ? p.a[(int64_t)(kk + k) * p.lda + m0 + r] : p.a[(int64_t)(m0 + r) * p.lda + kk + k];
-        }
-        for (int i = tid; i < kBN * kBK; i += 256) {
-            const int c = KIND == kRaggedNT ? i / kBK : i % kBN, k = KIND == kRaggedNT ? i % kBK : i / kBN;
-            const bool in = n0 + c < p.n && kk + k < k_end;
-            s_b[c * kPitch + k] = !in                 ? (uint16_t)0
-                                  : KIND == kRaggedNT ? b[(int64_t)(n0 + c) * p.ldb + kk + k]
-                                                      : load_b(p, kk + k, n0 + c, b);
-        }
-        __syncthreads();
+
+    const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_address(smem));
+    Fragments<BM, A_KMAJOR, SM> fa;
+    Fragments<BN, B_KMAJOR, SN> fb;
+    fa.init(wm * WM, lane);
+    fb.init(wn * WN, lane);
+    bf16x8 op_b[SN][KS], op_a[2][KS];
+    auto read_a = [&](const uint8_t* stage, int buf, int slab) {
 #pragma unroll
-        for (int ks = 0; ks < kBK / 16; ++ks) {
-            const int off = ks * 16 + (lane >> 5) * 8;
-            bf16x8 fa[2], fb[2];
+        for (int ks = 0; ks < KS; ++ks) op_a[buf][ks] = fa.read(stage, slab, ks);
+    };
+    auto read_b = [&](const uint8_t* stage, int slab) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                fa[i] = *reinterpret_cast<const bf16x8*>(&s_a[(wm + i * 32 + (lane & 31)) * kPitch + off]);
-                fb[i] = *reinterpret_cast<const bf16x8*>(&s_b[(wn + i * 32 + (lane & 31)) * kPitch + off]);
+        for (int ks = 0; ks < KS; ++ks) op_b[slab][ks] = fb.read(stage, slab, ks);
+    };
+
+    const int steps = (reduced + BK - 1) / BK;
+    constexpr int A_LOADS = decltype(oa)::kInstr, B_LOADS = EIGHT ? 0 : decltype(ob)::kInstr;
+    oa.issue(lds0, wave);
+    if constexpr (!EIGHT) ob.issue(lds0 + B_AT, wave);
+    oa.issue(lds0 + A_STEP, wave);
+    if constexpr (!EIGHT) ob.issue(lds0 + B_AT + B_STEP, wave);
+    if constexpr (EIGHT) {
+        oc.load();
+        oc.store(smem + B_AT);
+        oc.load();
+        oc.store(smem + B_AT + B_STEP);
+        oc.load();
+    }
+    oa.issue(lds0 + 2 * A_STEP, wave);
+    __builtin_amdgcn_sched_barrier(0);
+    wait_vmcnt_barrier<2 * A_LOADS + B_LOADS>();
+    __builtin_amdgcn_sched_barrier(0);
+    read_a(smem, 0, 0);
+#pragma unroll
+    for (int j = 0; j < SN; ++j) read_b(smem + B_AT, j);
+
+    uint32_t a_cur = 0, a_next = A_STEP, a_last = 2 * A_STEP;   // A's steps kb, kb + 1, kb + 2
+    const bool computes = m0 + wm * WM < m_end;   // else a wave of rows past the group's: it loads and synchronises only
+    if (!computes) {
+        for (int kb = 0; kb < steps; ++kb) {
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            if constexpr (EIGHT) {
+                oc.store(smem + B_AT + (kb & 1) * B_STEP);
+                oc.load();
+            } else {
+                ob.issue(lds0 + B_AT + (kb & 1) * B_STEP, wave);
+            }
+            wait_vmcnt_barrier<A_LOADS + B_LOADS>();
+            oa.issue(lds0 + a_cur, wave);
+            const uint32_t freed = a_cur;
+            a_cur = a_next, a_next = a_last, a_last = freed;
+        }
+    } else
+    for (int kb = 0; kb < steps; ++kb) {
+        const uint32_t b_cur = B_AT + (kb & 1) * B_STEP, b_next = B_AT + (~kb & 1) * B_STEP;
+        // every wave holds its B fragments of this step: their place is free
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if constexpr (EIGHT) {
+            oc.store(smem + b_cur);
+            oc.load();
+        } else {
+            ob.issue(lds0 + b_cur, wave);
+        }
+#pragma unroll
+        for (int i = 0; i < SM; ++i) {
+            if (i + 1 < SM) {
+                read_a(smem + a_cur, (i + 1) & 1, i + 1);
+            } else {
+                __builtin_amdgcn_sched_barrier(0);
+                wait_vmcnt_barrier<A_LOADS + B_LOADS>();
+                __builtin_amdgcn_sched_barrier(0);
+                oa.issue(lds0 + a_cur, wave);
+                read_a(smem + a_next, 0, 0);
             }
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int j = 0; j < SN; ++j) {
 #pragma unroll
-                for (int j = 0; j < 2; ++j)
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fb[j], fa[i], acc[i][j], 0, 0, 0);
+                for (int ks = 0; ks < KS; ++ks)
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(op_b[j][ks], op_a[i & 1][ks], acc[i][j], 0, 0, 0);
+                if (i + 1 == SM) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    read_b(smem + b_next, j);
+                }
+            }
+        }
+        const uint32_t freed = a_cur;
+        a_cur = a_next, a_next = a_last, a_last = freed;
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    wait_vmcnt_barrier<0>();   // (loads of steps past the end wrote zeros to LDS)
+    __builtin_amdgcn_sched_barrier(0);
+    store_wave_tile<SM, SN>(p, acc, smem + wave * (32 * WN * 4), KIND == kRaggedTN ? g : 0, m0 + wm * WM, m_end, n0 + wn * WN,
+                            lane, l.vec != 0);
+}
+
+// D (+ C) from the pieces' sums in the workspace, added in the order of the pieces: four
+// columns a thread, 1024 of a row a workgroup. rows: of D, in all groups (TN).
+template <int KIND>
+__global__ void __launch_bounds__(256) ragged_join_kernel(const RaggedGemmArgs p, const float* ws, const int64_t ws_ld,
+                                                          const int splits, const int chunks) {
+    const int64_t row = blockIdx.x / chunks;
+    const int c = ((int)(blockIdx.x - row * chunks) * 256 + (int)threadIdx.x) * 4;
+    int64_t to, from = 0;
+    if constexpr (KIND == kRaggedTN) {
+        const int64_t g = row / p.m, m = row - g * p.m;
+        to = g * p.d_gs + m * p.ldd, from = g * p.c_gs + m * p.ldc;
+    } else {
+        // the first group whose end is past the row has it, or none
+        int lo = 0, hi = p.groups;
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (p.ends[mid] > row) hi = mid;
+            else lo = mid + 1;
+        }
+        if (lo == p.groups) return;
+        int start, end;
+        group_rows(p.ends, lo, p.rows, p.alignment, start, end);
+        if (row < start) return;
+        to = row * p.ldd;
+    }
+    if (c >= p.n) return;
+    const float* src = ws + row * ws_ld + c;   // (ws_ld: n up to a multiple of 4)
+    f32x4 v = *reinterpret_cast<const f32x4*>(src);
+    for (int s = 1; s < splits; ++s) {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(src + s * p.d_split);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] += x[e];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if (c + e >= p.n) break;
+        if (p.out_f32) {
+            if (p.c) v[e] += static_cast<const float*>(p.c)[from + c + e];
+            static_cast<float*>(p.d)[to + c + e] = v[e];
+        } else {
+            if (p.c) v[e] += bf16_to_f32(static_cast<const uint16_t*>(p.c)[from + c + e]);
+            static_cast<uint16_t*>(p.d)[to + c + e] = bf16_bits(v[e]);
         }
     }
-    // lane: row lane & 31 of D, columns 8 (e / 4) + 4 (lane >> 5) + e % 4
-    const int64_t d_off = KIND == kRaggedTN ? (int64_t)g * p.d_gs : 0, c_off = (int64_t)g * p.c_gs;
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const int r = m0 + wm + i * 32 + (lane & 31), c = n0 + wn + j * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
-                if (r >= m_end || c >= p.n) continue;
-                float v = acc[i][j][e];
-                const int64_t at = c_off + (int64_t)r * p.ldc + c;
-                if (p.c) v += p.out_f32 ? static_cast<const float*>(p.c)[at] : bf16_to_f32(static_cast<const uint16_t*>(p.c)[at]);
-                const int64_t to = d_off + (int64_t)r * p.ldd + c;
-                if (p.out_f32) static_cast<float*>(p.d)[to] = v;
-                else static_cast<uint16_t*>(p.d)[to] = bf16_bits(v);
-            }
+}
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Row blocks of `bm` rows at most: whole ones, and a partial one for each group that has rows.
+int64_t row_blocks(RaggedKind kind, const RaggedGemmArgs& a, int bm) {
+    return kind == kRaggedTN ? ceil_div(a.m, bm) : a.rows / bm + std::min<int64_t>(a.groups, a.rows);
+}
+
+template <int KIND, int BM, int BN, int WGM, int WGN, int PART, int EIGHT>
+void launch_tiles(const RaggedGemmArgs& a, int slots, int splits, hipStream_t stream) {
+    constexpr int LIST = PART == 2 ? 2 : 1;
+    const int64_t mb = row_blocks((RaggedKind)KIND, a, LIST * BM), nb = ceil_div(a.n, LIST * BN);
+    const int64_t tiles = mb * nb * (KIND == kRaggedTN ? a.groups : 1);
+    DG_CHECK(tiles < ((int64_t)1 << 28) && (KIND != kRaggedTN || ceil_div(mb * nb, 8) * 8 * a.groups < ((int64_t)1 << 30)));
+    int64_t blocks = KIND == kRaggedTN ? ceil_div(mb * nb, 8) * 8 * a.groups : tiles;
+    // (a tail has at most 58% of a round's tiles, for each XCD by itself in TN)
+    if (PART == 2) blocks = std::min<int64_t>(blocks, KIND == kRaggedTN ? std::max(slots / 8, 1) * 8 : slots) * 4;
+    const int64_t size = a.out_f32 ? 4 : 2;
+    const bool vec = reinterpret_cast<uintptr_t>(a.d) % 16 == 0 && a.ldd * size % 16 == 0 && a.d_gs * size % 16 == 0 &&
+                     (!a.c || (reinterpret_cast<uintptr_t>(a.c) % 16 == 0 && a.ldc * size % 16 == 0 && a.c_gs * size % 16 == 0));
+    const RaggedLaunch l{(int)mb, (int)nb, slots, splits, (int)vec};
+    hipLaunchKernelGGL((ragged_tile_kernel<KIND, BM, BN, WGM, WGN, PART, EIGHT>), dim3((unsigned)blocks, (unsigned)splits),
+                       dim3(WGM * WGN * 64), 0, stream, a, l);
+    DG_HIP_CHECK(hipGetLastError());
+}
+
+template <int KIND, int EIGHT>
+void launch_kind(const RaggedGemmArgs& a, const RaggedPlan& plan, float* ws, int slots, hipStream_t stream) {
+    if (plan.block == 256) {
+        launch_tiles<KIND, 256, 256, 2, 4, 1, EIGHT>(a, slots, 1, stream);
+        launch_tiles<KIND, 128, 128, 2, 2, 2, EIGHT>(a, slots, 1, stream);
+        return;
+    }
+    if (plan.splits == 1) {
+        launch_tiles<KIND, 128, 128, 2, 2, 0, EIGHT>(a, slots, 1, stream);
+        return;
+    }
+    const int64_t rows = KIND == kRaggedTN ? (int64_t)a.groups * a.m : a.rows, ld = ceil_div(a.n, 4) * 4;
+    RaggedGemmArgs part = a;
+    part.d = ws, part.ldd = ld, part.d_gs = KIND == kRaggedTN ? a.m * ld : 0, part.d_split = rows * ld;
+    part.c = nullptr, part.out_f32 = 1;
+    launch_tiles<KIND, 128, 128, 2, 2, 0, EIGHT>(part, slots, plan.splits, stream);
+    RaggedGemmArgs whole = a;
+    whole.d_split = part.d_split;
+    const int64_t chunks = ceil_div(a.n, 1024);
+    DG_CHECK(rows * chunks < ((int64_t)1 << 31));
+    hipLaunchKernelGGL(ragged_join_kernel<KIND>, dim3((unsigned)(rows * chunks)), dim3(256), 0, stream, whole,
+                       (const float*)ws, ld, plan.splits, (int)chunks);
+    DG_HIP_CHECK(hipGetLastError());
 }
 
 }  // namespace
 
-void launch_ragged_gemm(RaggedKind kind, const RaggedGemmArgs& a, hipStream_t stream) {
-    const int64_t nb = (a.n + kBN - 1) / kBN;
-    // (row blocks at most: whole ones, and one partial block for each group that has rows)
-    const int64_t mb = kind == kRaggedTN ? (int64_t)a.groups * ((a.m + kBM - 1) / kBM)
-                                         : a.rows / kBM + std::min<int64_t>(a.groups, a.rows);
-    DG_CHECK(mb * nb < ((int64_t)1 << 31));
-    const dim3 grid((unsigned)(mb * nb)), block(256);
-    switch (kind) {
-        case kRaggedNT: hipLaunchKernelGGL(ragged_gemm_kernel<kRaggedNT>, grid, block, 0, stream, a, (int)nb); break;
-        case kRaggedNN: hipLaunchKernelGGL(ragged_gemm_kernel<kRaggedNN>, grid, block, 0, stream, a, (int)nb); break;
-        case kRaggedTN: hipLaunchKernelGGL(ragged_gemm_kernel<kRaggedTN>, grid, block, 0, stream, a, (int)nb); break;
+RaggedPlan plan_ragged_gemm(RaggedKind kind, const RaggedGemmArgs& a, int slots, int block, int splits) {
+    const int64_t used = std::max<int64_t>(1, std::min<int64_t>(a.groups, a.rows));   // groups with rows, at most
+    const int64_t length = kind == kRaggedTN ? ceil_div(a.rows, used) : a.k;
+    auto tiles = [&](int b) {   // expected
+        const double mb = kind == kRaggedTN ? (double)ceil_div(a.m, b) * a.groups
+                          : a.rows <= used * b ? (double)used
+                                               : (double)a.rows / b + 0.5 * used;
+        return mb * ceil_div(a.n, b);
+    };
+    RaggedPlan plan{128, 1, 0};
+    const bool long_groups = kind == kRaggedTN || a.rows >= 256 * used;
+    if (block == 256 || (block == 0 && long_groups && tiles(256) * 128 >= slots * 75)) {
+        plan.block = 256;
+        return plan;
     }
-    DG_HIP_CHECK(hipGetLastError());
+    const double t = tiles(128), steps = (double)ceil_div(length, BK);
+    const double bytes = (double)(kind == kRaggedTN ? (int64_t)a.groups * a.m : a.rows) * a.n * 4;   // of a piece's sums
+    double best = 1e300;
+    for (int s = 1; s <= 32; ++s) {
+        if (splits > 0 ? s != splits : (s > 1 && steps < 4 * s)) continue;
+        const double rounds = std::ceil(t * s / (2 * slots)), step_us = t * s <= slots ? 0.6 : 1.05;
+        const double cost = rounds * std::ceil(steps / s) * step_us + (s > 1 ? 4.0 + 2 * bytes * s / 3e6 : 0.0);
+        if (cost < best) best = cost, plan.splits = s;
+    }
+    if (plan.splits > 1)
+        plan.workspace_bytes = (kind == kRaggedTN ? (int64_t)a.groups * a.m : a.rows) * ceil_div(a.n, 4) * 16 * plan.splits;
+    return plan;
+}
+
+void launch_ragged_gemm(RaggedKind kind, const RaggedGemmArgs& a, const RaggedPlan& plan, float* ws, int slots,
+                        hipStream_t stream) {
+    DG_CHECK(plan.splits == 1 || ws != nullptr);
+    switch (kind) {
+        case kRaggedNT: launch_kind<kRaggedNT, 0>(a, plan, ws, slots, stream); break;
+        case kRaggedNN: launch_kind<kRaggedNN, 0>(a, plan, ws, slots, stream); break;
+        case kRaggedTN:
+            if (a.b_sf) launch_kind<kRaggedTN, 1>(a, plan, ws, slots, stream);
+            else launch_kind<kRaggedTN, 0>(a, plan, ws, slots, stream);
+            break;
+    }
 }
 
 }  // namespace dgm

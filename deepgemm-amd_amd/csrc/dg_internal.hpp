@@ -327,8 +327,18 @@ struct RaggedGemmArgs {
     const int32_t* ends;       // [groups]
     int32_t rows, m, n, k, groups, alignment, out_f32;
     int64_t lda, ldb, ldd, ldc, b_gs, d_gs, c_gs, sf_sr, sf_sc;
+    int64_t d_split;           // from one piece's sums to the next's, where the reduced axis is split
 };
-void launch_ragged_gemm(RaggedKind kind, const RaggedGemmArgs& args, hipStream_t stream);
+// Tiles of 256 x 256 or 128 x 128, and the pieces the reduced axis is split into (more than
+// one: FP32 sums of each piece in a workspace, then added in their order).
+struct RaggedPlan {
+    int block, splits;
+    int64_t workspace_bytes;
+};
+// slots: CUs. block, splits: 0 = by the sizes, otherwise as given (splits: 128 x 128 tiles).
+RaggedPlan plan_ragged_gemm(RaggedKind kind, const RaggedGemmArgs& args, int slots, int block, int splits);
+void launch_ragged_gemm(RaggedKind kind, const RaggedGemmArgs& args, const RaggedPlan& plan, float* workspace, int slots,
+                        hipStream_t stream);
 
 // SwiGLU with an 8-bit checkpoint, and its backward pass (dg_swiglu_grad.hip). n: columns
 // of h; gate columns [0, n), up columns [n, 2n) of x, q and dx; scales of the gate half

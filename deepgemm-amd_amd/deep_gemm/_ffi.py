@@ -95,9 +95,10 @@ SIGNATURES = {
     'dg_m_grouped_fp8_gemm_nt_masked_swiglu': (_I, [_T, _T, _T, _T, _T, _I, _T, ctypes.c_float, _T, _T, _V]),
     'dg_k_grouped_fp8_gemm_nt_contiguous': (_I, [_T, _T, _T, _T, _T, _P(_I), _I, _T, _T, _P(_I), _I, _V]),
     'dg_k_grouped_fp8_gemm_tn_contiguous': (_I, [_T, _T, _T, _T, _T, _P(_I), _I, _T, _T, _P(_I), _I, _V]),
-    'dg_m_grouped_bf16_gemm_nt_ragged': (_I, [_T, _T, _T, _T, _I, _V]),
-    'dg_m_grouped_bf16_gemm_nn_ragged': (_I, [_T, _T, _T, _T, _I, _V]),
-    'dg_k_grouped_bf16_gemm_tn_ragged': (_I, [_T, _T, _T, _T, _T, _T, _I, _V]),
+    'dg_bf16_gemm_ragged_workspace_size': (ctypes.c_int64, [_I] + [ctypes.c_int64] * 4 + [_I]),
+    'dg_m_grouped_bf16_gemm_nt_ragged': (_I, [_T, _T, _T, _T, _I, _T, _V]),
+    'dg_m_grouped_bf16_gemm_nn_ragged': (_I, [_T, _T, _T, _T, _I, _T, _V]),
+    'dg_k_grouped_bf16_gemm_tn_ragged': (_I, [_T, _T, _T, _T, _T, _T, _I, _T, _V]),
     'dg_moe_swiglu_checkpoint': (_I, [_T, _T, _T, ctypes.c_float, _T, _T, _T, _V]),
     'dg_moe_swiglu_backward': (_I, [_T, _T, _T, _T, _T, ctypes.c_float, _T, _T, _T, _V]),
     'dg_set_num_sms': (_I, [_I]),
@@ -142,7 +143,8 @@ def _load_bind():
                     'dg_m_grouped_fp8_gemm_nt_contiguous_swiglu', 'dg_m_grouped_fp8_gemm_nt_masked_swiglu',
                     'dg_moe_combine'))
     _dgbind.init_bf16(*addresses('dg_m_grouped_bf16_gemm_nt_ragged', 'dg_m_grouped_bf16_gemm_nn_ragged',
-                                 'dg_k_grouped_bf16_gemm_tn_ragged', 'dg_moe_swiglu_checkpoint',
+                                 'dg_k_grouped_bf16_gemm_tn_ragged', 'dg_bf16_gemm_ragged_workspace_size',
+                                 'dg_moe_swiglu_checkpoint',
                                  'dg_moe_swiglu_backward'))
     return _dgbind
 

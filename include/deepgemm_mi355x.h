@@ -405,17 +405,27 @@ int dg_moe_combine(const dg_tensor* y, const dg_tensor* pos, const dg_tensor* to
  * The reference's BF16 grouped GEMMs (csrc/apis/gemm.hpp) take segments padded to the MK
  * alignment and K-group sizes on the host. */
 
+/* Workspace bytes of a call of the three products (0: none; -1 on error): calls of few
+ * tiles split the reduced axis over workgroups, the FP32 sums of its pieces go to the
+ * workspace and a second kernel adds them in a fixed order. form 0: NT, 1: NN (rows, n,
+ * k), 2: TN (rows, m, n). `workspace` below is a 1-D device tensor of that size, 16-byte
+ * aligned, used until the call's kernels finish on `stream`; NULL, or one too small: the
+ * axis stays whole. */
+int64_t dg_bf16_gemm_ragged_workspace_size(int32_t form, int64_t rows, int64_t m, int64_t n, int64_t k, int32_t groups);
+
 /* Forward: d[r] = a[r] @ b[g(r)]^T. Rows outside every group are left as they were.
  *   a  bf16 [M, K], b bf16 [G, N, K], unit stride along K, K % 8 == 0, 16-byte rows
  *   d  bf16 or fp32 [M, N], unit stride along N, any row pitch from N on
  * Row pitches of at most 2^22 elements. */
 int dg_m_grouped_bf16_gemm_nt_ragged(const dg_tensor* a, const dg_tensor* b, const dg_tensor* d,
-                                     const dg_tensor* group_ends, int32_t alignment, void* stream);
+                                     const dg_tensor* group_ends, int32_t alignment, const dg_tensor* workspace,
+                                     void* stream);
 
 /* Gradient of the input: d[r] = a[r] @ b[g(r)], b bf16 [G, K, N] with unit stride along N
  * (the forward weight as it lies: its rows are this product's K). Otherwise as the NT form. */
 int dg_m_grouped_bf16_gemm_nn_ragged(const dg_tensor* a, const dg_tensor* b, const dg_tensor* d,
-                                     const dg_tensor* group_ends, int32_t alignment, void* stream);
+                                     const dg_tensor* group_ends, int32_t alignment, const dg_tensor* workspace,
+                                     void* stream);
 
 /* Gradient of the weights: d[g] = c[g] + a_g^T @ b_g over the rows of group g.
  *   a     bf16 [R, M], unit stride along M, 16-byte rows
@@ -427,7 +437,8 @@ int dg_m_grouped_bf16_gemm_nn_ragged(const dg_tensor* a, const dg_tensor* b, con
  *   c     NULL (zeros), or d's type and shape; may be d (accumulation in place)
  * A group without rows gets c. Sums in FP32. */
 int dg_k_grouped_bf16_gemm_tn_ragged(const dg_tensor* a, const dg_tensor* b, const dg_tensor* b_sf, const dg_tensor* d,
-                                     const dg_tensor* group_ends, const dg_tensor* c, int32_t alignment, void* stream);
+                                     const dg_tensor* group_ends, const dg_tensor* c, int32_t alignment,
+                                     const dg_tensor* workspace, void* stream);
 
 /* SwiGLU x routing weight in BF16, leaving its input in 8 bits for the backward pass:
  * h = silu(gate) * up * w, gate = x[:, :I], up = x[:, I:], in FP32, rounded once.
@@ -484,7 +495,8 @@ int32_t dg_get_theoretical_mk_alignment_for_contiguous_layout(int32_t expected_m
  * 10 = the split-K kernel of dg_fp8_fp4_gemm_nt_ws (block_m 0; block_n = K
  * chunks, 0 for the heuristic's count), 11 = the UE8M0 tiny-M kernel (block_m and
  * block_n 32 or 64: rows and columns per workgroup), 12 = the K-split kernel of
- * dense calls (128 x 128);
+ * dense calls (128 x 128), 13 = the tile of the ragged BF16 products (block_m 128 or
+ * 256; block_n = pieces of the reduced axis, at 128, 0 for the heuristic's count);
  * variant 0 restores the heuristic. Only compiled tile shapes are accepted. */
 int dg_set_tile_override(int32_t variant, int32_t block_m, int32_t block_n);
 

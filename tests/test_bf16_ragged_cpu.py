@@ -23,11 +23,11 @@ def rejected(name, *args, match=''):
 
 
 def nt(m=64, n=48, k=32, g=3):
-    return dict(a=fake((m, k), BF), b=fake((g, n, k), BF), d=fake((m, n), BF), ends=fake((g,), I32), alignment=1)
+    return dict(a=fake((m, k), BF), b=fake((g, n, k), BF), d=fake((m, n), BF), ends=fake((g,), I32), alignment=1, ws=None)
 
 
 def nn(m=64, n=48, k=32, g=3):
-    return dict(a=fake((m, k), BF), b=fake((g, k, n), BF), d=fake((m, n), BF), ends=fake((g,), I32), alignment=1)
+    return dict(a=fake((m, k), BF), b=fake((g, k, n), BF), d=fake((m, n), BF), ends=fake((g,), I32), alignment=1, ws=None)
 
 
 @pytest.mark.parametrize('name,make', [('dg_m_grouped_bf16_gemm_nt_ragged', nt), ('dg_m_grouped_bf16_gemm_nn_ragged', nn)])
@@ -42,7 +42,7 @@ def nn(m=64, n=48, k=32, g=3):
     ('d', fake((64, 48), BF, strides=(1, 64))), ('d', fake((64, 48), BF, device=-1)),
     ('ends', fake((4,), I32)), ('ends', fake((3,), _ffi.DG_I64)), ('ends', fake((3,), I32, strides=(2,))),
     ('ends', fake((3,), I32, device=-1)), ('ends', fake((3, 1), I32)),
-    ('alignment', 0), ('alignment', -16), ('alignment', (1 << 20) + 1)])
+    ('alignment', 0), ('alignment', -16), ('alignment', (1 << 20) + 1), ('ws', fake((64,), F32, device=1))])
 def test_m_grouped_refusals(name, make, key, value):
     args = make()
     args[key] = value
@@ -60,7 +60,7 @@ def test_m_grouped_reduced_length_and_null(name, make):
 
 def tn(r=64, m=40, n=48, g=3, eight=False):
     return dict(a=fake((r, m), BF), b=fake((r, n), E4 if eight else BF), sf=fake((r, -(-n // 128)), F32) if eight else None,
-                d=fake((g, m, n), F32), ends=fake((g,), I32), c=None, alignment=1)
+                d=fake((g, m, n), F32), ends=fake((g,), I32), c=None, alignment=1, ws=None)
 
 
 @pytest.mark.parametrize('key,value', [

@@ -15,6 +15,16 @@ pytestmark = pytest.mark.gpu
 MIXED = [5, 0, 1, 130, 0, 64, 257, 31, 0]
 
 
+@pytest.fixture(autouse=True, params=['heuristic', '256', '128', '128 in 3 pieces'])
+def tiles(request):
+    """Every test with the tiles the sizes choose, and with each kind forced."""
+    block, pieces = {'heuristic': (0, 0), '256': (256, 0), '128': (128, 1), '128 in 3 pieces': (128, 3)}[request.param]
+    if block:
+        deep_gemm.set_tile_override(block, pieces, variant=13)
+    yield request.param
+    deep_gemm.set_tile_override(0, 0)
+
+
 def m_grouped(direction, sizes, n, k, alignment=1, out=torch.bfloat16, spare=3, seed=0, d_pitch=None):
     print(f'{direction} sizes={sizes} n={n} k={k} alignment={alignment} {out}', flush=True)
     seg = segments(sizes, alignment)
