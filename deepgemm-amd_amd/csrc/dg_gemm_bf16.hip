@@ -53,7 +53,7 @@ __device__ __forceinline__ void group_rows(const int32_t* ends, int g, int rows,
 // of a 256 x 256 round (PART 1 and 2; 0 is a launch by itself). Both launches work it
 // out alike, from the tiles that there are. 8 experts, 16384 x 4096 x 7168 (NT, 1088
 // tiles, 4.25 rounds): see launch_ragged_gemm.
-__device__ __forceinline__ int tail_tiles(int tiles, int slots) {
+__host__ __device__ __forceinline__ int tail_tiles(int tiles, int slots) {
     const int rest = tiles % slots;
     return rest * 128 <= slots * 75 ? rest : 0;
 }
@@ -144,18 +144,20 @@ __device__ __forceinline__ int group_by_length(const RaggedGemmArgs& p, int q) {
     return __ffsll((unsigned long long)__ballot(place == q && lane < p.groups)) - 1;
 }
 
+__host__ __device__ __forceinline__ bool deals_eighths(int per) { return per % 8 == 0 || per >= 64; }
+__host__ __device__ __forceinline__ int eighth_start(int x, int per) { return (int)((int64_t)x * per / 8); }
+
 // TN: every group has the same tiles. Every XCD takes an eighth of each group's, group
 // after group, so that groups of different lengths weigh on all of them alike (groups
 // of few tiles: tiles dealt out one by one).
 template <int BM, int BN, int PART>
 __device__ __forceinline__ bool locate_outputs(const RaggedGemmArgs& p, const RaggedLaunch& l, RaggedTile& t) {
     const int per = l.row_blocks * l.col_blocks;
-    const bool eighths = per % 8 == 0 || per >= 64;
     int lo = 0, mine = per, i = blockIdx.x, slots = l.slots;
-    if (eighths) {
+    if (deals_eighths(per)) {
         const int x = blockIdx.x & 7;
-        lo = (int)((int64_t)x * per / 8);
-        mine = (int)((int64_t)(x + 1) * per / 8) - lo;
+        lo = eighth_start(x, per);
+        mine = eighth_start(x + 1, per) - lo;
         i = blockIdx.x >> 3;
         slots = max(l.slots / 8, 1);
     }
@@ -246,22 +248,31 @@ struct Operand {
             vlane = col < valid ? (uint32_t)(lane / LPR * (int)pitch) + col * 2 : kPastEnd;
         }
     }
-    // The next step to lds (this operand's part of a stage).
-    __device__ __forceinline__ void issue(uint32_t lds, int wave) {
-        constexpr int PER = 512 / (KMAJOR ? BK : ROWS);   // rows of a wave load
+    // Loads of the next step: its descriptor and lane offset, then wave load i to lds (this
+    // operand's part of LDS), and on to the step after it.
+    static constexpr int kRows = 512 / (KMAJOR ? BK : ROWS);   // rows of a wave load
+    struct Step {
+        i32x4 rsrc;
+        uint32_t v;
+    };
+    __device__ __forceinline__ Step next() {
         // (without branches, which would split the loop's instruction sequence; nothing
         // left: every lane past the end, or no bytes, as a row is no longer than the pitch)
         const int n = min(max(left, 0), BK);
         const int bytes = KMAJOR ? (rows - 1) * (int)pitch + n * 2 : max((n - 1) * (int)pitch + ((rows * 2 + 3) & ~3), 0);
-        const uint32_t v = !KMAJOR || chunk < left ? vlane : kPastEnd;
-        const i32x4 rsrc = descriptor(base, bytes);
-#pragma unroll
-        for (int i = 0; i < kInstr; ++i) {
-            const int seg = i * NW + wave;
-            dma16_buffer(rsrc, v + (uint32_t)(seg * PER * (int)pitch), lds + seg * 1024);
-        }
+        const Step s{descriptor(base, bytes), !KMAJOR || chunk < left ? vlane : kPastEnd};
         base += KMAJOR ? (int64_t)BK * 2 : BK * pitch;
         left -= BK;
+        return s;
+    }
+    __device__ __forceinline__ void load(const Step& s, int i, uint32_t lds, int wave) const {
+        const int seg = i * NW + wave;
+        dma16_buffer(s.rsrc, s.v + (uint32_t)(seg * kRows * (int)pitch), lds + seg * 1024);
+    }
+    __device__ __forceinline__ void issue(uint32_t lds, int wave) {
+        const Step s = next();
+#pragma unroll
+        for (int i = 0; i < kInstr; ++i) load(s, i, lds, wave);
     }
 };
 
@@ -297,54 +308,80 @@ struct Fragments {
     }
 };
 
-// An 8-bit B of TN: 64 reduced rows of BN codes through registers (32 codes of one row, so
-// one scale, per thread), to BF16, into the MN-major layout.
-template <int BN, int NT>
+// An 8-bit B of TN: the codes of 64 reduced rows and their scales go to LDS as they are, three
+// steps ahead (each lane's 16 codes of one row, and their scale, to a place of its own, so
+// that only the lane's own loads have to be waited for), and from there as BF16 into the
+// MN-major layout. code x scale is rounded to BF16 (exact for powers of two); doing it once
+// per value on the way to LDS takes 64 vector instructions a thread and step, doing it on
+// fragments 128 (two waves hold the same fragment).
+template <int BN, int NW>
 struct CodeOperand {
-    static constexpr int TPR = BN / 32;   // threads per reduced row
-    static_assert(NT == TPR * BK, "32 codes per thread");
-    const uint8_t* base;
-    const float* sf;
-    int64_t pitch, sf_pitch;
-    int left, row;
-    int pieces;          // valid 8-code pieces of this thread (columns)
-    uint32_t to[4];      // where its 8-column pieces go
-    uint2 raw[4];
-    float scale;
+    static constexpr int kPieces = BN * BK / (16 * 64 * NW);   // 16-code pieces of each lane
+    static constexpr int kLoads = 2 * kPieces;                 // loads of a step for each wave
+    static constexpr int kCodes = BN * BK, kBytes = kCodes + NW * kPieces * 256;   // LDS of a step
+    static constexpr int LPR = BN / 16;                        // lanes per reduced row
+    static_assert(kPieces * 16 * 64 * NW == BN * BK, "whole wave loads");
 
-    __device__ __forceinline__ void init(const RaggedGemmArgs& p, int k0, int reduced, int n0, int tid) {
-        row = tid / TPR;
-        const int col = tid % TPR * 32;
-        pitch = p.ldb, sf_pitch = p.sf_sr;
-        base = static_cast<const uint8_t*>(p.b) + (int64_t)(k0 + row) * pitch + n0 + col;
-        const int valid = p.n - n0 - col;   // columns from there on
-        pieces = min(max((valid + 7) / 8, 0), 4);
-        sf = p.b_sf + (int64_t)(k0 + row) * sf_pitch + (int64_t)min((n0 + col) >> 7, (p.n - 1) >> 7) * p.sf_sc;
+    const uint8_t* base;   // the tile's first code of the step to be loaded next
+    const float* sf;       // the scales' first row of that step
+    int64_t pitch, sf_row;
+    int64_t sf_col;        // this lane's column of scales
+    int cols, left;
+    uint32_t vlane;
+    int row;               // this lane's reduced row in a wave load
+
+    __device__ __forceinline__ void init(const RaggedGemmArgs& p, int k0, int reduced, int n0, int lane) {
+        pitch = p.ldb, sf_row = p.sf_sr;
+        base = static_cast<const uint8_t*>(p.b) + (int64_t)k0 * pitch + n0;
+        cols = min(BN, p.n - n0);
         left = reduced;
-        const int a = col >> 5;
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-            to[q] = row * (BN * 2) + (q >> 1) * 128 + (((a & 3) ^ (row & 3)) << 5) + (a >> 2) * 256 + (q & 1) * 16;
+        row = lane / LPR;
+        const int col = lane % LPR * 16;
+        vlane = col < cols ? (uint32_t)(row * (int)pitch) + col : kPastEnd;
+        sf = p.b_sf + (int64_t)k0 * sf_row;
+        sf_col = (int64_t)min((n0 + col) >> 7, (p.n - 1) >> 7) * p.sf_sc;
     }
-    __device__ __forceinline__ void load() {
-        const bool in = row < left;
+    // The next step's codes and scales to lds (codes, then scales). Rows past the end: zero
+    // codes; a scale is read of the last row there is.
+    __device__ __forceinline__ void issue(uint32_t lds, int wave) {
+        if (left <= 0) {   // (uniform) nothing left: as many loads, of no bytes
+            const i32x4 none = descriptor(base, 0);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) raw[q] = in && q < pieces ? *reinterpret_cast<const uint2*>(base + q * 8) : uint2{0u, 0u};
-        scale = in ? *sf : 0.f;
-        base += BK * pitch, sf += BK * sf_pitch, left -= BK;
-    }
-    __device__ __forceinline__ void store(uint8_t* tile) const {
+            for (int i = 0; i < kLoads; ++i) dma16_buffer(none, kPastEnd, lds + (uint32_t)((i % kPieces * NW + wave) * 1024));
+        } else {
+            const int n = min(left, BK);
+            const i32x4 rsrc = descriptor(base, (n - 1) * (int)pitch + ((cols + 3) & ~3));
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            uint32_t w[4];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int c = (int)(h ? raw[q].y : raw[q].x);
-                const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(c, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(c, true);
-                w[2 * h] = pack2(lo[0] * scale, lo[1] * scale);
-                w[2 * h + 1] = pack2(hi[0] * scale, hi[1] * scale);
+            for (int i = 0; i < kPieces; ++i) {
+                const int seg = i * NW + wave;
+                dma16_buffer(rsrc, vlane + (uint32_t)(seg * (1024 / BN) * (int)pitch), lds + seg * 1024);
+                const float* at = sf + (int64_t)min(seg * (1024 / BN) + row, n - 1) * sf_row + sf_col;
+                dma4_vaddr(at, lds + kCodes + seg * 256);
             }
-            *reinterpret_cast<uint4*>(tile + to[q]) = uint4{w[0], w[1], w[2], w[3]};
+        }
+        base += BK * pitch, sf += BK * sf_row, left -= BK;
+    }
+    // The codes of the step at `from` (already there) to BF16 in `to`; valid: its rows.
+    __device__ __forceinline__ void convert(const uint8_t* from, uint8_t* to, int valid, int wave, int lane) const {
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+            const int seg = i * NW + wave, k = seg * (1024 / BN) + row;
+            const uint4 c = *reinterpret_cast<const uint4*>(from + seg * 1024 + lane * 16);
+            float scale = *reinterpret_cast<const float*>(from + kCodes + seg * 256 + lane * 4);
+            scale = k < valid ? scale : 0.f;   // (a scale of another row may be anything)
+            const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+            uint32_t o[8];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[q], false);
+                const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[q], true);
+                o[2 * q] = pack2(lo[0] * scale, lo[1] * scale);
+                o[2 * q + 1] = pack2(hi[0] * scale, hi[1] * scale);
+            }
+            const int u = lane % LPR, a = u >> 1;   // 16-column unit of the row: 2a + (u & 1)
+            uint8_t* at = to + k * (BN * 2) + (u & 1) * 128 + (((a & 3) ^ (k & 3)) << 5) + (a >> 2) * 256;
+            reinterpret_cast<uint4*>(at)[0] = uint4{o[0], o[1], o[2], o[3]};
+            reinterpret_cast<uint4*>(at)[1] = uint4{o[4], o[5], o[6], o[7]};
         }
     }
 };
@@ -447,15 +484,19 @@ __device__ __forceinline__ void store_wave_tile(const RaggedGemmArgs& p, const f
 template <int KIND, int BM, int BN, int WGM, int WGN, int PART, int EIGHT>
 __global__ void __launch_bounds__(WGM * WGN * 64, WGM * WGN == 4 ? 2 : 1)
 ragged_tile_kernel(const RaggedGemmArgs p, const RaggedLaunch l) {
-    constexpr int NW = WGM * WGN, NT = NW * 64;
+    constexpr int NW = WGM * WGN;
     constexpr int WM = BM / WGM, WN = BN / WGN, SM = WM / 32, SN = WN / 32;
     constexpr int A_KMAJOR = KIND != kRaggedTN, B_KMAJOR = KIND == kRaggedNT;
     constexpr int KS = BK / 16;
     constexpr int A_STEP = BM * BK * 2, B_STEP = BN * BK * 2;   // bytes of a step
-    constexpr int B_AT = 3 * A_STEP;
+    // LDS: A's steps, B's (8-bit: one, beside three steps of codes, which take A's third)
+    using Codes = CodeOperand<BN, NW>;
+    constexpr int A_SLOTS = EIGHT ? 2 : 3, B_SLOTS = EIGHT ? 1 : 2;
+    constexpr int B_AT = A_SLOTS * A_STEP, C_AT = B_AT + B_SLOTS * B_STEP;
+    constexpr int LDS_BYTES = C_AT + (EIGHT ? 3 * Codes::kBytes : 0);
     static_assert(SM % 2 == 0, "A fragments alternate between two buffers");
-    static_assert(NW * 32 * WN * 4 <= 3 * A_STEP + 2 * B_STEP, "the epilogue's rows fit");
-    __shared__ __attribute__((aligned(1024))) uint8_t smem[3 * A_STEP + 2 * B_STEP];
+    static_assert(NW * 32 * WN * 4 <= LDS_BYTES && LDS_BYTES <= 160 * 1024, "the epilogue's rows fit");
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[LDS_BYTES];
 
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -477,13 +518,13 @@ ragged_tile_kernel(const RaggedGemmArgs p, const RaggedLaunch l) {
 
     Operand<BM, A_KMAJOR, NW> oa;
     Operand<BN, B_KMAJOR, NW> ob;
-    CodeOperand<EIGHT ? BN : 256, EIGHT ? NT : 512> oc;
+    Codes oc;
     if constexpr (A_KMAJOR)
         oa.init(p.a + (int64_t)m0 * p.lda + k0, p.lda, min(BM, m_end - m0), reduced, wave, lane);
     else
         oa.init(p.a + (int64_t)k0 * p.lda + m0, p.lda, min(BM, p.m - m0), reduced, wave, lane);
     if constexpr (EIGHT)
-        oc.init(p, k0, reduced, n0, tid);
+        oc.init(p, k0, reduced, n0, lane);
     else if constexpr (KIND == kRaggedNT)
         ob.init(b + (int64_t)g * p.b_gs + (int64_t)n0 * p.ldb + k0, p.ldb, min(BN, p.n - n0), reduced, wave, lane);
     else if constexpr (KIND == kRaggedNN)
@@ -515,77 +556,109 @@ ragged_tile_kernel(const RaggedGemmArgs p, const RaggedLaunch l) {
     };
 
     const int steps = (reduced + BK - 1) / BK;
-    constexpr int A_LOADS = decltype(oa)::kInstr, B_LOADS = EIGHT ? 0 : decltype(ob)::kInstr;
-    oa.issue(lds0, wave);
-    if constexpr (!EIGHT) ob.issue(lds0 + B_AT, wave);
-    oa.issue(lds0 + A_STEP, wave);
-    if constexpr (!EIGHT) ob.issue(lds0 + B_AT + B_STEP, wave);
+    // Loads of a wave for a step of A and of B (codes and scales). At a hand-off those of the
+    // step after the next may be in flight: A's and B's, or the codes of four steps on.
+    constexpr int A_LOADS = decltype(oa)::kInstr, B_LOADS = EIGHT ? Codes::kLoads : decltype(ob)::kInstr;
+    constexpr int IN_FLIGHT = EIGHT ? B_LOADS : A_LOADS + B_LOADS;
     if constexpr (EIGHT) {
-        oc.load();
-        oc.store(smem + B_AT);
-        oc.load();
-        oc.store(smem + B_AT + B_STEP);
-        oc.load();
+        oc.issue(lds0 + C_AT, wave);
+        oa.issue(lds0, wave);
+        oc.issue(lds0 + C_AT + Codes::kBytes, wave);
+        oa.issue(lds0 + A_STEP, wave);
+        oc.issue(lds0 + C_AT + 2 * Codes::kBytes, wave);
+        // (waits for the first step's codes, and for A's)
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * B_LOADS + A_LOADS) : "memory");
+        oc.convert(smem + C_AT, smem + B_AT, reduced, wave, lane);
+        oc.issue(lds0 + C_AT, wave);
+        __builtin_amdgcn_sched_barrier(0);
+        wait_vmcnt_barrier<2 * B_LOADS + A_LOADS>();
+    } else {
+        oa.issue(lds0, wave);
+        ob.issue(lds0 + B_AT, wave);
+        oa.issue(lds0 + A_STEP, wave);
+        ob.issue(lds0 + B_AT + B_STEP, wave);
+        oa.issue(lds0 + 2 * A_STEP, wave);
+        __builtin_amdgcn_sched_barrier(0);
+        wait_vmcnt_barrier<2 * A_LOADS + B_LOADS>();
     }
-    oa.issue(lds0 + 2 * A_STEP, wave);
-    __builtin_amdgcn_sched_barrier(0);
-    wait_vmcnt_barrier<2 * A_LOADS + B_LOADS>();
     __builtin_amdgcn_sched_barrier(0);
     read_a(smem, 0, 0);
 #pragma unroll
     for (int j = 0; j < SN; ++j) read_b(smem + B_AT, j);
 
-    uint32_t a_cur = 0, a_next = A_STEP, a_last = 2 * A_STEP;   // A's steps kb, kb + 1, kb + 2
+    // A's steps kb, kb + 1 (and kb + 2), and the codes of steps kb + 1, kb + 2, kb + 3
+    uint32_t a_cur = 0, a_next = A_STEP, a_last = A_SLOTS > 2 ? 2 * A_STEP : 0;
+    uint32_t c_next = C_AT + Codes::kBytes, c_after = C_AT + 2 * Codes::kBytes, c_last = C_AT;
+    auto advance = [&] {
+        const uint32_t a_freed = a_cur, c_freed = c_next;
+        a_cur = a_next, a_next = A_SLOTS > 2 ? a_last : a_freed, a_last = a_freed;
+        c_next = c_after, c_after = c_last, c_last = c_freed;
+    };
+    // B's place of this step is free: the next step's codes go there as BF16, and the codes
+    // of the step three after that one to the place they leave (the lane has read its own:
+    // it has stored what they became).
+    auto next_codes = [&](int kb) {
+        oc.convert(smem + c_next, smem + B_AT, reduced - (kb + 1) * BK, wave, lane);
+        oc.issue(lds0 + c_next, wave);
+    };
     const bool computes = m0 + wm * WM < m_end;   // else a wave of rows past the group's: it loads and synchronises only
     if (!computes) {
         for (int kb = 0; kb < steps; ++kb) {
             asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-            if constexpr (EIGHT) {
-                oc.store(smem + B_AT + (kb & 1) * B_STEP);
-                oc.load();
-            } else {
-                ob.issue(lds0 + B_AT + (kb & 1) * B_STEP, wave);
-            }
-            wait_vmcnt_barrier<A_LOADS + B_LOADS>();
+            if constexpr (EIGHT) next_codes(kb);
+            else ob.issue(lds0 + B_AT + (kb & 1) * B_STEP, wave);
+            wait_vmcnt_barrier<IN_FLIGHT>();
             oa.issue(lds0 + a_cur, wave);
-            const uint32_t freed = a_cur;
-            a_cur = a_next, a_next = a_last, a_last = freed;
+            advance();
         }
     } else
     for (int kb = 0; kb < steps; ++kb) {
-        const uint32_t b_cur = B_AT + (kb & 1) * B_STEP, b_next = B_AT + (~kb & 1) * B_STEP;
-        // every wave holds its B fragments of this step: their place is free
-        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if constexpr (EIGHT) {
-            oc.store(smem + b_cur);
-            oc.load();
-        } else {
-            ob.issue(lds0 + b_cur, wave);
-        }
+        const uint32_t b_cur = B_AT + (EIGHT ? 0 : (kb & 1) * B_STEP), b_next = B_AT + (EIGHT ? 0 : (~kb & 1) * B_STEP);
+        // A slice's matrix instructions with the LDS reads and loads of the steps to come
+        // set between them one by one, in this order: a burst of loads keeps a wave from
+        // issuing matrix instructions for as long as the address unit takes them in.
+        constexpr int N = SN * KS, TOP = SM > 2 ? 1 : 0;
 #pragma unroll
         for (int i = 0; i < SM; ++i) {
-            if (i + 1 < SM) {
-                read_a(smem + a_cur, (i + 1) & 1, i + 1);
-            } else {
-                __builtin_amdgcn_sched_barrier(0);
-                wait_vmcnt_barrier<A_LOADS + B_LOADS>();
-                __builtin_amdgcn_sched_barrier(0);
-                oa.issue(lds0 + a_cur, wave);
-                read_a(smem + a_next, 0, 0);
+            const bool last = i + 1 == SM;
+            typename decltype(oa)::Step sa;
+            typename decltype(ob)::Step sb;
+            __builtin_amdgcn_sched_barrier(0);
+            if (i == TOP) {
+                // every wave holds its B fragments of this step: their place is free
+                asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                if constexpr (EIGHT) next_codes(kb);
+                else sb = ob.next();
             }
+            if (last) {
+                wait_vmcnt_barrier<IN_FLIGHT>();
+                sa = oa.next();
+            }
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int j = 0; j < SN; ++j) {
-#pragma unroll
-                for (int ks = 0; ks < KS; ++ks)
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(op_b[j][ks], op_a[i & 1][ks], acc[i][j], 0, 0, 0);
-                if (i + 1 == SM) {
-                    __builtin_amdgcn_sched_barrier(0);
-                    read_b(smem + b_next, j);
+            for (int n = 0; n < N; ++n) {
+                // (the last slice by columns of fragments, whose registers are then free)
+                const int j = last ? n / KS : n % SN, ks = last ? n % KS : n / SN;
+                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(op_b[j][ks], op_a[i & 1][ks], acc[i][j], 0, 0, 0);
+                __builtin_amdgcn_sched_barrier(0);
+                if (n < KS) {
+                    if (last) op_a[0][n] = fa.read(smem + a_next, 0, n);
+                    else op_a[(i + 1) & 1][n] = fa.read(smem + a_cur, i + 1, n);
                 }
+                if (last && n >= KS) op_b[n / KS - 1][n % KS] = fb.read(smem + b_next, n / KS - 1, n % KS);
+                if (!EIGHT && i == TOP) {
+#pragma unroll
+                    for (int q = n * B_LOADS / N; q < (n + 1) * B_LOADS / N; ++q) ob.load(sb, q, lds0 + b_cur, wave);
+                }
+                if (last) {
+#pragma unroll
+                    for (int q = n * A_LOADS / N; q < (n + 1) * A_LOADS / N; ++q) oa.load(sa, q, lds0 + a_cur, wave);
+                }
+                __builtin_amdgcn_sched_barrier(0);
             }
+            if (last) read_b(smem + b_next, SN - 1);
         }
-        const uint32_t freed = a_cur;
-        a_cur = a_next, a_next = a_last, a_last = freed;
+        advance();
     }
     __builtin_amdgcn_sched_barrier(0);
     wait_vmcnt_barrier<0>();   // (loads of steps past the end wrote zeros to LDS)
@@ -597,8 +670,8 @@ ragged_tile_kernel(const RaggedGemmArgs p, const RaggedLaunch l) {
 // D (+ C) from the pieces' sums in the workspace, added in the order of the pieces: four
 // columns a thread, 1024 of a row a workgroup. rows: of D, in all groups (TN).
 template <int KIND>
-__global__ void __launch_bounds__(256) ragged_join_kernel(const RaggedGemmArgs p, const float* ws, const int64_t ws_ld,
-                                                          const int splits, const int chunks) {
+__global__ void __launch_bounds__(256) ragged_join_kernel(const RaggedGemmArgs p, const float* __restrict__ ws,
+                                                          const int64_t ws_ld, const int splits, const int chunks) {
     const int64_t row = blockIdx.x / chunks;
     const int c = ((int)(blockIdx.x - row * chunks) * 256 + (int)threadIdx.x) * 4;
     int64_t to, from = 0;
@@ -622,10 +695,16 @@ __global__ void __launch_bounds__(256) ragged_join_kernel(const RaggedGemmArgs p
     if (c >= p.n) return;
     const float* src = ws + row * ws_ld + c;   // (ws_ld: n up to a multiple of 4)
     f32x4 v = *reinterpret_cast<const f32x4*>(src);
-    for (int s = 1; s < splits; ++s) {
-        const f32x4 x = *reinterpret_cast<const f32x4*>(src + s * p.d_split);
+    for (int s = 1; s < splits; s += 8) {   // eight loads at a time
+        f32x4 x[8];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] += x[e];
+        for (int q = 0; q < 8; ++q)
+            if (s + q < splits) x[q] = *reinterpret_cast<const f32x4*>(src + (s + q) * p.d_split);
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (s + q < splits) v[e] += x[q][e];
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -665,11 +744,26 @@ void launch_tiles(const RaggedGemmArgs& a, int slots, int splits, hipStream_t st
     DG_HIP_CHECK(hipGetLastError());
 }
 
+// Whether a TN launch of 256 x 256 tiles leaves tiles to a second one.
+bool has_tail(const RaggedGemmArgs& a, int slots) {
+    const int64_t per = ceil_div(a.m, 256) * ceil_div(a.n, 256);
+    DG_CHECK(per * a.groups < ((int64_t)1 << 28));
+    if (!deals_eighths((int)per)) return tail_tiles((int)per * a.groups, slots) > 0;
+    for (int x = 0; x < 8; ++x)
+        if (tail_tiles((eighth_start(x + 1, (int)per) - eighth_start(x, (int)per)) * a.groups, std::max(slots / 8, 1)) > 0)
+            return true;
+    return false;
+}
+
 template <int KIND, int EIGHT>
 void launch_kind(const RaggedGemmArgs& a, const RaggedPlan& plan, float* ws, int slots, hipStream_t stream) {
     if (plan.block == 256) {
-        launch_tiles<KIND, 256, 256, 2, 4, 1, EIGHT>(a, slots, 1, stream);
-        launch_tiles<KIND, 128, 128, 2, 2, 2, EIGHT>(a, slots, 1, stream);
+        if (KIND == kRaggedTN && !has_tail(a, slots)) {   // (known here: its tiles do not depend on group_ends)
+            launch_tiles<KIND, 256, 256, 2, 4, 0, EIGHT>(a, slots, 1, stream);
+        } else {
+            launch_tiles<KIND, 256, 256, 2, 4, 1, EIGHT>(a, slots, 1, stream);
+            launch_tiles<KIND, 128, 128, 2, 2, 2, EIGHT>(a, slots, 1, stream);
+        }
         return;
     }
     if (plan.splits == 1) {
@@ -692,6 +786,16 @@ void launch_kind(const RaggedGemmArgs& a, const RaggedPlan& plan, float* ws, int
 
 }  // namespace
 
+// The tile, and the pieces of the reduced axis. 256 x 256 tiles for groups of 256 rows and
+// more (TN: 1792 reduced rows and more) that fill 150 CUs. Measured in us, 256 x 256
+// against 128 x 128: NT, 4096 columns, K = 2048, 8 groups of 256 rows 38.1 and 35.5, of 512
+// 61.9 and 67.2, 32 of 512 252 and 311; TN, 8 groups to 4096 x 4096, of 1024 rows 368 and
+// 329 (two small workgroups on a CU store one's sums under the other's products), of 1536
+// 459 and 452, of 2048 551 and 567.
+// Pieces: the fewest microseconds by the time of a step (0.42 with a workgroup on a CU,
+// 1.02 with two) and of the sums' way through the workspace. Measured in us, whole and in 4, 8 and 16 pieces: NT of 8 x 4096 x 7168
+// 47.6, 18.8, 15.9, 17.4; 256 x 2112 x 7168 50.9, 22.5, 24.2, 31.0; 512 x 4096 x 2048
+// 19.5, 28.4, 41.9, 66.3; TN of 20000 rows to 104 x 504 124, 39.2, 24.8, 19.5.
 RaggedPlan plan_ragged_gemm(RaggedKind kind, const RaggedGemmArgs& a, int slots, int block, int splits) {
     const int64_t used = std::max<int64_t>(1, std::min<int64_t>(a.groups, a.rows));   // groups with rows, at most
     const int64_t length = kind == kRaggedTN ? ceil_div(a.rows, used) : a.k;
@@ -702,22 +806,22 @@ RaggedPlan plan_ragged_gemm(RaggedKind kind, const RaggedGemmArgs& a, int slots,
         return mb * ceil_div(a.n, b);
     };
     RaggedPlan plan{128, 1, 0};
-    const bool long_groups = kind == kRaggedTN || a.rows >= 256 * used;
-    if (block == 256 || (block == 0 && long_groups && tiles(256) * 128 >= slots * 75)) {
+    const bool large = kind == kRaggedTN ? length >= 1792 : a.rows >= 256 * used;
+    if (block == 256 || (block == 0 && large && tiles(256) * 128 >= slots * 75)) {
         plan.block = 256;
         return plan;
     }
-    const double t = tiles(128), steps = (double)ceil_div(length, BK);
-    const double bytes = (double)(kind == kRaggedTN ? (int64_t)a.groups * a.m : a.rows) * a.n * 4;   // of a piece's sums
+    const int64_t out_rows = kind == kRaggedTN ? (int64_t)a.groups * a.m : a.rows;
+    const double t = tiles(128), steps = (double)ceil_div(length, BK), sums = (double)out_rows * a.n * 4;
     double best = 1e300;
     for (int s = 1; s <= 32; ++s) {
         if (splits > 0 ? s != splits : (s > 1 && steps < 4 * s)) continue;
-        const double rounds = std::ceil(t * s / (2 * slots)), step_us = t * s <= slots ? 0.6 : 1.05;
-        const double cost = rounds * std::ceil(steps / s) * step_us + (s > 1 ? 4.0 + 2 * bytes * s / 3e6 : 0.0);
-        if (cost < best) best = cost, plan.splits = s;
+        const double per_cu = t * s / slots, rounds = std::ceil(per_cu / 2);
+        const double step_us = 0.42 + 0.6 * std::min(1.0, std::max(0.0, per_cu - 1));
+        const double us = rounds * std::ceil(steps / s) * step_us + (s > 1 ? 3.0 + 2 * sums * s / 3e6 : 0.0);
+        if (us < best) best = us, plan.splits = s;
     }
-    if (plan.splits > 1)
-        plan.workspace_bytes = (kind == kRaggedTN ? (int64_t)a.groups * a.m : a.rows) * ceil_div(a.n, 4) * 16 * plan.splits;
+    if (plan.splits > 1) plan.workspace_bytes = out_rows * ceil_div(a.n, 4) * 16 * plan.splits;
     return plan;
 }
 
