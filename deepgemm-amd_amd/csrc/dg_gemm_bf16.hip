@@ -386,35 +386,33 @@ struct CodeOperand {
     }
 };
 
-// One wave's WM x WN sums to D (+ C), 32 rows at a time through its own part of LDS
-// (32 rows of WN floats), so that a store covers whole 128-byte pieces of rows. C's values
-// of the next 32 rows are loaded ahead of the ones in hand: their latency would otherwise
-// come once for every 8 rows.
-template <int SM, int SN>
+// One wave's sums to D (+ C), 32 rows at a time through its own part of LDS (32 rows of WN
+// floats), so that every lane has 16 bytes of D (4 FP32 or 8 BF16 columns) beside those of
+// the next lane. C's values of the next 32 rows are loaded ahead of the ones in hand: their
+// latency would otherwise come with every access. (Streaming stores lose: without C, 32
+// groups of 47 rows to 2048 x 2048 222 against 141 us.)
+template <int F32, int SM, int SN>
 __device__ __forceinline__ void store_wave_tile(const RaggedGemmArgs& p, const f32x16 (&acc)[SM][SN], uint8_t* buf, int g,
                                                 int r0, int row_end, int c0, int lane, bool vec) {
-    constexpr int WN = SN * 32;
-    constexpr int LPR = WN / 8;          // lanes per row, 8 columns each
-    constexpr int RPT = 64 / LPR, T = 32 / RPT;   // rows of one access, accesses of 32 rows
+    constexpr int WN = SN * 32, CPL = F32 ? 4 : 8;     // columns of a lane
+    constexpr int LPR = WN / CPL, RPT = 64 / LPR, T = 32 / RPT;   // lanes of a row, rows of an access, accesses of 32 rows
     constexpr int kRowBytes = WN * 4;
     constexpr int kSwz = WN >= 64 ? 2 : 1;
     const int lrow = lane & 31, lhalf = lane >> 5;
-    const int my_row = lane / LPR, c = c0 + lane % LPR * 8;
-    const bool whole = vec && c + 8 <= p.n;
+    const int my_row = lane / LPR, c = c0 + lane % LPR * CPL;
+    const bool whole = vec && c + CPL <= p.n;
     const int64_t d_off = (int64_t)blockIdx.y * p.d_split + (int64_t)g * p.d_gs + c, c_off = (int64_t)g * p.c_gs + c;
-    f32x4 cv[2][T][2];   // C's values (BF16: packed in the first of each pair)
+    auto element = [](const void* base, int64_t at) {
+        return F32 ? static_cast<const float*>(base)[at] : bf16_to_f32(static_cast<const uint16_t*>(base)[at]);
+    };
+    constexpr int kSize = F32 ? 4 : 2;
+    uint4 cv[2][T];
     auto load_c = [&](int i, int b) {
 #pragma unroll
         for (int t = 0; t < T; ++t) {
             const int r = r0 + i * 32 + t * RPT + my_row;
-            if (r >= row_end || !whole) continue;
-            const int64_t from = c_off + (int64_t)r * p.ldc;
-            if (p.out_f32) {
-                const f32x4* at = reinterpret_cast<const f32x4*>(static_cast<const float*>(p.c) + from);
-                cv[b][t][0] = at[0], cv[b][t][1] = at[1];
-            } else {
-                cv[b][t][0] = *reinterpret_cast<const f32x4*>(static_cast<const uint16_t*>(p.c) + from);
-            }
+            if (r < row_end && whole)
+                cv[b][t] = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.c) + (c_off + (int64_t)r * p.ldc) * kSize);
         }
     };
     if (p.c) load_c(0, 0);
@@ -434,45 +432,39 @@ __device__ __forceinline__ void store_wave_tile(const RaggedGemmArgs& p, const f
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
         for (int t = 0; t < T; ++t) {
-            const int lr = t * RPT + my_row, cu = lane % LPR, sw = (lr & 7) * kSwz;
-            const f32x4 x0 = *reinterpret_cast<const f32x4*>(buf + lr * kRowBytes + (((2 * cu) ^ sw) & (WN / 4 - 1)) * 16);
-            const f32x4 x1 = *reinterpret_cast<const f32x4*>(buf + lr * kRowBytes + (((2 * cu + 1) ^ sw) & (WN / 4 - 1)) * 16);
-            float v[8] = {x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]};
+            const int lr = t * RPT + my_row, sw = (lr & 7) * kSwz;
+            float v[CPL];
+#pragma unroll
+            for (int h = 0; h < CPL / 4; ++h) {
+                const int u = lane % LPR * (CPL / 4) + h;
+                const f32x4 x = *reinterpret_cast<const f32x4*>(buf + lr * kRowBytes + ((u ^ sw) & (WN / 4 - 1)) * 16);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[4 * h + e] = x[e];
+            }
             const int r = r0 + i * 32 + lr;
             if (r >= row_end || c >= p.n) continue;
             const int64_t to = d_off + (int64_t)r * p.ldd, from = c_off + (int64_t)r * p.ldc;
-            if (p.out_f32) {
-                float* d = static_cast<float*>(p.d) + to;
-                if (whole) {
-                    if (p.c) {
+            if (whole) {
+                const uint32_t w[4] = {cv[i & 1][t].x, cv[i & 1][t].y, cv[i & 1][t].z, cv[i & 1][t].w};
+                if (p.c) {
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) v[e] += cv[i & 1][t][e >> 2][e & 3];
-                    }
-                    __builtin_nontemporal_store(f32x4{v[0], v[1], v[2], v[3]}, reinterpret_cast<f32x4*>(d));
-                    __builtin_nontemporal_store(f32x4{v[4], v[5], v[6], v[7]}, reinterpret_cast<f32x4*>(d + 4));
-                } else {
-                    const float* cc = static_cast<const float*>(p.c) + from;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if (c + e < p.n) d[e] = p.c ? v[e] + cc[e] : v[e];
+                    for (int e = 0; e < CPL; ++e)
+                        v[e] += F32 ? __uint_as_float(w[e & 3])
+                                    : __uint_as_float(e & 1 ? w[e >> 1] & 0xFFFF0000u : w[e >> 1] << 16);
                 }
+                uint4 o;
+                if constexpr (F32)
+                    o = uint4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
+                else
+                    o = uint4{pack2(v[0], v[1]), pack2(v[2], v[3]), pack2(v[CPL - 4], v[CPL - 3]), pack2(v[CPL - 2], v[CPL - 1])};
+                *reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.d) + to * kSize) = o;
             } else {
-                uint16_t* d = static_cast<uint16_t*>(p.d) + to;
-                if (whole) {
-                    if (p.c) {
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            const uint32_t w = __float_as_uint(cv[i & 1][t][0][e >> 1]);
-                            v[e] += __uint_as_float(e & 1 ? w & 0xFFFF0000u : w << 16);
-                        }
-                    }
-                    *reinterpret_cast<uint4*>(d) =
-                        uint4{pack2(v[0], v[1]), pack2(v[2], v[3]), pack2(v[4], v[5]), pack2(v[6], v[7])};
-                } else {
-                    const uint16_t* cc = static_cast<const uint16_t*>(p.c) + from;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if (c + e < p.n) d[e] = bf16_bits(p.c ? v[e] + bf16_to_f32(cc[e]) : v[e]);
+                for (int e = 0; e < CPL; ++e) {
+                    if (c + e >= p.n) break;
+                    const float x = p.c ? v[e] + element(p.c, from + e) : v[e];
+                    if constexpr (F32) static_cast<float*>(p.d)[to + e] = x;
+                    else static_cast<uint16_t*>(p.d)[to + e] = bf16_bits(x);
                 }
             }
         }
@@ -663,8 +655,10 @@ ragged_tile_kernel(const RaggedGemmArgs p, const RaggedLaunch l) {
     __builtin_amdgcn_sched_barrier(0);
     wait_vmcnt_barrier<0>();   // (loads of steps past the end wrote zeros to LDS)
     __builtin_amdgcn_sched_barrier(0);
-    store_wave_tile<SM, SN>(p, acc, smem + wave * (32 * WN * 4), KIND == kRaggedTN ? g : 0, m0 + wm * WM, m_end, n0 + wn * WN,
-                            lane, l.vec != 0);
+    uint8_t* buf = smem + wave * (32 * WN * 4);
+    const int g_out = KIND == kRaggedTN ? g : 0;
+    if (p.out_f32) store_wave_tile<1, SM, SN>(p, acc, buf, g_out, m0 + wm * WM, m_end, n0 + wn * WN, lane, l.vec != 0);
+    else store_wave_tile<0, SM, SN>(p, acc, buf, g_out, m0 + wm * WM, m_end, n0 + wn * WN, lane, l.vec != 0);
 }
 
 // D (+ C) from the pieces' sums in the workspace, added in the order of the pieces: four
@@ -786,12 +780,13 @@ void launch_kind(const RaggedGemmArgs& a, const RaggedPlan& plan, float* ws, int
 
 }  // namespace
 
-// The tile, and the pieces of the reduced axis. 256 x 256 tiles for groups of 256 rows and
-// more (TN: 1792 reduced rows and more) that fill 150 CUs. Measured in us, 256 x 256
-// against 128 x 128: NT, 4096 columns, K = 2048, 8 groups of 256 rows 38.1 and 35.5, of 512
-// 61.9 and 67.2, 32 of 512 252 and 311; TN, 8 groups to 4096 x 4096, of 1024 rows 368 and
-// 329 (two small workgroups on a CU store one's sums under the other's products), of 1536
-// 459 and 452, of 2048 551 and 567.
+// The tile, and the pieces of the reduced axis. 256 x 256 tiles that fill 150 CUs, for NT
+// and NN with groups of 256 rows and more, for TN with C of 512 and more. Measured in us,
+// 256 x 256 against 128 x 128: NT, 4096 columns, K = 2048, 8 groups of 256 rows 38.1 and 35.5, of
+// 512 61.9 and 67.2, 32 of 512 252 and 311; TN without C, 32 groups of 47 rows to 2048 x
+// 2048 128 and 145, 8 of 1024 to 4096 x 4096 312 and 401; with C, the same 273 and 215, 8
+// of 512 to 4096 x 2048 178 and 180, 8 of 1024 to 4096 x 4096 444 and 450 (two small
+// workgroups on a CU read C for one under the other's products).
 // Pieces: the fewest microseconds by the time of a step (0.42 with a workgroup on a CU,
 // 1.02 with two) and of the sums' way through the workspace. Measured in us, whole and in 4, 8 and 16 pieces: NT of 8 x 4096 x 7168
 // 47.6, 18.8, 15.9, 17.4; 256 x 2112 x 7168 50.9, 22.5, 24.2, 31.0; 512 x 4096 x 2048
@@ -806,7 +801,7 @@ RaggedPlan plan_ragged_gemm(RaggedKind kind, const RaggedGemmArgs& a, int slots,
         return mb * ceil_div(a.n, b);
     };
     RaggedPlan plan{128, 1, 0};
-    const bool large = kind == kRaggedTN ? length >= 1792 : a.rows >= 256 * used;
+    const bool large = kind == kRaggedTN ? !a.c || length >= 512 : a.rows >= 256 * used;
     if (block == 256 || (block == 0 && large && tiles(256) * 128 >= slots * 75)) {
         plan.block = 256;
         return plan;
