@@ -318,7 +318,7 @@ PyObject* k_grouped_ragged(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const int32_t alignment = (int32_t)integer(a[6]);
         void* stream = pointer<void>(a[7]);
         const bool fits = ta.d.ndim == 2 && tb.d.ndim == 2 && d.d.ndim == 3;
-        const Workspace ws(2, tensor(a[3]), ta.d.sizes[0], ta.d.sizes[1], fits ? tb.d.sizes[1] : 0, 0, d.d.sizes[0]);
+        const Workspace ws(sf.given ? 3 : 2, tensor(a[3]), ta.d.sizes[0], ta.d.sizes[1], fits ? tb.d.sizes[1] : 0, 0, d.d.sizes[0]);
         return call(g_entry.ragged_tn, ta.get(), tb.get(), sf.get(), d.get(), ends.get(), c.get(), alignment, ws.arg.get(),
                     stream);
     });

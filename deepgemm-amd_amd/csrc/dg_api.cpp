@@ -1992,12 +1992,14 @@ int dg_moe_combine(const dg_tensor* y, const dg_tensor* pos, const dg_tensor* to
 int64_t dg_bf16_gemm_ragged_workspace_size(int32_t form, int64_t rows, int64_t m, int64_t n, int64_t k, int32_t groups) {
     int64_t bytes = -1;
     guarded([&] {
-        DG_CHECK(form >= 0 && form <= 2);
+        DG_CHECK(form >= 0 && form <= 3);
         for (int64_t v : {rows, m, n, k, (int64_t)groups}) DG_CHECK(v >= 0 && v < ((int64_t)1 << 30));
         RaggedGemmArgs a{};
         a.rows = (int32_t)rows, a.m = (int32_t)m, a.n = (int32_t)n, a.k = (int32_t)k, a.groups = groups;
-        const bool nothing = n == 0 || groups == 0 || (form == 2 ? m == 0 : rows == 0);
-        bytes = nothing ? 0 : ragged_plan((RaggedKind)form, a).workspace_bytes;
+        static const float scales = 1.f;
+        if (form == 3) a.b_sf = &scales;   // (never read: an 8-bit B to the plan)
+        const bool nothing = n == 0 || groups == 0 || (form >= 2 ? m == 0 : rows == 0);
+        bytes = nothing ? 0 : ragged_plan((RaggedKind)std::min(form, 2), a).workspace_bytes;
     });
     return bytes;
 }

@@ -14,6 +14,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "dg_internal.hpp"
 #include "dg_kernel_common.hpp"
@@ -128,10 +129,11 @@ __device__ __forceinline__ bool locate_rows(const RaggedGemmArgs& p, const Ragge
     return false;
 }
 
-// Group at place q of the groups from the longest to the shortest (up to 64 groups; in
-// their own order otherwise), so that the last tiles of a launch are the short ones.
+// Group at place q of the groups from the longest to the shortest, so that the last tiles of
+// a launch are the short ones; more than 16 groups in their own order (one of them weighs
+// little, and the ranking takes a workgroup 20 instructions a group).
 __device__ __forceinline__ int group_by_length(const RaggedGemmArgs& p, int q) {
-    if (p.groups > 64) return q;
+    if (p.groups > 16) return q;
     const int lane = threadIdx.x & 63;
     int start = 0, end = -1;
     if (lane < p.groups) group_rows(p.ends, lane, p.rows, p.alignment, start, end);
@@ -386,89 +388,125 @@ struct CodeOperand {
     }
 };
 
-// One wave's sums to D (+ C), 32 rows at a time through its own part of LDS (32 rows of WN
-// floats), so that every lane has 16 bytes of D (4 FP32 or 8 BF16 columns) beside those of
-// the next lane. C's values of the next 32 rows are loaded ahead of the ones in hand: their
-// latency would otherwise come with every access. (Streaming stores lose: without C, 32
-// groups of 47 rows to 2048 x 2048 222 against 141 us.)
-template <int F32, int SM, int SN>
-__device__ __forceinline__ void store_wave_tile(const RaggedGemmArgs& p, const f32x16 (&acc)[SM][SN], uint8_t* buf, int g,
-                                                int r0, int row_end, int c0, int lane, bool vec) {
-    constexpr int WN = SN * 32, CPL = F32 ? 4 : 8;     // columns of a lane
-    constexpr int LPR = WN / CPL, RPT = 64 / LPR, T = 32 / RPT;   // lanes of a row, rows of an access, accesses of 32 rows
-    constexpr int kRowBytes = WN * 4;
-    constexpr int kSwz = WN >= 64 ? 2 : 1;
-    const int lrow = lane & 31, lhalf = lane >> 5;
-    const int my_row = lane / LPR, c = c0 + lane % LPR * CPL;
-    const bool whole = vec && c + CPL <= p.n;
-    const int64_t d_off = (int64_t)blockIdx.y * p.d_split + (int64_t)g * p.d_gs + c, c_off = (int64_t)g * p.c_gs + c;
-    auto element = [](const void* base, int64_t at) {
-        return F32 ? static_cast<const float*>(base)[at] : bf16_to_f32(static_cast<const uint16_t*>(base)[at]);
-    };
-    constexpr int kSize = F32 ? 4 : 2;
-    uint4 cv[2][T];
-    auto load_c = [&](int i, int b) {
+// The tile's sums to D (+ C) through LDS, so that each access of a wave covers whole rows of
+// the tile (256 to 1024 bytes in one piece; every lane 16 of them). OUT: 0 BF16 without C
+// (staged as BF16), 1 FP32, 2 BF16 with C (staged as FP32: the sum is rounded once).
+// Staged as FP32, 256 rows take two passes of 128 (64 of each wave row). C's values of a
+// pass are loaded before its sums are in LDS: their latency would otherwise come with
+// every access.
+template <int OUT, int BM, int BN, int WGM, int WGN, int SM, int SN>
+__device__ __forceinline__ void store_tile(const RaggedGemmArgs& p, const f32x16 (&acc)[SM][SN], uint8_t* lds, int g, int m0,
+                                           int m_end, int n0, int wave, int lane, bool vec) {
+    constexpr int NW = WGM * WGN, SIZE = OUT == 1 ? 4 : 2, CPL = 16 / SIZE;   // columns of a lane
+    constexpr int PASSES = OUT && BM == 256 ? 2 : 1, PS = SM / PASSES;        // slabs of a pass
+    constexpr int STAGED = OUT ? 4 : 2, ROW_BYTES = BN * STAGED;
+    constexpr int LPR = BN / CPL, RPT = 64 / LPR, T = BM / PASSES / (NW * RPT);   // lanes of a row, rows of an access
+    static_assert(T * NW * RPT * PASSES == BM, "whole accesses");
+    const int lrow = lane & 31, lhalf = lane >> 5, wm = wave / WGN, wn = wave % WGN;
+    const int c = n0 + lane % LPR * CPL;
+    const bool whole = vec && c + CPL <= p.n, add = OUT && p.c;
+    const int64_t d_tile = (int64_t)blockIdx.y * p.d_split + (int64_t)g * p.d_gs + n0, c_tile = (int64_t)g * p.c_gs + n0;
+    const int64_t d_off = d_tile + (c - n0), c_off = c_tile + (c - n0);
 #pragma unroll
-        for (int t = 0; t < T; ++t) {
-            const int r = r0 + i * 32 + t * RPT + my_row;
-            if (r < row_end && whole)
-                cv[b][t] = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.c) + (c_off + (int64_t)r * p.ldc) * kSize);
+    for (int pass = 0; pass < PASSES; ++pass) {
+        // row of D of the pass's row r (which has PS slabs of each wave row)
+        auto row_of = [&](int r) { return m0 + (r / (PS * 32)) * (SM * 32) + pass * (PS * 32) + r % (PS * 32); };
+        uint4 cv[T];
+        if (add) {
+#pragma unroll
+            for (int t = 0; t < T; ++t) {
+                const int r = row_of((t * NW + wave) * RPT + lane / LPR);
+                if (r < m_end && whole)
+                    cv[t] = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.c) + (c_off + (int64_t)r * p.ldc) * SIZE);
+            }
         }
-    };
-    if (p.c) load_c(0, 0);
+        if (pass > 0) __syncthreads();
+        // 16-byte unit u of row r at u ^ (r & 7): 8 rows on distinct banks
 #pragma unroll
-    for (int i = 0; i < SM; ++i) {
-        if (r0 + i * 32 >= row_end) break;   // wave-uniform
-        if (p.c && i + 1 < SM) load_c(i + 1, (i + 1) & 1);
-        // 16-byte unit u (4 columns) of row r at u ^ (r & 7) * 2: 16 rows on distinct banks
+        for (int i = 0; i < PS; ++i)
 #pragma unroll
-        for (int j = 0; j < SN; ++j)
+            for (int j = 0; j < SN; ++j)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int u = j * 8 + 2 * q + lhalf;
-                const f32x4 v{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
-                *reinterpret_cast<f32x4*>(buf + lrow * kRowBytes + ((u ^ ((lrow & 7) * kSwz)) & (WN / 4 - 1)) * 16) = v;
+                for (int q = 0; q < 4; ++q) {
+                    const f32x16& v = acc[pass * PS + i][j];
+                    const int r = wm * (PS * 32) + i * 32 + lrow, col = wn * (SN * 32) + j * 32 + 8 * q + 4 * lhalf;
+                    uint8_t* at = lds + r * ROW_BYTES + ((col * STAGED >> 4 ^ (r & 7)) << 4) + (OUT ? 0 : lhalf * 8);
+                    if constexpr (OUT)
+                        *reinterpret_cast<f32x4*>(at) = f32x4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
+                    else
+                        *reinterpret_cast<uint2*>(at) = uint2{pack2(v[4 * q], v[4 * q + 1]), pack2(v[4 * q + 2], v[4 * q + 3])};
+                }
+        __syncthreads();
+        if (!vec) {   // rows that begin anywhere: 64 elements of a row an access, one a lane
+            for (int t = 0; t < T * RPT; ++t) {
+                const int lr = t * NW + wave, r = row_of(lr);
+                if (r >= m_end) continue;
+#pragma unroll
+                for (int q = 0; q < BN / 64; ++q) {
+                    const int col = q * 64 + lane, at = col * STAGED;
+                    if (n0 + col >= p.n) continue;
+                    const uint8_t* src = lds + lr * ROW_BYTES + (((at >> 4) ^ (lr & 7)) << 4) + (at & 15);
+                    const int64_t to = d_tile + (int64_t)r * p.ldd + col, from = c_tile + (int64_t)r * p.ldc + col;
+                    if constexpr (OUT == 0) {
+                        static_cast<uint16_t*>(p.d)[to] = *reinterpret_cast<const uint16_t*>(src);
+                    } else {
+                        float v = *reinterpret_cast<const float*>(src);
+                        if constexpr (OUT == 1) {
+                            if (add) v += static_cast<const float*>(p.c)[from];
+                            static_cast<float*>(p.d)[to] = v;
+                        } else {
+                            v += bf16_to_f32(static_cast<const uint16_t*>(p.c)[from]);
+                            static_cast<uint16_t*>(p.d)[to] = bf16_bits(v);
+                        }
+                    }
+                }
             }
-        __builtin_amdgcn_wave_barrier();
+            continue;
+        }
 #pragma unroll
         for (int t = 0; t < T; ++t) {
-            const int lr = t * RPT + my_row, sw = (lr & 7) * kSwz;
-            float v[CPL];
+            const int lr = (t * NW + wave) * RPT + lane / LPR, r = row_of(lr);
+            auto unit = [&](int u) { return *reinterpret_cast<const uint4*>(lds + lr * ROW_BYTES + ((u ^ (lr & 7)) << 4)); };
+            const uint4 x = unit(lane % LPR * (OUT == 2 ? 2 : 1));
+            uint32_t w[4] = {x.x, x.y, x.z, x.w};   // D's 16 bytes
+            float f[OUT ? CPL : 1];
+            if constexpr (OUT) {
 #pragma unroll
-            for (int h = 0; h < CPL / 4; ++h) {
-                const int u = lane % LPR * (CPL / 4) + h;
-                const f32x4 x = *reinterpret_cast<const f32x4*>(buf + lr * kRowBytes + ((u ^ sw) & (WN / 4 - 1)) * 16);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[4 * h + e] = x[e];
+                for (int e = 0; e < 4; ++e) f[e] = __uint_as_float(w[e]);
+                if constexpr (OUT == 2) {
+                    const uint4 y = unit(lane % LPR * 2 + 1);
+                    f[4] = __uint_as_float(y.x), f[5] = __uint_as_float(y.y), f[6] = __uint_as_float(y.z), f[7] = __uint_as_float(y.w);
+                }
             }
-            const int r = r0 + i * 32 + lr;
-            if (r >= row_end || c >= p.n) continue;
+            if (r >= m_end || c >= p.n) continue;
             const int64_t to = d_off + (int64_t)r * p.ldd, from = c_off + (int64_t)r * p.ldc;
             if (whole) {
-                const uint32_t w[4] = {cv[i & 1][t].x, cv[i & 1][t].y, cv[i & 1][t].z, cv[i & 1][t].w};
-                if (p.c) {
+                if constexpr (OUT) {
+                    if (add) {
+                        const uint32_t y[4] = {cv[t].x, cv[t].y, cv[t].z, cv[t].w};
 #pragma unroll
-                    for (int e = 0; e < CPL; ++e)
-                        v[e] += F32 ? __uint_as_float(w[e & 3])
-                                    : __uint_as_float(e & 1 ? w[e >> 1] & 0xFFFF0000u : w[e >> 1] << 16);
+                        for (int e = 0; e < CPL; ++e)
+                            f[e] += OUT == 1 ? __uint_as_float(y[e & 3])
+                                             : __uint_as_float(e & 1 ? y[e >> 1] & 0xFFFF0000u : y[e >> 1] << 16);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) w[e] = OUT == 1 ? __float_as_uint(f[e]) : pack2(f[(2 * e) % CPL], f[(2 * e + 1) % CPL]);
                 }
-                uint4 o;
-                if constexpr (F32)
-                    o = uint4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
-                else
-                    o = uint4{pack2(v[0], v[1]), pack2(v[2], v[3]), pack2(v[CPL - 4], v[CPL - 3]), pack2(v[CPL - 2], v[CPL - 1])};
-                *reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.d) + to * kSize) = o;
+                *reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.d) + to * SIZE) = uint4{w[0], w[1], w[2], w[3]};
             } else {
 #pragma unroll
                 for (int e = 0; e < CPL; ++e) {
                     if (c + e >= p.n) break;
-                    const float x = p.c ? v[e] + element(p.c, from + e) : v[e];
-                    if constexpr (F32) static_cast<float*>(p.d)[to + e] = x;
-                    else static_cast<uint16_t*>(p.d)[to + e] = bf16_bits(x);
+                    if constexpr (OUT == 1)
+                        static_cast<float*>(p.d)[to + e] = add ? f[e] + static_cast<const float*>(p.c)[from + e] : f[e];
+                    else if constexpr (OUT == 2)
+                        static_cast<uint16_t*>(p.d)[to + e] =
+                            bf16_bits(f[e] + bf16_to_f32(static_cast<const uint16_t*>(p.c)[from + e]));
+                    else
+                        static_cast<uint16_t*>(p.d)[to + e] = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
                 }
             }
         }
-        __builtin_amdgcn_wave_barrier();
     }
 }
 
@@ -487,7 +525,7 @@ ragged_tile_kernel(const RaggedGemmArgs p, const RaggedLaunch l) {
     constexpr int B_AT = A_SLOTS * A_STEP, C_AT = B_AT + B_SLOTS * B_STEP;
     constexpr int LDS_BYTES = C_AT + (EIGHT ? 3 * Codes::kBytes : 0);
     static_assert(SM % 2 == 0, "A fragments alternate between two buffers");
-    static_assert(NW * 32 * WN * 4 <= LDS_BYTES && LDS_BYTES <= 160 * 1024, "the epilogue's rows fit");
+    static_assert(128 * BN * 4 <= LDS_BYTES && LDS_BYTES <= 160 * 1024, "the epilogue's rows fit");
     __shared__ __attribute__((aligned(1024))) uint8_t smem[LDS_BYTES];
 
     const int tid = threadIdx.x, lane = tid & 63;
@@ -655,10 +693,13 @@ ragged_tile_kernel(const RaggedGemmArgs p, const RaggedLaunch l) {
     __builtin_amdgcn_sched_barrier(0);
     wait_vmcnt_barrier<0>();   // (loads of steps past the end wrote zeros to LDS)
     __builtin_amdgcn_sched_barrier(0);
-    uint8_t* buf = smem + wave * (32 * WN * 4);
-    const int g_out = KIND == kRaggedTN ? g : 0;
-    if (p.out_f32) store_wave_tile<1, SM, SN>(p, acc, buf, g_out, m0 + wm * WM, m_end, n0 + wn * WN, lane, l.vec != 0);
-    else store_wave_tile<0, SM, SN>(p, acc, buf, g_out, m0 + wm * WM, m_end, n0 + wn * WN, lane, l.vec != 0);
+    auto store = [&](auto out) {
+        store_tile<decltype(out)::value, BM, BN, WGM, WGN>(p, acc, smem, KIND == kRaggedTN ? g : 0, m0, m_end, n0, wave, lane,
+                                                           l.vec != 0);
+    };
+    if (p.out_f32) store(std::integral_constant<int, 1>{});
+    else if (KIND == kRaggedTN && p.c) store(std::integral_constant<int, KIND == kRaggedTN ? 2 : 0>{});
+    else store(std::integral_constant<int, 0>{});
 }
 
 // D (+ C) from the pieces' sums in the workspace, added in the order of the pieces: four
@@ -780,40 +821,52 @@ void launch_kind(const RaggedGemmArgs& a, const RaggedPlan& plan, float* ws, int
 
 }  // namespace
 
-// The tile, and the pieces of the reduced axis. 256 x 256 tiles that fill 150 CUs, for NT
-// and NN with groups of 256 rows and more, for TN with C of 512 and more. Measured in us,
-// 256 x 256 against 128 x 128: NT, 4096 columns, K = 2048, 8 groups of 256 rows 38.1 and 35.5, of
-// 512 61.9 and 67.2, 32 of 512 252 and 311; TN without C, 32 groups of 47 rows to 2048 x
-// 2048 128 and 145, 8 of 1024 to 4096 x 4096 312 and 401; with C, the same 273 and 215, 8
-// of 512 to 4096 x 2048 178 and 180, 8 of 1024 to 4096 x 4096 444 and 450 (two small
-// workgroups on a CU read C for one under the other's products).
-// Pieces: the fewest microseconds by the time of a step (0.42 with a workgroup on a CU,
-// 1.02 with two) and of the sums' way through the workspace. Measured in us, whole and in 4, 8 and 16 pieces: NT of 8 x 4096 x 7168
-// 47.6, 18.8, 15.9, 17.4; 256 x 2112 x 7168 50.9, 22.5, 24.2, 31.0; 512 x 4096 x 2048
-// 19.5, 28.4, 41.9, 66.3; TN of 20000 rows to 104 x 504 124, 39.2, 24.8, 19.5.
+// The tile and the pieces of the reduced axis that take the fewest microseconds by measured
+// times: of a 64-element step of a round of tiles (256 x 256: 1.7; 128 x 128: 0.42 with one
+// workgroup on a CU, 1.05 with two; more with an 8-bit B), of a round's stores in TN, and
+// of the pieces' sums on their way through the workspace. 256 x 256 tiles have to fill 150
+// CUs, and win where they are within 15%: with K long the 128 x 128 ones' operands, read
+// twice as often, slow their steps (8 groups, 17648 x 517 x 7272 231 and 289 us). What it decides between, in us, 256 x 256 against 128 x 128: NT, 4096 columns, K =
+// 2048, 8 groups of 256 rows 38.1 and 35.5, of 512 61.9 and 67.2, 32 of 512 252 and 311; TN
+// without C, 8 groups of 512 rows to 4096 x 2048 133 and 114, of 1024 to 4096 x 4096 312
+// and 408; with C, 32 of 47 to 2048 x 2048 273 and 202 (two small workgroups on a CU read
+// C for one under the other's products), 8 of 2048 to 4096 x 7168 1072 and 1207. Whole and
+// in 4, 8 and 16 pieces: NT of 8 x 4096 x 7168 47.6, 18.8, 15.9, 17.4; 256 x 2112 x 7168
+// 50.9, 22.5, 24.2, 31.0; 512 x 4096 x 2048 19.5, 28.4, 41.9, 66.3; TN of 20000 rows to
+// 104 x 504 124, 39.2, 24.8, 19.5.
 RaggedPlan plan_ragged_gemm(RaggedKind kind, const RaggedGemmArgs& a, int slots, int block, int splits) {
+    const bool tn = kind == kRaggedTN, eight = a.b_sf != nullptr;
     const int64_t used = std::max<int64_t>(1, std::min<int64_t>(a.groups, a.rows));   // groups with rows, at most
-    const int64_t length = kind == kRaggedTN ? ceil_div(a.rows, used) : a.k;
+    const int64_t length = tn ? ceil_div(a.rows, used) : a.k;
     auto tiles = [&](int b) {   // expected
-        const double mb = kind == kRaggedTN ? (double)ceil_div(a.m, b) * a.groups
+        const double mb = tn ? (double)ceil_div(a.m, b) * a.groups
                           : a.rows <= used * b ? (double)used
                                                : (double)a.rows / b + 0.5 * used;
         return mb * ceil_div(a.n, b);
     };
+    // (the longest of several groups counts in TN: half as long again as the others, say)
+    const double steps = (double)ceil_div(length, BK) * (tn && used > 1 ? 1.5 : 1.0), t256 = tiles(256), t128 = tiles(128);
+    const double alone = eight ? 1.1 : 0.42, both = eight ? 1.3 : 1.05;   // a step of 128 x 128
+    const double store256 = !tn ? 0 : a.c ? 30 : a.out_f32 ? 15 : 9, store128 = !tn ? 0 : a.c ? 11.5 : a.out_f32 ? 7.7 : 5;
+    auto us128 = [&](double t, double n) {   // t tiles of n steps: whole rounds, and what is left for a CU
+        const double per_cu = t / slots, whole = std::floor(per_cu / 2), rest = per_cu - 2 * whole;
+        return whole * (n * both + store128) +
+               (rest > 0 ? n * (alone + (both - alone) * std::max(0.0, rest - 1)) + store128 * rest / 2 : 0.0);
+    };
     RaggedPlan plan{128, 1, 0};
-    const bool large = kind == kRaggedTN ? !a.c || length >= 512 : a.rows >= 256 * used;
-    if (block == 256 || (block == 0 && large && tiles(256) * 128 >= slots * 75)) {
+    if (block == 0 && t256 * 128 >= slots * 75 &&
+        std::max(1.0, t256 / slots) * (steps * (eight ? 1.95 : 1.7) + store256) < 1.15 * us128(t128, steps))
+        block = 256;
+    if (block == 256) {
         plan.block = 256;
         return plan;
     }
-    const int64_t out_rows = kind == kRaggedTN ? (int64_t)a.groups * a.m : a.rows;
-    const double t = tiles(128), steps = (double)ceil_div(length, BK), sums = (double)out_rows * a.n * 4;
+    const int64_t out_rows = tn ? (int64_t)a.groups * a.m : a.rows;
+    const double sums = (double)out_rows * a.n * 4;   // bytes of a piece's
     double best = 1e300;
     for (int s = 1; s <= 32; ++s) {
         if (splits > 0 ? s != splits : (s > 1 && steps < 4 * s)) continue;
-        const double per_cu = t * s / slots, rounds = std::ceil(per_cu / 2);
-        const double step_us = 0.42 + 0.6 * std::min(1.0, std::max(0.0, per_cu - 1));
-        const double us = rounds * std::ceil(steps / s) * step_us + (s > 1 ? 3.0 + 2 * sums * s / 3e6 : 0.0);
+        const double us = us128(t128 * s, std::ceil(steps / s)) + (s > 1 ? 3.0 + 2 * sums * s / 3e6 : 0.0);
         if (us < best) best = us, plan.splits = s;
     }
     if (plan.splits > 1) plan.workspace_bytes = out_rows * ceil_div(a.n, 4) * 16 * plan.splits;

@@ -408,7 +408,7 @@ int dg_moe_combine(const dg_tensor* y, const dg_tensor* pos, const dg_tensor* to
 /* Workspace bytes of a call of the three products (0: none; -1 on error): calls of few
  * tiles split the reduced axis over workgroups, the FP32 sums of its pieces go to the
  * workspace and a second kernel adds them in a fixed order. form 0: NT, 1: NN (rows, n,
- * k), 2: TN (rows, m, n). `workspace` below is a 1-D device tensor of that size, 16-byte
+ * k), 2: TN (rows, m, n), 3: TN with an 8-bit b. `workspace` below is a 1-D device tensor of that size, 16-byte
  * aligned, used until the call's kernels finish on `stream`; NULL, or one too small: the
  * axis stays whole. */
 int64_t dg_bf16_gemm_ragged_workspace_size(int32_t form, int64_t rows, int64_t m, int64_t n, int64_t k, int32_t groups);
