@@ -825,7 +825,7 @@ void launch_kind(const RaggedGemmArgs& a, const RaggedPlan& plan, float* ws, int
 // times: of a 64-element step of a round of tiles (256 x 256: 1.7; 128 x 128: 0.42 with one
 // workgroup on a CU, 1.05 with two; more with an 8-bit B), of a round's stores in TN, and
 // of the pieces' sums on their way through the workspace. 256 x 256 tiles have to fill 150
-// CUs, and win where they are within 15%: with K long the 128 x 128 ones' operands, read
+// CUs, and in NT and NN win where they are within 15%: with K long the 128 x 128 ones' operands, read
 // twice as often, slow their steps (8 groups, 17648 x 517 x 7272 231 and 289 us). What it decides between, in us, 256 x 256 against 128 x 128: NT, 4096 columns, K =
 // 2048, 8 groups of 256 rows 38.1 and 35.5, of 512 61.9 and 67.2, 32 of 512 252 and 311; TN
 // without C, 8 groups of 512 rows to 4096 x 2048 133 and 114, of 1024 to 4096 x 4096 312
@@ -855,7 +855,7 @@ RaggedPlan plan_ragged_gemm(RaggedKind kind, const RaggedGemmArgs& a, int slots,
     };
     RaggedPlan plan{128, 1, 0};
     if (block == 0 && t256 * 128 >= slots * 75 &&
-        std::max(1.0, t256 / slots) * (steps * (eight ? 1.95 : 1.7) + store256) < 1.15 * us128(t128, steps))
+        std::max(1.0, t256 / slots) * (steps * (eight ? 1.95 : 1.7) + store256) < (tn ? 1.0 : 1.15) * us128(t128, steps))
         block = 256;
     if (block == 256) {
         plan.block = 256;
