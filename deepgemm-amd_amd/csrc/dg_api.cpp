@@ -1575,6 +1575,7 @@ void check_sizes(const View& t) {
 // least their length (outputs: so that no two elements share memory). The kernels' tile
 // offsets are 32-bit: 256 rows of at most kRaggedMaxPitch elements.
 constexpr int64_t kRaggedMaxPitch = (int64_t)1 << 22;
+constexpr int64_t kRaggedMaxGroups = 65536;   // (every workgroup looks through group_ends)
 void check_ragged_matrix(const View& t, int dims) {
     check_shape(t, dims);
     check_sizes(t);
@@ -1595,7 +1596,7 @@ bool has_elements(const View& t) {
 
 void check_group_ends(const View& t, int64_t groups, int32_t alignment) {
     DG_CHECK(t.dim() == 1 && t.dtype() == DG_I32 && t.on_device() && contiguous_view(t));
-    DG_CHECK(t.size(0) == groups);
+    DG_CHECK(t.size(0) == groups && groups <= kRaggedMaxGroups);
     DG_CHECK(alignment > 0 && alignment <= (1 << 20));
 }
 

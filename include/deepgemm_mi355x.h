@@ -401,7 +401,8 @@ int dg_moe_combine(const dg_tensor* y, const dg_tensor* pos, const dg_tensor* to
  * not decreasing) holds the end of each group's rows: group g owns rows
  * [align(group_ends[g-1], alignment), group_ends[g]) (group 0 from row 0). alignment 1:
  * segments back to back; dg_moe_dispatch's psum layout with the alignment it was made
- * with otherwise. Groups may be empty. Ends past the rows that exist are cut off there.
+ * with otherwise. At most 65536 groups, any of them empty. Ends past the rows that exist
+ * are cut off there. The ends are read when the call runs: a captured graph follows them.
  * The reference's BF16 grouped GEMMs (csrc/apis/gemm.hpp) take segments padded to the MK
  * alignment and K-group sizes on the host. */
 

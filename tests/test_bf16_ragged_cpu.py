@@ -52,6 +52,7 @@ def test_m_grouped_refusals(name, make, key, value):
 @pytest.mark.parametrize('name,make', [('dg_m_grouped_bf16_gemm_nt_ragged', nt), ('dg_m_grouped_bf16_gemm_nn_ragged', nn)])
 def test_m_grouped_reduced_length_and_null(name, make):
     rejected(name, *make(k=36).values())
+    rejected(name, *make(n=8, k=8, g=65537).values(), match='kRaggedMaxGroups')
     for key in ('a', 'b', 'd', 'ends'):
         args = make()
         args[key] = None
@@ -141,3 +142,26 @@ def test_python_entry_points_refuse_host_tensors():
 def test_calls_with_nothing_to_do_launch_nothing(name, make):
     for args in (make(m=0), make(n=0), make(g=0)):
         assert call(name, *args.values())[0] == _ffi.DG_OK
+
+
+def test_workspace_sizes_and_plans():
+    """Few tiles split a long reduced axis, with a workspace of the pieces' FP32 sums; large
+    calls and short axes do not. A given number of pieces is taken as it is."""
+    size = _ffi.lib.dg_bf16_gemm_ragged_workspace_size
+    deep_gemm.set_num_sms(256)
+    try:
+        assert size(0, 8, 0, 4096, 7168, 1) % (8 * 4096 * 4) == 0 and size(0, 8, 0, 4096, 7168, 1) > 8 * 4096 * 4
+        assert size(2, 20000, 104, 504, 0, 1) > 0 and size(3, 20000, 104, 504, 0, 1) > 0
+        assert size(0, 16384, 0, 4096, 7168, 8) == 0 and size(1, 8, 0, 4096, 64, 1) == 0
+        assert size(0, 0, 0, 4096, 7168, 1) == 0 and size(2, 64, 0, 512, 0, 1) == 0 and size(0, 64, 0, 512, 512, 0) == 0
+        deep_gemm.set_tile_override(128, 5, variant=13)
+        assert size(0, 10, 0, 30, 640, 2) == 5 * 10 * 32 * 4
+        deep_gemm.set_tile_override(256, 0, variant=13)
+        assert size(0, 10, 0, 30, 640, 2) == 0
+        for args in ((4, 8, 8, 8, 8, 1), (0, -1, 8, 8, 8, 1), (0, 8, 8, 1 << 30, 8, 1)):
+            assert size(*args) == -1 and 'Assertion error' in _ffi.lib.dg_last_error().decode()
+        for bad in ((64, 0), (256, 2), (128, 33), (128, -1)):
+            with pytest.raises(RuntimeError, match='Unsupported'):
+                deep_gemm.set_tile_override(*bad, variant=13)
+    finally:
+        deep_gemm.init()

@@ -338,6 +338,88 @@ def test_graphs_replay_the_eager_results():
             assert torch.equal(bits(out), bits(ref)) and torch.equal(bits(other), bits(ref)) and torch.equal(bits(third), bits(ref))
 
 
+def test_graphs_follow_the_group_ends():
+    """A graph replayed with other ends in the same tensor: other segments, other counts."""
+    a, _ = matrix((300, 64), 1)
+    w, _ = matrix((5, 72, 64), 2)
+    t, _ = matrix((300, 72), 3)
+    ends = ends_of(segments([10, 0, 200, 30, 60]))
+    d, e = torch.zeros((300, 72), device=DEV), torch.zeros((5, 72, 64), device=DEV)
+
+    def run(d, e, ends):
+        deep_gemm.m_grouped_bf16_gemm_nt_ragged(a, w, d, ends)
+        deep_gemm.k_grouped_bf16_gemm_tn_ragged(t, a, e, ends)
+    run(d, e, ends)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        run(d, e, ends)
+    for sizes in ([300, 0, 0, 0, 0], [60] * 5, [0, 0, 1, 0, 0], [1, 120, 1, 130, 48]):
+        now = ends_of(segments(sizes))
+        d.fill_(3.0), e.fill_(3.0)
+        d2, e2 = torch.full_like(d, 3.0), torch.full_like(e, 3.0)
+        ends.copy_(now)
+        g.replay()
+        run(d2, e2, now)
+        torch.cuda.synchronize()
+        assert torch.equal(bits(d), bits(d2)) and torch.equal(bits(e), bits(e2))
+
+
+@pytest.mark.parametrize('sms', [7, 64])
+def test_fewer_compute_units(sms):
+    """Rounds, tails and plans of another number of CUs."""
+    deep_gemm.set_num_sms(sms)
+    try:
+        m_grouped('nt', [700, 0, 1300, 65], 776, 192)
+        m_grouped('nn', [700, 0, 1300, 65], 776, 192)
+        k_grouped([300, 0, 130, 65], 776, 520, add=True)
+        k_grouped([300, 0, 130, 65], 520, 776, eight=True)
+    finally:
+        deep_gemm.set_num_sms(256)
+
+
+def test_offsets_past_32_bits(tiles):
+    """Operands and results of more than 2^31 elements: their last group, row and column."""
+    if tiles not in ('256', '128'):
+        pytest.skip('the two kinds of tiles are enough')
+    n, k = 36000, 32768
+    print('nt, weights of 3.5e9 elements', flush=True)
+    b = torch.empty((3, n, k), dtype=torch.bfloat16, device=DEV)
+    b[2].normal_(generator=torch.Generator(DEV).manual_seed(1))
+    a, a64 = matrix((5, k), 2)
+    d = torch.full((5, n), 7.0, device=DEV)
+    deep_gemm.m_grouped_bf16_gemm_nt_ragged(a, b, d, torch.tensor([0, 0, 5], dtype=torch.int32, device=DEV))
+    cols = [0, 1, 17999, n - 1]
+    w = b[2, cols].double().cpu()
+    ref = a64 @ w.T
+    check(d[:, cols], ref, rounding(d.dtype, ref) + sum_error(k, a64.abs() @ w.T.abs()), 'weights past 2^31')
+    del b, d
+    print('tn, rows past 2^31 elements', flush=True)
+    rows, m = 70000, 32768
+    t = torch.empty((rows, m), dtype=torch.bfloat16, device=DEV)
+    t[-30:].normal_(generator=torch.Generator(DEV).manual_seed(3))
+    x, x64 = matrix((rows, 40), 4)
+    d = torch.empty((2, m, 40), device=DEV)
+    seg = [(0, rows - 30), (rows - 30, rows)]
+    t[:-30] = 0
+    deep_gemm.k_grouped_bf16_gemm_tn_ragged(t, x, d, ends_of(seg))
+    ms = [0, 5, m - 1]
+    tv = t[-30:, ms].double().cpu()
+    ref = tv.T @ x64[-30:]
+    check(d[1, ms], ref, rounding(d.dtype, ref) + sum_error(30, tv.abs().T @ x64[-30:].abs()), 'rows past 2^31')
+    assert (d[0] == 0).all()
+    del t, d
+    print('tn, a result of 2.4e9 elements', flush=True)
+    m, n = 32768, 36864
+    t, t64 = matrix((9, m), 5)
+    x, x64 = matrix((9, n), 6)
+    d = torch.full((2, m, n), 7.0, dtype=torch.bfloat16, device=DEV)
+    deep_gemm.k_grouped_bf16_gemm_tn_ragged(t, x, d, ends_of([(0, 4), (4, 9)]))
+    ref = t64[4:].T[-3:] @ x64[4:][:, -70:]
+    mag = t64[4:].abs().T[-3:] @ x64[4:].abs()[:, -70:]
+    check(d[1, -3:, -70:], ref, rounding(d.dtype, ref) + sum_error(5, mag) * 1.01, 'result past 2^31')
+
+
 def test_two_streams_at_once():
     for run, out in _calls():
         run(out)
