@@ -10,6 +10,13 @@
 // BF16 products are exact in FP32 and summed there by v_mfma_f32_32x32x16_bf16; the sum
 // (with C added in FP32) is rounded once, to D's type. A checkpoint value is rounded to
 // BF16 after its scale, which is exact where the scale is a power of two.
+//
+// Measured on MI355X: 8192^3 as one group NT 930-980 us (16 KB rows of both operands meet in
+// few L2 channels; with 128 bytes more 905), NN 825-880, TN 805-855, with an 8-bit B
+// 960-1010; torch's library product 802, 888, 996. Under matrix load the clock falls to
+// 1.4-1.7 GHz: 2091 TFLOP/s of zeros become 1371 of random values in the library's NT
+// product, 1814 and 1250 in NN here, so bytes moved cost time even where they are hidden.
+// Matrix cores busy 74-78% of the cycles of NT 16384 x 4096 x 7168 and NN 8192 x 7168 x 4096.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -53,7 +60,7 @@ __device__ __forceinline__ void group_rows(const int32_t* ends, int g, int rows,
 // workgroups of those fit a CU, so 150 tiles' quarters take 1.2 rounds of 512, about 0.65
 // of a 256 x 256 round (PART 1 and 2; 0 is a launch by itself). Both launches work it
 // out alike, from the tiles that there are. 8 experts, 16384 x 4096 x 7168 (NT, 1088
-// tiles, 4.25 rounds): see launch_ragged_gemm.
+// tiles, 4.25 rounds): 889 -> 861 us; 8192 x 7168 x 4096 (NN, 3.94 rounds, no tail) 437 and 439.
 __host__ __device__ __forceinline__ int tail_tiles(int tiles, int slots) {
     const int rest = tiles % slots;
     return rest * 128 <= slots * 75 ? rest : 0;
@@ -178,7 +185,11 @@ __device__ __forceinline__ bool locate_outputs(const RaggedGemmArgs& p, const Ra
 
 // ---------------------------------------------------------------- tiles
 //
-// One workgroup per BM x BN tile of D, 64 reduced elements a step, two steps in LDS.
+// One workgroup per BM x BN tile of D: 256 x 256 on eight waves (128 x 64 each), one
+// workgroup on a CU, or 128 x 128 on four (64 x 64), two on a CU. 64 reduced elements a step,
+// three steps of A and two of B in LDS (160 or 80 KB), so that every load has most of two
+// steps to arrive: with two of each, 128 x 128 tiles of few rows, which wait for HBM, took
+// 35.4 us instead of 25.7 (1001 x 1413 x 2048 over 16 groups), 256 x 256 the same.
 // Operands go straight to LDS by buffer loads (16 bytes a lane) whose descriptor ends at
 // the last valid byte: rows past the group's, columns past N and reduced elements past the
 // end arrive as zeros, in both operands, and nothing is read there. So there are no edge
@@ -193,9 +204,11 @@ __device__ __forceinline__ bool locate_outputs(const RaggedGemmArgs& p, const Ra
 // permuted (column unit 2a + b of reduced row k at b * 4 + (a & 3 ^ k & 3) + (a >> 2) * 8)
 // so that the four rows of a block, and the two blocks side by side, lie in distinct banks.
 //
-// The hand-off to the next step (wait for its loads, barrier, issue the loads of the step
-// after it into the freed half of LDS) comes before the last 32-row slice of a step's
-// matrix instructions, with the next step's fragments read under them.
+// Two barriers a step. The hand-off (the next step's loads have arrived, and every wave has
+// read A's last slice of this one: A's step after the next three goes there) comes before
+// the last 32-row slice of a step's matrix instructions, with the next step's fragments read
+// under them; the other one, a slice after the step's start (128 x 128: at it), when every
+// wave holds its B fragments, hands B's place on.
 
 __device__ __forceinline__ int swz_g(int r) { return ((r >> 1) ^ ((r & 1) << 2)) & 7; }
 
@@ -519,7 +532,7 @@ ragged_tile_kernel(const RaggedGemmArgs p, const RaggedLaunch l) {
     constexpr int A_KMAJOR = KIND != kRaggedTN, B_KMAJOR = KIND == kRaggedNT;
     constexpr int KS = BK / 16;
     constexpr int A_STEP = BM * BK * 2, B_STEP = BN * BK * 2;   // bytes of a step
-    // LDS: A's steps, B's (8-bit: one, beside three steps of codes, which take A's third)
+    // LDS: A's steps, B's (8-bit: one, beside three steps of codes, in the place of A's third)
     using Codes = CodeOperand<BN, NW>;
     constexpr int A_SLOTS = EIGHT ? 2 : 3, B_SLOTS = EIGHT ? 1 : 2;
     constexpr int B_AT = A_SLOTS * A_STEP, C_AT = B_AT + B_SLOTS * B_STEP;

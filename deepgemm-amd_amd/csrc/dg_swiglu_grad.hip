@@ -11,8 +11,11 @@
 //   du = dh w g s,  dg = dh w u s (1 + g (1 - s)),  dw = sum over the row of dh g s u.
 // With a clamp c, u is clamped to [-c, c] and g to at most c before all of it, and du, dg
 // are zero where the clamp holds the value (|u| > c, g > c).
-// Both are one pass over HBM: forward 8 bytes per element of h (4 in, 2 + 2 out), backward
-// 10 (2 + 2 in, 4 + 2 out).
+// Both are one pass over HBM, which bounds them: forward 8 bytes per element of h (4 in, 2 +
+// 2 out), backward 10 (2 + 2 in, 4 + 2 out). A lane owns 8 columns: 16-byte accesses of the
+// BF16 rows, 8 of the codes. 16384 x 2048: forward 48.6 us (5.6 TB/s; the kernel alone 43),
+// backward 60.7 (5.6 TB/s), a copy of 1 GiB 5.1 TB/s; the exponentials and reciprocals hide
+// under it. 33 x 1024: 11.5 us a call, of which the kernel 4.
 #include <hip/hip_runtime.h>
 
 #include "dg_internal.hpp"
@@ -36,7 +39,8 @@ __device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
     return uint4{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7])};
 }
 
-// s = 1 / (1 + exp(-g)); NaN for NaN.
+// s = 1 / (1 + exp(-g)) by the hardware's exponential and reciprocal (a few units in the last
+// place of FP32; results are rounded to BF16); zero below g = -87.3, NaN for NaN.
 __device__ __forceinline__ float sigmoid(float g) { return __builtin_amdgcn_rcpf(1.0f + __expf(-g)); }
 
 // The power-of-two scale and the codes of one lane's 8 values, the group being the 16

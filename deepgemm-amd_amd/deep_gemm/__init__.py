@@ -9,8 +9,10 @@ functions return None. Launches are asynchronous on the current stream.
 
 Scope: fp8_gemm_nt (and its fp8_fp4/fp4 aliases and nn/tn/tt transposing
 wrappers), m_grouped_fp8_gemm_nt_contiguous (m_indices and psum layouts),
-m_grouped_fp8_gemm_nt_masked, and the SF layout helpers. The reference's
-BF16/einsum/attention/Mega-MoE/cuBLASLt kernels are not provided.
+m_grouped_fp8_gemm_nt_masked, the SF layout helpers, and BF16 training of an MoE layer's
+experts (m_grouped_bf16_gemm_{nt,nn}_ragged, k_grouped_bf16_gemm_tn_ragged,
+moe_swiglu_checkpoint, moe_swiglu_backward). The reference's own
+BF16/einsum/attention/Mega-MoE/cuBLASLt entry points are not provided.
 """
 from typing import Optional, Tuple
 
