@@ -2084,7 +2084,7 @@ int dg_set_tile_override(int32_t variant, int32_t block_m, int32_t block_n) {
             return;
         }
         if (variant == 13) {
-            if ((block_m != 128 && block_m != 256) || block_n < 0 || block_n > (block_m == 128 ? 32 : 0))
+            if ((block_m != 32 && block_m != 128 && block_m != 256) || block_n < 0 || block_n > (block_m == 256 ? 0 : 32))
                 DG_UNSUPPORTED("tile shape not compiled");
             g_ragged_block = block_m, g_ragged_splits = block_n;
             return;

@@ -44,9 +44,11 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 // Tiles of a launch: row and column blocks (NT, NN: row blocks at most; of 256 for quarters),
 // CUs, pieces of the reduced axis (blockIdx.y), and whether D and C take 16-byte accesses.
 struct RaggedLaunch {
-    int row_blocks, col_blocks, slots, splits, vec;
+    int row_blocks, col_blocks, slots, splits;
+    bool vec;
 };
 constexpr int kRasterBlocks = 8;   // row blocks of a raster band
+constexpr int kFewRows = 32;       // rows of the tile for decode
 
 // Rows [start, end) of group g, inside the `rows` that exist whatever group_ends holds.
 __device__ __forceinline__ void group_rows(const int32_t* ends, int g, int rows, int alignment, int& start, int& end) {
@@ -708,11 +710,79 @@ ragged_tile_kernel(const RaggedGemmArgs p, const RaggedLaunch l) {
     __builtin_amdgcn_sched_barrier(0);
     auto store = [&](auto out) {
         store_tile<decltype(out)::value, BM, BN, WGM, WGN>(p, acc, smem, KIND == kRaggedTN ? g : 0, m0, m_end, n0, wave, lane,
-                                                           l.vec != 0);
+                                                           l.vec);
     };
     if (p.out_f32) store(std::integral_constant<int, 1>{});
     else if (KIND == kRaggedTN && p.c) store(std::integral_constant<int, KIND == kRaggedTN ? 2 : 0>{});
     else store(std::integral_constant<int, 0>{});
+}
+
+// NT and NN with at most 32 rows a group (decode): 32 x 128 tiles on four waves of 32 x 32, two
+// workgroups on a CU, which stream the weights from HBM. A step is 4 KB of A and 16 of B, so
+// four steps fit where a 128 x 128 tile has three and two, and a workgroup keeps 60 KB in
+// flight; one barrier a step (it certifies the next step's loads and frees this one's
+// place, whose fragments every wave holds).
+template <int KIND>
+__global__ void __launch_bounds__(256, 2) ragged_few_rows_kernel(const RaggedGemmArgs p, const RaggedLaunch l) {
+    static_assert(KIND == kRaggedNT || KIND == kRaggedNN, "A is K-major");
+    constexpr int BM = kFewRows, BN = 128, NW = 4, KS = BK / 16, SLOTS = 4;
+    constexpr int A_STEP = BM * BK * 2, STEP = A_STEP + BN * BK * 2;
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[SLOTS * STEP];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    RaggedTile t{};
+    if (!locate_rows<BM, BN, 0>(p, l, t)) return;
+    const int piece = ((p.k + BK - 1) / BK + l.splits - 1) / l.splits * BK;   // (as in the tile kernel)
+    const int k0 = min((int)blockIdx.y * piece, p.k);
+    const int reduced = min(piece, p.k - k0);
+    const uint16_t* b = static_cast<const uint16_t*>(p.b) + (int64_t)t.g * p.b_gs;
+
+    Operand<BM, 1, NW> oa;
+    Operand<BN, KIND == kRaggedNT, NW> ob;
+    oa.init(p.a + (int64_t)t.m0 * p.lda + k0, p.lda, min(BM, t.m_end - t.m0), reduced, wave, lane);
+    ob.init(KIND == kRaggedNT ? b + (int64_t)t.n0 * p.ldb + k0 : b + (int64_t)k0 * p.ldb + t.n0, p.ldb, min(BN, p.n - t.n0),
+            reduced, wave, lane);
+    constexpr int LOADS = decltype(oa)::kInstr + decltype(ob)::kInstr;
+    const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_address(smem));
+    auto issue = [&](int slot) {
+        oa.issue(lds0 + slot * STEP, wave);
+        ob.issue(lds0 + slot * STEP + A_STEP, wave);
+    };
+    Fragments<BM, 1, 1> fa;
+    Fragments<BN, KIND == kRaggedNT, 1> fb;
+    fa.init(0, lane);
+    fb.init(wave * 32, lane);
+    bf16x8 op_a[2][KS], op_b[2][KS];
+    auto read = [&](int to, int slot) {
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            op_a[to][ks] = fa.read(smem + slot * STEP, 0, ks);
+            op_b[to][ks] = fb.read(smem + slot * STEP + A_STEP, 0, ks);
+        }
+    };
+    f32x16 acc[1][1];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[0][0][e] = 0.f;
+
+    const int steps = (reduced + BK - 1) / BK;
+#pragma unroll
+    for (int st = 0; st < SLOTS; ++st) issue(st);
+    wait_vmcnt_barrier<(SLOTS - 1) * LOADS>();
+    read(0, 0);
+    for (int kb = 0; kb < steps; kb += 2) {   // (a step past an odd end: zeros)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            wait_vmcnt_barrier<(SLOTS - 2) * LOADS>();
+            issue((kb + h) % SLOTS);
+            read(h ^ 1, (kb + h + 1) % SLOTS);
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+                acc[0][0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(op_b[h][ks], op_a[h][ks], acc[0][0], 0, 0, 0);
+        }
+    }
+    wait_vmcnt_barrier<0>();   // (loads of steps past the end wrote zeros to LDS)
+    if (p.out_f32) store_tile<1, BM, BN, 1, NW>(p, acc, smem, 0, t.m0, t.m_end, t.n0, wave, lane, l.vec);
+    else store_tile<0, BM, BN, 1, NW>(p, acc, smem, 0, t.m0, t.m_end, t.n0, wave, lane, l.vec);
 }
 
 // D (+ C) from the pieces' sums in the workspace, added in the order of the pieces: four
@@ -774,6 +844,22 @@ int64_t row_blocks(RaggedKind kind, const RaggedGemmArgs& a, int bm) {
     return kind == kRaggedTN ? ceil_div(a.m, bm) : a.rows / bm + std::min<int64_t>(a.groups, a.rows);
 }
 
+// Whether D's rows, and C's, begin at multiples of 16 bytes.
+bool takes_vectors(const RaggedGemmArgs& a) {
+    const int64_t size = a.out_f32 ? 4 : 2;
+    return reinterpret_cast<uintptr_t>(a.d) % 16 == 0 && a.ldd * size % 16 == 0 && a.d_gs * size % 16 == 0 &&
+           (!a.c || (reinterpret_cast<uintptr_t>(a.c) % 16 == 0 && a.ldc * size % 16 == 0 && a.c_gs * size % 16 == 0));
+}
+
+template <int KIND>
+void launch_few_rows(const RaggedGemmArgs& a, int slots, int splits, hipStream_t stream) {
+    const int64_t mb = row_blocks((RaggedKind)KIND, a, kFewRows), nb = ceil_div(a.n, 128);
+    DG_CHECK(mb * nb < ((int64_t)1 << 28));
+    const RaggedLaunch l{(int)mb, (int)nb, slots, splits, takes_vectors(a)};
+    hipLaunchKernelGGL(ragged_few_rows_kernel<KIND>, dim3((unsigned)(mb * nb), (unsigned)splits), dim3(256), 0, stream, a, l);
+    DG_HIP_CHECK(hipGetLastError());
+}
+
 template <int KIND, int BM, int BN, int WGM, int WGN, int PART, int EIGHT>
 void launch_tiles(const RaggedGemmArgs& a, int slots, int splits, hipStream_t stream) {
     constexpr int LIST = PART == 2 ? 2 : 1;
@@ -783,10 +869,7 @@ void launch_tiles(const RaggedGemmArgs& a, int slots, int splits, hipStream_t st
     int64_t blocks = KIND == kRaggedTN ? ceil_div(mb * nb, 8) * 8 * a.groups : tiles;
     // (a tail has at most 58% of a round's tiles, for each XCD by itself in TN)
     if (PART == 2) blocks = std::min<int64_t>(blocks, KIND == kRaggedTN ? std::max(slots / 8, 1) * 8 : slots) * 4;
-    const int64_t size = a.out_f32 ? 4 : 2;
-    const bool vec = reinterpret_cast<uintptr_t>(a.d) % 16 == 0 && a.ldd * size % 16 == 0 && a.d_gs * size % 16 == 0 &&
-                     (!a.c || (reinterpret_cast<uintptr_t>(a.c) % 16 == 0 && a.ldc * size % 16 == 0 && a.c_gs * size % 16 == 0));
-    const RaggedLaunch l{(int)mb, (int)nb, slots, splits, (int)vec};
+    const RaggedLaunch l{(int)mb, (int)nb, slots, splits, takes_vectors(a)};
     hipLaunchKernelGGL((ragged_tile_kernel<KIND, BM, BN, WGM, WGN, PART, EIGHT>), dim3((unsigned)blocks, (unsigned)splits),
                        dim3(WGM * WGN * 64), 0, stream, a, l);
     DG_HIP_CHECK(hipGetLastError());
@@ -814,15 +897,21 @@ void launch_kind(const RaggedGemmArgs& a, const RaggedPlan& plan, float* ws, int
         }
         return;
     }
+    auto launch = [&](const RaggedGemmArgs& args) {
+        if constexpr (KIND != kRaggedTN) {
+            if (plan.block == kFewRows) return launch_few_rows<KIND>(args, slots, plan.splits, stream);
+        }
+        launch_tiles<KIND, 128, 128, 2, 2, 0, EIGHT>(args, slots, plan.splits, stream);
+    };
     if (plan.splits == 1) {
-        launch_tiles<KIND, 128, 128, 2, 2, 0, EIGHT>(a, slots, 1, stream);
+        launch(a);
         return;
     }
     const int64_t rows = KIND == kRaggedTN ? (int64_t)a.groups * a.m : a.rows, ld = ceil_div(a.n, 4) * 4;
     RaggedGemmArgs part = a;
     part.d = ws, part.ldd = ld, part.d_gs = KIND == kRaggedTN ? a.m * ld : 0, part.d_split = rows * ld;
     part.c = nullptr, part.out_f32 = 1;
-    launch_tiles<KIND, 128, 128, 2, 2, 0, EIGHT>(part, slots, plan.splits, stream);
+    launch(part);
     RaggedGemmArgs whole = a;
     whole.d_split = part.d_split;
     const int64_t chunks = ceil_div(a.n, 1024);
@@ -836,17 +925,21 @@ void launch_kind(const RaggedGemmArgs& a, const RaggedPlan& plan, float* ws, int
 
 // The tile and the pieces of the reduced axis that take the fewest microseconds by measured
 // times: of a 64-element step of a round of tiles (256 x 256: 1.7; 128 x 128: 0.42 with one
-// workgroup on a CU, 1.05 with two; more with an 8-bit B), of a round's stores in TN, and
-// of the pieces' sums on their way through the workspace. 256 x 256 tiles have to fill 150
-// CUs, and in NT and NN win where they are within 15%: with K long the 128 x 128 ones' operands, read
-// twice as often, slow their steps (8 groups, 17648 x 517 x 7272 231 and 289 us). What it decides between, in us, 256 x 256 against 128 x 128: NT, 4096 columns, K =
-// 2048, 8 groups of 256 rows 38.1 and 35.5, of 512 61.9 and 67.2, 32 of 512 252 and 311; TN
-// without C, 8 groups of 512 rows to 4096 x 2048 133 and 114, of 1024 to 4096 x 4096 312
-// and 408; with C, 32 of 47 to 2048 x 2048 273 and 202 (two small workgroups on a CU read
-// C for one under the other's products), 8 of 2048 to 4096 x 7168 1072 and 1207. Whole and
-// in 4, 8 and 16 pieces: NT of 8 x 4096 x 7168 47.6, 18.8, 15.9, 17.4; 256 x 2112 x 7168
-// 50.9, 22.5, 24.2, 31.0; 512 x 4096 x 2048 19.5, 28.4, 41.9, 66.3; TN of 20000 rows to
-// 104 x 504 124, 39.2, 24.8, 19.5.
+// workgroup on a CU, 1.05 with two; more with an 8-bit B; 32 x 128, for at most 32 rows a
+// group: 0.25 and 0.5), of a round's stores in TN, and of the pieces' sums on their way
+// through the workspace. 256 x 256 tiles have to fill 150 CUs, and in NT and NN win where
+// they are within 15%: with K long the 128 x 128 ones' operands, read twice as often, slow
+// their steps (8 groups, 17648 x 517 x 7272 231 and 289 us). What it decides between, in us:
+// 256 x 256 against 128 x 128: NT, 4096 columns, K = 2048, 8 groups of 256 rows 38.1 and 35.5,
+//   of 512 61.9 and 67.2, 32 of 512 252 and 311; TN without C, 8 groups of 512 rows to 4096 x
+//   2048 133 and 114, of 1024 to 4096 x 4096 312 and 408; with C, 32 of 47 to 2048 x 2048 273
+//   and 202 (two small workgroups on a CU read C for one under the other's products), 8 of
+//   2048 to 4096 x 7168 1072 and 1207.
+// 128 x 128 against 32 x 128: NT, 64 x 2048 x 2048 over 8 groups 17.8 and 13.3, 14 x 512 x
+//   8192 over 2, in pieces, 14.0 and 9.6; even where HBM bounds both.
+// Whole and in 4, 8 and 16 pieces: 32 x 128, 8 x 4096 x 7168 30.4, 15.4, 15.4, 16.8; 128 x
+//   128, 256 x 2112 x 7168 50.9, 22.5, 24.2, 31.0, 512 x 4096 x 2048 19.5, 28.4, 41.9, 66.3,
+//   TN of 20000 rows to 104 x 504 124, 39.2, 24.8, 19.5.
 RaggedPlan plan_ragged_gemm(RaggedKind kind, const RaggedGemmArgs& a, int slots, int block, int splits) {
     const bool tn = kind == kRaggedTN, eight = a.b_sf != nullptr;
     const int64_t used = std::max<int64_t>(1, std::min<int64_t>(a.groups, a.rows));   // groups with rows, at most
@@ -859,15 +952,16 @@ RaggedPlan plan_ragged_gemm(RaggedKind kind, const RaggedGemmArgs& a, int slots,
     };
     // (the longest of several groups counts in TN: half as long again as the others, say)
     const double steps = (double)ceil_div(length, BK) * (tn && used > 1 ? 1.5 : 1.0), t256 = tiles(256), t128 = tiles(128);
-    const double alone = eight ? 1.1 : 0.42, both = eight ? 1.3 : 1.05;   // a step of 128 x 128
+    const bool few = !tn && (block == kFewRows || (block == 0 && a.rows <= kFewRows * used));
+    const double alone = few ? 0.25 : eight ? 1.1 : 0.42, both = few ? 0.5 : eight ? 1.3 : 1.05;   // a step of 32 or 128 rows
     const double store256 = !tn ? 0 : a.c ? 30 : a.out_f32 ? 15 : 9, store128 = !tn ? 0 : a.c ? 11.5 : a.out_f32 ? 7.7 : 5;
     auto us128 = [&](double t, double n) {   // t tiles of n steps: whole rounds, and what is left for a CU
         const double per_cu = t / slots, whole = std::floor(per_cu / 2), rest = per_cu - 2 * whole;
         return whole * (n * both + store128) +
                (rest > 0 ? n * (alone + (both - alone) * std::max(0.0, rest - 1)) + store128 * rest / 2 : 0.0);
     };
-    RaggedPlan plan{128, 1, 0};
-    if (block == 0 && t256 * 128 >= slots * 75 &&
+    RaggedPlan plan{few ? kFewRows : 128, 1, 0};
+    if (block == 0 && !few && t256 * 128 >= slots * 75 &&
         std::max(1.0, t256 / slots) * (steps * (eight ? 1.95 : 1.7) + store256) < (tn ? 1.0 : 1.15) * us128(t128, steps))
         block = 256;
     if (block == 256) {
@@ -879,7 +973,7 @@ RaggedPlan plan_ragged_gemm(RaggedKind kind, const RaggedGemmArgs& a, int slots,
     double best = 1e300;
     for (int s = 1; s <= 32; ++s) {
         if (splits > 0 ? s != splits : (s > 1 && steps < 4 * s)) continue;
-        const double us = us128(t128 * s, std::ceil(steps / s)) + (s > 1 ? 3.0 + 2 * sums * s / 3e6 : 0.0);
+        const double us = us128(t128 * s, std::ceil(steps / s)) + (s > 1 ? 5.0 + 2 * sums * s / 3e6 : 0.0);
         if (us < best) best = us, plan.splits = s;
     }
     if (plan.splits > 1) plan.workspace_bytes = out_rows * ceil_div(a.n, 4) * 16 * plan.splits;

@@ -15,10 +15,10 @@ pytestmark = pytest.mark.gpu
 MIXED = [5, 0, 1, 130, 0, 64, 257, 31, 0]
 
 
-@pytest.fixture(autouse=True, params=['heuristic', '256', '128', '128 in 3 pieces'])
+@pytest.fixture(autouse=True, params=['heuristic', '256', '128', '128 in 3 pieces', '32', '32 in 2 pieces'])
 def tiles(request):
     """Every test with the tiles the sizes choose, and with each kind forced."""
-    block, pieces = {'heuristic': (0, 0), '256': (256, 0), '128': (128, 1), '128 in 3 pieces': (128, 3)}[request.param]
+    block, pieces = {'heuristic': (0, 0), '256': (256, 0), '128': (128, 1), '128 in 3 pieces': (128, 3), '32': (32, 1), '32 in 2 pieces': (32, 2)}[request.param]
     if block:
         deep_gemm.set_tile_override(block, pieces, variant=13)
     yield request.param
@@ -380,8 +380,8 @@ def test_fewer_compute_units(sms):
 
 def test_offsets_past_32_bits(tiles):
     """Operands and results of more than 2^31 elements: their last group, row and column."""
-    if tiles not in ('256', '128'):
-        pytest.skip('the two kinds of tiles are enough')
+    if tiles not in ('256', '128', '32'):
+        pytest.skip('each kind of tile is enough')
     n, k = 36000, 32768
     print('nt, weights of 3.5e9 elements', flush=True)
     b = torch.empty((3, n, k), dtype=torch.bfloat16, device=DEV)
