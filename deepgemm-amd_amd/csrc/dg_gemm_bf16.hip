@@ -231,9 +231,9 @@ __device__ __forceinline__ i32x4 descriptor(const void* base, int bytes) {
 // No offset of a valid byte: past the end of every descriptor here.
 constexpr uint32_t kPastEnd = 0x80000000u;
 
-// One operand of a tile: where its steps come from. ROWS: BM or BN; KMAJOR as above.
 constexpr int BK = 64;
 
+// One operand of a tile: where its steps come from. ROWS: BM or BN; KMAJOR as above.
 template <int ROWS, int KMAJOR, int NW>
 struct Operand {
     static constexpr int kInstr = ROWS * BK / (512 * NW);   // wave loads (1 KB) of a step for each wave

@@ -15,7 +15,7 @@
 // 2 out), backward 10 (2 + 2 in, 4 + 2 out). A lane owns 8 columns: 16-byte accesses of the
 // BF16 rows, 8 of the codes. 16384 x 2048: forward 48.6 us (5.6 TB/s; the kernel alone 43),
 // backward 60.7 (5.6 TB/s), a copy of 1 GiB 5.1 TB/s; the exponentials and reciprocals hide
-// under it. 33 x 1024: 11.5 us a call, of which the kernel 4.
+// under it. 33 x 1024: 9 us a call, of which the kernel 4.
 #include <hip/hip_runtime.h>
 
 #include "dg_internal.hpp"

@@ -639,11 +639,8 @@ def moe_swiglu_checkpoint(x: torch.Tensor, row_weights: Optional[torch.Tensor] =
     [M, 2 ceil(I / 128)]) with power-of-two scales, each half as per_token_cast_to_fp8(half,
     use_ue8m0=True). One HBM pass. row_layout (m_indices): rows with a negative entry count
     as zeros. clamp_value: up within [-c, c] and gate at most c in h (x is kept unclamped)."""
-    m, i2 = x.shape
-    h = torch.empty((m, i2 // 2), dtype=torch.bfloat16, device=x.device)
-    q = torch.empty((m, i2), dtype=torch.float8_e4m3fn, device=x.device)
-    sf = torch.empty((m, 2 * ((i2 // 2 + 127) // 128)), dtype=torch.float32, device=x.device)
-    _check(_bind.swiglu_checkpoint(x, row_weights, row_layout, float(clamp_value or 0.0), h, q, sf, _raw_stream_of(x)))
+    status, h, q, sf = _bind.swiglu_checkpoint(x, row_weights, row_layout, float(clamp_value or 0.0), _raw_stream_of(x))
+    _check(status)
     return h, (q, sf)
 
 
@@ -656,10 +653,7 @@ def moe_swiglu_backward(dh: torch.Tensor, checkpoint: Tuple[torch.Tensor, torch.
     gradient of the product after it, float32 [M] gradient of row_weights or None without
     them). The other arguments as in the forward pass."""
     q, sf = _pair(checkpoint, 'checkpoint')
-    m, i = dh.shape
-    dx = torch.empty((m, 2 * i), dtype=torch.bfloat16, device=dh.device)
-    h = torch.empty((m, i), dtype=torch.bfloat16, device=dh.device)
-    dw = torch.empty((m,), dtype=torch.float32, device=dh.device) if row_weights is not None else None
-    _check(_bind.swiglu_backward(dh, q, sf, row_weights, row_layout, float(clamp_value or 0.0), dx, h, dw,
-                                 _raw_stream_of(dh)))
+    status, dx, h, dw = _bind.swiglu_backward(dh, q, sf, row_weights, row_layout, float(clamp_value or 0.0),
+                                              _raw_stream_of(dh))
+    _check(status)
     return dx, h, dw
