@@ -1747,6 +1747,7 @@ void swiglu_checkpoint_impl(const dg_tensor* x_, const dg_tensor* w_, const dg_t
     p.row_weight = row_weights_of(w_, m), p.row_layout = row_layout_of(rl_, m);
     const int device = one_device({x_, w_, rl_, h_, q_, sf_});
     if (m == 0 || n == 0) return;
+    DG_CHECK_GRID(swiglu_checkpoint_blocks(m, n), 256);
     p.x = static_cast<const uint16_t*>(x.data()), p.ldx = x.stride(0);
     p.clamp = clamp;
     p.h = static_cast<uint16_t*>(const_cast<void*>(h.data())), p.ldh = h.stride(0);
@@ -1777,6 +1778,7 @@ void swiglu_backward_impl(const dg_tensor* dh_, const dg_tensor* q_, const dg_te
     DG_CHECK((dw_ == nullptr) || (w_ != nullptr));   // a gradient of weights that were not given
     const int device = one_device({dh_, q_, sf_, w_, rl_, dx_, h_, dw_});
     if (m == 0) return;
+    DG_CHECK_GRID(swiglu_backward_blocks(m, n), 256);
     p.dh = static_cast<const uint16_t*>(dh.data()), p.lddh = dh.stride(0);
     p.q = static_cast<const uint8_t*>(q.data()), p.ldq = q.stride(0);
     p.sf = static_cast<const float*>(sf.data()), p.sf_sm = sf.stride(0), p.sf_sk = sf.stride(1);

@@ -854,7 +854,7 @@ bool takes_vectors(const RaggedGemmArgs& a) {
 template <int KIND>
 void launch_few_rows(const RaggedGemmArgs& a, int slots, int splits, hipStream_t stream) {
     const int64_t mb = row_blocks((RaggedKind)KIND, a, kFewRows), nb = ceil_div(a.n, 128);
-    DG_CHECK(mb * nb < ((int64_t)1 << 28));
+    DG_CHECK_GRID(mb * nb, 256);
     const RaggedLaunch l{(int)mb, (int)nb, slots, splits, takes_vectors(a)};
     hipLaunchKernelGGL(ragged_few_rows_kernel<KIND>, dim3((unsigned)(mb * nb), (unsigned)splits), dim3(256), 0, stream, a, l);
     DG_HIP_CHECK(hipGetLastError());
@@ -869,6 +869,7 @@ void launch_tiles(const RaggedGemmArgs& a, int slots, int splits, hipStream_t st
     int64_t blocks = KIND == kRaggedTN ? ceil_div(mb * nb, 8) * 8 * a.groups : tiles;
     // (a tail has at most 58% of a round's tiles, for each XCD by itself in TN)
     if (PART == 2) blocks = std::min<int64_t>(blocks, KIND == kRaggedTN ? std::max(slots / 8, 1) * 8 : slots) * 4;
+    DG_CHECK_GRID(blocks, WGM * WGN * 64);
     const RaggedLaunch l{(int)mb, (int)nb, slots, splits, takes_vectors(a)};
     hipLaunchKernelGGL((ragged_tile_kernel<KIND, BM, BN, WGM, WGN, PART, EIGHT>), dim3((unsigned)blocks, (unsigned)splits),
                        dim3(WGM * WGN * 64), 0, stream, a, l);
@@ -915,7 +916,7 @@ void launch_kind(const RaggedGemmArgs& a, const RaggedPlan& plan, float* ws, int
     RaggedGemmArgs whole = a;
     whole.d_split = part.d_split;
     const int64_t chunks = ceil_div(a.n, 1024);
-    DG_CHECK(rows * chunks < ((int64_t)1 << 31));
+    DG_CHECK_GRID(rows * chunks, 256);
     hipLaunchKernelGGL(ragged_join_kernel<KIND>, dim3((unsigned)(rows * chunks)), dim3(256), 0, stream, whole,
                        (const float*)ws, ld, plan.splits, (int)chunks);
     DG_HIP_CHECK(hipGetLastError());

@@ -37,6 +37,9 @@ private:
         if (!(cond)) throw ::dgm::Error(DG_ERR_INVALID, "Assertion", __FILE__, __LINE__, #cond); \
     } while (0)
 
+// Workgroups of a launch: all of its threads are counted in 32 bits.
+#define DG_CHECK_GRID(blocks, threads) DG_CHECK((int64_t)(blocks) * (threads) < ((int64_t)1 << 32))
+
 #define DG_UNSUPPORTED(reason) \
     throw ::dgm::Error(DG_ERR_UNSUPPORTED, "Unsupported", __FILE__, __LINE__, (reason))
 
@@ -335,7 +338,7 @@ struct RaggedPlan {
     int block, splits;
     int64_t workspace_bytes;
 };
-// slots: CUs. block, splits: 0 = by the sizes, otherwise as given (splits: 128 x 128 tiles).
+// slots: CUs. block, splits: 0 = by the sizes, otherwise as given (splits: of the smaller tiles).
 RaggedPlan plan_ragged_gemm(RaggedKind kind, const RaggedGemmArgs& args, int slots, int block, int splits);
 void launch_ragged_gemm(RaggedKind kind, const RaggedGemmArgs& args, const RaggedPlan& plan, float* workspace, int slots,
                         hipStream_t stream);
@@ -354,6 +357,13 @@ struct SwigluCheckpointArgs {
     int64_t ldx, ldh, ldq, sf_sm, sf_sk;
     int32_t m, n;
 };
+// Workgroups of the two kernels: a row and 512 columns a wave; rows by 1, 2 or 4 waves.
+inline int64_t swiglu_checkpoint_blocks(int64_t m, int64_t n) { return (m + 3) / 4 * ((n + 511) / 512); }
+inline int swiglu_backward_waves(int64_t n) { return n <= 512 ? 1 : n <= 1024 ? 2 : 4; }
+inline int64_t swiglu_backward_blocks(int64_t m, int64_t n) {
+    const int64_t rows = 4 / swiglu_backward_waves(n);
+    return (m + rows - 1) / rows;
+}
 void launch_swiglu_checkpoint(const SwigluCheckpointArgs& args, hipStream_t stream);
 struct SwigluBackwardArgs {
     const uint16_t* dh;        // bf16 [m, n]

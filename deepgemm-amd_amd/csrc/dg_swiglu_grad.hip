@@ -198,19 +198,18 @@ __global__ void __launch_bounds__(kSwThreads) swiglu_backward_kernel(const Swigl
 
 void launch_swiglu_checkpoint(const SwigluCheckpointArgs& a, hipStream_t stream) {
     if (a.m == 0 || a.n == 0) return;
-    const int64_t row_blocks = (a.m + 3) / 4, slices = (a.n + 511) / 512;
-    DG_CHECK(row_blocks * slices < ((int64_t)1 << 31));
-    hipLaunchKernelGGL(swiglu_checkpoint_kernel, dim3((unsigned)(row_blocks * slices)), dim3(kSwThreads), 0, stream, a,
-                       (int)slices);
+    const int64_t blocks = swiglu_checkpoint_blocks(a.m, a.n);
+    DG_CHECK_GRID(blocks, kSwThreads);
+    hipLaunchKernelGGL(swiglu_checkpoint_kernel, dim3((unsigned)blocks), dim3(kSwThreads), 0, stream, a, (a.n + 511) / 512);
     DG_HIP_CHECK(hipGetLastError());
 }
 
 void launch_swiglu_backward(const SwigluBackwardArgs& a, hipStream_t stream) {
     if (a.m == 0) return;
-    const int wpr = a.n <= 512 ? 1 : a.n <= 1024 ? 2 : 4;
-    const int64_t per = 4 / wpr;
-    const dim3 grid((unsigned)((a.m + per - 1) / per)), block(kSwThreads);
-    switch (wpr) {
+    const int64_t blocks = swiglu_backward_blocks(a.m, a.n);
+    DG_CHECK_GRID(blocks, kSwThreads);
+    const dim3 grid((unsigned)blocks), block(kSwThreads);
+    switch (swiglu_backward_waves(a.n)) {
         case 1: hipLaunchKernelGGL(swiglu_backward_kernel<1>, grid, block, 0, stream, a); break;
         case 2: hipLaunchKernelGGL(swiglu_backward_kernel<2>, grid, block, 0, stream, a); break;
         default: hipLaunchKernelGGL(swiglu_backward_kernel<4>, grid, block, 0, stream, a); break;

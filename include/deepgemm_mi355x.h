@@ -451,7 +451,9 @@ int dg_k_grouped_bf16_gemm_tn_ragged(const dg_tensor* a, const dg_tensor* b, con
  *   q            e4m3 [M, 2I] in 8-byte rows, the codes of x (not clamped)
  *   sf           f32 [M, 2 ceil(I/128)], any strides: power-of-two scales of 128 columns,
  *                of the gate half first; each half as dg_per_token_cast_to_fp8 (gran_k 128,
- *                use_ue8m0) gives it */
+ *                use_ue8m0) gives it
+ * ceil(M/4) ceil(I/512) < 2^24, in the backward pass also M < 2^24 where I > 1024: the
+ * threads of a launch are counted in 32 bits. */
 int dg_moe_swiglu_checkpoint(const dg_tensor* x, const dg_tensor* row_weights, const dg_tensor* row_layout,
                              float clamp_value, const dg_tensor* h, const dg_tensor* q, const dg_tensor* sf,
                              void* stream);

@@ -121,6 +121,12 @@ def test_swiglu_backward_refusals(key, value):
     rejected('dg_moe_swiglu_backward', *args.values())
 
 
+def test_swiglu_refuses_more_rows_than_a_launch_holds():
+    # a wave a row, four a workgroup of 256 threads: 2^26 rows are 2^32 threads
+    rejected('dg_moe_swiglu_checkpoint', *fwd(m=1 << 26).values(), match='<< 32')
+    rejected('dg_moe_swiglu_backward', *bwd(m=1 << 26).values(), match='<< 32')
+
+
 def test_python_entry_points_refuse_host_tensors():
     z = lambda *s: torch.zeros(s, dtype=torch.bfloat16)
     ends = torch.zeros(2, dtype=torch.int32)
