@@ -283,8 +283,11 @@ struct Operand {
         return s;
     }
     __device__ __forceinline__ void load(const Step& s, int i, uint32_t lds, int wave) const {
+        load(s, i, lds, wave, kRows * (int)pitch);
+    }
+    __device__ __forceinline__ void load(const Step& s, int i, uint32_t lds, int wave, int apart) const {
         const int seg = i * NW + wave;
-        dma16_buffer(s.rsrc, s.v + (uint32_t)(seg * kRows * (int)pitch), lds + seg * 1024);
+        dma16_buffer(s.rsrc, s.v + (uint32_t)(seg * apart), lds + seg * 1024);
     }
     __device__ __forceinline__ void issue(uint32_t lds, int wave) {
         const Step s = next();
@@ -408,8 +411,9 @@ struct CodeOperand {
 // (staged as BF16), 1 FP32, 2 BF16 with C (staged as FP32: the sum is rounded once).
 // Staged as FP32, 256 rows take two passes of 128 (64 of each wave row). C's values of a
 // pass are loaded before its sums are in LDS: their latency would otherwise come with
-// every access.
-template <int OUT, int BM, int BN, int WGM, int WGN, int SM, int SN>
+// every access. AHEAD: the first pass's are in the sums already, and the second's are loaded
+// before the first is stored (both passes' would not fit the registers).
+template <int OUT, int BM, int BN, int WGM, int WGN, bool AHEAD = false, int SM, int SN>
 __device__ __forceinline__ void store_tile(const RaggedGemmArgs& p, const f32x16 (&acc)[SM][SN], uint8_t* lds, int g, int m0,
                                            int m_end, int n0, int wave, int lane, bool vec) {
     constexpr int NW = WGM * WGN, SIZE = OUT == 1 ? 4 : 2, CPL = 16 / SIZE;   // columns of a lane
@@ -419,18 +423,20 @@ __device__ __forceinline__ void store_tile(const RaggedGemmArgs& p, const f32x16
     static_assert(T * NW * RPT * PASSES == BM, "whole accesses");
     const int lrow = lane & 31, lhalf = lane >> 5, wm = wave / WGN, wn = wave % WGN;
     const int c = n0 + lane % LPR * CPL;
-    const bool whole = vec && c + CPL <= p.n, add = OUT && p.c;
+    const bool whole = vec && c + CPL <= p.n;
     const int64_t d_tile = (int64_t)blockIdx.y * p.d_split + (int64_t)g * p.d_gs + n0, c_tile = (int64_t)g * p.c_gs + n0;
     const int64_t d_off = d_tile + (c - n0), c_off = c_tile + (c - n0);
+    uint4 cv[T];
 #pragma unroll
     for (int pass = 0; pass < PASSES; ++pass) {
-        // row of D of the pass's row r (which has PS slabs of each wave row)
-        auto row_of = [&](int r) { return m0 + (r / (PS * 32)) * (SM * 32) + pass * (PS * 32) + r % (PS * 32); };
-        uint4 cv[T];
-        if (add) {
+        const bool add = OUT && p.c && !(AHEAD && pass == 0);
+        // row of D of the row r of a pass (which has PS slabs of each wave row)
+        auto row_in = [&](int r, int of) { return m0 + (r / (PS * 32)) * (SM * 32) + of * (PS * 32) + r % (PS * 32); };
+        auto row_of = [&](int r) { return row_in(r, pass); };
+        if (AHEAD ? pass == 0 : add) {
 #pragma unroll
             for (int t = 0; t < T; ++t) {
-                const int r = row_of((t * NW + wave) * RPT + lane / LPR);
+                const int r = row_in((t * NW + wave) * RPT + lane / LPR, AHEAD ? PASSES - 1 : pass);
                 if (r < m_end && whole)
                     cv[t] = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.c) + (c_off + (int64_t)r * p.ldc) * SIZE);
             }
@@ -526,7 +532,7 @@ __device__ __forceinline__ void store_tile(const RaggedGemmArgs& p, const f32x16
 }
 
 // PART 2: 128 x 128 tiles, quarters of 256 x 256 ones.
-template <int KIND, int BM, int BN, int WGM, int WGN, int PART, int EIGHT>
+template <int KIND, int BM, int BN, int WGM, int WGN, int PART, int EIGHT, bool AHEAD>
 __global__ void __launch_bounds__(WGM * WGN * 64, WGM * WGN == 4 ? 2 : 1)
 ragged_tile_kernel(const RaggedGemmArgs p, const RaggedLaunch l) {
     constexpr int NW = WGM * WGN;
@@ -646,14 +652,55 @@ ragged_tile_kernel(const RaggedGemmArgs p, const RaggedLaunch l) {
         oc.convert(smem + c_next, smem + B_AT, reduced - (kb + 1) * BK, wave, lane);
         oc.issue(lds0 + c_next, wave);
     };
+    // FP32 C of 256 x 256 tiles: half of it on its way to LDS under the last three steps, in
+    // the places that the steps past the end would take, a 32-row slab for each: slab i of
+    // wave row e as A (i = 0) or B (i = 1) of step `steps + e`. A wave load is a row of the
+    // tile, whose 16-byte unit u goes to u ^ (row & 7). Otherwise every CU waits for all of
+    // its C at the same time as the others: 16384 rows to 8 x 4096 x 7168 1087 -> 1028 us, 5000
+    // to 8 x 4000 x 7000 674 -> 602. (A kernel of its own: without C the loop's
+    // conditions would cost 1 to 2%.)
+    static_assert(!AHEAD || (KIND == kRaggedTN && !EIGHT && BM == 256));
+    const bool ahead = AHEAD && p.c && p.out_f32 && l.vec && steps >= 3;
+    const int c_pitch = (int)p.ldc * 4;
+    auto c_slab = [&](int e, int i) {
+        const int row = m0 + e * WM + i * 32, rows = min(m_end - row, 32), cols = min(BN, p.n - n0);
+        const float* at = static_cast<const float*>(p.c) + (int64_t)g * p.c_gs + (int64_t)row * p.ldc + n0;
+        const uint32_t unit = (uint32_t)((lane ^ (wave & 7)) * 16);
+        return typename decltype(oa)::Step{descriptor(at, rows > 0 ? (rows - 1) * c_pitch + cols * 4 : 0),
+                                           unit < (uint32_t)cols * 4 ? unit : kPastEnd};
+    };
+    // The loads of A for step kb + 3 and of B for kb + 2; `apart`: bytes between wave loads.
+    auto next_a = [&](int kb, int& apart) {
+        auto s = oa.next();
+        apart = oa.kRows * (int)oa.pitch;
+        if constexpr (AHEAD)
+            if (ahead && kb + 3 >= steps && kb + 3 <= steps + 1) s = c_slab(kb + 3 - steps, 0), apart = c_pitch;
+        return s;
+    };
+    auto next_b = [&](int kb, int& apart) {
+        auto s = ob.next();
+        apart = ob.kRows * (int)ob.pitch;
+        if constexpr (AHEAD)
+            if (ahead && kb + 2 >= steps) s = c_slab(kb + 2 - steps, 1), apart = c_pitch;
+        return s;
+    };
     const bool computes = m0 + wm * WM < m_end;   // else a wave of rows past the group's: it loads and synchronises only
     if (!computes) {
         for (int kb = 0; kb < steps; ++kb) {
             asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-            if constexpr (EIGHT) next_codes(kb);
-            else ob.issue(lds0 + B_AT + (kb & 1) * B_STEP, wave);
+            if constexpr (EIGHT) {
+                next_codes(kb);
+            } else {
+                int apart = 0;
+                const auto s = next_b(kb, apart);
+#pragma unroll
+                for (int q = 0; q < B_LOADS; ++q) ob.load(s, q, lds0 + B_AT + (kb & 1) * B_STEP, wave, apart);
+            }
             wait_vmcnt_barrier<IN_FLIGHT>();
-            oa.issue(lds0 + a_cur, wave);
+            int apart = 0;
+            const auto s = next_a(kb, apart);
+#pragma unroll
+            for (int q = 0; q < A_LOADS; ++q) oa.load(s, q, lds0 + a_cur, wave, apart);
             advance();
         }
     } else
@@ -668,16 +715,17 @@ ragged_tile_kernel(const RaggedGemmArgs p, const RaggedLaunch l) {
             const bool last = i + 1 == SM;
             typename decltype(oa)::Step sa;
             typename decltype(ob)::Step sb;
+            int a_apart = 0, b_apart = 0;
             __builtin_amdgcn_sched_barrier(0);
             if (i == TOP) {
                 // every wave holds its B fragments of this step: their place is free
                 asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
                 if constexpr (EIGHT) next_codes(kb);
-                else sb = ob.next();
+                else sb = next_b(kb, b_apart);
             }
             if (last) {
                 wait_vmcnt_barrier<IN_FLIGHT>();
-                sa = oa.next();
+                sa = next_a(kb, a_apart);
             }
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -693,11 +741,11 @@ ragged_tile_kernel(const RaggedGemmArgs p, const RaggedLaunch l) {
                 if (last && n >= KS) op_b[n / KS - 1][n % KS] = fb.read(smem + b_next, n / KS - 1, n % KS);
                 if (!EIGHT && i == TOP) {
 #pragma unroll
-                    for (int q = n * B_LOADS / N; q < (n + 1) * B_LOADS / N; ++q) ob.load(sb, q, lds0 + b_cur, wave);
+                    for (int q = n * B_LOADS / N; q < (n + 1) * B_LOADS / N; ++q) ob.load(sb, q, lds0 + b_cur, wave, b_apart);
                 }
                 if (last) {
 #pragma unroll
-                    for (int q = n * A_LOADS / N; q < (n + 1) * A_LOADS / N; ++q) oa.load(sa, q, lds0 + a_cur, wave);
+                    for (int q = n * A_LOADS / N; q < (n + 1) * A_LOADS / N; ++q) oa.load(sa, q, lds0 + a_cur, wave, a_apart);
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
@@ -708,6 +756,29 @@ ragged_tile_kernel(const RaggedGemmArgs p, const RaggedLaunch l) {
     __builtin_amdgcn_sched_barrier(0);
     wait_vmcnt_barrier<0>();   // (loads of steps past the end wrote zeros to LDS)
     __builtin_amdgcn_sched_barrier(0);
+    if constexpr (AHEAD) {
+        if (ahead) {
+            if (computes) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const uint8_t* slab = smem + (i == 0 ? (steps + wm) % 3 * A_STEP : B_AT + ((steps + wm) & 1) * B_STEP);
+#pragma unroll
+                    for (int j = 0; j < SN; ++j)
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            const int unit = (wn * WN + j * 32 + 8 * q) / 4 + (lane >> 5);
+                            const f32x4 v = *reinterpret_cast<const f32x4*>(slab + (lane & 31) * (BN * 4) +
+                                                                            ((unit ^ (lane & 7)) << 4));
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) acc[i][j][4 * q + e] += v[e];
+                        }
+                }
+            }
+            __syncthreads();
+            store_tile<1, BM, BN, WGM, WGN, true>(p, acc, smem, g, m0, m_end, n0, wave, lane, true);
+            return;
+        }
+    }
     auto store = [&](auto out) {
         store_tile<decltype(out)::value, BM, BN, WGM, WGN>(p, acc, smem, KIND == kRaggedTN ? g : 0, m0, m_end, n0, wave, lane,
                                                            l.vec);
@@ -851,6 +922,11 @@ bool takes_vectors(const RaggedGemmArgs& a) {
            (!a.c || (reinterpret_cast<uintptr_t>(a.c) % 16 == 0 && a.ldc * size % 16 == 0 && a.c_gs * size % 16 == 0));
 }
 
+// Whether 256 x 256 tiles load FP32 C under their last products.
+bool loads_c_ahead(RaggedKind kind, const RaggedGemmArgs& a) {
+    return kind == kRaggedTN && !a.b_sf && a.c && a.out_f32 && takes_vectors(a);
+}
+
 template <int KIND>
 void launch_few_rows(const RaggedGemmArgs& a, int slots, int splits, hipStream_t stream) {
     const int64_t mb = row_blocks((RaggedKind)KIND, a, kFewRows), nb = ceil_div(a.n, 128);
@@ -860,7 +936,7 @@ void launch_few_rows(const RaggedGemmArgs& a, int slots, int splits, hipStream_t
     DG_HIP_CHECK(hipGetLastError());
 }
 
-template <int KIND, int BM, int BN, int WGM, int WGN, int PART, int EIGHT>
+template <int KIND, int BM, int BN, int WGM, int WGN, int PART, int EIGHT, bool AHEAD = false>
 void launch_tiles(const RaggedGemmArgs& a, int slots, int splits, hipStream_t stream) {
     constexpr int LIST = PART == 2 ? 2 : 1;
     const int64_t mb = row_blocks((RaggedKind)KIND, a, LIST * BM), nb = ceil_div(a.n, LIST * BN);
@@ -871,7 +947,7 @@ void launch_tiles(const RaggedGemmArgs& a, int slots, int splits, hipStream_t st
     if (PART == 2) blocks = std::min<int64_t>(blocks, KIND == kRaggedTN ? std::max(slots / 8, 1) * 8 : slots) * 4;
     DG_CHECK_GRID(blocks, WGM * WGN * 64);
     const RaggedLaunch l{(int)mb, (int)nb, slots, splits, takes_vectors(a)};
-    hipLaunchKernelGGL((ragged_tile_kernel<KIND, BM, BN, WGM, WGN, PART, EIGHT>), dim3((unsigned)blocks, (unsigned)splits),
+    hipLaunchKernelGGL((ragged_tile_kernel<KIND, BM, BN, WGM, WGN, PART, EIGHT, AHEAD>), dim3((unsigned)blocks, (unsigned)splits),
                        dim3(WGM * WGN * 64), 0, stream, a, l);
     DG_HIP_CHECK(hipGetLastError());
 }
@@ -890,12 +966,17 @@ bool has_tail(const RaggedGemmArgs& a, int slots) {
 template <int KIND, int EIGHT>
 void launch_kind(const RaggedGemmArgs& a, const RaggedPlan& plan, float* ws, int slots, hipStream_t stream) {
     if (plan.block == 256) {
-        if (KIND == kRaggedTN && !has_tail(a, slots)) {   // (known here: its tiles do not depend on group_ends)
-            launch_tiles<KIND, 256, 256, 2, 4, 0, EIGHT>(a, slots, 1, stream);
-        } else {
-            launch_tiles<KIND, 256, 256, 2, 4, 1, EIGHT>(a, slots, 1, stream);
-            launch_tiles<KIND, 128, 128, 2, 2, 2, EIGHT>(a, slots, 1, stream);
-        }
+        auto launch_256 = [&](auto ahead) {
+            if (KIND == kRaggedTN && !has_tail(a, slots)) {   // (known here: its tiles do not depend on group_ends)
+                launch_tiles<KIND, 256, 256, 2, 4, 0, EIGHT, decltype(ahead)::value>(a, slots, 1, stream);
+            } else {
+                launch_tiles<KIND, 256, 256, 2, 4, 1, EIGHT, decltype(ahead)::value>(a, slots, 1, stream);
+                launch_tiles<KIND, 128, 128, 2, 2, 2, EIGHT>(a, slots, 1, stream);
+            }
+        };
+        constexpr bool CAN = KIND == kRaggedTN && !EIGHT;
+        if (loads_c_ahead((RaggedKind)KIND, a)) launch_256(std::bool_constant<CAN>{});
+        else launch_256(std::false_type{});
         return;
     }
     auto launch = [&](const RaggedGemmArgs& args) {
@@ -933,9 +1014,10 @@ void launch_kind(const RaggedGemmArgs& a, const RaggedPlan& plan, float* ws, int
 // their steps (8 groups, 17648 x 517 x 7272 231 and 289 us). What it decides between, in us:
 // 256 x 256 against 128 x 128: NT, 4096 columns, K = 2048, 8 groups of 256 rows 38.1 and 35.5,
 //   of 512 61.9 and 67.2, 32 of 512 252 and 311; TN without C, 8 groups of 512 rows to 4096 x
-//   2048 133 and 114, of 1024 to 4096 x 4096 312 and 408; with C, 32 of 47 to 2048 x 2048 273
-//   and 202 (two small workgroups on a CU read C for one under the other's products), 8 of
-//   2048 to 4096 x 7168 1072 and 1207.
+//   2048 133 and 114, of 1024 to 4096 x 4096 312 and 408; with FP32 C, 32 of 47 to 2048 x 2048
+//   271 and 196 (two small workgroups on a CU read C for one under the other's products; two
+//   steps leave no time to load it ahead), 8 of 256 to 4096 x 2048 119 and 128, of 512 152 and
+//   164, to 2048 x 2048 76 and 68, of 2048 to 4096 x 7168 1028 and 1207.
 // 128 x 128 against 32 x 128: NT, 64 x 2048 x 2048 over 8 groups 17.8 and 13.3, 14 x 512 x
 //   8192 over 2, in pieces, 14.0 and 9.6; even where HBM bounds both.
 // Whole and in 4, 8 and 16 pieces: 32 x 128, 8 x 4096 x 7168 30.4, 15.4, 15.4, 16.8; 128 x
@@ -955,7 +1037,8 @@ RaggedPlan plan_ragged_gemm(RaggedKind kind, const RaggedGemmArgs& a, int slots,
     const double steps = (double)ceil_div(length, BK) * (tn && used > 1 ? 1.5 : 1.0), t256 = tiles(256), t128 = tiles(128);
     const bool few = !tn && (block == kFewRows || (block == 0 && a.rows <= kFewRows * used));
     const double alone = few ? 0.25 : eight ? 1.1 : 0.42, both = few ? 0.5 : eight ? 1.3 : 1.05;   // a step of 32 or 128 rows
-    const double store256 = !tn ? 0 : a.c ? 30 : a.out_f32 ? 15 : 9, store128 = !tn ? 0 : a.c ? 11.5 : a.out_f32 ? 7.7 : 5;
+    const bool ahead = loads_c_ahead(kind, a) && length > 2 * BK;   // (shorter groups have no steps to load C under)
+    const double store256 = !tn ? 0 : ahead ? 24 : a.c ? 30 : a.out_f32 ? 15 : 9, store128 = !tn ? 0 : a.c ? 11.5 : a.out_f32 ? 7.7 : 5;
     auto us128 = [&](double t, double n) {   // t tiles of n steps: whole rounds, and what is left for a CU
         const double per_cu = t / slots, whole = std::floor(per_cu / 2), rest = per_cu - 2 * whole;
         return whole * (n * both + store128) +

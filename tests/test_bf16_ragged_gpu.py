@@ -242,6 +242,30 @@ def test_k_grouped_large():
     k_grouped([700, 0, 1300, 65], 1030, 1544, eight=True, add=True)
 
 
+@pytest.mark.parametrize('m,n', [(1, 4), (33, 100), (129, 260), (161, 516), (300, 101)])
+def test_k_grouped_adds_c_to_the_sums(m, n):
+    """FP32 D with C is D without it plus C, to the bit, for groups of 0 to 11 steps, C's rows
+    as they lie (in place with a pitch, and apart with another one)."""
+    sizes = [128, 129, 64, 192, 193, 0, 257, 700]
+    seg = segments(sizes)
+    a, _ = matrix((seg[-1][1], m), 21)
+    b, _ = matrix((seg[-1][1], n), 22)
+    gen = torch.Generator(DEV).manual_seed(23)
+    wide = torch.randn((len(sizes), m + 3, -(-n // 4) * 4 + 8), generator=gen, device=DEV)
+    c = wide[:, :m, :n]
+    plain = torch.empty((len(sizes), m, n), device=DEV)
+    deep_gemm.k_grouped_bf16_gemm_tn_ragged(a, b, plain, ends_of(seg))
+    d = torch.full((len(sizes), m, -(-n // 4) * 4), 7.0, device=DEV)
+    deep_gemm.k_grouped_bf16_gemm_tn_ragged(a, b, d[..., :n], ends_of(seg), c=c)
+    torch.cuda.synchronize()
+    assert torch.equal(d[..., :n], plain + c) and (d[..., n:] == 7.0).all()
+    ref = wide.clone()
+    ref[:, :m, :n] += plain
+    deep_gemm.k_grouped_bf16_gemm_tn_ragged(a, b, c, ends_of(seg), c=c)
+    torch.cuda.synchronize()
+    assert torch.equal(wide, ref)
+
+
 def test_k_grouped_empty_calls():
     z = lambda *s: torch.zeros(s, dtype=torch.bfloat16, device=DEV)
     ends = torch.tensor([0, 0], dtype=torch.int32, device=DEV)
