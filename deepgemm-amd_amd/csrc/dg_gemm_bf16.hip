@@ -411,13 +411,14 @@ struct CodeOperand {
 // (staged as BF16), 1 FP32, 2 BF16 with C (staged as FP32: the sum is rounded once).
 // Staged as FP32, 256 rows take two passes of 128 (64 of each wave row). C's values of a
 // pass are loaded before its sums are in LDS: their latency would otherwise come with
-// every access. AHEAD: the first pass's are in the sums already, and the second's are loaded
-// before the first is stored (both passes' would not fit the registers).
-template <int OUT, int BM, int BN, int WGM, int WGN, bool AHEAD = false, int SM, int SN>
+// every access. AHEAD: four passes of 64 rows, the first AHEAD of which have C in the sums
+// already; C of the next two is loaded at once, of a fourth when the registers of the
+// second's are free.
+template <int OUT, int BM, int BN, int WGM, int WGN, int AHEAD = 0, int SM, int SN>
 __device__ __forceinline__ void store_tile(const RaggedGemmArgs& p, const f32x16 (&acc)[SM][SN], uint8_t* lds, int g, int m0,
                                            int m_end, int n0, int wave, int lane, bool vec) {
     constexpr int NW = WGM * WGN, SIZE = OUT == 1 ? 4 : 2, CPL = 16 / SIZE;   // columns of a lane
-    constexpr int PASSES = OUT && BM == 256 ? 2 : 1, PS = SM / PASSES;        // slabs of a pass
+    constexpr int PASSES = AHEAD ? 4 : OUT && BM == 256 ? 2 : 1, PS = SM / PASSES;        // slabs of a pass
     constexpr int STAGED = OUT ? 4 : 2, ROW_BYTES = BN * STAGED;
     constexpr int LPR = BN / CPL, RPT = 64 / LPR, T = BM / PASSES / (NW * RPT);   // lanes of a row, rows of an access
     static_assert(T * NW * RPT * PASSES == BM, "whole accesses");
@@ -426,19 +427,24 @@ __device__ __forceinline__ void store_tile(const RaggedGemmArgs& p, const f32x16
     const bool whole = vec && c + CPL <= p.n;
     const int64_t d_tile = (int64_t)blockIdx.y * p.d_split + (int64_t)g * p.d_gs + n0, c_tile = (int64_t)g * p.c_gs + n0;
     const int64_t d_off = d_tile + (c - n0), c_off = c_tile + (c - n0);
-    uint4 cv[T];
+    uint4 c_values[AHEAD ? PASSES : 1][T];
 #pragma unroll
     for (int pass = 0; pass < PASSES; ++pass) {
-        const bool add = OUT && p.c && !(AHEAD && pass == 0);
+        const bool add = OUT && p.c && pass >= AHEAD;
         // row of D of the row r of a pass (which has PS slabs of each wave row)
         auto row_in = [&](int r, int of) { return m0 + (r / (PS * 32)) * (SM * 32) + of * (PS * 32) + r % (PS * 32); };
         auto row_of = [&](int r) { return row_in(r, pass); };
-        if (AHEAD ? pass == 0 : add) {
+        uint4 (&cv)[T] = c_values[AHEAD ? pass : 0];
+#pragma unroll
+        for (int of = pass; of < PASSES; ++of) {
+            const int when = !AHEAD ? of : of < AHEAD + 2 ? 0 : of - 1;
+            if (of < AHEAD || pass != when || (!AHEAD && !add)) continue;
 #pragma unroll
             for (int t = 0; t < T; ++t) {
-                const int r = row_in((t * NW + wave) * RPT + lane / LPR, AHEAD ? PASSES - 1 : pass);
+                const int r = row_in((t * NW + wave) * RPT + lane / LPR, of);
                 if (r < m_end && whole)
-                    cv[t] = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.c) + (c_off + (int64_t)r * p.ldc) * SIZE);
+                    c_values[AHEAD ? of : 0][t] =
+                        *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.c) + (c_off + (int64_t)r * p.ldc) * SIZE);
             }
         }
         if (pass > 0) __syncthreads();
@@ -532,7 +538,7 @@ __device__ __forceinline__ void store_tile(const RaggedGemmArgs& p, const f32x16
 }
 
 // PART 2: 128 x 128 tiles, quarters of 256 x 256 ones.
-template <int KIND, int BM, int BN, int WGM, int WGN, int PART, int EIGHT, bool AHEAD>
+template <int KIND, int BM, int BN, int WGM, int WGN, int PART, int EIGHT, int AHEAD>
 __global__ void __launch_bounds__(WGM * WGN * 64, WGM * WGN == 4 ? 2 : 1)
 ragged_tile_kernel(const RaggedGemmArgs p, const RaggedLaunch l) {
     constexpr int NW = WGM * WGN;
@@ -652,15 +658,16 @@ ragged_tile_kernel(const RaggedGemmArgs p, const RaggedLaunch l) {
         oc.convert(smem + c_next, smem + B_AT, reduced - (kb + 1) * BK, wave, lane);
         oc.issue(lds0 + c_next, wave);
     };
-    // FP32 C of 256 x 256 tiles: half of it on its way to LDS under the last three steps, in
-    // the places that the steps past the end would take, a 32-row slab for each: slab i of
-    // wave row e as A (i = 0) or B (i = 1) of step `steps + e`. A wave load is a row of the
-    // tile, whose 16-byte unit u goes to u ^ (row & 7). Otherwise every CU waits for all of
-    // its C at the same time as the others: 16384 rows to 8 x 4096 x 7168 1087 -> 1028 us, 5000
-    // to 8 x 4000 x 7000 674 -> 602. (A kernel of its own: without C the loop's
-    // conditions would cost 1 to 2%.)
-    static_assert(!AHEAD || (KIND == kRaggedTN && !EIGHT && BM == 256));
-    const bool ahead = AHEAD && p.c && p.out_f32 && l.vec && steps >= 3;
+    // FP32 C of 256 x 256 tiles: half of it on its way to LDS under the last three steps (with
+    // codes, whose places are smaller, a quarter under the last two), in the places that
+    // the steps past the end would take, a 32-row slab for each: slab i of wave row e as
+    // A (i = 0) or B (i = 1) of step `steps + e`. A wave load is a row of the tile, whose
+    // 16-byte unit u goes to u ^ (row & 7). Otherwise every CU waits for all of its C at the
+    // same time as the others: 16384 rows to 8 x 4096 x 7168 1087 -> 1028 us, 5000 to 8 x 4000
+    // x 7000 664 -> 593, with codes 692 -> 618. (Kernels of their own: without C the
+    // loop's conditions would cost 1 to 2%.)
+    static_assert(!AHEAD || (KIND == kRaggedTN && BM == 256 && AHEAD == (EIGHT ? 1 : 2)));
+    const bool ahead = AHEAD && p.c && p.out_f32 && l.vec && steps >= A_SLOTS;
     const int c_pitch = (int)p.ldc * 4;
     auto c_slab = [&](int e, int i) {
         const int row = m0 + e * WM + i * 32, rows = min(m_end - row, 32), cols = min(BN, p.n - n0);
@@ -669,18 +676,18 @@ ragged_tile_kernel(const RaggedGemmArgs p, const RaggedLaunch l) {
         return typename decltype(oa)::Step{descriptor(at, rows > 0 ? (rows - 1) * c_pitch + cols * 4 : 0),
                                            unit < (uint32_t)cols * 4 ? unit : kPastEnd};
     };
-    // The loads of A for step kb + 3 and of B for kb + 2; `apart`: bytes between wave loads.
+    // The loads of A for step kb + A_SLOTS and of B for kb + 2; `apart`: bytes between wave loads.
     auto next_a = [&](int kb, int& apart) {
         auto s = oa.next();
         apart = oa.kRows * (int)oa.pitch;
-        if constexpr (AHEAD)
-            if (ahead && kb + 3 >= steps && kb + 3 <= steps + 1) s = c_slab(kb + 3 - steps, 0), apart = c_pitch;
+        if constexpr (AHEAD != 0)
+            if (ahead && kb + A_SLOTS >= steps && kb + A_SLOTS <= steps + 1) s = c_slab(kb + A_SLOTS - steps, 0), apart = c_pitch;
         return s;
     };
     auto next_b = [&](int kb, int& apart) {
         auto s = ob.next();
         apart = ob.kRows * (int)ob.pitch;
-        if constexpr (AHEAD)
+        if constexpr (AHEAD != 0)
             if (ahead && kb + 2 >= steps) s = c_slab(kb + 2 - steps, 1), apart = c_pitch;
         return s;
     };
@@ -756,12 +763,12 @@ ragged_tile_kernel(const RaggedGemmArgs p, const RaggedLaunch l) {
     __builtin_amdgcn_sched_barrier(0);
     wait_vmcnt_barrier<0>();   // (loads of steps past the end wrote zeros to LDS)
     __builtin_amdgcn_sched_barrier(0);
-    if constexpr (AHEAD) {
+    if constexpr (AHEAD != 0) {
         if (ahead) {
             if (computes) {
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const uint8_t* slab = smem + (i == 0 ? (steps + wm) % 3 * A_STEP : B_AT + ((steps + wm) & 1) * B_STEP);
+                for (int i = 0; i < AHEAD; ++i) {
+                    const uint8_t* slab = smem + (i == 0 ? (steps + wm) % A_SLOTS * A_STEP : B_AT + ((steps + wm) & 1) * B_STEP);
 #pragma unroll
                     for (int j = 0; j < SN; ++j)
 #pragma unroll
@@ -775,7 +782,7 @@ ragged_tile_kernel(const RaggedGemmArgs p, const RaggedLaunch l) {
                 }
             }
             __syncthreads();
-            store_tile<1, BM, BN, WGM, WGN, true>(p, acc, smem, g, m0, m_end, n0, wave, lane, true);
+            store_tile<1, BM, BN, WGM, WGN, AHEAD>(p, acc, smem, g, m0, m_end, n0, wave, lane, true);
             return;
         }
     }
@@ -924,7 +931,7 @@ bool takes_vectors(const RaggedGemmArgs& a) {
 
 // Whether 256 x 256 tiles load FP32 C under their last products.
 bool loads_c_ahead(RaggedKind kind, const RaggedGemmArgs& a) {
-    return kind == kRaggedTN && !a.b_sf && a.c && a.out_f32 && takes_vectors(a);
+    return kind == kRaggedTN && a.c && a.out_f32 && takes_vectors(a);
 }
 
 template <int KIND>
@@ -936,7 +943,7 @@ void launch_few_rows(const RaggedGemmArgs& a, int slots, int splits, hipStream_t
     DG_HIP_CHECK(hipGetLastError());
 }
 
-template <int KIND, int BM, int BN, int WGM, int WGN, int PART, int EIGHT, bool AHEAD = false>
+template <int KIND, int BM, int BN, int WGM, int WGN, int PART, int EIGHT, int AHEAD = 0>
 void launch_tiles(const RaggedGemmArgs& a, int slots, int splits, hipStream_t stream) {
     constexpr int LIST = PART == 2 ? 2 : 1;
     const int64_t mb = row_blocks((RaggedKind)KIND, a, LIST * BM), nb = ceil_div(a.n, LIST * BN);
@@ -974,9 +981,9 @@ void launch_kind(const RaggedGemmArgs& a, const RaggedPlan& plan, float* ws, int
                 launch_tiles<KIND, 128, 128, 2, 2, 2, EIGHT>(a, slots, 1, stream);
             }
         };
-        constexpr bool CAN = KIND == kRaggedTN && !EIGHT;
-        if (loads_c_ahead((RaggedKind)KIND, a)) launch_256(std::bool_constant<CAN>{});
-        else launch_256(std::false_type{});
+        constexpr int AHEAD = KIND == kRaggedTN ? (EIGHT ? 1 : 2) : 0;
+        if (loads_c_ahead((RaggedKind)KIND, a)) launch_256(std::integral_constant<int, AHEAD>{});
+        else launch_256(std::integral_constant<int, 0>{});
         return;
     }
     auto launch = [&](const RaggedGemmArgs& args) {

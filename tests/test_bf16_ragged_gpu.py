@@ -242,14 +242,20 @@ def test_k_grouped_large():
     k_grouped([700, 0, 1300, 65], 1030, 1544, eight=True, add=True)
 
 
+@pytest.mark.parametrize('eight', [False, True])
 @pytest.mark.parametrize('m,n', [(1, 4), (33, 100), (129, 260), (161, 516), (300, 101)])
-def test_k_grouped_adds_c_to_the_sums(m, n):
+def test_k_grouped_adds_c_to_the_sums(m, n, eight):
     """FP32 D with C is D without it plus C, to the bit, for groups of 0 to 11 steps, C's rows
     as they lie (in place with a pitch, and apart with another one)."""
     sizes = [128, 129, 64, 192, 193, 0, 257, 700]
     seg = segments(sizes)
     a, _ = matrix((seg[-1][1], m), 21)
-    b, _ = matrix((seg[-1][1], n), 22)
+    b, b64 = matrix((seg[-1][1], n), 22)
+    if eight:
+        q, sf, _ = cast8(b64)
+        codes = torch.full((seg[-1][1], -(-n // 8) * 8), 0x7F, dtype=torch.uint8)
+        codes[:, :n] = q.view(torch.uint8)
+        b = (codes.to(DEV).view(torch.float8_e4m3fn)[:, :n], sf.to(DEV))
     gen = torch.Generator(DEV).manual_seed(23)
     wide = torch.randn((len(sizes), m + 3, -(-n // 4) * 4 + 8), generator=gen, device=DEV)
     c = wide[:, :m, :n]
