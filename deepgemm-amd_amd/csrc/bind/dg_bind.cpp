@@ -103,11 +103,16 @@ struct Arg {
     const dg_tensor* get() const { return given ? &d : nullptr; }
 };
 
-// Integers; a pointer argument (a ctypes structure's address) is 0 for NULL.
-int64_t integer(PyObject* o) {
+// Integers (the ABI's are 32 bits wide: a longer one is refused, not cut); a pointer argument
+// (a ctypes structure's address) is 0 for NULL.
+int32_t integer(PyObject* o) {
     const long long v = PyLong_AsLongLong(o);
     if (v == -1 && PyErr_Occurred()) throw TypeMismatch("");
-    return v;
+    if (v != (int32_t)v) {
+        PyErr_Format(PyExc_OverflowError, "%lld does not fit a 32-bit integer", v);
+        throw TypeMismatch("");
+    }
+    return (int32_t)v;
 }
 float real(PyObject* o) {
     const double v = PyFloat_AsDouble(o);
@@ -186,7 +191,7 @@ PyObject* gemm_nt(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded(n, 10, [&] {
         const Arg ta(a[0]), sfa(a[1]), tb(a[2]), sfb(a[3]), d(a[4]), c(a[5], true);
         const auto* recipe = pointer<const dg_recipe>(a[6]);
-        const auto disable = (int32_t)integer(a[7]);
+        const int32_t disable = integer(a[7]);
         const auto* epilogue = pointer<const dg_epilogue>(a[8]);
         void* stream = pointer<void>(a[9]);
         // Decode-sized calls (at most 64 rows) split K over workgroups when given a
@@ -213,8 +218,8 @@ PyObject* contiguous(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded(n, 13, [&] {
         const Arg ta(a[0]), sfa(a[1]), tb(a[2]), sfb(a[3]), d(a[4]), layout(a[5]);
         return call(g_entry.contiguous, ta.get(), sfa.get(), tb.get(), sfb.get(), d.get(), layout.get(),
-                    pointer<const dg_recipe>(a[6]), (int32_t)integer(a[7]), (int32_t)integer(a[8]),
-                    (int32_t)integer(a[9]), (int32_t)integer(a[10]), pointer<const dg_epilogue>(a[11]),
+                    pointer<const dg_recipe>(a[6]), integer(a[7]), integer(a[8]),
+                    integer(a[9]), integer(a[10]), pointer<const dg_epilogue>(a[11]),
                     pointer<void>(a[12]));
     });
 }
@@ -224,7 +229,7 @@ PyObject* masked(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded(n, 11, [&] {
         const Arg ta(a[0]), sfa(a[1]), tb(a[2]), sfb(a[3]), d(a[4]), masked_m(a[5]);
         return call(g_entry.masked, ta.get(), sfa.get(), tb.get(), sfb.get(), d.get(), masked_m.get(),
-                    (int32_t)integer(a[6]), pointer<const dg_recipe>(a[7]), (int32_t)integer(a[8]),
+                    integer(a[6]), pointer<const dg_recipe>(a[7]), integer(a[8]),
                     pointer<const dg_epilogue>(a[9]), pointer<void>(a[10]));
     });
 }
@@ -233,7 +238,7 @@ PyObject* masked(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyObject* cast(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded(n, 6, [&] {
         const Arg x(a[0]), q(a[1]), sf(a[2]);
-        return call(g_entry.cast, x.get(), q.get(), sf.get(), (int32_t)integer(a[3]), (int32_t)integer(a[4]),
+        return call(g_entry.cast, x.get(), q.get(), sf.get(), integer(a[3]), integer(a[4]),
                     pointer<void>(a[5]));
     });
 }
@@ -244,8 +249,8 @@ PyObject* dispatch(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded(n, 14, [&] {
         const Arg x(a[0]), x_sf(a[1]), topk(a[2]), topk_w(a[3], true), out(a[7]), sf(a[8]), layout(a[9]), pos(a[10]),
             w(a[11], true), ws(a[12]);
-        return call(g_entry.dispatch, x.get(), x_sf.get(), topk.get(), topk_w.get(), (int32_t)integer(a[4]),
-                    (int32_t)integer(a[5]), (int32_t)integer(a[6]), out.get(), sf.get(), layout.get(), pos.get(),
+        return call(g_entry.dispatch, x.get(), x_sf.get(), topk.get(), topk_w.get(), integer(a[4]),
+                    integer(a[5]), integer(a[6]), out.get(), sf.get(), layout.get(), pos.get(),
                     w.get(), ws.get(), pointer<void>(a[13]));
     });
 }
@@ -255,7 +260,7 @@ PyObject* swiglu(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded(n, 8, [&] {
         const Arg x(a[0]), w(a[1], true), layout(a[2], true), q(a[4]), sf(a[5]);
         return call(g_entry.swiglu, x.get(), w.get(), layout.get(), real(a[3]), q.get(), sf.get(),
-                    (int32_t)integer(a[6]), pointer<void>(a[7]));
+                    integer(a[6]), pointer<void>(a[7]));
     });
 }
 
@@ -264,7 +269,7 @@ PyObject* contiguous_swiglu(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded(n, 12, [&] {
         const Arg ta(a[0]), sfa(a[1]), tb(a[2]), sfb(a[3]), layout(a[4]), w(a[5], true), q(a[7]), sf(a[8]);
         return call(g_entry.contiguous_swiglu, ta.get(), sfa.get(), tb.get(), sfb.get(), layout.get(), w.get(),
-                    real(a[6]), q.get(), sf.get(), (int32_t)integer(a[9]), (int32_t)integer(a[10]),
+                    real(a[6]), q.get(), sf.get(), integer(a[9]), integer(a[10]),
                     pointer<void>(a[11]));
     });
 }
@@ -274,7 +279,7 @@ PyObject* masked_swiglu(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded(n, 11, [&] {
         const Arg ta(a[0]), sfa(a[1]), tb(a[2]), sfb(a[3]), masked_m(a[4]), w(a[6], true), q(a[8]), sf(a[9]);
         return call(g_entry.masked_swiglu, ta.get(), sfa.get(), tb.get(), sfb.get(), masked_m.get(),
-                    (int32_t)integer(a[5]), w.get(), real(a[7]), q.get(), sf.get(), pointer<void>(a[10]));
+                    integer(a[5]), w.get(), real(a[7]), q.get(), sf.get(), pointer<void>(a[10]));
     });
 }
 
@@ -306,7 +311,7 @@ PyObject* m_grouped_ragged(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const bool nn = integer(a[0]) != 0;
         const auto entry = nn ? g_entry.ragged_nn : g_entry.ragged_nt;
         const Arg ta(a[1]), tb(a[2]), d(a[3]), ends(a[4]);
-        const int32_t alignment = (int32_t)integer(a[5]);
+        const int32_t alignment = integer(a[5]);
         void* stream = pointer<void>(a[6]);
         const bool fits = ta.d.ndim == 2 && tb.d.ndim == 3;
         const Workspace ws(nn, tensor(a[3]), fits ? ta.d.sizes[0] : 0, 0, tb.d.sizes[nn ? 2 : 1], ta.d.sizes[1], tb.d.sizes[0]);
@@ -318,7 +323,7 @@ PyObject* m_grouped_ragged(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyObject* k_grouped_ragged(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded(n, 8, [&] {
         const Arg ta(a[0]), tb(a[1]), sf(a[2], true), d(a[3]), ends(a[4]), c(a[5], true);
-        const int32_t alignment = (int32_t)integer(a[6]);
+        const int32_t alignment = integer(a[6]);
         void* stream = pointer<void>(a[7]);
         const bool fits = ta.d.ndim == 2 && tb.d.ndim == 2 && d.d.ndim == 3;
         const Workspace ws(sf.given ? 3 : 2, tensor(a[3]), ta.d.sizes[0], ta.d.sizes[1], fits ? tb.d.sizes[1] : 0, 0, d.d.sizes[0]);
