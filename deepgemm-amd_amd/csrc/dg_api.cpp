@@ -1601,7 +1601,10 @@ void check_group_ends(const View& t, int64_t groups, int32_t alignment) {
 }
 
 RaggedPlan ragged_plan(RaggedKind kind, const RaggedGemmArgs& a) {
-    return plan_ragged_gemm(kind, a, num_sms_now(), g_ragged_block.load(), g_ragged_splits.load());
+    const int slots = num_sms_now();
+    const RaggedPlan plan = plan_ragged_gemm(kind, a, slots, g_ragged_block.load(), g_ragged_splits.load());
+    check_ragged_launches(kind, a, plan, slots);
+    return plan;
 }
 
 // Plans and launches a call; without a workspace, or with one too small, the reduced axis

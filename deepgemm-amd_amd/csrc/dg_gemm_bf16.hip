@@ -934,10 +934,22 @@ bool loads_c_ahead(RaggedKind kind, const RaggedGemmArgs& a) {
     return kind == kRaggedTN && a.c && a.out_f32 && takes_vectors(a);
 }
 
+// Workgroups of a launch of `tile` x `tile` tiles (quarters: of its tail).
+int64_t tile_blocks(RaggedKind kind, const RaggedGemmArgs& a, int tile, bool quarters, int slots) {
+    const int64_t tiles = row_blocks(kind, a, tile) * ceil_div(a.n, tile);
+    const int64_t blocks = kind == kRaggedTN ? ceil_div(tiles, 8) * 8 * a.groups : tiles;
+    // (a tail has at most 58% of a round's tiles, for each XCD by itself in TN)
+    return quarters ? std::min<int64_t>(blocks, kind == kRaggedTN ? std::max(slots / 8, 1) * 8 : slots) * 4 : blocks;
+}
+
+// Workgroups of the join of a call's pieces: 1024 columns of a row each.
+int64_t join_blocks(RaggedKind kind, const RaggedGemmArgs& a) {
+    return (kind == kRaggedTN ? (int64_t)a.groups * a.m : a.rows) * ceil_div(a.n, 1024);
+}
+
 template <int KIND>
 void launch_few_rows(const RaggedGemmArgs& a, int slots, int splits, hipStream_t stream) {
     const int64_t mb = row_blocks((RaggedKind)KIND, a, kFewRows), nb = ceil_div(a.n, 128);
-    DG_CHECK_GRID(mb * nb, 256);
     const RaggedLaunch l{(int)mb, (int)nb, slots, splits, takes_vectors(a)};
     hipLaunchKernelGGL(ragged_few_rows_kernel<KIND>, dim3((unsigned)(mb * nb), (unsigned)splits), dim3(256), 0, stream, a, l);
     DG_HIP_CHECK(hipGetLastError());
@@ -947,12 +959,7 @@ template <int KIND, int BM, int BN, int WGM, int WGN, int PART, int EIGHT, int A
 void launch_tiles(const RaggedGemmArgs& a, int slots, int splits, hipStream_t stream) {
     constexpr int LIST = PART == 2 ? 2 : 1;
     const int64_t mb = row_blocks((RaggedKind)KIND, a, LIST * BM), nb = ceil_div(a.n, LIST * BN);
-    const int64_t tiles = mb * nb * (KIND == kRaggedTN ? a.groups : 1);
-    DG_CHECK(tiles < ((int64_t)1 << 28) && (KIND != kRaggedTN || ceil_div(mb * nb, 8) * 8 * a.groups < ((int64_t)1 << 30)));
-    int64_t blocks = KIND == kRaggedTN ? ceil_div(mb * nb, 8) * 8 * a.groups : tiles;
-    // (a tail has at most 58% of a round's tiles, for each XCD by itself in TN)
-    if (PART == 2) blocks = std::min<int64_t>(blocks, KIND == kRaggedTN ? std::max(slots / 8, 1) * 8 : slots) * 4;
-    DG_CHECK_GRID(blocks, WGM * WGN * 64);
+    const int64_t blocks = tile_blocks((RaggedKind)KIND, a, LIST * BM, PART == 2, slots);
     const RaggedLaunch l{(int)mb, (int)nb, slots, splits, takes_vectors(a)};
     hipLaunchKernelGGL((ragged_tile_kernel<KIND, BM, BN, WGM, WGN, PART, EIGHT, AHEAD>), dim3((unsigned)blocks, (unsigned)splits),
                        dim3(WGM * WGN * 64), 0, stream, a, l);
@@ -962,7 +969,6 @@ void launch_tiles(const RaggedGemmArgs& a, int slots, int splits, hipStream_t st
 // Whether a TN launch of 256 x 256 tiles leaves tiles to a second one.
 bool has_tail(const RaggedGemmArgs& a, int slots) {
     const int64_t per = ceil_div(a.m, 256) * ceil_div(a.n, 256);
-    DG_CHECK(per * a.groups < ((int64_t)1 << 28));
     if (!deals_eighths((int)per)) return tail_tiles((int)per * a.groups, slots) > 0;
     for (int x = 0; x < 8; ++x)
         if (tail_tiles((eighth_start(x + 1, (int)per) - eighth_start(x, (int)per)) * a.groups, std::max(slots / 8, 1)) > 0)
@@ -1003,10 +1009,8 @@ void launch_kind(const RaggedGemmArgs& a, const RaggedPlan& plan, float* ws, int
     launch(part);
     RaggedGemmArgs whole = a;
     whole.d_split = part.d_split;
-    const int64_t chunks = ceil_div(a.n, 1024);
-    DG_CHECK_GRID(rows * chunks, 256);
-    hipLaunchKernelGGL(ragged_join_kernel<KIND>, dim3((unsigned)(rows * chunks)), dim3(256), 0, stream, whole,
-                       (const float*)ws, ld, plan.splits, (int)chunks);
+    hipLaunchKernelGGL(ragged_join_kernel<KIND>, dim3((unsigned)join_blocks((RaggedKind)KIND, a)), dim3(256), 0, stream, whole,
+                       (const float*)ws, ld, plan.splits, (int)ceil_div(a.n, 1024));
     DG_HIP_CHECK(hipGetLastError());
 }
 
@@ -1069,6 +1073,18 @@ RaggedPlan plan_ragged_gemm(RaggedKind kind, const RaggedGemmArgs& a, int slots,
     }
     if (plan.splits > 1) plan.workspace_bytes = out_rows * ceil_div(a.n, 4) * 16 * plan.splits;
     return plan;
+}
+
+// (Every launch of a call is within these before the first of them is queued; they keep the
+// kernels' tile numbers within 32 bits too.)
+void check_ragged_launches(RaggedKind kind, const RaggedGemmArgs& a, const RaggedPlan& plan, int slots) {
+    if (plan.block == kFewRows) {
+        DG_CHECK_GRID(row_blocks(kind, a, kFewRows) * ceil_div(a.n, 128), 256);
+    } else {
+        DG_CHECK_GRID(tile_blocks(kind, a, plan.block, false, slots), plan.block * 2);
+        if (plan.block == 256) DG_CHECK_GRID(tile_blocks(kind, a, 256, true, slots), 256);
+    }
+    if (plan.splits > 1) DG_CHECK_GRID(join_blocks(kind, a), 256);
 }
 
 void launch_ragged_gemm(RaggedKind kind, const RaggedGemmArgs& a, const RaggedPlan& plan, float* ws, int slots,

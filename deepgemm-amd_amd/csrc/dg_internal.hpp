@@ -340,6 +340,8 @@ struct RaggedPlan {
 };
 // slots: CUs. block, splits: 0 = by the sizes, otherwise as given (splits: of the smaller tiles).
 RaggedPlan plan_ragged_gemm(RaggedKind kind, const RaggedGemmArgs& args, int slots, int block, int splits);
+// Throws if a launch of the plan would have 2^32 threads or more.
+void check_ragged_launches(RaggedKind kind, const RaggedGemmArgs& args, const RaggedPlan& plan, int slots);
 void launch_ragged_gemm(RaggedKind kind, const RaggedGemmArgs& args, const RaggedPlan& plan, float* workspace, int slots,
                         hipStream_t stream);
 

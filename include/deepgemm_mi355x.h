@@ -403,15 +403,19 @@ int dg_moe_combine(const dg_tensor* y, const dg_tensor* pos, const dg_tensor* to
  * segments back to back; dg_moe_dispatch's psum layout with the alignment it was made
  * with otherwise. At most 65536 groups, any of them empty. Ends past the rows that exist
  * are cut off there. The ends are read when the call runs: a captured graph follows them.
+ * A call one of whose launches would have 2^32 threads or more is refused before any is
+ * made: 2^24 workgroups of 32 x 128 or 128 x 128 tiles, 2^23 of 256 x 256 (M / T + min(G, M)
+ * row blocks of T rows for each column block in NT and NN; in TN the tiles of a group, up to
+ * a multiple of 8, G times). No such call has less than 4 GB of operands.
  * The reference's BF16 grouped GEMMs (csrc/apis/gemm.hpp) take segments padded to the MK
  * alignment and K-group sizes on the host. */
 
-/* Workspace bytes of a call of the three products (0: none; -1 on error): calls of few
- * tiles split the reduced axis over workgroups, the FP32 sums of its pieces go to the
- * workspace and a second kernel adds them in a fixed order. form 0: NT, 1: NN (rows, n,
- * k), 2: TN (rows, m, n), 3: TN with an 8-bit b. `workspace` below is a 1-D device tensor of that size, 16-byte
- * aligned, used until the call's kernels finish on `stream`; NULL, or one too small: the
- * axis stays whole. */
+/* Workspace bytes of a call of the three products (0: none; -1 on error, as for sizes that
+ * the call refuses): calls of few tiles split the reduced axis over workgroups, the FP32
+ * sums of its pieces go to the workspace and a second kernel adds them in a fixed order.
+ * form 0: NT, 1: NN (rows, n, k), 2: TN (rows, m, n), 3: TN with an 8-bit b. `workspace`
+ * below is a 1-D device tensor of that size, 16-byte aligned, used until the call's kernels
+ * finish on `stream`; NULL, or one too small: the axis stays whole. */
 int64_t dg_bf16_gemm_ragged_workspace_size(int32_t form, int64_t rows, int64_t m, int64_t n, int64_t k, int32_t groups);
 
 /* Forward: d[r] = a[r] @ b[g(r)]^T. Rows outside every group are left as they were.
