@@ -625,8 +625,8 @@ def k_grouped_bf16_gemm_tn_ragged(a: torch.Tensor, b, d: torch.Tensor, group_end
     the gradient of its weight, with a = the gradient of its output [R, M] and b = its input
     [R, N], in BF16 or as an 8-bit checkpoint (e4m3 [R, N], float32 [R, ceil(N / 128)]) such
     as per_token_cast_to_fp8(x, use_ue8m0=True) or moe_dispatch gives (values are rounded to
-    BF16 after their scale: exact where it is a power of two). d bf16 or float32 [G, M, N];
-    c None (zeros) or like d, also d itself. Groups without rows get c."""
+    BF16 after their scale: exact where it is a power of two, otherwise off by up to 2^-8 of
+    the value). d bf16 or float32 [G, M, N]; c None (zeros) or like d, also d itself. Groups without rows get c."""
     b_t, b_sf = _pair(b, 'b') if isinstance(b, (tuple, list)) else (b, None)
     _check(_bind.k_grouped_ragged(a, b_t, b_sf, d, group_ends, c, int(alignment), _raw_stream_of(d)))
 

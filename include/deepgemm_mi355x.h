@@ -437,7 +437,7 @@ int dg_m_grouped_bf16_gemm_nn_ragged(const dg_tensor* a, const dg_tensor* b, con
  *   b     bf16 [R, N] likewise (b_sf NULL), or an 8-bit checkpoint: e4m3 [R, N] in 8-byte
  *         rows with b_sf f32 [R, ceil(N/128)] (any strides), the 1 x 128 scales of
  *         dg_per_token_cast_to_fp8 or dg_moe_dispatch; a value is bf16(code * scale), exact
- *         where the scale is a power of two (use_ue8m0)
+ *         where the scale is a power of two (use_ue8m0), else off by up to 2^-8 of it
  *   d     bf16 or fp32 [G, M, N], unit stride along N
  *   c     NULL (zeros), or d's type and shape; may be d (accumulation in place)
  * A group without rows gets c. Sums in FP32. */
