@@ -61,7 +61,8 @@ __device__ __forceinline__ void group_rows(const int32_t* ends, int g, int rows,
 // leaves that round's tiles to a second launch, as four 128 x 128 quarters each: two
 // workgroups of those fit a CU, so 150 tiles' quarters take 1.2 rounds of 512, about 0.65
 // of a 256 x 256 round (PART 1 and 2; 0 is a launch by itself). Both launches work it
-// out alike, from the tiles that there are. 8 experts, 16384 x 4096 x 7168 (NT, 1088
+// out alike, from the tiles that there are; in NT and NN the host does not know them, and
+// the second one is made also where it has nothing to do (4 to 5 us). 8 experts, 16384 x 4096 x 7168 (NT, 1088
 // tiles, 4.25 rounds): 889 -> 861 us; 8192 x 7168 x 4096 (NN, 3.94 rounds, no tail) 437 and 439.
 __host__ __device__ __forceinline__ int tail_tiles(int tiles, int slots) {
     const int rest = tiles % slots;
@@ -804,8 +805,8 @@ ragged_tile_kernel(const RaggedGemmArgs p, const RaggedLaunch l) {
     else store(std::integral_constant<int, 0>{});
 }
 
-// NT and NN with at most 32 rows a group (decode): 32 x 128 tiles on four waves of 32 x 32, two
-// workgroups on a CU, which stream the weights from HBM. A step is 4 KB of A and 16 of B, so
+// NT and NN with at most 32 rows a group on average (decode): 32 x 128 tiles on four waves of 32 x
+// 32, two workgroups on a CU, which stream the weights from HBM. A step is 4 KB of A and 16 of B, so
 // four steps fit where a 128 x 128 tile has three and two, and a workgroup keeps 60 KB in
 // flight; one barrier a step (it certifies the next step's loads and frees this one's
 // place, whose fragments every wave holds).
@@ -1028,7 +1029,7 @@ void launch_kind(const RaggedGemmArgs& a, const RaggedPlan& plan, float* ws, int
 // The tile and the pieces of the reduced axis that take the fewest microseconds by measured
 // times: of a 64-element step of a round of tiles (256 x 256: 1.7; 128 x 128: 0.42 with one
 // workgroup on a CU, 1.05 with two; more with an 8-bit B; 32 x 128, for at most 32 rows a
-// group: 0.25 and 0.5), of a round's stores in TN, and of the pieces' sums on their way
+// group on average: 0.25 and 0.5), of a round's stores in TN, and of the pieces' sums on their way
 // through the workspace. 256 x 256 tiles have to fill 150 CUs, and in NT and NN win where
 // they are within 15%: with K long the 128 x 128 ones' operands, read twice as often, slow
 // their steps (8 groups, 17648 x 517 x 7272 231 and 289 us). What it decides between, in us:
@@ -1040,6 +1041,11 @@ void launch_kind(const RaggedGemmArgs& a, const RaggedPlan& plan, float* ws, int
 //   164, to 2048 x 2048 76 and 68, of 2048 to 4096 x 7168 1028 and 1207.
 // 128 x 128 against 32 x 128: NT, 64 x 2048 x 2048 over 8 groups 17.8 and 13.3, 14 x 512 x
 //   8192 over 2, in pieces, 14.0 and 9.6; even where HBM bounds both.
+// It knows the buffer's rows, not which of them are in groups (the ends are on the device), and
+// no group's own: 32 experts of 32 rows to 4096 x 2048 with FP32 C 367 in a buffer of their
+// 1024 rows, 522 in one of 8672, which a dispatch of 8192 ids takes (371 on 128 x 128); NT, 32
+// of 4096 x 7168, 2 rows each 303 and, in 4224 rows, 312; 1024 rows 109 all in one group (32 x
+// 128 tiles, each of which reads its weights; 65 on 128 x 128), 309 spread over them.
 // Whole and in 4, 8 and 16 pieces: 32 x 128, 8 x 4096 x 7168 30.4, 15.4, 15.4, 16.8; 128 x
 //   128, 256 x 2112 x 7168 50.9, 22.5, 24.2, 31.0, 512 x 4096 x 2048 19.5, 28.4, 41.9, 66.3,
 //   TN of 20000 rows to 104 x 504 124, 39.2, 24.8, 19.5.

@@ -332,7 +332,7 @@ struct RaggedGemmArgs {
     int64_t lda, ldb, ldd, ldc, b_gs, d_gs, c_gs, sf_sr, sf_sc;
     int64_t d_split;           // from one piece's sums to the next's, where the reduced axis is split
 };
-// Tiles of 256 x 256 or 128 x 128, and the pieces the reduced axis is split into (more than
+// Tiles of 256 x 256, 128 x 128 or 32 x 128 (block 32), and the pieces the reduced axis is split into (more than
 // one: FP32 sums of each piece in a workspace, then added in their order).
 struct RaggedPlan {
     int block, splits;

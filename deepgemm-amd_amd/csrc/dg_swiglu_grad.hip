@@ -15,7 +15,8 @@
 // 2 out), backward 10 (2 + 2 in, 4 + 2 out). A lane owns 8 columns: 16-byte accesses of the
 // BF16 rows, 8 of the codes. 16384 x 2048: forward 48.6 us (5.6 TB/s; the kernel alone 43),
 // backward 60.7 (5.6 TB/s), a copy of 1 GiB 5.1 TB/s; the exponentials and reciprocals hide
-// under it. 33 x 1024: 9 us a call, of which the kernel 4.
+// under it. (Columns in whole 512s; the forward pass gives a wave 512 of them, so at 768 a
+// quarter of the lanes have nothing to do, at 520 almost half.) 33 x 1024: 9 us a call, of which the kernel 4.
 #include <hip/hip_runtime.h>
 
 #include "dg_internal.hpp"
@@ -39,8 +40,9 @@ __device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
     return uint4{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7])};
 }
 
-// s = 1 / (1 + exp(-g)) by the hardware's exponential and reciprocal (a few units in the last
-// place of FP32; results are rounded to BF16); zero below g = -87.3, NaN for NaN.
+// s = 1 / (1 + exp(-g)) by the hardware's exponential and reciprocal: off by (|g| + 8) 2^-23 of
+// itself at most (the exponent is an FP32 product), beside BF16's half step of 2^-8 in all
+// results but dw; zero below g = -87.3, NaN for NaN.
 __device__ __forceinline__ float sigmoid(float g) { return __builtin_amdgcn_rcpf(1.0f + __expf(-g)); }
 
 // The power-of-two scale and the codes of one lane's 8 values, the group being the 16
