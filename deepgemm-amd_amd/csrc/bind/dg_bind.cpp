@@ -16,6 +16,7 @@
 #include <ATen/ATen.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <cstdint>
 #include <stdexcept>
 #include <string>
@@ -45,6 +46,14 @@ struct EntryPoints {
     decltype(&dg_bf16_gemm_ragged_workspace_size) ragged_workspace_size;
     decltype(&dg_moe_swiglu_checkpoint) swiglu_checkpoint;
     decltype(&dg_moe_swiglu_backward) swiglu_backward;
+    decltype(&dg_moe_dispatch_max_rows) dispatch_max_rows;
+    decltype(&dg_moe_dispatch_workspace_size) dispatch_workspace_size;
+    decltype(&dg_moe_dispatch_backward) dispatch_backward;
+    decltype(&dg_moe_combine_backward) combine_backward;
+    decltype(&dg_per_token_cast_to_fp4) cast4;
+    decltype(&dg_cast_back_from_fp4) cast_back4;
+    decltype(&dg_m_grouped_fp4_gemm_nt_ragged) ragged_fp4;
+    decltype(&dg_fp4_gemm_ragged_workspace_size) ragged_fp4_workspace_size;
 } g_entry{};
 
 struct TypeMismatch : std::runtime_error {
@@ -186,6 +195,18 @@ PyObject* init_bf16(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
+// init_rows(addresses of the entry points after those)
+PyObject* init_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded(n, 8, [&] {
+        auto set = [&](auto& entry, int i) { entry = reinterpret_cast<std::decay_t<decltype(entry)>>(pointer<void>(a[i])); };
+        set(g_entry.dispatch_max_rows, 0), set(g_entry.dispatch_workspace_size, 1);
+        set(g_entry.dispatch_backward, 2), set(g_entry.combine_backward, 3);
+        set(g_entry.cast4, 4), set(g_entry.cast_back4, 5);
+        set(g_entry.ragged_fp4, 6), set(g_entry.ragged_fp4_workspace_size, 7);
+        return 0;
+    });
+}
+
 // gemm_nt(a, sfa, b, sfb, d, c | None, recipe, disable_ue8m0_cast, epilogue, stream)
 PyObject* gemm_nt(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded(n, 10, [&] {
@@ -296,8 +317,9 @@ PyObject* combine(PyObject*, PyObject* const* a, Py_ssize_t n) {
 struct Workspace {
     at::Tensor tensor;
     Arg arg;
-    Workspace(int form, const at::Tensor& out, int64_t rows, int64_t m, int64_t n, int64_t k, int64_t groups) {
-        const int64_t bytes = out.is_cuda() ? g_entry.ragged_workspace_size(form, rows, m, n, k, (int32_t)groups) : 0;
+    Workspace(int form, const at::Tensor& out, int64_t rows, int64_t m, int64_t n, int64_t k, int64_t groups)
+        : Workspace(out, out.is_cuda() ? g_entry.ragged_workspace_size(form, rows, m, n, k, (int32_t)groups) : 0) {}
+    Workspace(const at::Tensor& out, int64_t bytes) {
         if (bytes <= 0) return;   // (-1: sizes that the call itself refuses)
         tensor = unlocked([&] { return at::empty({bytes}, out.options().dtype(at::kByte)); });
         arg.fill(tensor);
@@ -413,6 +435,146 @@ PyObject* swiglu_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
+// ragged_fp4(a, a_sf, b, b_sf, d, group_ends, alignment, stream)
+PyObject* ragged_fp4(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded(n, 8, [&] {
+        const Arg ta(a[0]), sa(a[1]), tb(a[2]), sb(a[3]), d(a[4]), ends(a[5]);
+        const int32_t alignment = integer(a[6]);
+        void* stream = pointer<void>(a[7]);
+        const bool fits = ta.d.ndim == 2 && tb.d.ndim == 3 && tensor(a[4]).is_cuda();
+        const Workspace ws(tensor(a[4]), fits ? g_entry.ragged_fp4_workspace_size(ta.d.sizes[0], tb.d.sizes[1], 2 * ta.d.sizes[1],
+                                                                                  (int32_t)tb.d.sizes[0]) : 0);
+        return call(g_entry.ragged_fp4, ta.get(), sa.get(), tb.get(), sb.get(), d.get(), ends.get(), alignment, ws.arg.get(),
+                    stream);
+    });
+}
+
+// cast4(x, gran_k, use_ue8m0, packed, stream) -> (status, q, sf)
+PyObject* cast4(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded_new(n, 5, [&]() -> NewTensors {
+        const Arg x(a[0]);
+        const int32_t gran = integer(a[1]), ue8m0 = integer(a[2]), packed = integer(a[3]);
+        void* stream = pointer<void>(a[4]);
+        const at::Tensor& like = tensor(a[0]);
+        const bool matrix = x.d.ndim == 2 && gran > 0;   // (otherwise the call refuses it)
+        const int64_t m = matrix ? x.d.sizes[0] : 0, cols = matrix ? x.d.sizes[1] : 0;
+        const int64_t groups = matrix ? (cols + gran - 1) / gran : 0;
+        at::Tensor q, sf;
+        unlocked([&] {
+            q = new_matrix(like, m, cols / 2, at::kChar);
+            sf = packed ? new_matrix(like, m, (groups + 3) / 4, at::kInt) : new_matrix(like, m, groups, at::kFloat);
+            return 0;
+        });
+        Arg dq, ds;
+        dq.fill(q), ds.fill(sf);
+        return {call(g_entry.cast4, x.get(), &dq.d, &ds.d, gran, ue8m0, stream), {q, sf}};
+    });
+}
+
+// cast_back4(q, sf, gran_k, bf16, stream) -> (status, y)
+PyObject* cast_back4(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded_new(n, 5, [&]() -> NewTensors {
+        const Arg q(a[0]), sf(a[1]);
+        const int32_t gran = integer(a[2]), bf16 = integer(a[3]);
+        void* stream = pointer<void>(a[4]);
+        const at::Tensor& like = tensor(a[0]);
+        const bool matrix = q.d.ndim == 2;
+        at::Tensor y;
+        unlocked([&] {
+            y = new_matrix(like, matrix ? q.d.sizes[0] : 0, matrix ? 2 * q.d.sizes[1] : 0, bf16 ? at::kBFloat16 : at::kFloat);
+            return 0;
+        });
+        Arg dy;
+        dy.fill(y);
+        return {call(g_entry.cast_back4, q.get(), sf.get(), &dy.d, gran, stream), {y}};
+    });
+}
+
+// dispatch_rows(x, x_sf | None, topk, topk_weights | None, experts, layout, alignment, max_m, out | None, out_sf | None,
+//               stream) -> (status, a, sf | None, grouped_layout, pos, row_weights | None)
+// (its five to seven allocations here, not in Python)
+PyObject* dispatch_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded_new(n, 11, [&]() -> NewTensors {
+        const Arg x(a[0]), x_sf(a[1], true), topk(a[2]), topk_w(a[3], true);
+        const int32_t experts = integer(a[4]), layout = integer(a[5]), alignment = integer(a[6]), max_m = integer(a[7]);
+        const bool given = a[8] != Py_None, given_sf = a[9] != Py_None;
+        at::Tensor out = given ? tensor(a[8]) : at::Tensor(), sf = given_sf ? tensor(a[9]) : at::Tensor();
+        void* stream = pointer<void>(a[10]);
+        const at::Tensor& like = tensor(a[0]);
+        if (x.d.ndim != 2 || topk.d.ndim != 2)
+            throw std::runtime_error("Assertion error (deep_gemm): x.dim() == 2 and topk_idx.dim() == 2");
+        const bool masked = layout == 2;
+        const int64_t t = x.d.sizes[0], k = topk.d.sizes[1];
+        int64_t rows = masked ? (int64_t)experts * max_m : g_entry.dispatch_max_rows(t, (int32_t)k, experts, alignment);
+        if (experts <= 0 || rows < 0)
+            throw std::runtime_error("Assertion error (deep_gemm): num_experts > 0, alignment > 0, max_m >= 0 and topk > 0");
+        if (given && !masked && out.dim() == 2) rows = out.size(0);   // (at least as many: the call checks it)
+        at::Tensor meta, pos, w, ws;
+        unlocked([&] {
+            auto fresh = [&](int64_t cols, at::ScalarType type) {
+                return masked ? at::empty({experts, max_m, cols}, like.options().dtype(type)) : new_matrix(like, rows, cols, type);
+            };
+            if (!given) out = fresh(x.d.sizes[1], like.scalar_type());
+            if (!given_sf && x_sf.given && x_sf.d.ndim == 2) sf = fresh(x_sf.d.sizes[1], x_sf.d.dtype == DG_I32 ? at::kInt : at::kFloat);
+            meta = at::empty({layout == 0 ? rows : (int64_t)experts}, like.options().dtype(at::kInt));
+            pos = new_matrix(like, t, k, at::kInt);
+            if (topk_w.given) w = at::empty({rows}, like.options().dtype(at::kFloat));
+            ws = at::empty({std::max<int64_t>(g_entry.dispatch_workspace_size(t, experts) / 4, 1)}, like.options().dtype(at::kInt));
+            return 0;
+        });
+        Arg da, dsf, dm, dp, dw, dws;
+        da.fill(out), dm.fill(meta), dp.fill(pos), dws.fill(ws);
+        if (sf.defined()) dsf.fill(sf), dsf.given = true;
+        if (w.defined()) dw.fill(w), dw.given = true;
+        const int32_t status = call(g_entry.dispatch, x.get(), x_sf.get(), topk.get(), topk_w.get(), experts, layout, alignment,
+                                    &da.d, dsf.get(), &dm.d, &dp.d, dw.get(), &dws.d, stream);
+        if (w.defined() && masked) w = w.view({experts, max_m});
+        return {status, {out, sf, meta, pos, w}};
+    });
+}
+
+// dispatch_backward(drows, pos, drow_weights | None, stream) -> (status, dx, d_topk_weights | None)
+PyObject* dispatch_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded_new(n, 4, [&]() -> NewTensors {
+        const Arg rows(a[0]), pos(a[1]), w(a[2], true);
+        void* stream = pointer<void>(a[3]);
+        const at::Tensor& like = tensor(a[0]);
+        const bool fits = rows.d.ndim >= 2 && pos.d.ndim == 2;   // (otherwise the call refuses them)
+        const int64_t t = fits ? pos.d.sizes[0] : 0, k = fits ? pos.d.sizes[1] : 0;
+        at::Tensor dx, dw;
+        unlocked([&] {
+            dx = new_matrix(like, t, fits ? rows.d.sizes[rows.d.ndim - 1] : 0, at::kBFloat16);
+            if (w.given) dw = new_matrix(like, t, k, at::kFloat);
+            return 0;
+        });
+        Arg ddx, ddw;
+        ddx.fill(dx);
+        if (w.given) ddw.fill(dw), ddw.given = true;
+        return {call(g_entry.dispatch_backward, rows.get(), pos.get(), w.get(), &ddx.d, ddw.get(), stream), {dx, dw}};
+    });
+}
+
+// combine_backward(dout, y, pos, topk_weights | None, dy | None, stream) -> (status, dy, d_topk_weights | None)
+PyObject* combine_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded_new(n, 6, [&]() -> NewTensors {
+        const Arg dout(a[0]), y(a[1]), pos(a[2]), w(a[3], true);
+        const bool given = a[4] != Py_None;
+        at::Tensor dy = given ? tensor(a[4]) : at::Tensor(), dw;
+        void* stream = pointer<void>(a[5]);
+        const at::Tensor& like = tensor(a[1]);
+        const bool fits = pos.d.ndim == 2;
+        unlocked([&] {
+            if (!given) dy = at::zeros(like.sizes(), like.options().dtype(at::kBFloat16));
+            if (w.given) dw = new_matrix(like, fits ? pos.d.sizes[0] : 0, fits ? pos.d.sizes[1] : 0, at::kFloat);
+            return 0;
+        });
+        Arg ddy, ddw;
+        ddy.fill(dy);
+        if (w.given) ddw.fill(dw), ddw.given = true;
+        return {call(g_entry.combine_backward, dout.get(), y.get(), pos.get(), w.get(), &ddy.d, ddw.get(), stream), {dy, dw}};
+    });
+}
+
 template <PyObject* (*F)(PyObject*, PyObject* const*, Py_ssize_t)>
 PyMethodDef method(const char* name) {
     return {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(F)), METH_FASTCALL, nullptr};
@@ -426,6 +588,10 @@ PyMethodDef g_methods[] = {method<init>("init"),     method<gemm_nt>("gemm_nt"),
                            method<k_grouped_ragged>("k_grouped_ragged"),
                            method<swiglu_checkpoint>("swiglu_checkpoint"),
                            method<swiglu_backward>("swiglu_backward"),
+                           method<init_rows>("init_rows"), method<ragged_fp4>("ragged_fp4"), method<cast4>("cast4"),
+                           method<cast_back4>("cast_back4"), method<dispatch_rows>("dispatch_rows"),
+                           method<dispatch_backward>("dispatch_backward"),
+                           method<combine_backward>("combine_backward"),
                            {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_dgbind", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};

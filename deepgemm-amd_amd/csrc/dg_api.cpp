@@ -1283,6 +1283,75 @@ void cast_impl(const dg_tensor* x_, const dg_tensor* q_, const dg_tensor* sf_, i
     t_last_config = buf;
 }
 
+// Every given tensor is on one device, which is made current for the launch (a null
+// stream, and a stream's kernels, belong to the current device) and set back after it.
+class OnDevice {
+public:
+    explicit OnDevice(int device) {
+        DG_HIP_CHECK(hipGetDevice(&before_));
+        if (before_ != device) {
+            DG_HIP_CHECK(hipSetDevice(device));
+            changed_ = true;
+        }
+    }
+    ~OnDevice() {
+        if (changed_) (void)hipSetDevice(before_);
+    }
+    OnDevice(const OnDevice&) = delete;
+    OnDevice& operator=(const OnDevice&) = delete;
+
+private:
+    int before_ = 0;
+    bool changed_ = false;
+};
+
+int one_device(std::initializer_list<const dg_tensor*> tensors) {
+    int device = -1;
+    for (const dg_tensor* t : tensors) {
+        if (t == nullptr) continue;
+        DG_CHECK(t->device >= 0);
+        if (device < 0) device = t->device;
+        DG_CHECK(t->device == device);   // all operands on one device
+    }
+    return device;
+}
+
+// The per-token casts to packed e2m1 (back = false: x BF16, read) and back (x f32 or BF16, written).
+void cast4_impl(bool back, const dg_tensor* x_, const dg_tensor* q_, const dg_tensor* sf_, int32_t gran_k, int32_t use_ue8m0,
+                hipStream_t stream) {
+    const View x = view(x_, back ? "y" : "x"), q = view(q_, "q"), sf = view(sf_, "sf");
+    DG_CHECK(x.dim() == 2 && q.dim() == 2 && sf.dim() == 2);
+    DG_CHECK((x.dtype() == DG_BF16 || (back && x.dtype() == DG_F32)) && q.dtype() == DG_I8);
+    DG_CHECK(gran_k == 32 || gran_k == 64 || gran_k == 128);
+    const int64_t m = x.size(0), n = x.size(1);
+    DG_CHECK(m < ((int64_t)1 << 30) && n < ((int64_t)1 << 27) && n % 2 == 0);
+    DG_CHECK(q.size(0) == m && q.size(1) == n / 2);
+    DG_CHECK((n <= 1 || x.stride(-1) == 1) && (n <= 2 || q.stride(-1) == 1));
+    const int64_t groups = ceil_div(n, (int64_t)gran_k);
+    const bool packed = sf.dtype() == DG_I32;
+    DG_CHECK(packed ? use_ue8m0 != 0 : sf.dtype() == DG_F32);
+    DG_CHECK(sf.size(0) == m && sf.size(1) == (packed ? ceil_div(groups, (int64_t)4) : groups));
+    const int device = one_device({x_, q_, sf_});
+    DG_CHECK_GRID(cast4_blocks(m, n), 256);
+    if (m == 0 || n == 0) return;
+    Cast4Args a{};
+    if (back) a.y = const_cast<void*>(x.data());
+    else a.x = static_cast<const uint16_t*>(x.data());
+    // (a single row's stride says nothing)
+    a.ldx = m > 1 ? x.stride(0) : align_up(n, 8), a.ldq = m > 1 ? q.stride(0) : align_up(n / 2, 4);
+    a.q = static_cast<uint8_t*>(const_cast<void*>(q.data()));
+    a.sf = const_cast<void*>(sf.data()), a.sf_sm = sf.stride(0), a.sf_sk = sf.stride(1);
+    a.m = (int32_t)m, a.n = (int32_t)n, a.gran = gran_k, a.ue8m0 = use_ue8m0 != 0, a.packed = packed;
+    a.out_f32 = x.dtype() == DG_F32;
+    const OnDevice on(device);
+    if (back) launch_cast_back4(a, stream);
+    else launch_cast4(a, stream);
+    char buf[160];
+    std::snprintf(buf, sizeof(buf), "%s kind=%s gran_k=%d ue8m0=%d m=%lld n=%lld", back ? "cast_back_from_fp4" : "per_token_cast_to_fp4",
+                  packed ? "packed" : "f32", gran_k, (int)a.ue8m0, (long long)m, (long long)n);
+    t_last_config = buf;
+}
+
 // ---------------------------------------------------------------- MoE plumbing
 // The layer around the grouped GEMMs on one GPU, as the reference's MoE baseline
 // runs it (tests/test_mega_moe.py:296-330): dispatch into the grouped layouts,
@@ -1306,15 +1375,26 @@ void moe_dispatch_impl(const dg_tensor* x_, const dg_tensor* x_sf_, const dg_ten
                        const dg_tensor* topk_w_, int32_t num_experts, int32_t layout, int32_t alignment,
                        const dg_tensor* a_, const dg_tensor* sf_, const dg_tensor* meta_, const dg_tensor* pos_,
                        const dg_tensor* w_out_, int32_t* workspace, int64_t workspace_ints, hipStream_t stream) {
-    const View x = view(x_, "x"), xs = view(x_sf_, "x_sf"), ti = view(topk_idx_, "topk_idx"), a = view(a_, "a"),
-               sf = view(sf_, "sf"), meta = view(meta_, "grouped_layout"), pos = view(pos_, "pos");
+    const View x = view(x_, "x"), ti = view(topk_idx_, "topk_idx"), a = view(a_, "a"),
+               meta = view(meta_, "grouped_layout"), pos = view(pos_, "pos");
+    // Rows are copied as bytes, scales as 4-byte words: e4m3 with f32 scales of 128 columns,
+    // packed e2m1 with words of four UE8M0 scales of 32, or BF16 without scales.
+    const bool bf16 = x.dtype() == DG_BF16, fp4 = x.dtype() == DG_I8;
+    DG_CHECK(bf16 || fp4 || x.dtype() == DG_E4M3);
+    if (bf16) DG_CHECK(x_sf_ == nullptr && sf_ == nullptr);   // BF16 rows have no scales
     DG_CHECK(layout == kMoeContiguous || layout == kMoePsum || layout == kMoeMasked);
     DG_CHECK(num_experts > 0 && num_experts <= kMoeMaxExperts);
-    DG_CHECK(x.dim() == 2 && x.dtype() == DG_E4M3 && x.stride(-1) == 1 && x.on_device());
-    const int64_t t = x.size(0), kdim = x.size(1), sfk = ceil_div(kdim, (int64_t)128);
-    DG_CHECK(kdim % 16 == 0 && t < ((int64_t)1 << 30));
+    DG_CHECK(x.dim() == 2 && x.stride(-1) == 1 && x.on_device());
+    const int64_t size = bf16 ? 2 : 1, t = x.size(0), cols = x.size(1), kdim = cols * size;
+    const int64_t sfk = bf16 ? 0 : ceil_div(fp4 ? 2 * cols : cols, (int64_t)128);
+    DG_CHECK(kdim % 16 == 0 && kdim < ((int64_t)1 << 30) && t < ((int64_t)1 << 30));
+    DG_CHECK_GRID((t + 3) / 4 + num_experts + 1, 256);
     check_vector_alignment(x, "x");
-    DG_CHECK(xs.dim() == 2 && xs.dtype() == DG_F32 && xs.on_device() && xs.size(0) == t && xs.size(1) == sfk);
+    const int sf_dtype = fp4 ? DG_I32 : DG_F32;
+    if (!bf16) {
+        const View xs = view(x_sf_, "x_sf");
+        DG_CHECK(xs.dim() == 2 && xs.dtype() == sf_dtype && xs.on_device() && xs.size(0) == t && xs.size(1) == sfk);
+    }
     DG_CHECK(ti.dim() == 2 && (ti.dtype() == DG_I32 || ti.dtype() == DG_I64) && ti.on_device() && ti.size(0) == t);
     const int64_t k = ti.size(1);
     DG_CHECK(k > 0 && k <= kMoeMaxTopk);
@@ -1324,19 +1404,24 @@ void moe_dispatch_impl(const dg_tensor* x_, const dg_tensor* x_sf_, const dg_ten
     }
     DG_CHECK(pos.dim() == 2 && pos.dtype() == DG_I32 && pos.on_device() && pos.size(0) == t && pos.size(1) == k &&
              contiguous_view(pos));
-    DG_CHECK(a.dtype() == DG_E4M3 && a.on_device() && a.stride(-1) == 1 && a.size(-1) == kdim);
-    DG_CHECK(sf.dtype() == DG_F32 && sf.on_device() && sf.size(-1) == sfk);
+    DG_CHECK(a.dim() == (layout == kMoeMasked ? 3 : 2));
+    DG_CHECK(a.dtype() == x.dtype() && a.on_device() && a.stride(-1) == 1 && a.size(-1) == cols);
+    if (!bf16) {
+        const View sf = view(sf_, "sf");
+        DG_CHECK(sf.dtype() == sf_dtype && sf.on_device() && sf.dim() == a.dim() && sf.size(-1) == sfk);
+    }
     DG_CHECK(meta.dtype() == DG_I32 && meta.on_device() && meta.dim() == 1 && contiguous_view(meta));
     check_vector_alignment(a, "a");
     int64_t cap = 0, max_m = 0;
     if (layout == kMoeMasked) {
-        DG_CHECK(a.dim() == 3 && a.size(0) == num_experts && sf.dim() == 3 && sf.size(0) == num_experts);
+        DG_CHECK(a.dim() == 3 && a.size(0) == num_experts && (bf16 || sf_->sizes[0] == num_experts));
         max_m = a.size(1);
-        DG_CHECK(max_m > 0 && sf.size(1) == max_m && meta.size(0) == num_experts);
+        DG_CHECK(max_m > 0 && (bf16 || sf_->sizes[1] == max_m) && meta.size(0) == num_experts);
         cap = num_experts * max_m;
     } else {
-        DG_CHECK(alignment > 0 && alignment % 16 == 0);
-        DG_CHECK(a.dim() == 2 && sf.dim() == 2 && sf.size(0) == a.size(0));
+        // (the padded products' block heights; the ragged ones take any)
+        DG_CHECK(alignment > 0 && alignment <= (1 << 20) && (alignment % 16 == 0 || x.dtype() != DG_E4M3));
+        DG_CHECK(a.dim() == 2 && (bf16 || sf_->sizes[0] == a.size(0)));
         cap = a.size(0);
         // every routing must fit: the segments take at most T*k + E*(alignment - 1) rows
         DG_CHECK(cap >= moe_worst_rows(t, k, num_experts, alignment));
@@ -1354,8 +1439,13 @@ void moe_dispatch_impl(const dg_tensor* x_, const dg_tensor* x_sf_, const dg_ten
     }
     DG_CHECK(workspace != nullptr && workspace_ints >= moe_dispatch_workspace_ints(t, num_experts));
     MoeDispatchArgs p{};
-    p.x = static_cast<const uint8_t*>(x.data()), p.ldx = x.stride(0);
-    p.x_sf = static_cast<const float*>(xs.data()), p.sf_st = xs.stride(0), p.sf_sk = xs.stride(1);
+    p.x = static_cast<const uint8_t*>(x.data()), p.ldx = x.stride(0) * size;
+    if (!bf16) {
+        const View xs{x_sf_}, sf{sf_};
+        p.x_sf = static_cast<const float*>(xs.data()), p.sf_st = xs.stride(0), p.sf_sk = xs.stride(1);
+        p.sf = static_cast<float*>(const_cast<void*>(sf.data()));
+        p.sf_sm = sf.stride(-2), p.sf_sk_o = sf.stride(-1), p.sf_gs = sf.dim() == 3 ? sf.stride(0) : 0;
+    }
     p.topk = ti.data(), p.topk_i64 = ti.dtype() == DG_I64, p.topk_st = ti.stride(0), p.topk_sk = ti.stride(1);
     if (topk_w_) {
         const View tw = view(topk_w_, "topk_weights");
@@ -1365,19 +1455,18 @@ void moe_dispatch_impl(const dg_tensor* x_, const dg_tensor* x_sf_, const dg_ten
     p.num_experts = num_experts, p.layout = layout, p.alignment = alignment, p.max_m = (int32_t)max_m;
     p.chunks = moe_dispatch_chunks(t);
     p.a = static_cast<uint8_t*>(const_cast<void*>(a.data()));
-    p.lda = a.stride(-2), p.a_gs = a.dim() == 3 ? a.stride(0) : 0;
-    p.sf = static_cast<float*>(const_cast<void*>(sf.data()));
-    p.sf_sm = sf.stride(-2), p.sf_sk_o = sf.stride(-1), p.sf_gs = sf.dim() == 3 ? sf.stride(0) : 0;
+    p.lda = a.stride(-2) * size, p.a_gs = a.dim() == 3 ? a.stride(0) * size : 0;
     p.meta = static_cast<int32_t*>(const_cast<void*>(meta.data()));
     p.cap_rows = cap;
     p.w_out = w_out;
     p.pos = static_cast<int32_t*>(const_cast<void*>(pos.data()));
     p.ws = workspace;
+    const OnDevice on(one_device({x_, x_sf_, topk_idx_, topk_w_, a_, sf_, meta_, pos_, w_out_}));
     launch_moe_dispatch(p, stream);
     char buf[160];
-    std::snprintf(buf, sizeof(buf), "moe_dispatch layout=%s experts=%d t=%lld k=%lld kdim=%lld",
-                  layout == kMoeContiguous ? "contiguous" : layout == kMoePsum ? "psum" : "masked", num_experts,
-                  (long long)t, (long long)k, (long long)kdim);
+    std::snprintf(buf, sizeof(buf), "moe_dispatch%s layout=%s experts=%d t=%lld k=%lld kdim=%lld",
+                  bf16 ? " x=bf16" : fp4 ? " x=e2m1" : "", layout == kMoeContiguous ? "contiguous" : layout == kMoePsum ? "psum" : "masked", num_experts,
+                  (long long)t, (long long)k, (long long)(fp4 ? 2 * cols : cols));
     t_last_config = buf;
 }
 
@@ -1447,6 +1536,98 @@ void moe_combine_impl(const dg_tensor* y_, const dg_tensor* pos_, const dg_tenso
     launch_moe_combine(p, stream);
     char buf[128];
     std::snprintf(buf, sizeof(buf), "moe_combine t=%lld k=%lld n=%lld", (long long)t, (long long)k, (long long)n);
+    t_last_config = buf;
+}
+
+// Expert rows [R, n] or [E, max_m, n] as the gradients' kernels address them.
+struct ExpertRows {
+    int64_t ld, gs, rows;
+    int32_t max_m;
+};
+ExpertRows expert_rows(const dg_tensor* t_, const char* name, int64_t n) {
+    const View t = view(t_, name);
+    DG_CHECK(t.dim() == 2 || t.dim() == 3);
+    DG_CHECK(t.dtype() == DG_BF16 && t.on_device() && t.size(-1) == n);
+    for (int i = 0; i < t.dim(); ++i) DG_CHECK(t.size(i) >= 0 && t.size(i) < ((int64_t)1 << 30));
+    DG_CHECK(n <= 1 || t.stride(-1) == 1);
+    DG_CHECK(t.size(-2) <= 1 || t.stride(-2) >= n);
+    if (t.dim() == 3 && t.size(0) > 1) DG_CHECK(t.stride(0) >= (t.size(1) > 0 ? (t.size(1) - 1) * t.stride(1) + n : 0));
+    const int64_t rows = t.dim() == 3 ? t.size(0) * t.size(1) : t.size(0);
+    DG_CHECK(rows < ((int64_t)1 << 31));
+    if (rows > 0 && n > 0) check_vector_alignment(t, name);
+    return {t.size(-2) > 1 ? t.stride(-2) : 0, t.dim() == 3 && t.size(0) > 1 ? t.stride(0) : 0, rows,
+            t.dim() == 3 ? (int32_t)t.size(1) : 0};
+}
+
+// pos and the token rows of both gradients, and what they share of the arguments.
+MoeGradArgs moe_grad_args(const dg_tensor* tokens_, const char* name, const dg_tensor* pos_) {
+    const View x = view(tokens_, name), pos = view(pos_, "pos");
+    DG_CHECK(x.dim() == 2 && x.dtype() == DG_BF16 && x.on_device());
+    DG_CHECK(pos.dim() == 2 && pos.dtype() == DG_I32 && pos.on_device() && contiguous_view(pos));
+    const int64_t t = x.size(0), n = x.size(1), k = pos.size(1);
+    DG_CHECK(pos.size(0) == t && k > 0 && k <= kMoeMaxTopk);
+    DG_CHECK(t < ((int64_t)1 << 30) && n < ((int64_t)1 << 30) && n % 8 == 0);
+    DG_CHECK((n <= 1 || x.stride(1) == 1) && (t <= 1 || x.stride(0) >= n));
+    if (t > 0 && n > 0) check_vector_alignment(x, name);
+    MoeGradArgs p{};
+    p.tokens = static_cast<uint16_t*>(const_cast<void*>(x.data())), p.ldt = x.stride(0);
+    p.pos = static_cast<const int32_t*>(pos.data());
+    p.t = (int32_t)t, p.k = (int32_t)k, p.n = (int32_t)n;
+    return p;
+}
+
+float* moe_weight_gradient(const dg_tensor* dw_, int64_t t, int64_t k) {
+    const View dw = view(dw_, "d_topk_weights");
+    DG_CHECK(dw.dim() == 2 && dw.dtype() == DG_F32 && dw.on_device() && dw.size(0) == t && dw.size(1) == k && contiguous_view(dw));
+    return static_cast<float*>(const_cast<void*>(dw.data()));
+}
+
+void dispatch_backward_impl(const dg_tensor* drows_, const dg_tensor* pos_, const dg_tensor* drow_w_, const dg_tensor* dx_,
+                            const dg_tensor* dw_, hipStream_t stream) {
+    MoeGradArgs p = moe_grad_args(dx_, "dx", pos_);
+    const ExpertRows r = expert_rows(drows_, "drows", p.n);
+    p.rows_in = static_cast<const uint16_t*>(drows_->data), p.ld_in = r.ld, p.gs_in = r.gs, p.rows = r.rows, p.max_m = r.max_m;
+    DG_CHECK((drow_w_ == nullptr) == (dw_ == nullptr));   // the weights' gradient goes with their rows'
+    if (drow_w_) {
+        const View w = view(drow_w_, "drow_weights");
+        DG_CHECK(w.dtype() == DG_F32 && w.on_device() && contiguous_view(w));
+        int64_t numel = 1;
+        for (int i = 0; i < w.dim(); ++i) numel *= w.size(i);
+        DG_CHECK(numel == r.rows);
+        p.w = static_cast<const float*>(w.data());
+        p.dw = moe_weight_gradient(dw_, p.t, p.k);
+    }
+    const int device = one_device({drows_, pos_, drow_w_, dx_, dw_});
+    DG_CHECK_GRID(dispatch_backward_blocks(p.t, p.n), 256);
+    const OnDevice on(device);
+    launch_dispatch_backward(p, stream);
+    char buf[96];
+    std::snprintf(buf, sizeof(buf), "moe_dispatch_backward t=%d k=%d n=%d", p.t, p.k, p.n);
+    t_last_config = buf;
+}
+
+void combine_backward_impl(const dg_tensor* dout_, const dg_tensor* y_, const dg_tensor* pos_, const dg_tensor* w_,
+                           const dg_tensor* dy_, const dg_tensor* dw_, hipStream_t stream) {
+    MoeGradArgs p = moe_grad_args(dout_, "dout", pos_);
+    const ExpertRows r = expert_rows(dy_, "dy", p.n);
+    p.rows_out = static_cast<uint16_t*>(dy_->data), p.ld_out = r.ld, p.gs_out = r.gs, p.rows = r.rows, p.max_m = r.max_m;
+    DG_CHECK((w_ == nullptr) == (dw_ == nullptr));   // a gradient for weights that are given
+    if (w_) {
+        const View w = view(w_, "topk_weights");
+        DG_CHECK(w.dim() == 2 && w.dtype() == DG_F32 && w.on_device() && w.size(0) == p.t && w.size(1) == p.k);
+        const ExpertRows y = expert_rows(y_, "y", p.n);
+        DG_CHECK(y_->ndim == dy_->ndim && y.rows == r.rows && y.max_m == r.max_m);
+        if (y_->data == dy_->data) DG_CHECK(y.ld == r.ld && y.gs == r.gs);   // in place: the same elements
+        p.rows_in = static_cast<const uint16_t*>(y_->data), p.ld_in = y.ld, p.gs_in = y.gs;
+        p.w = static_cast<const float*>(w.data()), p.w_st = w.stride(0), p.w_sk = w.stride(1);
+        p.dw = moe_weight_gradient(dw_, p.t, p.k);
+    }
+    const int device = one_device({dout_, y_, pos_, w_, dy_, dw_});
+    DG_CHECK_GRID(combine_backward_blocks(p.t, p.n), 256);
+    const OnDevice on(device);
+    launch_combine_backward(p, stream);
+    char buf[96];
+    std::snprintf(buf, sizeof(buf), "moe_combine_backward t=%d k=%d n=%d weights=%d", p.t, p.k, p.n, w_ != nullptr);
     t_last_config = buf;
 }
 
@@ -1534,39 +1715,6 @@ void k_grouped_impl(const dg_tensor* a_, const dg_tensor* sfa_, const dg_tensor*
 
 // ---------------------------------------------------------------- BF16 expert products, SwiGLU checkpoints
 
-// Every given tensor is on one device, which is made current for the launch (a null
-// stream, and a stream's kernels, belong to the current device) and set back after it.
-class OnDevice {
-public:
-    explicit OnDevice(int device) {
-        DG_HIP_CHECK(hipGetDevice(&before_));
-        if (before_ != device) {
-            DG_HIP_CHECK(hipSetDevice(device));
-            changed_ = true;
-        }
-    }
-    ~OnDevice() {
-        if (changed_) (void)hipSetDevice(before_);
-    }
-    OnDevice(const OnDevice&) = delete;
-    OnDevice& operator=(const OnDevice&) = delete;
-
-private:
-    int before_ = 0;
-    bool changed_ = false;
-};
-
-int one_device(std::initializer_list<const dg_tensor*> tensors) {
-    int device = -1;
-    for (const dg_tensor* t : tensors) {
-        if (t == nullptr) continue;
-        DG_CHECK(t->device >= 0);
-        if (device < 0) device = t->device;
-        DG_CHECK(t->device == device);   // all operands on one device
-    }
-    return device;
-}
-
 void check_sizes(const View& t) {
     for (int i = 0; i < t.dim(); ++i) DG_CHECK(t.size(i) >= 0 && t.size(i) < ((int64_t)1 << 30));
 }
@@ -1607,21 +1755,26 @@ RaggedPlan ragged_plan(RaggedKind kind, const RaggedGemmArgs& a) {
     return plan;
 }
 
+// The workspace of a plan that splits the reduced axis, or null, if it is not given or too small:
+// the axis stays whole then.
+float* ragged_workspace(RaggedPlan& plan, const dg_tensor* ws_) {
+    if (plan.splits <= 1) return nullptr;
+    if (ws_ != nullptr) {
+        const View w = view(ws_, "workspace");
+        DG_CHECK(w.on_device() && w.dim() == 1 && contiguous_view(w));
+        DG_CHECK(reinterpret_cast<uintptr_t>(w.data()) % 16 == 0);
+        if (w.size(0) * elem_size(w.dtype()) >= plan.workspace_bytes)
+            return static_cast<float*>(const_cast<void*>(w.data()));
+    }
+    plan.splits = 1, plan.workspace_bytes = 0;
+    return nullptr;
+}
+
 // Plans and launches a call; without a workspace, or with one too small, the reduced axis
 // stays whole.
 void run_ragged(const char* name, RaggedKind kind, const RaggedGemmArgs& a, const dg_tensor* ws_, hipStream_t stream) {
     RaggedPlan plan = ragged_plan(kind, a);
-    float* ws = nullptr;
-    if (plan.splits > 1) {
-        if (ws_ != nullptr) {
-            const View w = view(ws_, "workspace");
-            DG_CHECK(w.on_device() && w.dim() == 1 && contiguous_view(w));
-            DG_CHECK(reinterpret_cast<uintptr_t>(w.data()) % 16 == 0);
-            if (w.size(0) * elem_size(w.dtype()) >= plan.workspace_bytes)
-                ws = static_cast<float*>(const_cast<void*>(w.data()));
-        }
-        if (ws == nullptr) plan.splits = 1, plan.workspace_bytes = 0;
-    }
+    float* ws = ragged_workspace(plan, ws_);
     launch_ragged_gemm(kind, a, plan, ws, num_sms_now(), stream);
     char buf[160];
     std::snprintf(buf, sizeof(buf), "%s block=%d splits=%d rows=%d m=%d n=%d k=%d groups=%d", name, plan.block, plan.splits,
@@ -1655,6 +1808,64 @@ void m_grouped_ragged_impl(RaggedKind kind, const dg_tensor* a_, const dg_tensor
     p.out_f32 = d.dtype() == DG_F32;
     const OnDevice on(device);
     run_ragged(kind == kRaggedNT ? "bf16_ragged_nt" : "bf16_ragged_nn", kind, p, ws_, stream);
+}
+
+// Scales of a 4-bit operand of `k` elements a row: words of four UE8M0 bytes, [.., rows, ceil(k / 128)],
+// any strides within the kernels' 32-bit offsets (256 rows and a word).
+void check_fp4_scales(const View& sf, int dims, int64_t groups, int64_t rows, int64_t k) {
+    DG_CHECK(sf.dim() == dims && sf.dtype() == DG_I32 && sf.on_device());
+    DG_CHECK((dims == 2 || sf.size(0) == groups) && sf.size(-2) == rows && sf.size(-1) == ceil_div(k, (int64_t)128));
+    DG_CHECK(sf.size(-2) <= 1 || (sf.stride(-2) >= 0 && sf.stride(-2) <= ((int64_t)1 << 20)));
+    DG_CHECK(sf.size(-1) <= 1 || (sf.stride(-1) >= 0 && sf.stride(-1) < ((int64_t)1 << 28)));
+    if (has_elements(sf)) DG_CHECK(reinterpret_cast<uintptr_t>(sf.data()) % 4 == 0);
+}
+
+RaggedPlan ragged_fp4_plan(const RaggedFp4Args& a) {
+    const RaggedPlan plan = plan_ragged_fp4(a, num_sms_now(), g_ragged_block.load(), g_ragged_splits.load());
+    check_ragged_fp4_launches(a, plan);
+    return plan;
+}
+
+void ragged_fp4_impl(const dg_tensor* a_, const dg_tensor* a_sf_, const dg_tensor* b_, const dg_tensor* b_sf_,
+                     const dg_tensor* d_, const dg_tensor* ends_, int32_t alignment, const dg_tensor* ws_,
+                     hipStream_t stream) {
+    const View a = view(a_, "a"), a_sf = view(a_sf_, "a_sf"), b = view(b_, "b"), b_sf = view(b_sf_, "b_sf"), d = view(d_, "d"),
+               ends = view(ends_, "group_ends");
+    check_ragged_matrix(a, 2);
+    check_ragged_matrix(b, 3);
+    check_ragged_matrix(d, 2);
+    DG_CHECK(a.dtype() == DG_I8 && b.dtype() == DG_I8);   // packed e2m1
+    DG_CHECK(d.dtype() == DG_BF16 || d.dtype() == DG_F32);
+    const int64_t rows = a.size(0), k = 2 * a.size(1), groups = b.size(0), n = b.size(1);
+    DG_CHECK(b.size(2) * 2 == k);
+    DG_CHECK(d.size(0) == rows && d.size(1) == n);
+    DG_CHECK(k % 32 == 0);   // whole scales
+    check_fp4_scales(a_sf, 2, 0, rows, k);
+    check_fp4_scales(b_sf, 3, groups, n, k);
+    check_group_ends(ends, groups, alignment);
+    if (has_elements(a)) check_vector_alignment(a, "a");
+    if (has_elements(b)) check_vector_alignment(b, "b");
+    const int device = one_device({a_, a_sf_, b_, b_sf_, d_, ends_, ws_});
+    if (rows == 0 || n == 0 || groups == 0) return;
+    RaggedFp4Args p{};
+    auto pitch = [](const View& t) { return t.size(-2) > 1 ? t.stride(-2) : align_up(t.size(-1), 16); };
+    p.g.a = static_cast<const uint16_t*>(a.data()), p.g.lda = pitch(a) / 2;
+    p.g.b = b.data(), p.g.ldb = pitch(b) / 2, p.g.b_gs = b.stride(0) / 2;
+    p.g.d = const_cast<void*>(d.data()), p.g.ldd = d.stride(0);
+    p.g.ends = static_cast<const int32_t*>(ends.data());
+    p.g.rows = (int32_t)rows, p.g.n = (int32_t)n, p.g.k = (int32_t)(k / 4), p.g.groups = (int32_t)groups, p.g.alignment = alignment;
+    p.g.out_f32 = d.dtype() == DG_F32;
+    p.a_sf = static_cast<const uint32_t*>(a_sf.data()), p.b_sf = static_cast<const uint32_t*>(b_sf.data());
+    p.a_sr = rows > 1 ? a_sf.stride(0) : 0, p.a_sk = a_sf.size(1) > 1 ? a_sf.stride(1) : 0;
+    p.b_sr = n > 1 ? b_sf.stride(1) : 0, p.b_sk = b_sf.size(2) > 1 ? b_sf.stride(2) : 0, p.b_sg = b_sf.stride(0);
+    const OnDevice on(device);
+    RaggedPlan plan = ragged_fp4_plan(p);
+    float* ws = ragged_workspace(plan, ws_);
+    launch_ragged_fp4(p, plan, ws, num_sms_now(), stream);
+    char buf[160];
+    std::snprintf(buf, sizeof(buf), "fp4_ragged_nt block=%d splits=%d rows=%d n=%d k=%lld groups=%d", plan.block, plan.splits,
+                  p.g.rows, p.g.n, (long long)k, p.g.groups);
+    t_last_config = buf;
 }
 
 void k_grouped_ragged_impl(const dg_tensor* a_, const dg_tensor* b_, const dg_tensor* b_sf_, const dg_tensor* d_,
@@ -1936,6 +2147,15 @@ int dg_per_token_cast_to_fp8(const dg_tensor* x, const dg_tensor* q, const dg_te
     return guarded([&] { cast_impl(x, q, sf, gran_k, use_ue8m0, static_cast<hipStream_t>(stream)); });
 }
 
+int dg_per_token_cast_to_fp4(const dg_tensor* x, const dg_tensor* q, const dg_tensor* sf, int32_t gran_k,
+                             int32_t use_ue8m0, void* stream) {
+    return guarded([&] { cast4_impl(false, x, q, sf, gran_k, use_ue8m0, static_cast<hipStream_t>(stream)); });
+}
+
+int dg_cast_back_from_fp4(const dg_tensor* q, const dg_tensor* sf, const dg_tensor* y, int32_t gran_k, void* stream) {
+    return guarded([&] { cast4_impl(true, y, q, sf, gran_k, 1, static_cast<hipStream_t>(stream)); });
+}
+
 int64_t dg_moe_dispatch_workspace_size(int64_t num_tokens, int32_t num_experts) {
     if (num_tokens < 0 || num_experts <= 0) return -1;
     return moe_dispatch_workspace_ints(num_tokens, num_experts) * 4;
@@ -1993,6 +2213,40 @@ int dg_moe_swiglu_apply_weight_to_fp8(const dg_tensor* x, const dg_tensor* row_w
 int dg_moe_combine(const dg_tensor* y, const dg_tensor* pos, const dg_tensor* topk_weights, const dg_tensor* out,
                    void* stream) {
     return guarded([&] { moe_combine_impl(y, pos, topk_weights, out, static_cast<hipStream_t>(stream)); });
+}
+
+int dg_moe_dispatch_backward(const dg_tensor* drows, const dg_tensor* pos, const dg_tensor* drow_weights, const dg_tensor* dx,
+                             const dg_tensor* d_topk_weights, void* stream) {
+    return guarded([&] {
+        dispatch_backward_impl(drows, pos, drow_weights, dx, d_topk_weights, static_cast<hipStream_t>(stream));
+    });
+}
+
+int dg_moe_combine_backward(const dg_tensor* dout, const dg_tensor* y, const dg_tensor* pos, const dg_tensor* topk_weights,
+                            const dg_tensor* dy, const dg_tensor* d_topk_weights, void* stream) {
+    return guarded([&] {
+        combine_backward_impl(dout, y, pos, topk_weights, dy, d_topk_weights, static_cast<hipStream_t>(stream));
+    });
+}
+
+int64_t dg_fp4_gemm_ragged_workspace_size(int64_t rows, int64_t n, int64_t k, int32_t groups) {
+    int64_t bytes = -1;
+    guarded([&] {
+        for (int64_t v : {rows, n, k, (int64_t)groups}) DG_CHECK(v >= 0 && v < ((int64_t)1 << 30));
+        DG_CHECK(k % 32 == 0);
+        RaggedFp4Args a{};
+        a.g.rows = (int32_t)rows, a.g.n = (int32_t)n, a.g.k = (int32_t)(k / 4), a.g.groups = groups;
+        bytes = rows == 0 || n == 0 || groups == 0 ? 0 : ragged_fp4_plan(a).workspace_bytes;
+    });
+    return bytes;
+}
+
+int dg_m_grouped_fp4_gemm_nt_ragged(const dg_tensor* a, const dg_tensor* a_sf, const dg_tensor* b, const dg_tensor* b_sf,
+                                    const dg_tensor* d, const dg_tensor* group_ends, int32_t alignment,
+                                    const dg_tensor* workspace, void* stream) {
+    return guarded([&] {
+        ragged_fp4_impl(a, a_sf, b, b_sf, d, group_ends, alignment, workspace, static_cast<hipStream_t>(stream));
+    });
 }
 
 int64_t dg_bf16_gemm_ragged_workspace_size(int32_t form, int64_t rows, int64_t m, int64_t n, int64_t k, int32_t groups) {

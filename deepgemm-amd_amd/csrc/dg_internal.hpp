@@ -262,9 +262,9 @@ constexpr int kMoeMaxTopk = 16;
 constexpr int kMoeChunkTokens = 64;    // tokens per dispatch chunk (count / scatter workgroup)
 enum MoeLayout : int32_t { kMoeContiguous = 0, kMoePsum = 1, kMoeMasked = 2 };
 struct MoeDispatchArgs {
-    const uint8_t* x;          // e4m3 [t, kdim]
+    const uint8_t* x;          // rows of kdim bytes (e4m3, packed e2m1, BF16) [t]
     int64_t ldx;               // bytes
-    const float* x_sf;         // f32 [t, sfk]
+    const float* x_sf;         // [t, sfk] 4-byte scales or words of scales (copied as they are)
     int64_t sf_st, sf_sk;
     const void* topk;          // int32 / int64 [t, k]
     int32_t topk_i64;
@@ -272,7 +272,7 @@ struct MoeDispatchArgs {
     const float* topk_w;       // f32 [t, k] or null
     int64_t w_st, w_sk;
     int32_t t, k, kdim, sfk, num_experts, layout, alignment, max_m, chunks;
-    uint8_t* a;                // [cap, kdim] or [E, max_m, kdim]
+    uint8_t* a;                // [cap] or [E, max_m] rows
     int64_t lda, a_gs;         // bytes
     float* sf;                 // [cap, sfk] or [E, max_m, sfk]
     int64_t sf_sm, sf_sk_o, sf_gs;
@@ -344,6 +344,57 @@ RaggedPlan plan_ragged_gemm(RaggedKind kind, const RaggedGemmArgs& args, int slo
 void check_ragged_launches(RaggedKind kind, const RaggedGemmArgs& args, const RaggedPlan& plan, int slots);
 void launch_ragged_gemm(RaggedKind kind, const RaggedGemmArgs& args, const RaggedPlan& plan, float* workspace, int slots,
                         hipStream_t stream);
+
+// The 4-bit NT product over ragged segments (dg_gemm_fp4.hip). g.a, g.b: e2m1 in 16-bit
+// units of four elements, in which g.k, g.lda, g.ldb and g.b_gs count. Scales: words of
+// four UE8M0 bytes, strides in words.
+struct RaggedFp4Args {
+    RaggedGemmArgs g;
+    const uint32_t* a_sf;      // [rows, ceil(k / 32)]
+    const uint32_t* b_sf;      // [groups, n, ceil(k / 32)]
+    int64_t a_sr, a_sk, b_sr, b_sk, b_sg;
+};
+RaggedPlan plan_ragged_fp4(const RaggedFp4Args& args, int slots, int block, int splits);
+void check_ragged_fp4_launches(const RaggedFp4Args& args, const RaggedPlan& plan);
+void launch_ragged_fp4(const RaggedFp4Args& args, const RaggedPlan& plan, float* workspace, int slots, hipStream_t stream);
+
+// The per-token cast to e2m1 and back (dg_cast4.hip): codes two a byte, scales of `gran`
+// columns as f32 or as words of four UE8M0 bytes.
+struct Cast4Args {
+    const uint16_t* x;         // cast: bf16 [m, n], read
+    void* y;                   // cast back: f32 or bf16 [m, n], written
+    uint8_t* q;                // [m, n / 2]
+    void* sf;                  // f32 [m, ceil(n / gran)] or int32 [m, ceil(ceil(n / gran) / 4)]
+    int64_t ldx, ldq, sf_sm, sf_sk;
+    int32_t m, n, gran, ue8m0, packed, out_f32;
+};
+inline int64_t cast4_blocks(int64_t m, int64_t n) { return (m + 3) / 4 * ((n + 1023) / 1024); }
+void launch_cast4(const Cast4Args& args, hipStream_t stream);
+void launch_cast_back4(const Cast4Args& args, hipStream_t stream);
+
+// Gradients of the dispatch and of the combination (dg_moe_grad.hip). Rows as in CombineArgs.
+struct MoeGradArgs {
+    const uint16_t* rows_in;   // drows (dispatch) or y (combination; null without weights): bf16 rows
+    uint16_t* rows_out;        // dy (combination)
+    int64_t ld_in, gs_in, ld_out, gs_out;   // elements
+    int32_t max_m;             // 0: flat rows; else rows r = e * max_m + i
+    int64_t rows;
+    const int32_t* pos;        // [t, k] contiguous
+    const float* w;            // row weights' gradient [rows] (dispatch) or weights [t, k] (combination), or null
+    int64_t w_st, w_sk;
+    uint16_t* tokens;          // dx (dispatch, written) or dout (combination, read): bf16 [t, n]
+    int64_t ldt;
+    float* dw;                 // [t, k] contiguous, or null
+    int32_t t, k, n;
+};
+inline int moe_grad_waves(int64_t n) { return n <= 512 ? 1 : n <= 1024 ? 2 : 4; }   // of a token
+inline int64_t dispatch_backward_blocks(int64_t t, int64_t n) { return (t + 3) / 4 * (n > 0 ? (n + 511) / 512 : 1); }
+inline int64_t combine_backward_blocks(int64_t t, int64_t n) {
+    const int64_t per = 4 / moe_grad_waves(n);
+    return (t + per - 1) / per;
+}
+void launch_dispatch_backward(const MoeGradArgs& args, hipStream_t stream);
+void launch_combine_backward(const MoeGradArgs& args, hipStream_t stream);
 
 // SwiGLU with an 8-bit checkpoint, and its backward pass (dg_swiglu_grad.hip). n: columns
 // of h; gate columns [0, n), up columns [n, 2n) of x, q and dx; scales of the gate half

@@ -1,5 +1,5 @@
 // MoE plumbing around the grouped GEMMs on one GPU (gfx950): dispatch of
-// token-major FP8 activations into the expert-grouped layouts the grouped GEMMs
+// token-major FP8, BF16 or 4-bit activations into the expert-grouped layouts the grouped GEMMs
 // read, the fused SwiGLU x routing-weight -> FP8 cast between the two grouped
 // GEMMs, and combine. The reference runs this layer as DeepEP dispatch, L1 GEMM,
 // tilelang SwiGLU, L2 GEMM, DeepEP combine (tests/test_mega_moe.py:296-330); the
@@ -187,13 +187,15 @@ __global__ void __launch_bounds__(kThreads) moe_starts_kernel(const MoeDispatchA
 }
 
 // Contiguous and psum layouts: e < E fills expert e's padding rows (zero A, SF
-// and weight, m_indices = -1); e = E sets m_indices = -1 past the segments.
+// and weight, m_indices = -1); e = E sets m_indices = -1 and the weights to zero past the segments.
 __device__ __forceinline__ void pad_block(const MoeDispatchArgs& p, int e) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     if (e == p.num_experts) {
-        if (p.layout != kMoeContiguous) return;
         const int used = ws_totals(p)[p.num_experts];
-        for (int64_t r = used + threadIdx.x; r < p.cap_rows; r += kThreads) p.meta[r] = -1;
+        for (int64_t r = used + threadIdx.x; r < p.cap_rows; r += kThreads) {
+            if (p.layout == kMoeContiguous) p.meta[r] = -1;
+            if (p.w_out) p.w_out[r] = 0.f;
+        }
         return;
     }
     const int total = ws_totals(p)[e], start = ws_starts(p)[e];

@@ -11,7 +11,8 @@ Scope: fp8_gemm_nt (and its fp8_fp4/fp4 aliases and nn/tn/tt transposing
 wrappers), m_grouped_fp8_gemm_nt_contiguous (m_indices and psum layouts),
 m_grouped_fp8_gemm_nt_masked, the SF layout helpers, and BF16 training of an MoE layer's
 experts (m_grouped_bf16_gemm_{nt,nn}_ragged, k_grouped_bf16_gemm_tn_ragged,
-moe_swiglu_checkpoint, moe_swiglu_backward). The reference's own
+moe_swiglu_checkpoint, moe_swiglu_backward, moe_dispatch_backward, moe_combine_backward) and
+their 4-bit form (per_token_cast_to_fp4, cast_back_from_fp4, m_grouped_fp4_gemm_nt_ragged). The reference's own
 BF16/einsum/attention/Mega-MoE/cuBLASLt entry points are not provided.
 """
 from typing import Optional, Tuple
@@ -449,37 +450,83 @@ def per_token_cast_to_fp8(x: torch.Tensor, use_ue8m0: bool, gran_k: int = 128,
     return q, sf
 
 
+def per_token_cast_to_fp4(x: torch.Tensor, use_ue8m0: bool, gran_k: int = 128,
+                          use_packed_ue8m0: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
+    """[m, n] -> (packed e2m1 int8 [m, n / 2], element 2i in the low nibble, float32 SF
+    [m, ceil(n / gran_k)] or packed int32 UE8M0 words); gran_k 32 with use_ue8m0 is the microscaled
+    format that m_grouped_fp4_gemm_nt_ragged takes. Results of the reference's
+    (deep_gemm/utils/math.py) to the bit. BF16 device tensors take the fused HIP kernel (one HBM
+    pass); anything else takes the torch ops of deep_gemm.utils.math."""
+    if not _cast_on_device(x) or gran_k not in (32, 64, 128):
+        return utils.math.per_token_cast_to_fp4(x, use_ue8m0, gran_k, use_packed_ue8m0)
+    assert not use_packed_ue8m0 or use_ue8m0
+    status, q, sf = _bind.cast4(x, gran_k, int(bool(use_ue8m0)), int(bool(use_packed_ue8m0)), _raw_stream_of(x))
+    _check(status)
+    return q, sf
+
+
+def cast_back_from_fp4(packed: torch.Tensor, sf: torch.Tensor, gran_k: int = 128, use_packed_ue8m0: bool = False,
+                       dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """The values that per_token_cast_to_fp4's codes and scales stand for, float32 or bfloat16
+    (rounded once; exact for power-of-two scales from 2^-125 on): with it the BF16 products
+    take 4-bit weights, for gradients through them. Device tensors take one HIP kernel;
+    others the torch ops of deep_gemm.utils.math."""
+    if dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError('dtype must be torch.float32 or torch.bfloat16')
+    if not packed.is_cuda or packed.dtype != torch.int8 or packed.dim() != 2 or gran_k not in (32, 64, 128):
+        return utils.math.cast_back_from_fp4(packed, sf, gran_k, use_packed_ue8m0).to(dtype)
+    if sf.dtype != (torch.int32 if use_packed_ue8m0 else torch.float32):
+        raise RuntimeError('Assertion error (deep_gemm): sf must be int32 words with use_packed_ue8m0, else float32')
+    status, y = _bind.cast_back4(packed, sf, gran_k, int(dtype == torch.bfloat16), _raw_stream_of(packed))
+    _check(status)
+    return y
+
+
 # ------------------------------------------------------------------ MoE plumbing
 
 _MOE_LAYOUTS = {'contiguous': 0, 'psum': 1, 'masked': 2}
 
 
-def moe_dispatch(x: Tuple[torch.Tensor, torch.Tensor], topk_idx: torch.Tensor, num_experts: int,
+def moe_dispatch(x, topk_idx: torch.Tensor, num_experts: int,
                  layout: str = 'contiguous', alignment: Optional[int] = None, max_m: Optional[int] = None,
-                 topk_weights: Optional[torch.Tensor] = None):
-    """Token-major FP8 rows -> the expert-grouped layout a grouped GEMM reads, the
+                 topk_weights: Optional[torch.Tensor] = None, out=None):
+    """Token-major rows -> the expert-grouped layout a grouped GEMM reads, the
     one-GPU form of DeepEP's expanded / low-latency receive buffers that the
     reference feeds its grouped GEMMs (tests/test_mega_moe.py:296-310, README.md:78,86).
 
-    x = (e4m3 [T, K], f32 SF [T, ceil(K/128)]); topk_idx [T, topk] (negative ids are
+    x: (e4m3 [T, K], f32 SF [T, ceil(K/128)]) for the FP8 GEMMs; bf16 [T, K] (K a multiple of
+    8) or (packed e2m1 int8 [T, K/2], int32 UE8M0 words [T, ceil(K/128)]) (K a multiple of 32) for the
+    ragged ones. topk_idx [T, topk] (negative ids are
     not routed). Returns (a, a_sf, grouped_layout, pos, row_weights):
       contiguous: a [R, K], m_indices [R] (-1 on padding), R = dg_moe_dispatch_max_rows;
       psum:       a [R, K], psum ends [E];
       masked:     a [E, max_m, K], masked_m [E] (entries past max_m dropped);
-    pos [T, topk] int32 (row of each (token, slot), masked rows flattened as
+    a and a_sf of x's types (a_sf None for bf16); alignment a multiple of 16 for e4m3 rows, any
+    for the others; pos [T, topk] int32 (row of each (token, slot), masked rows flattened as
     e * max_m + r, -1 if none); row_weights: the routing weight of each row (None
-    without topk_weights). Deterministic: an expert's rows follow token order."""
-    xq, xs = _pair(x, 'x')
+    without topk_weights; 0 on rows of no token in the first two layouts). out: optional
+    preallocated a (bf16) or (a, a_sf), of R rows or more: rows past the segments are left
+    as they were. Deterministic: an expert's rows follow token order."""
     if layout not in _MOE_LAYOUTS:
         raise ValueError(f'layout must be one of {sorted(_MOE_LAYOUTS)}')
+    if layout == 'masked' and not max_m:
+        raise ValueError('the masked layout needs max_m')
+    alignment = int(alignment or get_mk_alignment_for_contiguous_layout())
+    bf16 = isinstance(x, torch.Tensor)
+    xq, xs = (x, None) if bf16 else _pair(x, 'x')
+    if not isinstance(xq, torch.Tensor):
+        raise TypeError('x must be a tensor or a (tensor, scaling factor) pair')
+    if bf16 or xq.dtype != torch.float8_e4m3fn or out is not None:
+        o, o_sf = (out, None) if bf16 or out is None else _pair(out, 'out')
+        status, *got = _bind.dispatch_rows(xq, xs, topk_idx, topk_weights, num_experts, _MOE_LAYOUTS[layout], alignment,
+                                           max_m or 0, o, o_sf, _raw_stream_of(xq))
+        _check(status)
+        return tuple(got)
     t, kdim = xq.shape
     k = topk_idx.shape[1]
     dev = xq.device
-    alignment = int(alignment or get_mk_alignment_for_contiguous_layout())
     sfk = (kdim + 127) // 128
     if layout == 'masked':
-        if not max_m:
-            raise ValueError('the masked layout needs max_m')
         a = torch.empty((num_experts, max_m, kdim), dtype=torch.float8_e4m3fn, device=dev)
         a_sf = torch.empty((num_experts, max_m, sfk), dtype=torch.float32, device=dev)
         gl = torch.empty((num_experts,), dtype=torch.int32, device=dev)
@@ -528,6 +575,32 @@ def moe_combine(y: torch.Tensor, pos: torch.Tensor, topk_weights: Optional[torch
     out = torch.empty((pos.shape[0], y.shape[-1]), dtype=torch.bfloat16, device=y.device)
     _check(_bind.combine(y, pos, topk_weights, out, _raw_stream_of(y)))
     return out
+
+
+def moe_dispatch_backward(drows: torch.Tensor, pos: torch.Tensor, drow_weights: Optional[torch.Tensor] = None
+                          ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """Gradient of moe_dispatch: drows bf16 ([R, K] or masked [E, max_m, K]) and the gradient of
+    its row_weights (float32, or None) -> (dx bf16 [T, K], float32 [T, topk] gradient of
+    topk_weights or None): dx[t] = sum over the slots of drows[pos[t, j]], in FP32 and their
+    order, rounded once. Entries that were not routed count as zeros. K a multiple of 8,
+    topk at most 16."""
+    status, dx, dw = _bind.dispatch_backward(drows, pos, drow_weights, _raw_stream_of(drows))
+    _check(status)
+    return dx, dw
+
+
+def moe_combine_backward(dout: torch.Tensor, y: torch.Tensor, pos: torch.Tensor,
+                         topk_weights: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None
+                         ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """Gradient of moe_combine(y, pos, topk_weights): dout bf16 [T, N] -> (dy bf16 like y, float32
+    [T, topk] gradient of topk_weights or None without them): dy[pos[t, j]] = w * dout[t], dw =
+    the products of dout[t] and y[pos[t, j]] summed. y is read only with topk_weights. Every row
+    is named at most once in pos, as moe_dispatch leaves it; rows that it does not name are
+    zeros, or with `out` (a preallocated dy, which may be y itself) left as they were: that
+    saves a pass over dy. N a multiple of 8, topk at most 16."""
+    status, dy, dw = _bind.combine_backward(dout, y, pos, topk_weights, out, _raw_stream_of(dout))
+    _check(status)
+    return dy, dw
 
 
 def transform_l1_weights_for_swiglu(b: Tuple[torch.Tensor, torch.Tensor]) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -629,6 +702,20 @@ def k_grouped_bf16_gemm_tn_ragged(a: torch.Tensor, b, d: torch.Tensor, group_end
     the value). d bf16 or float32 [G, M, N]; c None (zeros) or like d, also d itself. Groups without rows get c."""
     b_t, b_sf = _pair(b, 'b') if isinstance(b, (tuple, list)) else (b, None)
     _check(_bind.k_grouped_ragged(a, b_t, b_sf, d, group_ends, c, int(alignment), _raw_stream_of(d)))
+
+
+def m_grouped_fp4_gemm_nt_ragged(a: Tuple[torch.Tensor, torch.Tensor], b: Tuple[torch.Tensor, torch.Tensor],
+                                 d: torch.Tensor, group_ends: torch.Tensor, alignment: int = 1) -> None:
+    """m_grouped_bf16_gemm_nt_ragged of 4-bit operands: D[r] = A[r] @ B[g(r)].T with a = (packed
+    e2m1 int8 [M, K/2], int32 [M, ceil(K/128)]) and b = ([G, N, K/2], [G, N, ceil(K/128)]), as
+    per_token_cast_to_fp4(x, use_ue8m0=True, gran_k=32, use_packed_ue8m0=True) makes them: a
+    power-of-two scale for 32 elements of a row, four to a word. Sums in FP32, d bf16 or float32.
+    K a multiple of 32, rows of codes at multiples of 16 bytes; scales with any strides (words of a
+    row side by side are read fastest). Gradients: through the operands' values (cast_back_from_fp4 to
+    bfloat16 is exact) and the BF16 products."""
+    a_t, a_sf = _pair(a, 'a')
+    b_t, b_sf = _pair(b, 'b')
+    _check(_bind.ragged_fp4(a_t, a_sf, b_t, b_sf, d, group_ends, int(alignment), _raw_stream_of(d)))
 
 
 def moe_swiglu_checkpoint(x: torch.Tensor, row_weights: Optional[torch.Tensor] = None,

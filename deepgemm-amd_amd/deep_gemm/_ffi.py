@@ -101,6 +101,12 @@ SIGNATURES = {
     'dg_k_grouped_bf16_gemm_tn_ragged': (_I, [_T, _T, _T, _T, _T, _T, _I, _T, _V]),
     'dg_moe_swiglu_checkpoint': (_I, [_T, _T, _T, ctypes.c_float, _T, _T, _T, _V]),
     'dg_moe_swiglu_backward': (_I, [_T, _T, _T, _T, _T, ctypes.c_float, _T, _T, _T, _V]),
+    'dg_per_token_cast_to_fp4': (_I, [_T, _T, _T, _I, _I, _V]),
+    'dg_cast_back_from_fp4': (_I, [_T, _T, _T, _I, _V]),
+    'dg_moe_dispatch_backward': (_I, [_T, _T, _T, _T, _T, _V]),
+    'dg_moe_combine_backward': (_I, [_T, _T, _T, _T, _T, _T, _V]),
+    'dg_fp4_gemm_ragged_workspace_size': (ctypes.c_int64, [ctypes.c_int64] * 3 + [_I]),
+    'dg_m_grouped_fp4_gemm_nt_ragged': (_I, [_T, _T, _T, _T, _T, _T, _I, _T, _V]),
     'dg_set_num_sms': (_I, [_I]),
     'dg_get_num_sms': (_I, [_P(_I)]),
     'dg_set_mk_alignment_for_contiguous_layout': (_I, [_I]),
@@ -146,6 +152,9 @@ def _load_bind():
                                  'dg_k_grouped_bf16_gemm_tn_ragged', 'dg_bf16_gemm_ragged_workspace_size',
                                  'dg_moe_swiglu_checkpoint',
                                  'dg_moe_swiglu_backward'))
+    _dgbind.init_rows(*addresses('dg_moe_dispatch_max_rows', 'dg_moe_dispatch_workspace_size', 'dg_moe_dispatch_backward',
+                                 'dg_moe_combine_backward', 'dg_per_token_cast_to_fp4', 'dg_cast_back_from_fp4',
+                                 'dg_m_grouped_fp4_gemm_nt_ragged', 'dg_fp4_gemm_ragged_workspace_size'))
     return _dgbind
 
 

@@ -277,6 +277,22 @@ int dg_plan_sf_transform(const dg_tensor* sf, int32_t mn, int32_t k,
 int dg_per_token_cast_to_fp8(const dg_tensor* x, const dg_tensor* q, const dg_tensor* sf,
                              int32_t gran_k, int32_t use_ue8m0, void* stream);
 
+/* The same cast to packed e2m1 (4 bits), in the arithmetic of the reference's per_token_cast_to_fp4
+ * (deep_gemm/utils/math.py, torch ops there): amax of gran_k columns, at least 1e-4, times
+ * fl32(1/6), up to a power of two with use_ue8m0; codes e2m1(x * (1 / sf)), ties to the even
+ * code, no negative zero.
+ *   x   bf16 [M, N], N even (< 2^27), unit stride along N
+ *   q   int8 [M, N/2]: element 2i in the low nibble
+ *   sf  f32 [M, ceil(N/gran_k)], or int32 [M, ceil(ceil(N/gran_k)/4)] of packed UE8M0 exponents
+ *       (needs use_ue8m0; groups past the last as 1.0), any strides
+ *   gran_k 32 (microscaled formats), 64 or 128. ceil(M/4) ceil(N/1024) < 2^24. */
+int dg_per_token_cast_to_fp4(const dg_tensor* x, const dg_tensor* q, const dg_tensor* sf,
+                             int32_t gran_k, int32_t use_ue8m0, void* stream);
+
+/* Back: y = code * scale in FP32, y f32 or bf16 [M, N] (rounded once; exact in BF16 for powers
+ * of two from 2^-125 on). q, sf as above; an int32 sf holds UE8M0 bytes. */
+int dg_cast_back_from_fp4(const dg_tensor* q, const dg_tensor* sf, const dg_tensor* y, int32_t gran_k, void* stream);
+
 /* ---------------------------------------------------------------- MoE plumbing */
 
 /* The MoE layer around the grouped GEMMs, for one GPU's experts. The reference
@@ -292,25 +308,31 @@ int64_t dg_moe_dispatch_workspace_size(int64_t num_tokens, int32_t num_experts);
  * alignment), the capacity `a` must have (-1 on bad arguments). */
 int64_t dg_moe_dispatch_max_rows(int64_t num_tokens, int32_t num_topk, int32_t num_experts, int32_t alignment);
 
-/* Dispatch: token-major FP8 rows -> the expert-grouped layout of a grouped GEMM,
+/* Dispatch: token-major rows -> the expert-grouped layout of a grouped GEMM,
  * as DeepEP's expanded (normal) or low-latency (masked) receive buffers feed
  * m_grouped_fp8_gemm_nt_contiguous / _masked (README.md:78,86). Each (token t,
  * slot j) with expert e = topk_idx[t, j] in [0, E) gets the next row of e's
  * segment, in token-then-slot order (deterministic); negative ids are not routed.
- *   x            e4m3 [T, K], unit stride along K, K % 16 == 0, 16-byte rows
- *   x_sf         f32 [T, ceil(K/128)], any strides (1 x 128 per-token scales)
+ *   x            e4m3 [T, K], unit stride along K, K % 16 == 0, 16-byte rows; or, for the
+ *                ragged products, BF16 [T, K] (K % 8 == 0) or packed e2m1 int8 [T, K/2] (K % 32 == 0)
+ *   x_sf         f32 [T, ceil(K/128)], any strides (1 x 128 per-token scales); NULL for BF16; of
+ *                e2m1 rows int32 words of four UE8M0 scales of 32
  *   topk_idx     int32 / int64 [T, topk] (topk <= 16), any strides
  *   topk_weights f32 [T, topk] or null: copied to row_weights
  *   layout       0 contiguous: `a` [R, K], R >= dg_moe_dispatch_max_rows; segment e
- *                  starts at a multiple of `alignment` (tests/generators.py:383-407);
+ *                  starts at a multiple of `alignment` (tests/generators.py:383-407; of 16
+ *                  for e4m3 rows, any up to 2^20 for the others);
  *                  grouped_layout = int32 m_indices [R], -1 on padding and past the
- *                  segments; padding rows of a / sf / row_weights are zero
+ *                  segments; padding rows of a / sf / row_weights are zero, and row_weights
+ *                  also past the segments (a and sf are left as they were there)
  *                1 psum: the same rows, grouped_layout = int32 [E] with
  *                  psum[e] = align(psum[e-1]) + count_e (tests/generators.py:456-461)
  *                2 masked: `a` [E, max_m, K], rows [0, count_e) of slab e,
  *                  grouped_layout = masked_m [E] = min(count_e, max_m); entries past
  *                  max_m are dropped (pos -1); other rows are not written
- *   sf           f32 [R, ceil(K/128)] or [E, max_m, ceil(K/128)], any strides
+ *   a            rows of x's type
+ *   sf           [R, ceil(K/128)] or [E, max_m, ceil(K/128)] of x_sf's type, any strides (NULL
+ *                for BF16)
  *   pos          int32 [T, topk] contiguous: the row of (t, j) (masked: e * max_m + r),
  *                -1 if not routed or dropped
  *   row_weights  f32 with R (or E * max_m) elements, contiguous, or null
@@ -394,6 +416,33 @@ int dg_m_grouped_fp8_gemm_nt_masked_swiglu(const dg_tensor* a, const dg_tensor* 
 int dg_moe_combine(const dg_tensor* y, const dg_tensor* pos, const dg_tensor* topk_weights, const dg_tensor* out,
                    void* stream);
 
+/* Gradient of the dispatch: dx[t] = sum over slots j of drows[pos[t, j]] (FP32, in the slots'
+ * order, rounded once to BF16) and d_topk_weights[t, j] = drow_weights[pos[t, j]].
+ *   drows           bf16 [R, K] or [E, max_m, K], unit stride along K, K % 8 == 0, 16-byte rows
+ *   pos             int32 [T, topk] contiguous from dg_moe_dispatch (topk <= 16); entries that are
+ *                   no row (-1) count as zeros
+ *   drow_weights    f32 with R (or E * max_m) elements, contiguous, or NULL
+ *   dx              bf16 [T, K], 16-byte rows
+ *   d_topk_weights  f32 [T, topk] contiguous; given if and only if drow_weights is
+ * (dg_moe_combine is the gradient of the rows alone.) ceil(T/4) ceil(K/512) < 2^24. */
+int dg_moe_dispatch_backward(const dg_tensor* drows, const dg_tensor* pos, const dg_tensor* drow_weights, const dg_tensor* dx,
+                             const dg_tensor* d_topk_weights, void* stream);
+
+/* Gradient of dg_moe_combine: dy[pos[t, j]] = w[t, j] dout[t] (FP32, rounded once; a copy where
+ * topk_weights is NULL) and d_topk_weights[t, j] = sum over the columns of dout[t] y[pos[t, j]]
+ * (FP32, in a fixed order).
+ *   dout            bf16 [T, N], N % 8 == 0, 16-byte rows
+ *   y               dg_moe_combine's, read only where topk_weights is given (else it may be NULL)
+ *   pos             as above; every row is named by at most one entry, as dg_moe_dispatch leaves it
+ *   topk_weights    f32 [T, topk], any strides, or NULL (w = 1)
+ *   dy              y's shape, bf16, 16-byte rows; rows that no entry names are left as they were;
+ *                   may be y itself
+ *   d_topk_weights  f32 [T, topk] contiguous (0 where there is no row); given if and only if
+ *                   topk_weights is
+ * T < 2^24 where N > 1024. */
+int dg_moe_combine_backward(const dg_tensor* dout, const dg_tensor* y, const dg_tensor* pos, const dg_tensor* topk_weights,
+                            const dg_tensor* dy, const dg_tensor* d_topk_weights, void* stream);
+
 /* ---------------------------------------------------------------- BF16 expert products */
 
 /* Training and BF16 serving of an MoE layer's experts: products over ragged row segments,
@@ -444,6 +493,21 @@ int dg_m_grouped_bf16_gemm_nn_ragged(const dg_tensor* a, const dg_tensor* b, con
 int dg_k_grouped_bf16_gemm_tn_ragged(const dg_tensor* a, const dg_tensor* b, const dg_tensor* b_sf, const dg_tensor* d,
                                      const dg_tensor* group_ends, const dg_tensor* c, int32_t alignment,
                                      const dg_tensor* workspace, void* stream);
+
+/* 4-bit form of the NT product: d[r] = a[r] @ b[g(r)]^T with a and b in packed e2m1 and a
+ * power-of-two scale for 32 elements of a row, both applied by the matrix cores; sums in FP32.
+ *   a, b        int8 [M, K/2], [G, N, K/2] (element 2i in the low nibble), unit stride along K,
+ *               K % 32 == 0, 16-byte rows
+ *   a_sf, b_sf  int32 [M, ceil(K/128)], [G, N, ceil(K/128)]: words of four UE8M0 exponents along K
+ *               as dg_per_token_cast_to_fp4 (gran_k 32) gives them, row strides of at most 2^20
+ *               words, the others of less than 2^28. Bytes past the last scale may hold anything.
+ *   d           bf16 or fp32 [M, N], unit stride along N; rows outside every group left as they were
+ * group_ends, alignment, limits: as the BF16 products. `workspace`: likewise, of
+ * dg_fp4_gemm_ragged_workspace_size(M, N, K, G) bytes, or NULL. */
+int64_t dg_fp4_gemm_ragged_workspace_size(int64_t rows, int64_t n, int64_t k, int32_t groups);
+int dg_m_grouped_fp4_gemm_nt_ragged(const dg_tensor* a, const dg_tensor* a_sf, const dg_tensor* b, const dg_tensor* b_sf,
+                                    const dg_tensor* d, const dg_tensor* group_ends, int32_t alignment,
+                                    const dg_tensor* workspace, void* stream);
 
 /* SwiGLU x routing weight in BF16, leaving its input in 8 bits for the backward pass:
  * h = silu(gate) * up * w, gate = x[:, :I], up = x[:, I:], in FP32, rounded once.
