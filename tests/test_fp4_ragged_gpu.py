@@ -16,6 +16,15 @@ pytestmark = pytest.mark.gpu
 MIXED = [5, 0, 1, 130, 0, 64, 257, 31, 0]
 
 
+@pytest.fixture(autouse=True, params=['heuristic', '256', '128', '32'])
+def tiles(request):
+    """Every test with the tiles the sizes choose, and with each kind forced."""
+    if request.param != 'heuristic':
+        deep_gemm.set_tile_override(int(request.param), 0, variant=13)
+    yield request.param
+    deep_gemm.set_tile_override(0, 0)
+
+
 def product(sizes, n, k, alignment=1, out=torch.bfloat16, spare=3, seed=0, d_pitch=None, layout='rows', pitch=0, low=120, high=130):
     print(f'sizes={sizes} n={n} k={k} alignment={alignment} {out} {layout}', flush=True)
     seg = segments(sizes, alignment)
