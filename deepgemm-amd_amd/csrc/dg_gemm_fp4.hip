@@ -22,25 +22,34 @@ using namespace dev;
 
 constexpr int kFmtE2M1 = 4;   // operand format of the matrix instruction
 
-// The scales of 32 rows of a tile, two words a row for each step: word q of row r goes to
-// (q * 32 + r) * 4. One wave load; rows past the tile's read its last row's.
+// The scales of 32 rows of a tile (a slab), WORDS words a row at a time (2: a step's, 4: those of
+// two steps): word q of row r goes to (r * WORDS + q) * 4. Neighbouring lanes load neighbouring words
+// of a row, 64 / WORDS rows a wave load; rows past the tile's read its last row's.
+template <int WORDS>
 struct ScaleSlab {
-    const uint8_t* base;   // the first row's words of the step to be issued next
-    uint32_t row, word;    // byte offsets of this lane's row, and of its word
-    int64_t step;          // bytes between steps
-    int left;              // words from there on
+    static constexpr int kBytes = 32 * WORDS * 4, kLoads = WORDS / 2;   // wave loads
+    const uint8_t* base;    // the first row's words to be issued next
+    uint32_t row[kLoads];   // byte offsets of this lane's rows
+    uint32_t word;          // of its word
+    int64_t step;           // bytes to the next words
+    int left;               // words from there on
 
     __device__ __forceinline__ void init(const uint32_t* at, int64_t sr, int64_t sk, int first_row, int rows, int words, int lane) {
         base = reinterpret_cast<const uint8_t*>(at);
-        row = (uint32_t)(min(first_row + (lane & 31), rows - 1) * (int)sr * 4);
-        word = (uint32_t)((lane >> 5) * (int)sk * 4);
-        step = sk * 8;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i)
+            row[i] = (uint32_t)(min(first_row + i * (64 / WORDS) + lane / WORDS, rows - 1) * (int)sr * 4);
+        word = (uint32_t)(lane % WORDS * (int)sk * 4);
+        step = sk * 4 * WORDS;
         left = words;
     }
-    __device__ __forceinline__ void issue(uint32_t lds) {
-        dma4_saddr(base, row + (left > 1 ? word : 0u), lds);   // (an odd last word: twice)
-        base += left > 2 ? step : 0;                            // (steps past the end read the last one again)
-        left -= left > 2 ? 2 : 0;
+    __device__ __forceinline__ void issue(uint32_t lds, int lane) {
+        const uint32_t w = lane % WORDS < left ? word : 0u;   // (past the last word: the first again)
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) dma4_saddr(base, row[i] + w, lds + i * 256);
+        const bool more = left > WORDS;   // (past the end: the last ones again)
+        base += more ? step : 0;
+        left -= more ? WORDS : 0;
     }
 };
 
@@ -54,9 +63,11 @@ struct StepScales {
         m0 = left >= 4 ? ~0u : (1u << (8 * max(left, 0))) - 1u;
         m1 = left >= 8 ? ~0u : (1u << (8 * max(left - 4, 0))) - 1u;
     }
-    __device__ __forceinline__ static void read(const uint8_t* slab, int lane, uint32_t (&words)[2]) {
-        const uint32_t* w = reinterpret_cast<const uint32_t*>(slab) + (lane & 31);
-        words[0] = w[0], words[1] = w[32];
+    // WORDS: of a row in LDS; first: the step's first of them
+    template <int WORDS>
+    __device__ __forceinline__ static void read(const uint8_t* slab, int lane, uint32_t first, uint32_t (&words)[2]) {
+        const uint2 w = *reinterpret_cast<const uint2*>(slab + (lane & 31) * (WORDS * 4) + first * 4);
+        words[0] = w.x, words[1] = w.y;
     }
     __device__ __forceinline__ void get(const uint32_t (&words)[2], int lane, int (&out)[2]) const {
         const uint32_t ones = 0x7F7F7F7Fu;
@@ -78,19 +89,22 @@ __device__ __forceinline__ f32x16 mfma4(int ks, const bf16x8& b, const bf16x8& a
 
 // One workgroup per BM x BN tile: 256 x 256 on eight waves (128 x 64 each), one workgroup on a
 // CU, or 128 x 128 on four (64 x 64), two on a CU; PART 2: 128 x 128 quarters of 256 x 256 tiles
-// (dg_ragged.hpp). Two steps of A, of B and of the scales in LDS, and two barriers a step: the
-// hand-off before a step's last 32-row slice (the next step's loads have arrived, and every
-// wave has read A's last slice and the scales, whose places the step after the next takes), and
-// another one a slice after the step's start, when every wave holds its B fragments, whose
-// place is handed on.
+// (dg_ragged.hpp). Two steps of A and of B in LDS, and four of the scales; A's by slices (the
+// 32-row slabs that the waves multiply at a time, side by side), a wave load for each wave. Two
+// barriers a step, at which places are handed on and arrivals certified: before its last
+// slice (every wave holds the slices up to the last; slices of the first half, B and the scales of
+// the next step have arrived, and are read under the last slice), and at the start of its
+// second half (every wave holds B and the first half's slices; the second half's have arrived).
+// So a load is issued 1.5 steps before it is waited for.
 template <int BM, int BN, int WGM, int WGN, int PART>
 __global__ void __launch_bounds__(WGM * WGN * 64, WGM * WGN == 4 ? 2 : 1) fp4_tile_kernel(const RaggedFp4Args p, const RaggedLaunch l) {
     constexpr int NW = WGM * WGN, WM = BM / WGM, WN = BN / WGN, SM = WM / 32, SN = WN / 32, KS = 4;
-    constexpr int A_STEP = BM * BK * 2, B_STEP = BN * BK * 2, S_STEP = (BM + BN) / 32 * 256;   // bytes of a step
+    constexpr int A_STEP = BM * BK * 2, B_STEP = BN * BK * 2;   // bytes of a step
+    constexpr int SLAB = ScaleSlab<4>::kBytes, S_PAIR = (BM + BN) / 32 * SLAB, S_SLOTS = 3;   // scales of two steps
     constexpr int B_AT = 2 * A_STEP, S_AT = B_AT + 2 * B_STEP;
     static_assert(SM % 2 == 0 && BM / 32 == NW && BN / 32 == NW, "a slab of A's and of B's scales for each wave");
     static_assert(128 * BN * 4 <= S_AT, "the epilogue's rows fit");
-    __shared__ __attribute__((aligned(1024))) uint8_t smem[S_AT + 2 * S_STEP];
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[S_AT + S_SLOTS * S_PAIR];
 
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -107,7 +121,7 @@ __global__ void __launch_bounds__(WGM * WGN * 64, WGM * WGN == 4 ? 2 : 1) fp4_ti
 
     Operand<BM, 1, NW> oa;
     Operand<BN, 1, NW> ob;
-    ScaleSlab sa, sb;
+    ScaleSlab<4> sa, sb;
     oa.init(p.g.a + (int64_t)m0 * p.g.lda + k0, p.g.lda, a_rows, reduced, wave, lane);
     ob.init(static_cast<const uint16_t*>(p.g.b) + (int64_t)t.g * p.g.b_gs + (int64_t)n0 * p.g.ldb + k0, p.g.ldb, b_rows, reduced,
             wave, lane);
@@ -130,69 +144,101 @@ __global__ void __launch_bounds__(WGM * WGN * 64, WGM * WGN == 4 ? 2 : 1) fp4_ti
     fb.init(wn * WN, lane);
     bf16x8 op_b[SN][KS], op_a[2][KS];
     uint32_t wa[2][2], wb[SN][2];
-    auto a_scales = [&](uint32_t step, int slab) { return smem + S_AT + step + (wm * SM + slab) * 256; };
-    auto b_scales = [&](uint32_t step, int slab) { return smem + S_AT + step + (NW + wn * SN + slab) * 256; };
-    auto issue_scales = [&](uint32_t s) {
-        sa.issue(lds0 + S_AT + s + wave * 256);
-        sb.issue(lds0 + S_AT + s + (NW + wave) * 256);
+    // words of a slab's rows for a step: pair, the place of its two steps' scales; odd, which of them it is
+    auto read_a_scales = [&](uint32_t pair, uint32_t odd, int slab, uint32_t (&to)[2]) {
+        StepScales::read<4>(smem + pair + (wm * SM + slab) * SLAB, lane, odd * 2, to);
+    };
+    auto read_b_scales = [&](uint32_t pair, uint32_t odd, int slab, uint32_t (&to)[2]) {
+        StepScales::read<4>(smem + pair + (NW + wn * SN + slab) * SLAB, lane, odd * 2, to);
     };
 
     const int steps = (reduced + BK - 1) / BK;
-    constexpr int A_LOADS = decltype(oa)::kInstr, B_LOADS = decltype(ob)::kInstr;
-    constexpr int IN_FLIGHT = B_LOADS;   // at a hand-off: B of the step after the next
+    // Loads of a wave for a step: HALF of A at the hand-off of its last slice, TOP_LOADS (scales, A's
+    // first half, B) at the other one; in flight at either: those of the step after the next.
+    constexpr int HALF = decltype(oa)::kInstr / 2, B_LOADS = decltype(ob)::kInstr, S_LOADS = decltype(sa)::kLoads;
+    constexpr int TOP_LOADS = S_LOADS + HALF + B_LOADS;
+    constexpr int IN_FLIGHT = TOP_LOADS + HALF, PER_SLICE = HALF * 2 / SM;   // loads of a slice
+    auto load_a = [&](const typename decltype(oa)::Step& s, int q, uint32_t lds) {   // the q-th of a step's
+        const int x = q % PER_SLICE * NW + wave;   // 8-row piece of the slice, four of each wave row
+        oa.load_rows(s, (x >> 2) * (SM * 4) + q / PER_SLICE * 4 + (x & 3), lds, decltype(oa)::kRows * (int)oa.pitch);
+    };
+    // Scales come two steps at a time: A's of the pair after the next in even steps, B's in odd ones,
+    // to the place after the next pair's (three places).
+    uint32_t s_cur = S_AT, s_next = S_AT + S_PAIR, s_last = S_AT + 2 * S_PAIR;
+    auto issue_scales = [&](bool b, uint32_t pair) {
+        ScaleSlab<4> s = sa;
+        s.base = b ? sb.base : sa.base, s.left = b ? sb.left : sa.left, s.step = b ? sb.step : sa.step;
+        s.word = b ? sb.word : sa.word;
+#pragma unroll
+        for (int i = 0; i < S_LOADS; ++i) s.row[i] = b ? sb.row[i] : sa.row[i];
+        s.issue(lds0 + pair + (wave + (b ? NW : 0)) * SLAB, lane);
+        (b ? sb.base : sa.base) = s.base, (b ? sb.left : sa.left) = s.left;
+    };
+    auto next_pair = [&](int kb) {   // after an odd step
+        const uint32_t done = s_cur;
+        s_cur = kb & 1 ? s_next : s_cur, s_next = kb & 1 ? s_last : s_next, s_last = kb & 1 ? done : s_last;
+    };
     if (steps > 0) {
-        oa.issue(lds0, wave);
-        ob.issue(lds0 + B_AT, wave);
-        issue_scales(0);
-        oa.issue(lds0 + A_STEP, wave);
-        ob.issue(lds0 + B_AT + B_STEP, wave);
-        issue_scales(S_STEP);
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+            const auto s = oa.next();
+            issue_scales(false, S_AT + kb * S_PAIR);
+            issue_scales(true, S_AT + kb * S_PAIR);
+#pragma unroll
+            for (int q = 0; q < HALF; ++q) load_a(s, q, lds0 + kb * A_STEP);
+            ob.issue(lds0 + B_AT + kb * B_STEP, wave);
+#pragma unroll
+            for (int q = HALF; q < 2 * HALF; ++q) load_a(s, q, lds0 + kb * A_STEP);
+        }
         __builtin_amdgcn_sched_barrier(0);
-        wait_vmcnt_barrier<A_LOADS + B_LOADS + 2>();
+        wait_vmcnt_barrier<HALF + S_LOADS + IN_FLIGHT>();
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) op_a[0][ks] = fa.read(smem, 0, ks);
-        StepScales::read(a_scales(0, 0), lane, wa[0]);
+        read_a_scales(s_cur, 0, 0, wa[0]);
 #pragma unroll
         for (int j = 0; j < SN; ++j) {
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) op_b[j][ks] = fb.read(smem + B_AT, j, ks);
-            StepScales::read(b_scales(0, j), lane, wb[j]);
+            read_b_scales(s_cur, 0, j, wb[j]);
         }
     }
     const bool computes = m0 + wm * WM < m_end;   // else a wave of rows past the group's: it loads and synchronises only
     if (!computes) {
         for (int kb = 0; kb < steps; ++kb) {
-            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            wait_vmcnt_barrier<IN_FLIGHT>();
+            const auto s = oa.next();
+            issue_scales(kb & 1, s_last);
+            next_pair(kb);
+#pragma unroll
+            for (int q = 0; q < HALF; ++q) load_a(s, q, lds0 + (kb & 1) * A_STEP);
             ob.issue(lds0 + B_AT + (kb & 1) * B_STEP, wave);
             wait_vmcnt_barrier<IN_FLIGHT>();
-            oa.issue(lds0 + (kb & 1) * A_STEP, wave);
-            issue_scales((kb & 1) * S_STEP);
+#pragma unroll
+            for (int q = HALF; q < 2 * HALF; ++q) load_a(s, q, lds0 + (kb & 1) * A_STEP);
         }
     } else
     for (int kb = 0; kb < steps; ++kb) {
         const uint32_t odd = kb & 1, a_cur = odd * A_STEP, a_next = (odd ^ 1) * A_STEP;
-        const uint32_t b_cur = B_AT + odd * B_STEP, b_next = B_AT + (odd ^ 1) * B_STEP, s_cur = odd * S_STEP, s_next = (odd ^ 1) * S_STEP;
+        const uint32_t b_cur = B_AT + odd * B_STEP, b_next = B_AT + (odd ^ 1) * B_STEP;
+        const uint32_t s_ahead = odd ? s_next : s_cur;   // the next step's
         const StepScales scales(reduced / 8 - kb * 8);
         int eb[SN][2];
+        typename decltype(oa)::Step step_a;
+        typename decltype(ob)::Step step_b;
         // A slice's matrix instructions with the LDS reads and loads of the steps to come set
         // between them one by one (as the BF16 products').
-        constexpr int N = SN * KS, TOP = SM > 2 ? 1 : 0;
+        constexpr int N = SN * KS, TOP = SM / 2 - 1;
 #pragma unroll
         for (int i = 0; i < SM; ++i) {
             const bool last = i + 1 == SM;
-            typename decltype(oa)::Step step_a;
-            typename decltype(ob)::Step step_b;
             __builtin_amdgcn_sched_barrier(0);
             if (i == TOP) {
-                // every wave holds its B fragments and B's scales of this step, and A's up to slice TOP
-                asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-                step_b = ob.next();
-            }
-            if (last) {
                 wait_vmcnt_barrier<IN_FLIGHT>();
                 step_a = oa.next();
+                step_b = ob.next();
             }
+            if (last) wait_vmcnt_barrier<IN_FLIGHT>();
             int ea[2];
             scales.get(wa[i & 1], lane, ea);
             if (i == 0) {
@@ -210,25 +256,29 @@ __global__ void __launch_bounds__(WGM * WGN * 64, WGM * WGN == 4 ? 2 : 1) fp4_ti
                     if (last) op_a[0][n] = fa.read(smem + a_next, 0, n);
                     else op_a[(i + 1) & 1][n] = fa.read(smem + a_cur, i + 1, n);
                 }
-                if (n == 0) StepScales::read(last ? a_scales(s_next, 0) : a_scales(s_cur, i + 1), lane, wa[last ? 0 : (i + 1) & 1]);
-                if (last && n > 0 && n <= SN) StepScales::read(b_scales(s_next, n - 1), lane, wb[n - 1]);
+                if (n == 0) read_a_scales(last ? s_ahead : s_cur, last ? odd ^ 1 : odd, last ? 0 : i + 1, wa[last ? 0 : (i + 1) & 1]);
+                if (last && n > 0 && n <= SN) read_b_scales(s_ahead, odd ^ 1, n - 1, wb[n - 1]);
                 if (last && n >= KS) op_b[n / KS - 1][n % KS] = fb.read(smem + b_next, n / KS - 1, n % KS);
                 if (i == TOP) {
+                    if (n == 0) issue_scales(odd, s_last);
 #pragma unroll
-                    for (int q = n * B_LOADS / N; q < (n + 1) * B_LOADS / N; ++q) ob.load(step_b, q, lds0 + b_cur, wave);
+                    for (int q = n * (HALF + B_LOADS) / N; q < (n + 1) * (HALF + B_LOADS) / N; ++q) {
+                        if (q < HALF) load_a(step_a, q, lds0 + a_cur);
+                        else ob.load(step_b, q - HALF, lds0 + b_cur, wave);
+                    }
                 }
                 if (last) {
 #pragma unroll
-                    for (int q = n * A_LOADS / N; q < (n + 1) * A_LOADS / N; ++q) oa.load(step_a, q, lds0 + a_cur, wave);
+                    for (int q = n * HALF / N; q < (n + 1) * HALF / N; ++q) load_a(step_a, HALF + q, lds0 + a_cur);
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
             if (last) {
-                issue_scales(s_cur);
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks) op_b[SN - 1][ks] = fb.read(smem + b_next, SN - 1, ks);
             }
         }
+        next_pair(kb);
     }
     __builtin_amdgcn_sched_barrier(0);
     wait_vmcnt_barrier<0>();   // (loads of steps past the end wrote zeros to LDS)
@@ -250,7 +300,7 @@ __global__ void __launch_bounds__(256, 2) fp4_few_rows_kernel(const RaggedFp4Arg
 
     Operand<BM, 1, NW> oa;
     Operand<BN, 1, NW> ob;
-    ScaleSlab sa, sb;
+    ScaleSlab<2> sa, sb;
     const int a_rows = min(BM, t.m_end - t.m0), b_rows = min(BN, p.g.n - t.n0);
     oa.init(p.g.a + (int64_t)t.m0 * p.g.lda, p.g.lda, a_rows, reduced, wave, lane);
     ob.init(static_cast<const uint16_t*>(p.g.b) + (int64_t)t.g * p.g.b_gs + (int64_t)t.n0 * p.g.ldb, p.g.ldb, b_rows, reduced,
@@ -263,8 +313,8 @@ __global__ void __launch_bounds__(256, 2) fp4_few_rows_kernel(const RaggedFp4Arg
         const uint32_t at = lds0 + slot * STEP;
         oa.issue(at, wave);
         ob.issue(at + A_STEP, wave);
-        sa.issue(at + S_AT + wave * 512);
-        sb.issue(at + S_AT + wave * 512 + 256);
+        sa.issue(at + S_AT + wave * 512, lane);
+        sb.issue(at + S_AT + wave * 512 + 256, lane);
     };
     Fragments<BM, 1, 1> fa;
     Fragments<BN, 1, 1> fb;
@@ -291,8 +341,8 @@ __global__ void __launch_bounds__(256, 2) fp4_few_rows_kernel(const RaggedFp4Arg
             b[ks] = fb.read(at + A_STEP, 0, ks);
         }
         const StepScales scales(reduced / 8 - kb * 8);
-        scales.read(at + S_AT + wave * 512, lane, wa);
-        scales.read(at + S_AT + wave * 512 + 256, lane, wb);
+        scales.read<2>(at + S_AT + wave * 512, lane, 0, wa);
+        scales.read<2>(at + S_AT + wave * 512 + 256, lane, 0, wb);
         scales.get(wa, lane, ea), scales.get(wb, lane, eb);
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) acc[0][0] = mfma4(ks, b[ks], a[ks], acc[0][0], eb, ea);

@@ -203,7 +203,10 @@ struct Operand {
         load(s, i, lds, wave, kRows * (int)pitch);
     }
     __device__ __forceinline__ void load(const Step& s, int i, uint32_t lds, int wave, int apart) const {
-        const int seg = i * NW + wave;
+        load_rows(s, i * NW + wave, lds, apart);
+    }
+    // the wave load of rows (KMAJOR) 8 seg to 8 seg + 7; seg of the wave's parity
+    __device__ __forceinline__ void load_rows(const Step& s, int seg, uint32_t lds, int apart) const {
         dma16_buffer(s.rsrc, s.v + (uint32_t)(seg * apart), lds + seg * 1024);
     }
     __device__ __forceinline__ void issue(uint32_t lds, int wave) {
