@@ -87,6 +87,7 @@ std::atomic<int> g_num_sms{0};                 // 0: query the device
 std::atomic<int> g_mk_alignment{kDefaultMKAlignment};
 std::atomic<int> g_tile_variant{0}, g_tile_m{0}, g_tile_n{0};   // variant 0: heuristic
 std::atomic<int> g_ragged_block{0}, g_ragged_splits{0};         // variant 13: the ragged BF16 products'
+std::atomic<int> g_fp4_block{0}, g_fp4_splits{0};               // variant 14: the ragged 4-bit product's
 
 template <typename F>
 int guarded(F&& f) {
@@ -1821,7 +1822,7 @@ void check_fp4_scales(const View& sf, int dims, int64_t groups, int64_t rows, in
 }
 
 RaggedPlan ragged_fp4_plan(const RaggedFp4Args& a) {
-    const RaggedPlan plan = plan_ragged_fp4(a, num_sms_now(), g_ragged_block.load(), g_ragged_splits.load());
+    const RaggedPlan plan = plan_ragged_fp4(a, num_sms_now(), g_fp4_block.load(), g_fp4_splits.load());
     check_ragged_fp4_launches(a, plan);
     return plan;
 }
@@ -2026,6 +2027,7 @@ int dg_init(void) {
         g_tile_m = 0;
         g_tile_n = 0;
         g_ragged_block = 0, g_ragged_splits = 0;
+        g_fp4_block = 0, g_fp4_splits = 0;
     });
 }
 
@@ -2339,7 +2341,14 @@ int dg_set_tile_override(int32_t variant, int32_t block_m, int32_t block_n) {
     return guarded([&] {
         if (variant == 0) {
             g_tile_variant = 0, g_tile_m = 0, g_tile_n = 0;
-            g_ragged_block = 0, g_ragged_splits = 0;
+            g_ragged_block = 0, g_ragged_splits = 0, g_fp4_block = 0, g_fp4_splits = 0;
+            return;
+        }
+        if (variant == 14) {
+            if ((block_m != 32 && block_m != 64 && block_m != 128 && block_m != 256) || block_n < 0 ||
+                block_n > (block_m == 256 ? 0 : 32))
+                DG_UNSUPPORTED("tile shape not compiled");
+            g_fp4_block = block_m, g_fp4_splits = block_n;
             return;
         }
         if (variant == 13) {

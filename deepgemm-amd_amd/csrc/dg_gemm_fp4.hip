@@ -158,9 +158,23 @@ __global__ void __launch_bounds__(WGM * WGN * 64, WGM * WGN == 4 ? 2 : 1) fp4_ti
     constexpr int HALF = decltype(oa)::kInstr / 2, B_LOADS = decltype(ob)::kInstr, S_LOADS = decltype(sa)::kLoads;
     constexpr int TOP_LOADS = S_LOADS + HALF + B_LOADS;
     constexpr int IN_FLIGHT = TOP_LOADS + HALF, PER_SLICE = HALF * 2 / SM;   // loads of a slice
-    auto load_a = [&](const typename decltype(oa)::Step& s, int q, uint32_t lds) {   // the q-th of a step's
-        const int x = q % PER_SLICE * NW + wave;   // 8-row piece of the slice, four of each wave row
-        oa.load_rows(s, (x >> 2) * (SM * 4) + q / PER_SLICE * 4 + (x & 3), lds, decltype(oa)::kRows * (int)oa.pitch);
+    // The q-th load of a step of A: pieces of 8 rows of its slice, four of each wave row. (Offsets
+    // worked out where they are used, from few scalars: kept, they would fill the scalar registers.)
+    const uint32_t wave_lds = lds0 + wave * 1024;
+    const int wave_piece = NW == 8 ? (wave >> 2) * (SM * 4) + (wave & 3) : wave;
+    auto load_a = [&](const typename decltype(oa)::Step& s, int q, uint32_t at) {
+        static_assert(NW == 4 || NW == 8, "pieces of one wave row or of both by each load");
+        const int piece = q % PER_SLICE * (SM * 4) + q / PER_SLICE * 4;   // (+ wave_piece)
+        int apart = decltype(oa)::kRows * (int)oa.pitch, mine = wave_piece;
+        uint32_t lds = lds0 + at;
+        asm volatile("" : "+s"(apart), "+s"(lds), "+s"(mine));
+        dma16_buffer(s.rsrc, s.v + (uint32_t)((piece + mine) * apart), lds + (piece + mine) * 1024);
+    };
+    auto load_b = [&](const typename decltype(ob)::Step& s, int q, uint32_t at) {
+        int apart = decltype(ob)::kRows * (int)ob.pitch;
+        uint32_t lds = wave_lds + at;
+        asm volatile("" : "+s"(apart), "+s"(lds));
+        dma16_buffer(s.rsrc, s.v + (uint32_t)((q * NW + wave) * apart), lds + q * (NW * 1024));
     };
     // Scales come two steps at a time: A's of the pair after the next in even steps, B's in odd ones,
     // to the place after the next pair's (three places).
@@ -185,10 +199,10 @@ __global__ void __launch_bounds__(WGM * WGN * 64, WGM * WGN == 4 ? 2 : 1) fp4_ti
             issue_scales(false, S_AT + kb * S_PAIR);
             issue_scales(true, S_AT + kb * S_PAIR);
 #pragma unroll
-            for (int q = 0; q < HALF; ++q) load_a(s, q, lds0 + kb * A_STEP);
+            for (int q = 0; q < HALF; ++q) load_a(s, q, kb * A_STEP);
             ob.issue(lds0 + B_AT + kb * B_STEP, wave);
 #pragma unroll
-            for (int q = HALF; q < 2 * HALF; ++q) load_a(s, q, lds0 + kb * A_STEP);
+            for (int q = HALF; q < 2 * HALF; ++q) load_a(s, q, kb * A_STEP);
         }
         __builtin_amdgcn_sched_barrier(0);
         wait_vmcnt_barrier<HALF + S_LOADS + IN_FLIGHT>();
@@ -211,11 +225,11 @@ __global__ void __launch_bounds__(WGM * WGN * 64, WGM * WGN == 4 ? 2 : 1) fp4_ti
             issue_scales(kb & 1, s_last);
             next_pair(kb);
 #pragma unroll
-            for (int q = 0; q < HALF; ++q) load_a(s, q, lds0 + (kb & 1) * A_STEP);
+            for (int q = 0; q < HALF; ++q) load_a(s, q, (kb & 1) * A_STEP);
             ob.issue(lds0 + B_AT + (kb & 1) * B_STEP, wave);
             wait_vmcnt_barrier<IN_FLIGHT>();
 #pragma unroll
-            for (int q = HALF; q < 2 * HALF; ++q) load_a(s, q, lds0 + (kb & 1) * A_STEP);
+            for (int q = HALF; q < 2 * HALF; ++q) load_a(s, q, (kb & 1) * A_STEP);
         }
     } else
     for (int kb = 0; kb < steps; ++kb) {
@@ -263,13 +277,13 @@ __global__ void __launch_bounds__(WGM * WGN * 64, WGM * WGN == 4 ? 2 : 1) fp4_ti
                     if (n == 0) issue_scales(odd, s_last);
 #pragma unroll
                     for (int q = n * (HALF + B_LOADS) / N; q < (n + 1) * (HALF + B_LOADS) / N; ++q) {
-                        if (q < HALF) load_a(step_a, q, lds0 + a_cur);
-                        else ob.load(step_b, q - HALF, lds0 + b_cur, wave);
+                        if (q < HALF) load_a(step_a, q, a_cur);
+                        else load_b(step_b, q - HALF, b_cur);
                     }
                 }
                 if (last) {
 #pragma unroll
-                    for (int q = n * HALF / N; q < (n + 1) * HALF / N; ++q) load_a(step_a, HALF + q, lds0 + a_cur);
+                    for (int q = n * HALF / N; q < (n + 1) * HALF / N; ++q) load_a(step_a, HALF + q, a_cur);
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
@@ -287,68 +301,91 @@ __global__ void __launch_bounds__(WGM * WGN * 64, WGM * WGN == 4 ? 2 : 1) fp4_ti
     else store_tile<0, BM, BN, WGM, WGN>(p.g, acc, smem, 0, m0, m_end, n0, wave, lane, l.vec);
 }
 
-// 32 x 128 tiles on four waves of 32 x 32, two workgroups on a CU.
+// Few rows a group (decode): 32 x 128 or 64 x 128 tiles on four waves of 32 columns, two
+// workgroups on a CU, which stream the weights from HBM. Three steps of 21 or 26 KB in LDS and one
+// barrier a step: it certifies the next step's loads and frees this one's place, whose
+// fragments every wave holds. (A slab of A's scales is loaded by more than one wave, to one place.)
+template <int SM>
 __global__ void __launch_bounds__(256, 2) fp4_few_rows_kernel(const RaggedFp4Args p, const RaggedLaunch l) {
-    constexpr int BM = kFewRows, BN = 128, NW = 4, KS = 4, SLOTS = 3;
-    constexpr int A_STEP = BM * BK * 2, B_STEP = BN * BK * 2, S_AT = A_STEP + B_STEP, STEP = S_AT + NW * 512;
+    constexpr int BM = SM * 32, BN = 128, NW = 4, KS = 4, SLOTS = 3, SLAB = ScaleSlab<2>::kBytes;
+    constexpr int A_STEP = BM * BK * 2, B_STEP = BN * BK * 2, S_AT = A_STEP + B_STEP, STEP = S_AT + (SM + NW) * SLAB;
+    static_assert(NW % SM == 0 && BM * BN * 4 <= SLOTS * STEP, "whole slabs; the epilogue's rows fit");
     __shared__ __attribute__((aligned(1024))) uint8_t smem[SLOTS * STEP];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     RaggedTile t{};
     if (!locate_rows<BM, BN, 0>(p.g, l, t)) return;
-    const int reduced = p.g.k, words = (reduced + 31) / 32;
+    const int piece = ((p.g.k + BK - 1) / BK + l.splits - 1) / l.splits * BK;   // (as in the tile kernel)
+    const int k0 = min((int)blockIdx.y * piece, p.g.k);
+    const int reduced = min(piece, p.g.k - k0), words = (reduced + 31) / 32;
 
     Operand<BM, 1, NW> oa;
     Operand<BN, 1, NW> ob;
     ScaleSlab<2> sa, sb;
     const int a_rows = min(BM, t.m_end - t.m0), b_rows = min(BN, p.g.n - t.n0);
-    oa.init(p.g.a + (int64_t)t.m0 * p.g.lda, p.g.lda, a_rows, reduced, wave, lane);
-    ob.init(static_cast<const uint16_t*>(p.g.b) + (int64_t)t.g * p.g.b_gs + (int64_t)t.n0 * p.g.ldb, p.g.ldb, b_rows, reduced,
+    oa.init(p.g.a + (int64_t)t.m0 * p.g.lda + k0, p.g.lda, a_rows, reduced, wave, lane);
+    ob.init(static_cast<const uint16_t*>(p.g.b) + (int64_t)t.g * p.g.b_gs + (int64_t)t.n0 * p.g.ldb + k0, p.g.ldb, b_rows, reduced,
             wave, lane);
-    sa.init(p.a_sf + (int64_t)t.m0 * p.a_sr, p.a_sr, p.a_sk, 0, a_rows, words, lane);
-    sb.init(p.b_sf + (int64_t)t.g * p.b_sg + (int64_t)t.n0 * p.b_sr, p.b_sr, p.b_sk, wave * 32, b_rows, words, lane);
+    sa.init(p.a_sf + (int64_t)t.m0 * p.a_sr + (int64_t)(k0 / 32) * p.a_sk, p.a_sr, p.a_sk, wave % SM * 32, a_rows, words, lane);
+    sb.init(p.b_sf + (int64_t)t.g * p.b_sg + (int64_t)t.n0 * p.b_sr + (int64_t)(k0 / 32) * p.b_sk, p.b_sr, p.b_sk, wave * 32, b_rows,
+            words, lane);
     constexpr int LOADS = decltype(oa)::kInstr + decltype(ob)::kInstr + 2;
     const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_address(smem));
     auto issue = [&](int slot) {
         const uint32_t at = lds0 + slot * STEP;
         oa.issue(at, wave);
         ob.issue(at + A_STEP, wave);
-        sa.issue(at + S_AT + wave * 512, lane);
-        sb.issue(at + S_AT + wave * 512 + 256, lane);
+        sa.issue(at + S_AT + wave % SM * SLAB, lane);
+        sb.issue(at + S_AT + (SM + wave) * SLAB, lane);
     };
-    Fragments<BM, 1, 1> fa;
+    Fragments<BM, 1, SM> fa;
     Fragments<BN, 1, 1> fb;
     fa.init(0, lane);
     fb.init(wave * 32, lane);
-    f32x16 acc[1][1];
+    bf16x8 op_a[2][SM][KS], op_b[2][KS];
+    uint32_t wa[2][SM][2], wb[2][2];
+    auto read = [&](int to, int slot) {
+        const uint8_t* at = smem + slot * STEP;
 #pragma unroll
-    for (int e = 0; e < 16; ++e) acc[0][0][e] = 0.f;
+        for (int ks = 0; ks < KS; ++ks) {
+            op_b[to][ks] = fb.read(at + A_STEP, 0, ks);
+#pragma unroll
+            for (int i = 0; i < SM; ++i) op_a[to][i][ks] = fa.read(at, i, ks);
+        }
+        StepScales::read<2>(at + S_AT + (SM + wave) * SLAB, lane, 0, wb[to]);
+#pragma unroll
+        for (int i = 0; i < SM; ++i) StepScales::read<2>(at + S_AT + i * SLAB, lane, 0, wa[to][i]);
+    };
+    f32x16 acc[SM][1];
+#pragma unroll
+    for (int i = 0; i < SM; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[i][0][e] = 0.f;
 
     const int steps = (reduced + BK - 1) / BK;
     if (steps > 0) {   // (no reduced elements: no scales to read)
 #pragma unroll
         for (int st = 0; st < SLOTS; ++st) issue(st);
-    }
-    for (int kb = 0, slot = 0; kb < steps; ++kb) {
         wait_vmcnt_barrier<(SLOTS - 1) * LOADS>();
-        const uint8_t* at = smem + slot * STEP;
-        bf16x8 a[KS], b[KS];
-        uint32_t wa[2], wb[2];
-        int ea[2], eb[2];
+        read(0, 0);
+    }
+    for (int kb = 0, slot = 0; kb < steps; kb += 2) {   // (a step past an odd end: zeros)
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-            a[ks] = fa.read(at, 0, ks);
-            b[ks] = fb.read(at + A_STEP, 0, ks);
+        for (int h = 0; h < 2; ++h) {
+            wait_vmcnt_barrier<(SLOTS - 2) * LOADS>();
+            issue(slot);
+            slot = slot + 1 == SLOTS ? 0 : slot + 1;
+            read(h ^ 1, slot);
+            const StepScales scales(reduced / 8 - (kb + h) * 8);
+            int ea[SM][2], eb[2];
+            scales.get(wb[h], lane, eb);
+#pragma unroll
+            for (int i = 0; i < SM; ++i) scales.get(wa[h][i], lane, ea[i]);
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                for (int i = 0; i < SM; ++i) acc[i][0] = mfma4(ks, op_b[h][ks], op_a[h][i][ks], acc[i][0], eb, ea[i]);
         }
-        const StepScales scales(reduced / 8 - kb * 8);
-        scales.read<2>(at + S_AT + wave * 512, lane, 0, wa);
-        scales.read<2>(at + S_AT + wave * 512 + 256, lane, 0, wb);
-        scales.get(wa, lane, ea), scales.get(wb, lane, eb);
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) acc[0][0] = mfma4(ks, b[ks], a[ks], acc[0][0], eb, ea);
-        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");   // every wave has read this step
-        issue(slot);
-        slot = slot + 1 == SLOTS ? 0 : slot + 1;
     }
     wait_vmcnt_barrier<0>();   // (loads of steps past the end wrote zeros to LDS)
     if (p.g.out_f32) store_tile<1, BM, BN, 1, NW>(p.g, acc, smem, 0, t.m0, t.m_end, t.n0, wave, lane, l.vec);
@@ -357,19 +394,63 @@ __global__ void __launch_bounds__(256, 2) fp4_few_rows_kernel(const RaggedFp4Arg
 
 }  // namespace
 
-RaggedPlan plan_ragged_fp4(const RaggedFp4Args& a, int slots, int block, int) {
-    if (block) return RaggedPlan{block, 1, 0};
-    const int64_t used = std::max<int64_t>(1, std::min<int64_t>(a.g.groups, a.g.rows));
-    if (a.g.rows <= kFewRows * used) return RaggedPlan{kFewRows, 1, 0};
-    return RaggedPlan{(a.g.rows / 256 + 0.5 * used) * ceil_div(a.g.n, 256) * 128 >= slots * 75 ? 256 : 128, 1, 0};
+// Tiles and pieces of the reduced axis by a model of the time, in us: a step (256 elements) of a
+// tile on a CU takes 0.38, 0.5 and 0.7 (32, 64 and 128 rows) alone and 0.88, 0.98 and 1.35 beside another,
+// 1.9 of 256 x 256; a tile's start and end 2 (256 x 256: 10); a split call 3.5 more and its sums'
+// two ways at 2 TB/s. Row blocks of a group that has rows: as many as its average, and half a one,
+// at least one. Both sides measured (us; NT, groups x (rows in all), n, k):
+// 256 x 256 and 128 x 128: 8 x 16384, 4096, 7168 286 and 331; 8 x 8192, 7168, 2048 99 and 113; 8 x 2048, 4096,
+//   7168 61 and 66; 32 x 2048, 4096, 2048 42 and 32; 1 x 4096, 4096, 1024 22.1 and 20.7.
+// Where 128 x 128 tiles fill three quarters of the CUs, smaller ones only read weights again: 128,
+//   64 and 32 rows at 8 x 256, 4096, 7168 31, 49 and 45; 32 x 1024, 4096, 2048 30, 36 and 41; but up to 16 rows a group
+//   they are as fast or faster: 8 x 8, 4096, 7168 26.5, 26.6 and 26.1; 32 x 256, 4096, 2048 26.5, 25.8 and 25.1.
+// Where they do not: 1 x 512, 4096, 7168 22, 19 and 27; 1 x 256, 2112, 7168 22, 18 and 16; 2 x 128, 4096, 4096 14.7, 12.6
+//   and 11.4.
+// Whole, in 2, 4 and 8 pieces, 32 rows: 1 x 64, 2112, 7168 15.4, 13.9, 12.3, 14.3; 1 x 256, 2112, 7168 15.6, 20.2, 22.7, 23.1.
+RaggedPlan plan_ragged_fp4(const RaggedFp4Args& a, int slots, int block, int splits) {
+    const double used = (double)std::max<int64_t>(1, std::min<int64_t>(a.g.groups, a.g.rows));   // groups with rows, at most
+    const double steps = (double)ceil_div(a.g.k, BK), rows = (double)a.g.rows;
+    auto tiles = [&](int b) {   // expected
+        return std::max(used, rows / b + (rows > used ? 0.5 * used : 0.0)) * (double)ceil_div(a.g.n, b == 256 ? 256 : 128);
+    };
+    auto us = [&](int b, double t, double n) {   // t tiles of n steps, two of which fit a CU
+        const double alone = b == 32 ? 0.38 : b == 64 ? 0.5 : 0.7, both = b == 32 ? 0.88 : b == 64 ? 0.98 : 1.35, ends = 2.0;
+        const double per_cu = t / slots, whole = std::floor(per_cu / 2), rest = per_cu - 2 * whole;
+        return whole * (n * both + ends) +
+               (rest > 0 ? n * (alone + (both - alone) * std::max(0.0, rest - 1)) + ends * std::min(rest, 1.0) : 0.0);
+    };
+    if (block == 0) {
+        const double t128 = tiles(128), t256 = tiles(256);
+        if (t256 * 128 >= slots * 75 && std::max(1.0, t256 / slots) * (steps * 1.9 + 10) < 1.1 * us(128, t128, steps)) {
+            block = 256;
+        } else if (t128 * 4 >= slots * 3) {
+            block = rows <= 16 * used ? kFewRows : 128;
+        } else {   // (the larger of two that are about as fast)
+            block = 128;
+            for (int b : {64, 32})
+                if (us(b, tiles(b), steps) < 0.95 * us(block, tiles(block), steps)) block = b;
+        }
+    }
+    RaggedPlan plan{block, 1, 0};
+    if (block == 256) return plan;
+    const double sums = rows * a.g.n * 4;   // bytes of a piece's
+    double best = 1e300;
+    for (int s = 1; s <= 32; ++s) {
+        if (splits > 0 ? s != splits : (s > 1 && steps < 4 * s)) continue;
+        const double t = us(block, tiles(block) * s, std::ceil(steps / s)) + (s > 1 ? 3.5 + 2 * sums * s / 2e6 : 0.0);
+        if (t < best) best = t, plan.splits = s;
+    }
+    if (plan.splits > 1) plan.workspace_bytes = (int64_t)a.g.rows * ceil_div(a.g.n, 4) * 16 * plan.splits;
+    return plan;
 }
 
 void check_ragged_fp4_launches(const RaggedFp4Args& a, const RaggedPlan& plan) {
-    if (plan.block == kFewRows) {
-        DG_CHECK_GRID(row_blocks(kRaggedNT, a.g, kFewRows) * ceil_div(a.g.n, 128), 256);
+    if (plan.block <= 2 * kFewRows) {
+        DG_CHECK_GRID(row_blocks(kRaggedNT, a.g, plan.block) * ceil_div(a.g.n, 128), 256);
     } else {
         DG_CHECK_GRID(tile_blocks(kRaggedNT, a.g, plan.block, false, 1), plan.block * 2);
     }
+    if (plan.splits > 1) DG_CHECK_GRID(join_blocks(kRaggedNT, a.g), 256);
 }
 
 namespace {
@@ -385,18 +466,37 @@ void launch_fp4_tiles(const RaggedFp4Args& a, int slots, int splits, hipStream_t
     DG_HIP_CHECK(hipGetLastError());
 }
 
+template <int SM>
+void launch_fp4_few_rows(const RaggedFp4Args& a, int slots, int splits, hipStream_t stream) {
+    const int64_t mb = row_blocks(kRaggedNT, a.g, SM * 32), nb = ceil_div(a.g.n, 128);
+    const RaggedLaunch l{(int)mb, (int)nb, slots, splits, takes_vectors(a.g)};
+    hipLaunchKernelGGL(fp4_few_rows_kernel<SM>, dim3((unsigned)(mb * nb), (unsigned)splits), dim3(256), 0, stream, a, l);
+    DG_HIP_CHECK(hipGetLastError());
+}
+
 }  // namespace
 
-void launch_ragged_fp4(const RaggedFp4Args& a, const RaggedPlan& plan, float*, int slots, hipStream_t stream) {
+void launch_ragged_fp4(const RaggedFp4Args& a, const RaggedPlan& plan, float* ws, int slots, hipStream_t stream) {
+    DG_CHECK(plan.splits == 1 || ws != nullptr);
     if (plan.block == 256) {
         launch_fp4_tiles<256, 256, 2, 4, 1>(a, slots, 1, stream);
         launch_fp4_tiles<128, 128, 2, 2, 2>(a, slots, 1, stream);
         return;
     }
-    if (plan.block == 128) return launch_fp4_tiles<128, 128, 2, 2, 0>(a, slots, 1, stream);
-    const int64_t mb = row_blocks(kRaggedNT, a.g, kFewRows), nb = ceil_div(a.g.n, 128);
-    const RaggedLaunch l{(int)mb, (int)nb, slots, 1, takes_vectors(a.g)};
-    hipLaunchKernelGGL(fp4_few_rows_kernel, dim3((unsigned)(mb * nb)), dim3(256), 0, stream, a, l);
+    auto launch = [&](const RaggedFp4Args& args) {
+        if (plan.block == kFewRows) launch_fp4_few_rows<1>(args, slots, plan.splits, stream);
+        else if (plan.block == 2 * kFewRows) launch_fp4_few_rows<2>(args, slots, plan.splits, stream);
+        else launch_fp4_tiles<128, 128, 2, 2, 0>(args, slots, plan.splits, stream);
+    };
+    if (plan.splits == 1) return launch(a);
+    const int64_t ld = ceil_div(a.g.n, 4) * 4;
+    RaggedFp4Args part = a;
+    part.g.d = ws, part.g.ldd = ld, part.g.d_split = a.g.rows * ld, part.g.out_f32 = 1;
+    launch(part);
+    RaggedGemmArgs whole = a.g;
+    whole.d_split = part.g.d_split;
+    hipLaunchKernelGGL(ragged_join_kernel<kRaggedNT>, dim3((unsigned)join_blocks(kRaggedNT, a.g)), dim3(256), 0, stream, whole,
+                       (const float*)ws, ld, plan.splits, (int)ceil_div(a.g.n, 1024));
     DG_HIP_CHECK(hipGetLastError());
 }
 

@@ -568,6 +568,7 @@ int32_t dg_get_theoretical_mk_alignment_for_contiguous_layout(int32_t expected_m
  * block_n 32 or 64: rows and columns per workgroup), 12 = the K-split kernel of
  * dense calls (128 x 128), 13 = the tile of the ragged BF16 products (block_m 32
  * (TN: 128), 128 or 256; block_n = pieces of the reduced axis, below 256, 0 for the heuristic's count);
+ * 14 = the tile of the ragged 4-bit product (block_m 32, 64, 128 or 256; block_n = pieces as for 13);
  * variant 0 restores the heuristic. Only compiled tile shapes are accepted. */
 int dg_set_tile_override(int32_t variant, int32_t block_m, int32_t block_n);
 

@@ -16,11 +16,13 @@ pytestmark = pytest.mark.gpu
 MIXED = [5, 0, 1, 130, 0, 64, 257, 31, 0]
 
 
-@pytest.fixture(autouse=True, params=['heuristic', '256', '128', '32'])
+@pytest.fixture(autouse=True, params=['heuristic', '256', '128', '128 in 3 pieces', '64', '32', '32 in 2 pieces'])
 def tiles(request):
     """Every test with the tiles the sizes choose, and with each kind forced."""
-    if request.param != 'heuristic':
-        deep_gemm.set_tile_override(int(request.param), 0, variant=13)
+    block, pieces = {'heuristic': (0, 0), '256': (256, 0), '128': (128, 1), '128 in 3 pieces': (128, 3), '64': (64, 1), '32': (32, 1),
+                     '32 in 2 pieces': (32, 2)}[request.param]
+    if block:
+        deep_gemm.set_tile_override(block, pieces, variant=14)
     yield request.param
     deep_gemm.set_tile_override(0, 0)
 
