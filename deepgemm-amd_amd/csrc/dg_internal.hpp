@@ -260,6 +260,7 @@ void launch_per_token_cast(const CastArgs& args, hipStream_t stream);
 constexpr int kMoeMaxExperts = 1024;
 constexpr int kMoeMaxTopk = 16;
 constexpr int kMoeChunkTokens = 64;    // tokens per dispatch chunk (count / scatter workgroup)
+constexpr int64_t kMoeFewOne = 1 << 20, kMoeFewCounts = 1 << 23;   // entries x workgroups (launch_moe_dispatch)
 enum MoeLayout : int32_t { kMoeContiguous = 0, kMoePsum = 1, kMoeMasked = 2 };
 struct MoeDispatchArgs {
     const uint8_t* x;          // rows of kdim bytes (e4m3, packed e2m1, BF16) [t]

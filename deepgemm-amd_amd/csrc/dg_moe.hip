@@ -11,10 +11,9 @@
 //               among equal experts with ballots (in entry order; the rank goes
 //               to pos) and leaves the chunk's count per expert;
 //   2. scan:    one wave per expert: exclusive prefix over chunks, the total,
-//               and the masked counts;
-//   3. starts:  (contiguous / psum) one block scans the aligned totals into
-//               the segment starts and the psum ends;
-//   4. scatter: one wave per token turns its k ranks into rows, reads the
+//               and the masked counts; the last block to be done scans the aligned totals
+//               into the segment starts and the psum ends (contiguous / psum);
+//   3. scatter: one wave per token turns its k ranks into rows, reads the
 //               token's K bytes once and stores them to each routed row, with
 //               the SF row, the weight and m_indices; beside them (contiguous /
 //               psum) a block per expert fills its padding rows (zero A, SF and
@@ -112,52 +111,14 @@ __global__ void __launch_bounds__(kThreads) moe_count_kernel(const MoeDispatchAr
     __syncthreads();
     for (int e = threadIdx.x; e < p.num_experts; e += kThreads)
         ws_counts(p)[(int64_t)e * p.chunks + c] = run[e];
+    if (c == 0 && threadIdx.x == 0) ws_totals(p)[p.num_experts] = 0;   // (moe_scan_kernel counts its workgroups there)
 }
 
-// One wave per expert: the exclusive prefix of its chunk counts (in place, 256
-// chunks per round, 4 consecutive chunks per lane), its total, and for the
-// masked layout masked_m = min(total, max_m).
-__global__ void __launch_bounds__(kThreads) moe_scan_kernel(const MoeDispatchArgs p) {
-    const int lane = threadIdx.x & 63;
-    const int e = blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
-    if (e >= p.num_experts) return;   // wave-uniform
-    int32_t* cnt = ws_counts(p) + (int64_t)e * p.chunks;
-    int carry = 0;
-    for (int c0 = 0; c0 < p.chunks; c0 += 256) {
-        const int c = c0 + lane * 4;
-        int v[4], s = 0;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            v[q] = c + q < p.chunks ? cnt[c + q] : 0;
-            s += v[q];
-        }
-        const int incl = wave_inclusive_sum(s, lane);
-        int x = carry + incl - s;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            if (c + q < p.chunks) cnt[c + q] = x;
-            x += v[q];
-        }
-        carry += __shfl(incl, 63);
-    }
-    if (lane == 0) {
-        ws_totals(p)[e] = carry;
-        if (p.layout == kMoeMasked) p.meta[e] = min(carry, p.max_m);
-    }
-}
-
-// Row p of the output layout (flattened for masked: e * max_m + r).
-__device__ __forceinline__ int64_t row_a(const MoeDispatchArgs& p, int64_t r) {
-    return p.layout == kMoeMasked ? (r / p.max_m) * p.a_gs + (r % p.max_m) * p.lda : r * p.lda;
-}
-__device__ __forceinline__ int64_t row_sf(const MoeDispatchArgs& p, int64_t r) {
-    return p.layout == kMoeMasked ? (r / p.max_m) * p.sf_gs + (r % p.max_m) * p.sf_sm : r * p.sf_sm;
-}
-
-// Contiguous and psum layouts, one block: the exclusive prefix of the aligned
-// expert totals (E <= 4 * kThreads, 4 experts per thread) gives the segment
-// starts; also the psum ends and the rows the segments use.
-__global__ void __launch_bounds__(kThreads) moe_starts_kernel(const MoeDispatchArgs p) {
+// Contiguous and psum layouts, one workgroup: the exclusive prefix of the aligned expert totals
+// (E <= 4 * kThreads, 4 experts per thread) gives the segment starts. total(e): expert e's rows;
+// start(e, first row, rows). Returns, in the last thread, the rows that the segments use.
+template <typename Total, typename Start>
+__device__ __forceinline__ int segment_starts(const MoeDispatchArgs& p, Total&& total, Start&& start) {
     static_assert(kMoeMaxExperts <= 4 * kThreads, "4 experts per thread");
     __shared__ int wsum[kThreads / 64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -165,7 +126,7 @@ __global__ void __launch_bounds__(kThreads) moe_starts_kernel(const MoeDispatchA
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
         const int e = threadIdx.x * 4 + q;
-        tot[q] = e < p.num_experts ? ws_totals(p)[e] : 0;
+        tot[q] = e < p.num_experts ? total(e) : 0;
         v[q] = align_up(tot[q], p.alignment);
         s += v[q];
     }
@@ -177,29 +138,75 @@ __global__ void __launch_bounds__(kThreads) moe_starts_kernel(const MoeDispatchA
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
         const int e = threadIdx.x * 4 + q;
-        if (e < p.num_experts) {
-            ws_starts(p)[e] = x;
-            if (p.layout == kMoePsum) p.meta[e] = x + tot[q];   // psum[e] = align(psum[e-1]) + count
-        }
+        if (e < p.num_experts) start(e, x, tot[q]);
         x += v[q];
     }
-    if (threadIdx.x == kThreads - 1) ws_totals(p)[p.num_experts] = x;   // rows used by the segments
+    return x;
 }
 
-// Contiguous and psum layouts: e < E fills expert e's padding rows (zero A, SF
-// and weight, m_indices = -1); e = E sets m_indices = -1 and the weights to zero past the segments.
-__device__ __forceinline__ void pad_block(const MoeDispatchArgs& p, int e) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    if (e == p.num_experts) {
-        const int used = ws_totals(p)[p.num_experts];
-        for (int64_t r = used + threadIdx.x; r < p.cap_rows; r += kThreads) {
-            if (p.layout == kMoeContiguous) p.meta[r] = -1;
-            if (p.w_out) p.w_out[r] = 0.f;
+// One wave per expert: the exclusive prefix of its chunk counts (in place, 256
+// chunks per round, 4 consecutive chunks per lane), its total, and for the
+// masked layout masked_m = min(total, max_m). For the other layouts the workgroup that is the last
+// to have its totals written (a count in the place of the used rows, which moe_count_kernel has
+// cleared) goes on to the segment starts, the psum ends and the rows the segments use.
+__global__ void __launch_bounds__(kThreads) moe_scan_kernel(const MoeDispatchArgs p) {
+    __shared__ int s_done;
+    const int lane = threadIdx.x & 63;
+    const int e = blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
+    if (e < p.num_experts) {   // wave-uniform
+        int32_t* cnt = ws_counts(p) + (int64_t)e * p.chunks;
+        int carry = 0;
+        for (int c0 = 0; c0 < p.chunks; c0 += 256) {
+            const int c = c0 + lane * 4;
+            int v[4], s = 0;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                v[q] = c + q < p.chunks ? cnt[c + q] : 0;
+                s += v[q];
+            }
+            const int incl = wave_inclusive_sum(s, lane);
+            int x = carry + incl - s;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                if (c + q < p.chunks) cnt[c + q] = x;
+                x += v[q];
+            }
+            carry += __shfl(incl, 63);
         }
-        return;
+        if (lane == 0) {
+            __hip_atomic_store(ws_totals(p) + e, carry, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            if (p.layout == kMoeMasked) p.meta[e] = min(carry, p.max_m);
+        }
     }
-    const int total = ws_totals(p)[e], start = ws_starts(p)[e];
-    const int r0 = start + total, r1 = start + align_up(total, p.alignment);
+    if (p.layout == kMoeMasked) return;   // uniform over the launch
+    int32_t* used = ws_totals(p) + p.num_experts;
+    __threadfence();   // (each wave's total before the workgroup is counted)
+    __syncthreads();
+    if (threadIdx.x == 0) s_done = __hip_atomic_fetch_add(used, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    if (s_done != (int)gridDim.x - 1) return;   // workgroup-uniform
+    __threadfence();
+    const int rows = segment_starts(
+        p, [&](int x) { return __hip_atomic_load(ws_totals(p) + x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); },
+        [&](int x, int start, int total) {
+            ws_starts(p)[x] = start;
+            if (p.layout == kMoePsum) p.meta[x] = start + total;   // psum[e] = align(psum[e-1]) + count
+        });
+    if (threadIdx.x == kThreads - 1) *used = rows;
+}
+
+// Row p of the output layout (flattened for masked: e * max_m + r).
+__device__ __forceinline__ int64_t row_a(const MoeDispatchArgs& p, int64_t r) {
+    return p.layout == kMoeMasked ? (r / p.max_m) * p.a_gs + (r % p.max_m) * p.lda : r * p.lda;
+}
+__device__ __forceinline__ int64_t row_sf(const MoeDispatchArgs& p, int64_t r) {
+    return p.layout == kMoeMasked ? (r / p.max_m) * p.sf_gs + (r % p.max_m) * p.sf_sm : r * p.sf_sm;
+}
+
+// Contiguous and psum layouts: the padding rows [r0, r1) of a segment get zero A, SF and
+// weight and m_indices = -1.
+__device__ __forceinline__ void pad_rows(const MoeDispatchArgs& p, int r0, int r1) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     for (int r = r0 + wave; r < r1; r += kThreads / 64) {
         uint8_t* a = p.a + row_a(p, r);
         for (int c = lane * 16; c < p.kdim; c += 64 * 16)
@@ -211,6 +218,13 @@ __device__ __forceinline__ void pad_block(const MoeDispatchArgs& p, int e) {
         }
     }
 }
+// Past the segments (from row r0 on, every `step`-th): m_indices = -1, weights zero.
+__device__ __forceinline__ void pad_past(const MoeDispatchArgs& p, int64_t r0, int64_t step) {
+    for (int64_t r = r0; r < p.cap_rows; r += step) {
+        if (p.layout == kMoeContiguous) p.meta[r] = -1;
+        if (p.w_out) p.w_out[r] = 0.f;
+    }
+}
 
 // One wave per token: lane j < k turns slot j's chunk rank into its output row
 // (segment start + the expert's prefix over earlier chunks + the rank; for the
@@ -218,10 +232,16 @@ __device__ __forceinline__ void pad_block(const MoeDispatchArgs& p, int e) {
 // then the wave reads the token's K bytes once, 8 KB per round (8 x 16 B per
 // lane in flight), and stores them to each routed row, then the SF row. The
 // first pad_blocks blocks (E + 1 for the contiguous and psum layouts, else 0)
-// run pad_block instead, beside the copies.
+// fill an expert's padding rows each, and what is past the segments, beside the copies.
 __global__ void __launch_bounds__(kThreads) moe_scatter_kernel(const MoeDispatchArgs p, int pad_blocks) {
     if ((int)blockIdx.x < pad_blocks) {
-        pad_block(p, blockIdx.x);
+        const int e = blockIdx.x;
+        if (e == p.num_experts) {
+            pad_past(p, ws_totals(p)[p.num_experts] + (int)threadIdx.x, kThreads);
+        } else {
+            const int total = ws_totals(p)[e], start = ws_starts(p)[e];
+            pad_rows(p, start + total, start + align_up(total, p.alignment));
+        }
         return;
     }
     const int lane = threadIdx.x & 63;
@@ -280,6 +300,126 @@ __global__ void __launch_bounds__(kThreads) moe_scatter_kernel(const MoeDispatch
             const int r = __builtin_amdgcn_readfirstlane(__shfl(flat, j));
             if (r < 0) continue;
             if (s < p.sfk) p.sf[row_sf(p, r) + (int64_t)s * p.sf_sk_o] = sv;
+        }
+    }
+}
+
+// Few tokens: the whole dispatch in one launch, without a workspace. Every workgroup counts all
+// entries by expert in LDS, those before its own tokens apart, and scans the totals into the segment
+// starts for itself; its entries' rows are the starts, plus the earlier entries of their
+// experts, plus those among its own. TOKENS 1: the four waves share a token's row, 4: a token
+// each. The first 16 (8) KB of a row are loaded before the counting, whose latency they cover. The first
+// pad_blocks workgroups (contiguous and psum layouts) share the experts' padding rows and what
+// is past the segments, and the first one of all writes the ends.
+template <int TOKENS>
+__global__ void __launch_bounds__(kThreads) moe_dispatch_few_kernel(const MoeDispatchArgs p, int pad_blocks) {
+    constexpr int LANES = kThreads / TOKENS, UNITS = TOKENS == 1 ? 4 : 8;   // lanes of a row, 16-byte pieces of each at a time
+    __shared__ int s_total[kMoeMaxExperts], s_before[kMoeMaxExperts];
+    __shared__ int s_used;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const bool padding = (int)blockIdx.x < pad_blocks;
+    const int t0 = padding ? 0 : ((int)blockIdx.x - pad_blocks) * TOKENS;   // the first token
+    const int mine = TOKENS == 1 ? 0 : wave, t = t0 + mine;
+    const int at = (int)threadIdx.x % LANES, units = p.kdim / 16;
+    const bool live = !padding && t < p.t;
+    const i32x4* src = reinterpret_cast<const i32x4*>(p.x + (int64_t)(live ? t : 0) * p.ldx);
+    i32x4 v[UNITS];
+    if (live) {
+#pragma unroll
+        for (int q = 0; q < UNITS; ++q)
+            if (q * LANES + at < units) v[q] = src[q * LANES + at];
+    }
+    for (int e = threadIdx.x; e < p.num_experts; e += kThreads) s_total[e] = s_before[e] = 0;
+    __syncthreads();
+    // entry i: slot i % k of token i / k
+    const int entries = p.t * p.k, first = t0 * p.k;
+    const bool flat_ids = p.topk_st == p.k && p.topk_sk == 1;
+    auto id_of = [&](int i) {
+        if (flat_ids) return topk_at(p, 0, i);
+        const int row = i / p.k;
+        return topk_at(p, row, i - row * p.k);
+    };
+    for (int i0 = threadIdx.x; i0 < entries; i0 += 4 * kThreads) {
+        int e[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) e[q] = i0 + q * kThreads < entries ? id_of(i0 + q * kThreads) : -1;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            if (!routed(p, e[q])) continue;
+            atomicAdd(&s_total[e[q]], 1);
+            if (!padding && i0 + q * kThreads < first) atomicAdd(&s_before[e[q]], 1);
+        }
+    }
+    __syncthreads();
+    if (p.layout != kMoeMasked) {
+        // s_total becomes the first row; padding workgroups keep the rows in s_before
+        const int x = segment_starts(p, [&](int e) { return s_total[e]; }, [&](int e, int start, int total) {
+            s_total[e] = start;
+            if (padding) s_before[e] = total;
+            if (blockIdx.x == 0 && p.layout == kMoePsum) p.meta[e] = start + total;
+        });
+        if (threadIdx.x == kThreads - 1) s_used = x;
+        __syncthreads();
+    } else if (blockIdx.x == 0) {
+        for (int e = threadIdx.x; e < p.num_experts; e += kThreads) p.meta[e] = min(s_total[e], p.max_m);
+    }
+    if (padding) {
+        if (p.layout == kMoeMasked) return;   // (no tokens)
+        if (p.alignment > 1)
+            for (int e = blockIdx.x; e < p.num_experts; e += pad_blocks)
+                pad_rows(p, s_total[e] + s_before[e], s_total[e] + align_up(s_before[e], p.alignment));
+        pad_past(p, (int64_t)s_used + (int)blockIdx.x * kThreads + (int)threadIdx.x, (int64_t)pad_blocks * kThreads);
+        return;
+    }
+    // Lane i of every wave: the row of the workgroup's i-th entry.
+    const int own = min(TOKENS, p.t - t0) * p.k;
+    const int e = lane < own ? id_of(first + lane) : -1;
+    const bool ok = routed(p, e);
+    static_assert(kMoeMaxExperts <= 1024 && 4 * kMoeMaxTopk <= 64, "expert ids fit 10 bits, a workgroup's entries a wave");
+    uint64_t peers = __ballot(ok);   // the lanes with this lane's expert
+#pragma unroll
+    for (int bit = 0; bit < 10; ++bit) {
+        const bool set = (e >> bit) & 1;
+        const uint64_t m = __ballot(ok && set);
+        peers &= set ? m : ~m;
+    }
+    int flat = -1;
+    if (ok) {
+        const int r = s_before[e] + __popcll(peers & ((1ull << lane) - 1));
+        flat = p.layout == kMoeMasked ? (r < p.max_m ? e * p.max_m + r : -1) : s_total[e] + r;
+    }
+    if (wave == 0 && lane < own) {
+        p.pos[(int64_t)first + lane] = flat;
+        if (flat >= 0) {
+            const int row = lane / p.k;
+            if (p.w_out)
+                p.w_out[flat] = p.topk_w ? p.topk_w[(int64_t)(t0 + row) * p.w_st + (int64_t)(lane - row * p.k) * p.w_sk] : 1.f;
+            if (p.layout == kMoeContiguous) p.meta[flat] = e;
+        }
+    }
+    if (!live) return;   // wave-uniform; no barrier follows
+    for (int u0 = 0; u0 < units; u0 += UNITS * LANES) {
+        if (u0 > 0) {
+#pragma unroll
+            for (int q = 0; q < UNITS; ++q)
+                if (u0 + q * LANES + at < units) v[q] = src[u0 + q * LANES + at];
+        }
+        for (int j = 0; j < p.k; ++j) {
+            const int r = __builtin_amdgcn_readlane(flat, mine * p.k + j);
+            if (r < 0) continue;   // wave-uniform
+            i32x4* dst = reinterpret_cast<i32x4*>(p.a + row_a(p, r));
+#pragma unroll
+            for (int q = 0; q < UNITS; ++q) {
+                const int u = u0 + q * LANES + at;
+                if (u < units) __builtin_nontemporal_store(v[q], dst + u);
+            }
+        }
+    }
+    for (int s = at; s < p.sfk; s += LANES) {
+        const float sv = p.x_sf[(int64_t)t * p.sf_st + (int64_t)s * p.sf_sk];
+        for (int j = 0; j < p.k; ++j) {
+            const int r = __builtin_amdgcn_readlane(flat, mine * p.k + j);
+            if (r >= 0) p.sf[row_sf(p, r) + (int64_t)s * p.sf_sk_o] = sv;
         }
     }
 }
@@ -404,23 +544,32 @@ int64_t moe_dispatch_workspace_ints(int64_t tokens, int num_experts) {
 void launch_moe_dispatch(const MoeDispatchArgs& a, hipStream_t stream) {
     DG_CHECK(a.num_experts > 0 && a.num_experts <= kMoeMaxExperts && a.k > 0 && a.k <= kMoeMaxTopk);
     DG_CHECK(a.chunks == moe_dispatch_chunks(a.t));
-    if (a.t > 0) {
-        hipLaunchKernelGGL(moe_count_kernel, dim3(a.chunks), dim3(kThreads), 0, stream, a);
+    // One launch or three: every workgroup of the one counts all entries for itself, work that grows
+    // with the square of the tokens, against two launches and a workspace's round trip. Rows of a BF16
+    // or FP8 token each, in a graph, one launch against three, us: 4 tokens x 8 slots 4.9/12.6, 777 x 6
+    // 9.9/17.2, 1024 x 8 (2048 columns) 13.4/20, 2048 x 8 (2048) 25.2/28.4, 4096 x 2 (2048) 18.1/19.2,
+    // 4096 x 8 (1024) 35.5/31.3. One token a workgroup or four, us: 64 x 8 of 7168 10.2/11.9,
+    // 512 x 8 of 2048 8.3/8.2, 777 x 6 10.8/9.9.
+    const int64_t entries = (int64_t)a.t * a.k;
+    const int tokens = entries * a.t <= kMoeFewOne ? 1 : 4;   // of a workgroup
+    if (entries * ((a.t + tokens - 1) / tokens) <= kMoeFewCounts) {
+        // (without tokens or padding rows: one workgroup for the ends, masked counts and weights)
+        const int pad_blocks = a.layout != kMoeMasked ? (a.alignment > 1 ? a.num_experts : 1) : a.t == 0 ? 1 : 0;
+        const dim3 grid(pad_blocks + (a.t + tokens - 1) / tokens), block(kThreads);
+        if (tokens == 1) hipLaunchKernelGGL(moe_dispatch_few_kernel<1>, grid, block, 0, stream, a, pad_blocks);
+        else hipLaunchKernelGGL(moe_dispatch_few_kernel<4>, grid, block, 0, stream, a, pad_blocks);
         DG_HIP_CHECK(hipGetLastError());
+        return;
     }
+    hipLaunchKernelGGL(moe_count_kernel, dim3(a.chunks), dim3(kThreads), 0, stream, a);
+    DG_HIP_CHECK(hipGetLastError());
     hipLaunchKernelGGL(moe_scan_kernel, dim3((a.num_experts + kThreads / 64 - 1) / (kThreads / 64)), dim3(kThreads), 0,
                        stream, a);
     DG_HIP_CHECK(hipGetLastError());
     const int pad_blocks = a.layout == kMoeMasked ? 0 : a.num_experts + 1;
-    if (a.layout != kMoeMasked) {
-        hipLaunchKernelGGL(moe_starts_kernel, dim3(1), dim3(kThreads), 0, stream, a);
-        DG_HIP_CHECK(hipGetLastError());
-    }
     const int64_t blocks = pad_blocks + ((int64_t)a.t + kThreads / 64 - 1) / (kThreads / 64);
-    if (blocks > 0) {
-        hipLaunchKernelGGL(moe_scatter_kernel, dim3((unsigned)blocks), dim3(kThreads), 0, stream, a, pad_blocks);
-        DG_HIP_CHECK(hipGetLastError());
-    }
+    hipLaunchKernelGGL(moe_scatter_kernel, dim3((unsigned)blocks), dim3(kThreads), 0, stream, a, pad_blocks);
+    DG_HIP_CHECK(hipGetLastError());
 }
 
 void launch_moe_swiglu_cast(const SwigluCastArgs& a, hipStream_t stream) {
