@@ -1624,7 +1624,7 @@ void combine_backward_impl(const dg_tensor* dout_, const dg_tensor* y_, const dg
         p.dw = moe_weight_gradient(dw_, p.t, p.k);
     }
     const int device = one_device({dout_, y_, pos_, w_, dy_, dw_});
-    DG_CHECK_GRID(combine_backward_blocks(p.t, p.n), 256);
+    DG_CHECK_GRID(combine_backward_blocks(p.t, p.n), combine_backward_threads(p.t, p.n));
     const OnDevice on(device);
     launch_combine_backward(p, stream);
     char buf[96];

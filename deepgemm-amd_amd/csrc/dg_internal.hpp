@@ -388,12 +388,22 @@ struct MoeGradArgs {
     float* dw;                 // [t, k] contiguous, or null
     int32_t t, k, n;
 };
-inline int moe_grad_waves(int64_t n) { return n <= 512 ? 1 : n <= 1024 ? 2 : 4; }   // of a token
+// Waves of a token in the combination's gradient, one for each 512 columns: up to four, or up to 16
+// where the tokens alone do not fill the card's 256 CUs twice. Four / 16, h = 7168, k = 8, us (in a
+// graph): 1 token 11.2/7.4, 64 tokens 12.6/8.0, 256 16.2/13.2, 512 23.3/22.9.
+constexpr int64_t kMoeGradFewTokens = 512;
+inline int moe_grad_waves(int64_t t, int64_t n) {
+    const int most = t <= kMoeGradFewTokens ? 16 : 4;
+    int waves = 1;
+    while (waves < most && waves * 512 < n) waves *= 2;
+    return waves;
+}
 inline int64_t dispatch_backward_blocks(int64_t t, int64_t n) { return (t + 3) / 4 * (n > 0 ? (n + 511) / 512 : 1); }
 inline int64_t combine_backward_blocks(int64_t t, int64_t n) {
-    const int64_t per = 4 / moe_grad_waves(n);
+    const int64_t waves = moe_grad_waves(t, n), per = waves < 4 ? 4 / waves : 1;
     return (t + per - 1) / per;
 }
+inline int combine_backward_threads(int64_t t, int64_t n) { return std::max(moe_grad_waves(t, n), 4) * 64; }
 void launch_dispatch_backward(const MoeGradArgs& args, hipStream_t stream);
 void launch_combine_backward(const MoeGradArgs& args, hipStream_t stream);
 

@@ -19,6 +19,7 @@ namespace dgm {
 namespace {
 
 using namespace dev;
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 constexpr int kBatch = 8;   // slots whose rows are loaded at a time
 
 __device__ __forceinline__ void unpack8(const uint4& v, float (&x)[8]) {
@@ -37,6 +38,20 @@ __device__ __forceinline__ int64_t row_at(int r, int max_m, int64_t ld, int64_t 
     return max_m ? (int64_t)(r / max_m) * gs + (int64_t)(r % max_m) * ld : (int64_t)r * ld;
 }
 
+// 8 values of a row. STREAM: past the caches' usual order, for what is read once; see stream_rows.
+template <bool STREAM>
+__device__ __forceinline__ uint4 load8(const uint16_t* from) {
+    if constexpr (STREAM) {
+        const u32x4 v = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(from));
+        return uint4{v.x, v.y, v.z, v.w};
+    } else {
+        return *reinterpret_cast<const uint4*>(from);
+    }
+}
+__device__ __forceinline__ void store8(uint16_t* to, const uint4& v) {
+    __builtin_nontemporal_store(u32x4{v.x, v.y, v.z, v.w}, reinterpret_cast<u32x4*>(to));
+}
+
 // Lane j < k: the row of the token's slot j, or -1 (also for what is no row).
 __device__ __forceinline__ int lane_row(const MoeGradArgs& p, int64_t t, int lane) {
     const int r = lane < p.k ? p.pos[t * p.k + lane] : -1;
@@ -44,6 +59,7 @@ __device__ __forceinline__ int lane_row(const MoeGradArgs& p, int64_t t, int lan
 }
 
 // One wave per (token, 512 columns).
+template <bool STREAM>
 __global__ void __launch_bounds__(256) dispatch_backward_kernel(const MoeGradArgs p, int slices) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int tb = blockIdx.x / slices, slice = blockIdx.x - tb * slices;
@@ -60,7 +76,7 @@ __global__ void __launch_bounds__(256) dispatch_backward_kernel(const MoeGradArg
         for (int q = 0; q < kBatch; ++q) {
             const int r = __builtin_amdgcn_readlane(row, j + q);   // (lanes from k on hold -1)
             v[q] = uint4{0, 0, 0, 0};
-            if (r >= 0) v[q] = *reinterpret_cast<const uint4*>(p.rows_in + row_at(r, p.max_m, p.ld_in, p.gs_in) + col);
+            if (r >= 0) v[q] = load8<STREAM>(p.rows_in + row_at(r, p.max_m, p.ld_in, p.gs_in) + col);
         }
 #pragma unroll
         for (int q = 0; q < kBatch; ++q) {
@@ -70,16 +86,17 @@ __global__ void __launch_bounds__(256) dispatch_backward_kernel(const MoeGradArg
             for (int e = 0; e < 8; ++e) acc[e] += x[e];
         }
     }
-    *reinterpret_cast<uint4*>(p.tokens + t * p.ldt + col) = pack8(acc);
+    store8(p.tokens + t * p.ldt + col, pack8(acc));
 }
 
-// WPT waves per token (1, 2 or 4, one for each 512 columns up to four). dw: each lane's
-// columns in order, then the lanes of a wave, then the waves, always in the same order.
-template <int WPT>
-__global__ void __launch_bounds__(256) combine_backward_kernel(const MoeGradArgs p) {
-    __shared__ float s_dw[4][kMoeMaxTopk];
+// WPT waves per token: one for each 512 columns, up to four, or, for few tokens, up to 16. dw: each
+// lane's columns in order, then the lanes of a wave, then the waves, always in the same order.
+template <int WPT, bool STREAM>
+__global__ void __launch_bounds__(WPT > 4 ? WPT * 64 : 256) combine_backward_kernel(const MoeGradArgs p) {
+    constexpr int NW = WPT > 4 ? WPT : 4;
+    __shared__ float s_dw[NW][kMoeMaxTopk];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t t = (int64_t)blockIdx.x * (4 / WPT) + wave / WPT;
+    const int64_t t = (int64_t)blockIdx.x * (NW / WPT) + wave / WPT;
     const bool live = t < p.t;
     if (live) {
         const int row = lane_row(p, t, lane);
@@ -92,7 +109,7 @@ __global__ void __launch_bounds__(256) combine_backward_kernel(const MoeGradArgs
 #pragma unroll
                 for (int q = 0; q < kBatch; ++q) {
                     const int r = __builtin_amdgcn_readlane(row, j + q);
-                    if (p.w && r >= 0) v[q] = *reinterpret_cast<const uint4*>(p.rows_in + row_at(r, p.max_m, p.ld_in, p.gs_in) + col);
+                    if (p.w && r >= 0) v[q] = load8<STREAM>(p.rows_in + row_at(r, p.max_m, p.ld_in, p.gs_in) + col);
                 }
                 float d[8];
                 unpack8(raw, d);
@@ -102,7 +119,7 @@ __global__ void __launch_bounds__(256) combine_backward_kernel(const MoeGradArgs
                     if (r < 0) continue;   // wave-uniform
                     uint16_t* to = p.rows_out + row_at(r, p.max_m, p.ld_out, p.gs_out) + col;
                     if (!p.w) {
-                        *reinterpret_cast<uint4*>(to) = raw;
+                        store8(to, raw);
                         continue;
                     }
                     const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(weight), j + q));
@@ -110,7 +127,7 @@ __global__ void __launch_bounds__(256) combine_backward_kernel(const MoeGradArgs
                     unpack8(v[q], y);
 #pragma unroll
                     for (int e = 0; e < 8; ++e) dot[q] += d[e] * y[e], o[e] = w * d[e];
-                    *reinterpret_cast<uint4*>(to) = pack8(o);
+                    store8(to, pack8(o));
                 }
             }
             if (!p.dw) continue;
@@ -132,25 +149,43 @@ __global__ void __launch_bounds__(256) combine_backward_kernel(const MoeGradArgs
     }
 }
 
+// Routed rows larger than the 256 MB of the last cache would push each other out of it: from 100 MB of
+// them on, their loads are nontemporal. Plain / nontemporal, us (dispatch; combination, whose stores
+// are nontemporal in both): 2048 tokens x 8 of 2048 columns (67 MB) 12.8/13.5; 24.3/29.7, 1024 x 8 of
+// 7168 (117 MB) 24.6/23.0; 52.4/49.5, 16384 x 2 of 4096 (268 MB) 74.9/71.8; 129/126, 8192 x 8 of 7168
+// (940 MB) 193/180; 400/396. Plain stores: 13.0; 32.5, 25.0; 53.9, 79.3; 132, 205; 403.
+bool stream_rows(const MoeGradArgs& a) { return (int64_t)a.t * a.k * a.n >= 50'000'000; }
+
+template <int WPT>
+void run_combine_backward(const MoeGradArgs& a, dim3 grid, dim3 block, hipStream_t stream) {
+    if (stream_rows(a)) hipLaunchKernelGGL((combine_backward_kernel<WPT, true>), grid, block, 0, stream, a);
+    else hipLaunchKernelGGL((combine_backward_kernel<WPT, false>), grid, block, 0, stream, a);
+}
+
 }  // namespace
 
 void launch_dispatch_backward(const MoeGradArgs& a, hipStream_t stream) {
     if (a.t == 0) return;
     const int64_t slices = a.n > 0 ? (a.n + 511) / 512 : 1, blocks = dispatch_backward_blocks(a.t, a.n);
     DG_CHECK_GRID(blocks, 256);
-    hipLaunchKernelGGL(dispatch_backward_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, a, (int)slices);
+    const dim3 grid((unsigned)blocks), block(256);
+    if (stream_rows(a)) hipLaunchKernelGGL(dispatch_backward_kernel<true>, grid, block, 0, stream, a, (int)slices);
+    else hipLaunchKernelGGL(dispatch_backward_kernel<false>, grid, block, 0, stream, a, (int)slices);
     DG_HIP_CHECK(hipGetLastError());
 }
 
 void launch_combine_backward(const MoeGradArgs& a, hipStream_t stream) {
     if (a.t == 0) return;
     const int64_t blocks = combine_backward_blocks(a.t, a.n);
-    DG_CHECK_GRID(blocks, 256);
-    const dim3 grid((unsigned)blocks), block(256);
-    switch (moe_grad_waves(a.n)) {
-        case 1: hipLaunchKernelGGL(combine_backward_kernel<1>, grid, block, 0, stream, a); break;
-        case 2: hipLaunchKernelGGL(combine_backward_kernel<2>, grid, block, 0, stream, a); break;
-        default: hipLaunchKernelGGL(combine_backward_kernel<4>, grid, block, 0, stream, a); break;
+    const int threads = combine_backward_threads(a.t, a.n);
+    DG_CHECK_GRID(blocks, threads);
+    const dim3 grid((unsigned)blocks), block(threads);
+    switch (moe_grad_waves(a.t, a.n)) {
+        case 1: run_combine_backward<1>(a, grid, block, stream); break;
+        case 2: run_combine_backward<2>(a, grid, block, stream); break;
+        case 4: run_combine_backward<4>(a, grid, block, stream); break;
+        case 8: run_combine_backward<8>(a, grid, block, stream); break;
+        default: run_combine_backward<16>(a, grid, block, stream); break;
     }
     DG_HIP_CHECK(hipGetLastError());
 }
