@@ -11,10 +11,14 @@
 //
 // HBM-bound: 2 bytes in and 1/2 out an element (and the reverse), plus the scales. A lane has 8
 // columns, 16 bytes of BF16 and 4 of codes; a wave converts 1024 columns of a row, both of its
-// loads issued first; the gran / 8 lanes of a group find its largest magnitude by shuffles.
+// loads issued first; the gran / 8 lanes of a group find its largest magnitude by shuffles. BF16 and
+// FP32 values pass by the caches' order (nontemporal: plain / so, us: cast of 16384 x 7168 111/98,
+// 65536 x 2048 159/110, 4096 x 7168 28/28; back, 16384 x 7168, to BF16 69/41, to FP32 143/74); codes do not, which the
+// next kernel reads (nontemporal as well: 117 and 137 for the casts).
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "dg_internal.hpp"
 #include "dg_kernel_common.hpp"
@@ -23,6 +27,8 @@ namespace dgm {
 namespace {
 
 using namespace dev;
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kWaves = 4;      // rows per workgroup, one wave each
 constexpr int kChunk = 512;    // columns of a wave-wide access (64 lanes x 8)
@@ -69,7 +75,8 @@ __global__ void __launch_bounds__(kWaves * 64) cast4_kernel(const Cast4Args p, i
     for (int u = 0; u < kChunks; ++u) {
         const int col = s.col + u * kChunk + lane * 8;
         if (VEC && col + 8 <= p.n) {
-            raw[u] = *reinterpret_cast<const uint4*>(xr + col);
+            const u32x4 v = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(xr + col));
+            raw[u] = uint4{v.x, v.y, v.z, v.w};
         } else {
             uint32_t w[4];
 #pragma unroll
@@ -138,24 +145,27 @@ __global__ void __launch_bounds__(kWaves * 64) cast4_kernel(const Cast4Args p, i
     }
 }
 
-// VEC: rows begin at whole 4-byte (codes) and 16-byte (values) pieces.
-template <int GRAN, int VEC>
+// A lane's W values fill 16 bytes, so that a wave's store is one stretch: W is 8 for BF16, 4 for FP32.
+// VEC: rows begin at whole W / 2-byte (codes) and 16-byte (values) pieces.
+template <int GRAN, int VEC, int W>
 __global__ void __launch_bounds__(kWaves * 64) cast_back4_kernel(const Cast4Args p, int slices) {
+    constexpr int CHUNK = 64 * W, CHUNKS = kSlice / CHUNK;
+    using Codes = std::conditional_t<W == 8, uint32_t, uint16_t>;
     const Slice s(slices);
     if (s.row >= p.m) return;   // wave-uniform
     const int lane = threadIdx.x & 63;
     const uint8_t* qr = p.q + (int64_t)s.row * p.ldq;
-    uint32_t codes[kChunks];
-    float sf[kChunks];
+    uint32_t codes[CHUNKS];
+    float sf[CHUNKS];
 #pragma unroll
-    for (int u = 0; u < kChunks; ++u) {
-        const int col = s.col + u * kChunk + lane * 8;
+    for (int u = 0; u < CHUNKS; ++u) {
+        const int col = s.col + u * CHUNK + lane * W;
         codes[u] = 0, sf[u] = 0.f;
-        if (VEC && col + 8 <= p.n) {
-            codes[u] = *reinterpret_cast<const uint32_t*>(qr + col / 2);
+        if (VEC && col + W <= p.n) {
+            codes[u] = *reinterpret_cast<const Codes*>(qr + col / 2);
         } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
+            for (int e = 0; e < W / 2; ++e)
                 if (col + 2 * e < p.n) codes[u] |= (uint32_t)qr[col / 2 + e] << (8 * e);
         }
         if (col < p.n) {
@@ -169,36 +179,41 @@ __global__ void __launch_bounds__(kWaves * 64) cast_back4_kernel(const Cast4Args
         }
     }
 #pragma unroll
-    for (int u = 0; u < kChunks; ++u) {
-        const int col = s.col + u * kChunk + lane * 8;
+    for (int u = 0; u < CHUNKS; ++u) {
+        const int col = s.col + u * CHUNK + lane * W;
         if (col >= p.n) continue;
         typedef float f32x2 __attribute__((ext_vector_type(2)));
-        const f32x2 c[4] = {__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes[u], 1.0f, 0),
-                            __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes[u], 1.0f, 1),
-                            __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes[u], 1.0f, 2),
-                            __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes[u], 1.0f, 3)};
-        float v[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = __fmul_rn(c[e >> 1][e & 1], sf[u]);
+        float v[W];
+        auto pair = [&](auto at) {
+            constexpr int e = decltype(at)::value;
+            const f32x2 c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes[u], 1.0f, e);
+            v[2 * e] = __fmul_rn(c.x, sf[u]), v[2 * e + 1] = __fmul_rn(c.y, sf[u]);
+        };
+        pair(std::integral_constant<int, 0>{});
+        pair(std::integral_constant<int, 1>{});
+        if constexpr (W == 8) {
+            pair(std::integral_constant<int, 2>{});
+            pair(std::integral_constant<int, 3>{});
+        }
         const int64_t at = (int64_t)s.row * p.ldx + col;
-        if (p.out_f32) {
+        const bool whole = VEC && col + W <= p.n;
+        if constexpr (W == 4) {
             float* y = static_cast<float*>(p.y) + at;
-            if (VEC && col + 8 <= p.n) {
-                *reinterpret_cast<f32x4*>(y) = f32x4{v[0], v[1], v[2], v[3]};
-                *reinterpret_cast<f32x4*>(y + 4) = f32x4{v[4], v[5], v[6], v[7]};
+            if (whole) {
+                __builtin_nontemporal_store(f32x4{v[0], v[1], v[2], v[3]}, reinterpret_cast<f32x4*>(y));
             } else {
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
+                for (int e = 0; e < W; ++e)
                     if (col + e < p.n) y[e] = v[e];
             }
         } else {
             uint16_t* y = static_cast<uint16_t*>(p.y) + at;
-            if (VEC && col + 8 <= p.n) {
-                *reinterpret_cast<uint4*>(y) = uint4{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
-                                                     pack_bf16x2(v[6], v[7])};
+            if (whole) {
+                __builtin_nontemporal_store(u32x4{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
+                                                  pack_bf16x2(v[6], v[7])}, reinterpret_cast<u32x4*>(y));
             } else {
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
+                for (int e = 0; e < W; ++e)
                     if (col + e < p.n) y[e] = bf16_bits(v[e]);
             }
         }
@@ -238,9 +253,13 @@ void launch_cast_back4(const Cast4Args& a, hipStream_t stream) {
     if (a.m == 0 || a.n == 0) return;
     const int64_t blocks = cast4_blocks(a.m, a.n);
     DG_CHECK_GRID(blocks, kWaves * 64);
-    by_gran(a.gran, aligned(a.y, a.ldx * (a.out_f32 ? 4 : 2), 16) && aligned(a.q, a.ldq, 4), [&](auto gran, auto vec) {
-        hipLaunchKernelGGL((cast_back4_kernel<decltype(gran)::value, decltype(vec)::value>), dim3((unsigned)blocks),
-                           dim3(kWaves * 64), 0, stream, a, (a.n + kSlice - 1) / kSlice);
+    by_gran(a.gran, aligned(a.y, a.ldx * (a.out_f32 ? 4 : 2), 16) && aligned(a.q, a.ldq, a.out_f32 ? 2 : 4),
+            [&](auto gran, auto vec) {
+        constexpr int G = decltype(gran)::value, V = decltype(vec)::value;
+        const dim3 grid((unsigned)blocks), block(kWaves * 64);
+        const int slices = (a.n + kSlice - 1) / kSlice;
+        if (a.out_f32) hipLaunchKernelGGL((cast_back4_kernel<G, V, 4>), grid, block, 0, stream, a, slices);
+        else hipLaunchKernelGGL((cast_back4_kernel<G, V, 8>), grid, block, 0, stream, a, slices);
     });
     DG_HIP_CHECK(hipGetLastError());
 }
