@@ -307,28 +307,43 @@ __device__ __forceinline__ void store_tile(const RaggedGemmArgs& p, const f32x16
                 }
         __syncthreads();
         if (!vec) {   // rows that begin anywhere: 64 elements of a row an access, one a lane
-            for (int t = 0; t < T * RPT; ++t) {
-                const int lr = t * NW + wave, r = row_of(lr);
-                if (r >= m_end) continue;
+            // Four rows read from LDS at a time. One after the other / four, 4-bit products of 1001 rows over 16
+            // groups, n 1413, k 2080: BF16 14.6/13.5 us, FP32 15.6/14.1 us.
+            constexpr int ROWS = 4;
+            static_assert(T * RPT % ROWS == 0, "whole batches");
+            for (int t = 0; t < T * RPT; t += ROWS) {
+                uint32_t v[ROWS][BN / 64];
+                auto each = [&](auto&& body) {
 #pragma unroll
-                for (int q = 0; q < BN / 64; ++q) {
-                    const int col = q * 64 + lane, at = col * STAGED;
-                    if (n0 + col >= p.n) continue;
-                    const uint8_t* src = lds + lr * ROW_BYTES + (((at >> 4) ^ (lr & 7)) << 4) + (at & 15);
-                    const int64_t to = d_tile + (int64_t)r * p.ldd + col, from = c_tile + (int64_t)r * p.ldc + col;
-                    if constexpr (OUT == 0) {
-                        static_cast<uint16_t*>(p.d)[to] = *reinterpret_cast<const uint16_t*>(src);
-                    } else {
-                        float v = *reinterpret_cast<const float*>(src);
-                        if constexpr (OUT == 1) {
-                            if (add) v += static_cast<const float*>(p.c)[from];
-                            static_cast<float*>(p.d)[to] = v;
-                        } else {
-                            v += bf16_to_f32(static_cast<const uint16_t*>(p.c)[from]);
-                            static_cast<uint16_t*>(p.d)[to] = bf16_bits(v);
-                        }
+                    for (int u = 0; u < ROWS; ++u) {
+                        const int r = row_of((t + u) * NW + wave);
+                        if (r >= m_end) continue;
+#pragma unroll
+                        for (int q = 0; q < BN / 64; ++q)
+                            if (n0 + q * 64 + lane < p.n) body(v[u][q], r, q * 64 + lane);
                     }
-                }
+                };
+#pragma unroll
+                for (int u = 0; u < ROWS; ++u)
+#pragma unroll
+                    for (int q = 0; q < BN / 64; ++q) {
+                        const int lr = (t + u) * NW + wave, at = (q * 64 + lane) * STAGED;
+                        const uint8_t* src = lds + lr * ROW_BYTES + (((at >> 4) ^ (lr & 7)) << 4) + (at & 15);
+                        if constexpr (OUT == 0) v[u][q] = *reinterpret_cast<const uint16_t*>(src);
+                        else v[u][q] = *reinterpret_cast<const uint32_t*>(src);
+                    }
+                if (add)   // uniform over the launch
+                    each([&](uint32_t& x, int r, int col) {
+                        const int64_t from = c_tile + (int64_t)r * p.ldc + col;
+                        if constexpr (OUT == 1) x = __float_as_uint(__uint_as_float(x) + static_cast<const float*>(p.c)[from]);
+                        if constexpr (OUT == 2) x = __float_as_uint(__uint_as_float(x) + bf16_to_f32(static_cast<const uint16_t*>(p.c)[from]));
+                    });
+                each([&](uint32_t x, int r, int col) {
+                    const int64_t to = d_tile + (int64_t)r * p.ldd + col;
+                    if constexpr (OUT == 0) static_cast<uint16_t*>(p.d)[to] = (uint16_t)x;
+                    if constexpr (OUT == 1) static_cast<float*>(p.d)[to] = __uint_as_float(x);
+                    if constexpr (OUT == 2) static_cast<uint16_t*>(p.d)[to] = bf16_bits(__uint_as_float(x));
+                });
             }
             continue;
         }
