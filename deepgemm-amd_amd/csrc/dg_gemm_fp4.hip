@@ -423,12 +423,10 @@ RaggedPlan plan_ragged_fp4(const RaggedFp4Args& a, int slots, int block, int spl
         const double t128 = tiles(128), t256 = tiles(256);
         if (t256 * 128 >= slots * 75 && std::max(1.0, t256 / slots) * (steps * 1.9 + 10) < 1.1 * us(128, t128, steps)) {
             block = 256;
-        } else if (t128 * 4 >= slots * 3) {
+        } else {
             block = 128;
-        } else {   // (the larger of two that are about as fast)
-            block = 128;
-            for (int b : {64, 32})
-                if (us(b, tiles(b), steps) < 0.95 * us(block, tiles(block), steps)) block = b;
+            for (int b : {64, 32})   // (the larger of two that are about as fast)
+                if (t128 * 4 < slots * 3 && us(b, tiles(b), steps) < 0.95 * us(block, tiles(block), steps)) block = b;
         }
     }
     RaggedPlan plan{block, 1, 0};

@@ -379,3 +379,115 @@ def test_graphs_of_dispatch_and_gradients():
             torch.cuda.synchronize()
             for a, b in zip(out, want):
                 assert torch.equal(bits(a), bits(b))
+
+
+# Sizes at which the dispatch changes its form (one or four tokens a workgroup, one launch or three), around
+# the workgroups' last token, and ids that lie apart.
+@pytest.mark.parametrize('t', [3, 361, 362, 363, 365, 2045, 2048, 2049])
+@pytest.mark.parametrize('layout,alignment', [('psum', 1), ('psum', 48), ('contiguous', 16), ('masked', 0)])
+def test_dispatch_forms(t, layout, alignment):
+    print(f't={t} {layout}', flush=True)
+    k, e, h = 8, 1024 if t > 1000 else 40, 24
+    idx = routing(t, k, e, t, again=True)
+    x, x0 = tokens(t, h, t, pad=8)
+    w = torch.rand((t, k), generator=torch.Generator().manual_seed(1))
+    max_m = max(1, t * k // e)
+    wide = torch.full((t, 3 * k), 1, dtype=torch.int64)
+    wide[:, ::3] = idx
+    wide_w = torch.full((k, t), float('nan'))
+    wide_w[:] = w.t()
+    more = dict(max_m=max_m) if layout == 'masked' else dict(alignment=alignment)
+    a, _, gl, got, rw = deep_gemm.moe_dispatch(x, wide.to(DEV)[:, ::3], e, layout=layout, topk_weights=wide_w.to(DEV).t(), **more)
+    if layout == 'masked':
+        first, starts, ends, _ = places(idx, e, 1)
+        rank = first - torch.tensor(starts)[idx.clamp(min=0).long()]
+        pos = torch.where((idx >= 0) & (rank < max_m), idx.long() * max_m + rank, -1)
+        assert gl.tolist() == [min(n - s, max_m) for s, n in zip(starts, ends)]
+    else:
+        pos, starts, ends, used = places(idx, e, alignment)
+        if layout == 'psum':
+            assert gl.tolist() == ends
+        else:
+            want = torch.full((a.shape[0],), -1, dtype=torch.int32)
+            for g, (s, n) in enumerate(zip(starts, ends)):
+                want[s:n] = g
+            assert torch.equal(gl.cpu(), want)
+    live = pos >= 0
+    assert torch.equal(got.cpu().long(), pos)
+    flat, rw = a.reshape(-1, h).cpu(), rw.reshape(-1).cpu()
+    assert torch.equal(bits(flat[pos[live]]), bits(x0[live.nonzero()[:, 0]]))
+    assert torch.equal(rw[pos[live]], w[live])
+    if layout != 'masked':
+        rest = torch.ones(flat.shape[0], dtype=torch.bool)
+        rest[pos[live]] = False
+        assert not rw[rest].any()
+        rest[used:] = False
+        assert not flat[rest].any()
+
+
+@pytest.mark.parametrize('layout', ['psum', 'contiguous', 'masked'])
+def test_dispatch_no_tokens_of_any_layout(layout):
+    x = torch.empty((0, 64), dtype=torch.bfloat16, device=DEV)
+    a, _, gl, pos, rw = deep_gemm.moe_dispatch(x, torch.empty((0, 2), dtype=torch.int32, device=DEV), 4, layout=layout, alignment=16, max_m=8,
+                                               topk_weights=torch.empty((0, 2), device=DEV))
+    assert pos.shape == (0, 2) and not (gl.cpu() > 0).any()
+    if layout != 'masked':
+        assert not rw.any()
+
+
+def test_dispatches_beside_each_other():
+    """Calls on two streams, and two graphs replayed on them, share nothing."""
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    t, k, e, h = 3000, 8, 64, 264
+    sets = [(tokens(t, h, i)[0], routing(t, k, e, i).to(DEV)) for i in range(2)]
+    run = lambda x, idx: deep_gemm.moe_dispatch(x, idx, e, layout='psum', alignment=1)
+    want = [run(*s) for s in sets]
+    torch.cuda.synchronize()
+    graphs = []
+    for s in sets:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = run(*s)
+        graphs.append((graph, out))
+    for _ in range(5):
+        got = []
+        for (graph, out), stream, s in zip(graphs, streams, sets):
+            with torch.cuda.stream(stream):
+                graph.replay()
+                got.append(run(*s))
+        torch.cuda.synchronize()
+        for (_, out), eager, ref in zip(graphs, got, want):
+            used = int(ref[2][-1])
+            for res in (out, eager):
+                assert torch.equal(res[3], ref[3]) and torch.equal(res[2], ref[2])
+                assert torch.equal(bits(res[0][:used]), bits(ref[0][:used]))
+
+
+@pytest.mark.parametrize('t,k,h', [(3200, 16, 1024), (6300, 1, 8192), (513, 2, 4104), (512, 2, 4104), (512, 3, 2056), (100, 2, 16392)])
+def test_gradients_of_many_and_of_wide_rows(t, k, h):
+    """The forms for more than 100 MB of rows, and for up to and above 512 tokens."""
+    print(f't={t} k={k} h={h}', flush=True)
+    gen = torch.Generator().manual_seed(t)
+    pos = torch.randperm(t * k, generator=gen).view(t, k)
+    pos[torch.rand((t, k), generator=gen) < 0.1] = -1
+    rows = torch.randn((t * k, h), generator=gen).bfloat16()
+    dout = torch.randn((t, h), generator=gen).bfloat16()
+    w = torch.randn((t, k), generator=gen)
+    at, y = pos.int().to(DEV), rows.to(DEV)
+    dx, _ = deep_gemm.moe_dispatch_backward(y, at)
+    dy, dw = deep_gemm.moe_combine_backward(dout.to(DEV), y, at, w.to(DEV))
+    some = torch.randint(0, t, (150,), generator=gen)
+    some[:3] = torch.tensor([0, t // 2, t - 1])
+    live = pos[some] >= 0
+    each = torch.where(live[..., None], rows[pos[some].clamp(min=0)].double(), 0.0)
+    ref, mag = each.sum(1), each.abs().sum(1)
+    check(dx[some.to(DEV)], ref, rounding(torch.bfloat16, ref) + (k - 1) * 2.0 ** -24 * mag * (1 + 2.0 ** -8), 'dx')
+    terms = each * dout[some].double()[:, None]
+    # a product passes its lane's additions, six between lanes and up to fifteen between waves
+    length = 8 * -(-h // 512) + 22
+    check(dw[some.to(DEV)], terms.sum(2), length * 2.0 ** -24 * terms.abs().sum(2) + rounding(torch.float32, terms.sum(2)), 'dw')
+    ref = (dout[some].double()[:, None] * w[some].double()[..., None])[live]
+    check(dy.cpu()[pos[some][live]], ref, (1 + 2.0 ** -8) * 2.0 ** -24 * ref.abs() + rounding(torch.bfloat16, ref), 'dy')
+    none = torch.ones(t * k, dtype=torch.bool)
+    none[pos[pos >= 0]] = False
+    assert not dy[none.to(DEV)].any()
