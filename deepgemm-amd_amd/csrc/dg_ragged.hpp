@@ -376,7 +376,12 @@ __device__ __forceinline__ void store_tile(const RaggedGemmArgs& p, const f32x16
 #pragma unroll
                     for (int e = 0; e < 4; ++e) w[e] = OUT == 1 ? __float_as_uint(f[e]) : pack2(f[(2 * e) % CPL], f[(2 * e + 1) % CPL]);
                 }
-                *reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.d) + to * SIZE) = uint4{w[0], w[1], w[2], w[3]};
+                // Past the caches' order, in whole lines: it leaves them to the operands. Plain / so, us (4-bit NT, groups x
+                // rows, n, k): 8 x 16384, 7168, 2048 177/163 (FP32 226/196), 4096, 7168 284/282, 32 x 4096, 2048, 2048
+                // 28.0/25.4; BF16 TN 16384 rows to 8 x 4096 x 7168, FP32 + C, 1070/1034, NT 8 x 1000, 4096, 2048 38.4/37.1.
+                typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+                __builtin_nontemporal_store(u32x4{w[0], w[1], w[2], w[3]},
+                                            reinterpret_cast<u32x4*>(static_cast<uint8_t*>(p.d) + to * SIZE));
             } else {
 #pragma unroll
                 for (int e = 0; e < CPL; ++e) {
