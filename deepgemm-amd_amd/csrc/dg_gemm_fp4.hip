@@ -402,8 +402,9 @@ __global__ void __launch_bounds__(256, 2) fp4_few_rows_kernel(const RaggedFp4Arg
 // 256 x 256 and 128 x 128: 8 x 16384, 4096, 7168 286 and 331; 8 x 8192, 7168, 2048 99 and 113; 8 x 2048, 4096,
 //   7168 61 and 66; 32 x 2048, 4096, 2048 42 and 32; 1 x 4096, 4096, 1024 22.1 and 20.7.
 // Where 128 x 128 tiles fill three quarters of the CUs, smaller ones only read weights again: 128,
-//   64 and 32 rows at 8 x 256, 4096, 7168 31, 49 and 45; 32 x 1024, 4096, 2048 30, 36 and 41; 32 x 512, 4096, 7168 97, 107 and
-//   112; 32 x 64, 4096, 7168 86, 91 and 90; 32 x 64, 4096, 2048 29.5, 29.2 and 28.9.
+//   64 and 32 rows at 8 x 256, 4096, 7168 30, 48 and 45; 32 x 512, 4096, 7168 97, 107 and 112; 32 x 32, 4096, 7168 90, 95
+//   and 94, 5120 68, 73 and 71. But for up to 8 rows a group and a short reduced axis, where a tile's end
+//   counts: 32 x 32, 4096, 3584 48.9, 49.4 and 48.8, 2048 31.5, 31.0 and 30.5; 8 x 8, 4096, 2048 10.1, 9.5 and 9.2.
 // Where they do not: 1 x 512, 4096, 7168 22, 19 and 27; 1 x 256, 2112, 7168 22, 18 and 16; 2 x 128, 4096, 4096 14.7, 12.6
 //   and 11.4.
 // Whole, in 2, 4 and 8 pieces, 32 rows: 1 x 64, 2112, 7168 15.4, 13.9, 12.3, 14.3; 1 x 256, 2112, 7168 15.6, 20.2, 22.7, 23.1.
@@ -424,7 +425,7 @@ RaggedPlan plan_ragged_fp4(const RaggedFp4Args& a, int slots, int block, int spl
         if (t256 * 128 >= slots * 75 && std::max(1.0, t256 / slots) * (steps * 1.9 + 10) < 1.1 * us(128, t128, steps)) {
             block = 256;
         } else {
-            block = 128;
+            block = t128 * 4 >= slots * 3 && rows <= 8 * used && steps <= 12 ? kFewRows : 128;
             for (int b : {64, 32})   // (the larger of two that are about as fast)
                 if (t128 * 4 < slots * 3 && us(b, tiles(b), steps) < 0.95 * us(block, tiles(block), steps)) block = b;
         }
