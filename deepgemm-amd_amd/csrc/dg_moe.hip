@@ -6,14 +6,15 @@
 // layouts are those of its generators (tests/generators.py:383-478).
 //
 // Dispatch (all integer work, deterministic): each (token t, slot j) routed to
-// expert e gets the next row of e's segment, in token-then-slot order.
+// expert e gets the next row of e's segment, in token-then-slot order. Few tokens: in one launch
+// (moe_dispatch_few_kernel); others in three:
 //   1. count:   per chunk of 64 tokens, one wave ranks the chunk's entries
 //               among equal experts with ballots (in entry order; the rank goes
 //               to pos) and leaves the chunk's count per expert;
 //   2. scan:    one wave per expert: exclusive prefix over chunks, the total,
-//               and the masked counts; the last block to be done scans the aligned totals
-//               into the segment starts and the psum ends (contiguous / psum);
-//   3. scatter: one wave per token turns its k ranks into rows, reads the
+//               and the masked counts;
+//   3. scatter: each workgroup scans the aligned totals into the segment starts
+//               (contiguous / psum) and turns its ranks into rows; a wave reads a
 //               token's K bytes once and stores them to each routed row, with
 //               the SF row, the weight and m_indices; beside them (contiguous /
 //               psum) a block per expert fills its padding rows (zero A, SF and
@@ -34,6 +35,7 @@ namespace dgm {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kMoeShortRow = 512;   // bytes
 using dev::i32x4;
 
 __device__ __forceinline__ int align_up(int x, int a) { return (x + a - 1) / a * a; }
@@ -52,12 +54,9 @@ __device__ __forceinline__ int topk_at(const MoeDispatchArgs& p, int t, int j) {
 __device__ __forceinline__ bool routed(const MoeDispatchArgs& p, int e) { return e >= 0 && e < p.num_experts; }
 
 // Workspace: counts [E][chunks] (exclusive prefixes over chunks after the
-// scan), then starts [E], totals [E], rows [1].
+// scan), then totals [E].
 __device__ __forceinline__ int32_t* ws_counts(const MoeDispatchArgs& p) { return p.ws; }
-__device__ __forceinline__ int32_t* ws_starts(const MoeDispatchArgs& p) {
-    return p.ws + (int64_t)p.chunks * p.num_experts;
-}
-__device__ __forceinline__ int32_t* ws_totals(const MoeDispatchArgs& p) { return ws_starts(p) + p.num_experts; }
+__device__ __forceinline__ int32_t* ws_totals(const MoeDispatchArgs& p) { return p.ws + (int64_t)p.chunks * p.num_experts; }
 
 // Inclusive prefix sum over the 64 lanes of a wave.
 __device__ __forceinline__ int wave_inclusive_sum(int v, int lane) {
@@ -111,7 +110,6 @@ __global__ void __launch_bounds__(kThreads) moe_count_kernel(const MoeDispatchAr
     __syncthreads();
     for (int e = threadIdx.x; e < p.num_experts; e += kThreads)
         ws_counts(p)[(int64_t)e * p.chunks + c] = run[e];
-    if (c == 0 && threadIdx.x == 0) ws_totals(p)[p.num_experts] = 0;   // (moe_scan_kernel counts its workgroups there)
 }
 
 // Contiguous and psum layouts, one workgroup: the exclusive prefix of the aligned expert totals
@@ -146,53 +144,34 @@ __device__ __forceinline__ int segment_starts(const MoeDispatchArgs& p, Total&& 
 
 // One wave per expert: the exclusive prefix of its chunk counts (in place, 256
 // chunks per round, 4 consecutive chunks per lane), its total, and for the
-// masked layout masked_m = min(total, max_m). For the other layouts the workgroup that is the last
-// to have its totals written (a count in the place of the used rows, which moe_count_kernel has
-// cleared) goes on to the segment starts, the psum ends and the rows the segments use.
+// masked layout masked_m = min(total, max_m).
 __global__ void __launch_bounds__(kThreads) moe_scan_kernel(const MoeDispatchArgs p) {
-    __shared__ int s_done;
     const int lane = threadIdx.x & 63;
     const int e = blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
-    if (e < p.num_experts) {   // wave-uniform
-        int32_t* cnt = ws_counts(p) + (int64_t)e * p.chunks;
-        int carry = 0;
-        for (int c0 = 0; c0 < p.chunks; c0 += 256) {
-            const int c = c0 + lane * 4;
-            int v[4], s = 0;
+    if (e >= p.num_experts) return;   // wave-uniform
+    int32_t* cnt = ws_counts(p) + (int64_t)e * p.chunks;
+    int carry = 0;
+    for (int c0 = 0; c0 < p.chunks; c0 += 256) {
+        const int c = c0 + lane * 4;
+        int v[4], s = 0;
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                v[q] = c + q < p.chunks ? cnt[c + q] : 0;
-                s += v[q];
-            }
-            const int incl = wave_inclusive_sum(s, lane);
-            int x = carry + incl - s;
+        for (int q = 0; q < 4; ++q) {
+            v[q] = c + q < p.chunks ? cnt[c + q] : 0;
+            s += v[q];
+        }
+        const int incl = wave_inclusive_sum(s, lane);
+        int x = carry + incl - s;
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                if (c + q < p.chunks) cnt[c + q] = x;
-                x += v[q];
-            }
-            carry += __shfl(incl, 63);
+        for (int q = 0; q < 4; ++q) {
+            if (c + q < p.chunks) cnt[c + q] = x;
+            x += v[q];
         }
-        if (lane == 0) {
-            __hip_atomic_store(ws_totals(p) + e, carry, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            if (p.layout == kMoeMasked) p.meta[e] = min(carry, p.max_m);
-        }
+        carry += __shfl(incl, 63);
     }
-    if (p.layout == kMoeMasked) return;   // uniform over the launch
-    int32_t* used = ws_totals(p) + p.num_experts;
-    __threadfence();   // (each wave's total before the workgroup is counted)
-    __syncthreads();
-    if (threadIdx.x == 0) s_done = __hip_atomic_fetch_add(used, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
-    __syncthreads();
-    if (s_done != (int)gridDim.x - 1) return;   // workgroup-uniform
-    __threadfence();
-    const int rows = segment_starts(
-        p, [&](int x) { return __hip_atomic_load(ws_totals(p) + x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); },
-        [&](int x, int start, int total) {
-            ws_starts(p)[x] = start;
-            if (p.layout == kMoePsum) p.meta[x] = start + total;   // psum[e] = align(psum[e-1]) + count
-        });
-    if (threadIdx.x == kThreads - 1) *used = rows;
+    if (lane == 0) {
+        ws_totals(p)[e] = carry;
+        if (p.layout == kMoeMasked) p.meta[e] = min(carry, p.max_m);
+    }
 }
 
 // Row p of the output layout (flattened for masked: e * max_m + r).
@@ -226,80 +205,103 @@ __device__ __forceinline__ void pad_past(const MoeDispatchArgs& p, int64_t r0, i
     }
 }
 
-// One wave per token: lane j < k turns slot j's chunk rank into its output row
-// (segment start + the expert's prefix over earlier chunks + the rank; for the
-// masked layout -1 past max_m) and writes pos, the row weight and m_indices;
-// then the wave reads the token's K bytes once, 8 KB per round (8 x 16 B per
-// lane in flight), and stores them to each routed row, then the SF row. The
-// first pad_blocks blocks (E + 1 for the contiguous and psum layouts, else 0)
-// fill an expert's padding rows each, and what is past the segments, beside the copies.
+// A wave has TOKENS tokens: 1, or 4 of at most kMoeShortRow bytes. Lane i turns
+// the chunk rank of the wave's entry i into its output row (segment start + the expert's prefix over
+// earlier chunks + the rank; for the masked layout the slot in the group's buffer, -1 past max_m);
+// then the wave stores the tokens' K bytes, read once (8 KB per round of one token, 8 x 16 B per
+// lane in flight), to each routed row, then the SF row. Every workgroup scans the
+// totals into the segment starts for itself (a launch of its own for them: 8192 x 8 rows of 7168 columns
+// 235 us against 230, 4096 x 8 of 512 over 1000 experts 21.9 against 21.3; in the last workgroup of the scan 239 and 41).
+// The first pad_blocks blocks (E + 1 for the
+// contiguous and psum layouts, else 0) fill an expert's padding rows each, and what is past the
+// segments, beside the copies; the first writes the psum ends.
+template <int TOKENS>
 __global__ void __launch_bounds__(kThreads) moe_scatter_kernel(const MoeDispatchArgs p, int pad_blocks) {
-    if ((int)blockIdx.x < pad_blocks) {
-        const int e = blockIdx.x;
-        if (e == p.num_experts) {
-            pad_past(p, ws_totals(p)[p.num_experts] + (int)threadIdx.x, kThreads);
-        } else {
-            const int total = ws_totals(p)[e], start = ws_starts(p)[e];
-            pad_rows(p, start + total, start + align_up(total, p.alignment));
-        }
+    __shared__ int s_start[kMoeMaxExperts + 1];
+    constexpr int UNITS = TOKENS == 1 ? 8 : 1;   // 16-byte pieces of a token and lane at a time
+    static_assert(TOKENS * kMoeMaxTopk <= 64 && kMoeShortRow <= 64 * 16, "a wave's entries, a piece a lane");
+    const bool padding = (int)blockIdx.x < pad_blocks;
+    const int lane = threadIdx.x & 63;
+    const int t0 = padding ? p.t : ((int)blockIdx.x - pad_blocks) * (kThreads / 64 * TOKENS) + (int)(threadIdx.x >> 6) * TOKENS;
+    const int tokens = min(TOKENS, p.t - t0);   // wave-uniform; none or fewer behind the last
+    // The first 8 KB are loaded before the rows are looked up (the two
+    // are independent), so the lookup's load latency hides behind them.
+    const int units = p.kdim / 16;
+    i32x4 v[TOKENS][UNITS];
+#pragma unroll
+    for (int i = 0; i < TOKENS; ++i)
+#pragma unroll
+        for (int q = 0; q < UNITS; ++q)
+            if (i < tokens && q * 64 + lane < units)
+                v[i][q] = reinterpret_cast<const i32x4*>(p.x + (int64_t)(t0 + i) * p.ldx)[q * 64 + lane];
+    const bool mine = lane < tokens * p.k;
+    const int own = TOKENS == 1 ? 0 : lane / p.k, slot = lane - own * p.k;   // this lane's entry
+    const int64_t entry = (int64_t)t0 * p.k + lane;
+    int e = -1, rank = 0;
+    if (mine) {
+        e = topk_at(p, t0 + own, slot);
+        if (routed(p, e)) rank = ws_counts(p)[(int64_t)e * p.chunks + (t0 + own) / kMoeChunkTokens] + p.pos[entry];
+    }
+    if (p.layout != kMoeMasked) {
+        const int used = segment_starts(p, [&](int x) { return ws_totals(p)[x]; }, [&](int x, int start, int total) {
+            s_start[x] = start;
+            if (blockIdx.x == 0 && p.layout == kMoePsum) p.meta[x] = start + total;   // psum[e] = align(psum[e-1]) + count
+        });
+        if (threadIdx.x == kThreads - 1) s_start[p.num_experts] = used;
+        __syncthreads();
+    }
+    if (padding) {
+        const int x = blockIdx.x;
+        if (x == p.num_experts) pad_past(p, (int64_t)s_start[x] + (int)threadIdx.x, kThreads);
+        else pad_rows(p, s_start[x] + ws_totals(p)[x], s_start[x + 1]);
         return;
     }
-    const int lane = threadIdx.x & 63;
-    const int t = (blockIdx.x - pad_blocks) * (kThreads / 64) + (threadIdx.x >> 6);
-    if (t >= p.t) return;   // wave-uniform
-    // The row's first 8 KB are loaded before the rows are looked up (the two
-    // are independent), so the lookup's load latency hides behind them.
-    const i32x4* src = reinterpret_cast<const i32x4*>(p.x + (int64_t)t * p.ldx);
-    const int units = p.kdim / 16;
-    i32x4 v[8];
-#pragma unroll
-    for (int q = 0; q < 8; ++q) {
-        const int u = q * 64 + lane;
-        if (u < units) v[q] = src[u];
-    }
+    if (tokens <= 0) return;   // (no barrier follows)
     int flat = -1;
-    if (lane < p.k) {
-        const int e = topk_at(p, t, lane);
+    if (mine) {
         if (routed(p, e)) {
-            const int64_t pi = (int64_t)t * p.k + lane;
-            const int r = (p.layout == kMoeMasked ? 0 : ws_starts(p)[e]) +
-                          ws_counts(p)[(int64_t)e * p.chunks + t / kMoeChunkTokens] + p.pos[pi];
-            flat = p.layout == kMoeMasked ? (r < p.max_m ? e * p.max_m + r : -1) : r;
+            flat = p.layout == kMoeMasked ? (rank < p.max_m ? e * p.max_m + rank : -1) : s_start[e] + rank;
             if (flat >= 0) {
-                if (p.w_out) p.w_out[flat] = p.topk_w ? p.topk_w[(int64_t)t * p.w_st + (int64_t)lane * p.w_sk] : 1.f;
+                if (p.w_out) p.w_out[flat] = p.topk_w ? p.topk_w[(int64_t)(t0 + own) * p.w_st + (int64_t)slot * p.w_sk] : 1.f;
                 if (p.layout == kMoeContiguous) p.meta[flat] = e;
             }
         }
-        p.pos[(int64_t)t * p.k + lane] = flat;
+        p.pos[entry] = flat;
     }
     // The rows are written once and read by the next kernel, not by this one:
     // non-temporal stores (about 1.5x the copy rate of plain ones here).
-    for (int u0 = 0; u0 < units; u0 += 64 * 8) {
-        if (u0 > 0) {
 #pragma unroll
-            for (int q = 0; q < 8; ++q) {
-                const int u = u0 + q * 64 + lane;
-                if (u < units) v[q] = src[u];
+    for (int i = 0; i < TOKENS; ++i) {
+        if (i >= tokens) break;
+        for (int u0 = 0; u0 < units; u0 += 64 * UNITS) {
+            if (u0 > 0) {
+#pragma unroll
+                for (int q = 0; q < UNITS; ++q) {
+                    const int u = u0 + q * 64 + lane;
+                    if (u < units) v[i][q] = reinterpret_cast<const i32x4*>(p.x + (int64_t)(t0 + i) * p.ldx)[u];
+                }
             }
-        }
-        for (int j = 0; j < p.k; ++j) {
-            const int r = __builtin_amdgcn_readfirstlane(__shfl(flat, j));
-            if (r < 0) continue;   // wave-uniform
-            i32x4* dst = reinterpret_cast<i32x4*>(p.a + row_a(p, r));
+            for (int j = 0; j < p.k; ++j) {
+                const int r = __builtin_amdgcn_readlane(flat, i * p.k + j);
+                if (r < 0) continue;   // wave-uniform
+                i32x4* dst = reinterpret_cast<i32x4*>(p.a + row_a(p, r));
 #pragma unroll
-            for (int q = 0; q < 8; ++q) {
-                const int u = u0 + q * 64 + lane;
-                if (u < units) __builtin_nontemporal_store(v[q], dst + u);
+                for (int q = 0; q < UNITS; ++q) {
+                    const int u = u0 + q * 64 + lane;
+                    if (u < units) __builtin_nontemporal_store(v[i][q], dst + u);
+                }
             }
         }
     }
-    for (int s0 = 0; s0 < p.sfk; s0 += 64) {
-        const int s = s0 + lane;
-        const float sv = s < p.sfk ? p.x_sf[(int64_t)t * p.sf_st + (int64_t)s * p.sf_sk] : 0.f;
-        for (int j = 0; j < p.k; ++j) {
-            const int r = __builtin_amdgcn_readfirstlane(__shfl(flat, j));
-            if (r < 0) continue;
-            if (s < p.sfk) p.sf[row_sf(p, r) + (int64_t)s * p.sf_sk_o] = sv;
+#pragma unroll
+    for (int i = 0; i < TOKENS; ++i) {
+        if (i >= tokens) break;
+        for (int s = lane; s < p.sfk; s += 64) {
+            const float sv = p.x_sf[(int64_t)(t0 + i) * p.sf_st + (int64_t)s * p.sf_sk];
+            for (int j = 0; j < p.k; ++j) {
+                const int r = __builtin_amdgcn_readlane(flat, i * p.k + j);
+                if (r >= 0) p.sf[row_sf(p, r) + (int64_t)s * p.sf_sk_o] = sv;
+            }
         }
     }
 }
@@ -538,6 +540,7 @@ int32_t* moe_scratch_device_ptr() {
 int moe_dispatch_chunks(int64_t tokens) { return (int)((tokens + kMoeChunkTokens - 1) / kMoeChunkTokens); }
 
 int64_t moe_dispatch_workspace_ints(int64_t tokens, int num_experts) {
+    // (E + 1 more than counts and totals: the size that callers know)
     return (int64_t)moe_dispatch_chunks(tokens) * num_experts + 2 * (int64_t)num_experts + 1;
 }
 
@@ -545,11 +548,11 @@ void launch_moe_dispatch(const MoeDispatchArgs& a, hipStream_t stream) {
     DG_CHECK(a.num_experts > 0 && a.num_experts <= kMoeMaxExperts && a.k > 0 && a.k <= kMoeMaxTopk);
     DG_CHECK(a.chunks == moe_dispatch_chunks(a.t));
     // One launch or three: every workgroup of the one counts all entries for itself, work that grows
-    // with the square of the tokens, against two launches and a workspace's round trip. Rows of a BF16
-    // or FP8 token each, in a graph, one launch against three, us: 4 tokens x 8 slots 4.9/12.6, 777 x 6
-    // 9.9/17.2, 1024 x 8 (2048 columns) 13.4/20, 2048 x 8 (2048) 25.2/28.4, 4096 x 2 (2048) 18.1/19.2,
-    // 4096 x 8 (1024) 35.5/31.3. One token a workgroup or four, us: 64 x 8 of 7168 10.2/11.9,
-    // 512 x 8 of 2048 8.3/8.2, 777 x 6 10.8/9.9.
+    // with the square of the tokens, against two launches and a workspace's round trip. BF16 rows, tokens
+    // x slots (columns), one launch / three, us in a graph: 4 x 8 (7168) 6.1/12.9, 256 x 8 (7168) 15.2/22.8,
+    // 777 x 6 (2056) 10.1/14.8, 1024 x 8 (2048) 13.4/17.3, 2048 x 8 (2048) 25.0/24.8, 4096 x 2 (2048)
+    // 17.8/17.3, 3000 x 8 (2048) 38.5/31.9, 8192 x 1 (1024) 37.7/15.5. One token a workgroup or four, us:
+    // 64 x 8 of 7168 10.2/11.9, 512 x 8 of 2048 8.3/8.2, 777 x 6 10.8/9.9.
     const int64_t entries = (int64_t)a.t * a.k;
     const int tokens = entries * a.t <= kMoeFewOne ? 1 : 4;   // of a workgroup
     if (entries * ((a.t + tokens - 1) / tokens) <= kMoeFewCounts) {
@@ -567,8 +570,13 @@ void launch_moe_dispatch(const MoeDispatchArgs& a, hipStream_t stream) {
                        stream, a);
     DG_HIP_CHECK(hipGetLastError());
     const int pad_blocks = a.layout == kMoeMasked ? 0 : a.num_experts + 1;
-    const int64_t blocks = pad_blocks + ((int64_t)a.t + kThreads / 64 - 1) / (kThreads / 64);
-    hipLaunchKernelGGL(moe_scatter_kernel, dim3((unsigned)blocks), dim3(kThreads), 0, stream, a, pad_blocks);
+    // Short rows four tokens a wave: the scan of the totals weighs less. Four / one, us: 32768 x 4 rows of
+    // 512 bytes 27.9/32.6, 20000 x 8 of 128 22.8/30.8; of 1 KB 42.2/38.8, 16384 x 8 of 528 36.1/35.3.
+    const bool several = a.kdim <= kMoeShortRow;
+    const int per = kThreads / 64 * (several ? 4 : 1);   // tokens of a workgroup
+    const dim3 grid((unsigned)(pad_blocks + ((int64_t)a.t + per - 1) / per)), block(kThreads);
+    if (several) hipLaunchKernelGGL(moe_scatter_kernel<4>, grid, block, 0, stream, a, pad_blocks);
+    else hipLaunchKernelGGL(moe_scatter_kernel<1>, grid, block, 0, stream, a, pad_blocks);
     DG_HIP_CHECK(hipGetLastError());
 }
 

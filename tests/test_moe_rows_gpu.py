@@ -491,3 +491,27 @@ def test_gradients_of_many_and_of_wide_rows(t, k, h):
     none = torch.ones(t * k, dtype=torch.bool)
     none[pos[pos >= 0]] = False
     assert not dy[none.to(DEV)].any()
+
+
+@pytest.mark.parametrize('h', [8, 256, 264])
+@pytest.mark.parametrize('t', [4099, 8208])
+@pytest.mark.parametrize('layout', ['psum', 'masked'])
+def test_dispatch_of_many_short_rows(t, h, layout):
+    """Several tokens of a wave, the last wave's and workgroup's fewer."""
+    k, e = 16, 24
+    idx = routing(t, k, e, t)
+    x, x0 = tokens(t, h, t)
+    w = torch.rand((t, k), generator=torch.Generator().manual_seed(1))
+    kw = dict(alignment=16) if layout == 'psum' else dict(max_m=t // 2)
+    a, _, gl, got, rw = deep_gemm.moe_dispatch(x, idx.to(DEV), e, layout=layout, topk_weights=w.to(DEV), **kw)
+    pos, starts, ends, used = places(idx, e, 16 if layout == 'psum' else 1)
+    if layout == 'masked':
+        rank = pos - torch.tensor(starts)[idx.clamp(min=0).long()]
+        pos = torch.where((idx >= 0) & (rank < t // 2), idx.long() * (t // 2) + rank, -1)
+        assert gl.tolist() == [min(n - s, t // 2) for s, n in zip(starts, ends)]
+    else:
+        assert gl.tolist() == ends
+    live = pos >= 0
+    assert torch.equal(got.cpu().long(), pos)
+    assert torch.equal(bits(a.reshape(-1, h).cpu()[pos[live]]), bits(x0[live.nonzero()[:, 0]]))
+    assert torch.equal(rw.reshape(-1).cpu()[pos[live]], w[live])
