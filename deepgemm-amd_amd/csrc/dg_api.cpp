@@ -1465,9 +1465,9 @@ void moe_dispatch_impl(const dg_tensor* x_, const dg_tensor* x_sf_, const dg_ten
     const OnDevice on(one_device({x_, x_sf_, topk_idx_, topk_w_, a_, sf_, meta_, pos_, w_out_}));
     launch_moe_dispatch(p, stream);
     char buf[160];
-    std::snprintf(buf, sizeof(buf), "moe_dispatch%s layout=%s experts=%d t=%lld k=%lld kdim=%lld",
+    std::snprintf(buf, sizeof(buf), "moe_dispatch%s layout=%s experts=%d t=%lld k=%lld kdim=%lld launches=%d",
                   bf16 ? " x=bf16" : fp4 ? " x=e2m1" : "", layout == kMoeContiguous ? "contiguous" : layout == kMoePsum ? "psum" : "masked", num_experts,
-                  (long long)t, (long long)k, (long long)(fp4 ? 2 * cols : cols));
+                  (long long)t, (long long)k, (long long)(fp4 ? 2 * cols : cols), moe_few_tokens(p.t, p.k) ? 1 : 3);
     t_last_config = buf;
 }
 

@@ -260,7 +260,12 @@ void launch_per_token_cast(const CastArgs& args, hipStream_t stream);
 constexpr int kMoeMaxExperts = 1024;
 constexpr int kMoeMaxTopk = 16;
 constexpr int kMoeChunkTokens = 64;    // tokens per dispatch chunk (count / scatter workgroup)
-constexpr int64_t kMoeFewOne = 1 << 20, kMoeFewCounts = 1 << 23;   // entries x workgroups (launch_moe_dispatch)
+// Tokens of a workgroup of the dispatch in one launch, or 0: three launches (the figures: launch_moe_dispatch).
+inline int moe_few_tokens(int64_t t, int64_t k) {
+    if (t > 1 << 15) return 0;   // (the products below stay small)
+    const int tokens = t * k * t <= 1 << 20 ? 1 : 4;
+    return t * k * ((t + tokens - 1) / tokens) <= 1 << 23 ? tokens : 0;
+}
 enum MoeLayout : int32_t { kMoeContiguous = 0, kMoePsum = 1, kMoeMasked = 2 };
 struct MoeDispatchArgs {
     const uint8_t* x;          // rows of kdim bytes (e4m3, packed e2m1, BF16) [t]

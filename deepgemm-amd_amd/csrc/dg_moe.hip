@@ -553,9 +553,7 @@ void launch_moe_dispatch(const MoeDispatchArgs& a, hipStream_t stream) {
     // 777 x 6 (2056) 10.1/14.8, 1024 x 8 (2048) 13.4/17.3, 2048 x 8 (2048) 25.0/24.8, 4096 x 2 (2048)
     // 17.8/17.3, 3000 x 8 (2048) 38.5/31.9, 8192 x 1 (1024) 37.7/15.5. One token a workgroup or four, us:
     // 64 x 8 of 7168 10.2/11.9, 512 x 8 of 2048 8.3/8.2, 777 x 6 10.8/9.9.
-    const int64_t entries = (int64_t)a.t * a.k;
-    const int tokens = entries * a.t <= kMoeFewOne ? 1 : 4;   // of a workgroup
-    if (entries * ((a.t + tokens - 1) / tokens) <= kMoeFewCounts) {
+    if (const int tokens = moe_few_tokens(a.t, a.k)) {   // of a workgroup
         // (without tokens or padding rows: one workgroup for the ends, masked counts and weights)
         const int pad_blocks = a.layout != kMoeMasked ? (a.alignment > 1 ? a.num_experts : 1) : a.t == 0 ? 1 : 0;
         const dim3 grid(pad_blocks + (a.t + tokens - 1) / tokens), block(kThreads);

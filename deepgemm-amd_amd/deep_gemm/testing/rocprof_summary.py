@@ -33,7 +33,7 @@ import sys
 GEMM_KEYS = ('fp8_gemm_1d2d', 'fp8_fp4_gemm', 'fp8_gemm_1d2d_pipe', 'fp8_gemm_masked_stream', 'fp8_gemm_1d1d',
              'fp8_gemm_tinym', 'fp8_gemm_splitk', 'fp8_gemm_ksplit', 'moe_swiglu_cast_kernel')
 CAST_KEYS = ('per_token_cast_kernel',)   # the cast workload's kernel (GEMM workloads also cast while setting up)
-MOE_DISPATCH_KEYS = ('moe_count_kernel', 'moe_scan_kernel', 'moe_starts_kernel', 'moe_scatter_kernel')
+MOE_DISPATCH_KEYS = ('moe_count_kernel', 'moe_scan_kernel', 'moe_starts_kernel', 'moe_scatter_kernel', 'moe_dispatch_few_kernel')
 COPY_KEY = 'neg_kernel'
 _KEYS = GEMM_KEYS
 
@@ -93,11 +93,12 @@ def mfma_utilization(busy_cycles: float, gui_cycles: float, kernel_us: float, si
 def dispatches_per_call(config: str) -> int:
     """Kernels one bench launch dispatches: a dense column split, a contiguous row
     split or the split-K kernel (partials, then the reduction) runs two; a contiguous
-    layout longer than a block table runs `launches`; a MoE dispatch runs its count, scan, (segment starts,) scatter kernels; a launch of
+    layout longer than a block table runs `launches`; a MoE dispatch runs `launches` (in lines
+    without them, of older runs: its count, scan, (segment starts,) scatter kernels); a launch of
     several library calls (configs joined by ' + ') sums them."""
     if ' + ' in config:
         return sum(dispatches_per_call(c) for c in config.split(' + '))
-    if config.startswith('moe_dispatch'):   # count, scan, (starts,) scatter
+    if config.startswith('moe_dispatch') and ' launches=' not in config:   # count, scan, (starts,) scatter
         return 3 if 'layout=masked' in config else 4
     two = 'split_n=' in config or 'split_m=' in config or ' splits=' in config
     return (int(config.split(' launches=')[1].split()[0]) if ' launches=' in config else 1) + int(two)

@@ -211,3 +211,9 @@ def test_other_threads_run_during_a_call(stub, name):  # noqa: F811
     else:
         assert out[0] == 7
         assert [None if v is None else tuple(v.shape) for v in out[1:]] == shapes[name]
+
+
+def test_dispatches_of_a_moe_dispatch_that_names_its_launches():
+    from deep_gemm.testing import rocprof_summary
+    for n in (1, 3):
+        assert rocprof_summary.dispatches_per_call(f'moe_dispatch layout=psum experts=4 t=8 k=2 kdim=64 launches={n}') == n
