@@ -8,6 +8,10 @@
 // 256 elements are a step: 128 bytes of a row, as 64 BF16 values are, so that a step of the 4-bit
 // operands is one of the BF16 products' K-major operands, and is loaded, laid out in LDS and
 // read like it. A row has two words of scales a step.
+//
+// 16384 rows over 8 groups, n 4096, k 7168: 275 to 285 us, 3.4 to 3.5 PFLOP/s, bound by the clock that
+// the matrix load leaves (8192 x 4096 x 32768: 4.3 PFLOP/s of random values, 5.6 of zeros); k 2048,
+// n 7168 163 us (a tile's first loads and its stores); 32 rows over 32 groups, 4096 x 7168 90 us, 5.5 TB/s.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
