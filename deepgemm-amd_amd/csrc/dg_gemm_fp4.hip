@@ -43,7 +43,7 @@ struct ScaleSlab {
 #pragma unroll
         for (int i = 0; i < kLoads; ++i)
             row[i] = (uint32_t)(min(first_row + i * (64 / WORDS) + lane / WORDS, rows - 1) * (int)sr * 4);
-        word = (uint32_t)(lane % WORDS * (int)sk * 4);
+        word = (uint32_t)(lane % WORDS) * (uint32_t)sk * 4u;   // (up to 3 GiB)
         step = sk * 4 * WORDS;
         left = words;
     }

@@ -221,3 +221,46 @@ def test_graph_follows_its_ends():
                 check(d[lo:hi], ref, rounding(d.dtype, ref) + sum_error(1024, a64[lo:hi].abs() @ b64[g].T.abs()), f'{now} {g}')
             lo = hi
         assert (d[lo:] == 7.0).all()
+
+
+def test_rows_past_32_bits():
+    """A's codes, its scales' rows and D's rows of a group that begins past 2^32 bytes of A."""
+    k, n, first, rows = 8192, 64, 1 << 20, 70
+    total = first + rows
+    codes = torch.zeros((total, k // 2), dtype=torch.int8, device=DEV)
+    scales = torch.full((total, k // 128), -1, dtype=torch.int32, device=DEV)
+    (q0, s0), head = operand((5, k), 1)
+    (q1, s1), tail = operand((rows, k), 2)
+    codes[:5], scales[:5], codes[first:], scales[first:] = q0, s0, q1, s1
+    b, b64 = operand((2, n, k), 3)
+    d = torch.full((total, n), 7.0, dtype=torch.bfloat16, device=DEV)
+    deep_gemm.m_grouped_fp4_gemm_nt_ragged((codes, scales), b, d, torch.tensor([5, total], dtype=torch.int32, device=DEV), alignment=first)
+    torch.cuda.synchronize()
+    for got, a, w in ((d[:5], head, b64[0]), (d[first:], tail, b64[1])):
+        ref, mag = a @ w.T, a.abs() @ w.T.abs()
+        check(got, ref, rounding(torch.bfloat16, ref) + sum_error(k, mag) * (1 + 2.0 ** -7), 'rows')
+    assert (d[5:first] == 7.0).all()
+
+
+def test_scales_words_far_apart():
+    """Words of scales nearly 2^30 bytes apart, of A (a step has two of them, two steps four)."""
+    k, n, rows = 544, 40, 33
+    a, a64 = operand((rows, k), 1)
+    b, b64 = operand((1, n, k), 2)
+    pitch = (1 << 28) - 64
+    far = torch.empty(4 * pitch + rows, dtype=torch.int32, device=DEV)
+    words = far.as_strided((rows, 5), (1, pitch))
+    words.copy_(a[1])
+    d = torch.zeros((rows, n), dtype=torch.float32, device=DEV)
+    deep_gemm.m_grouped_fp4_gemm_nt_ragged((a[0], words), b, d, torch.tensor([rows], dtype=torch.int32, device=DEV))
+    torch.cuda.synchronize()
+    ref, mag = a64 @ b64[0].T, a64.abs() @ b64[0].T.abs()
+    check(d, ref, rounding(torch.float32, ref) + sum_error(k, mag) * (1 + 2.0 ** -7), 'far words')
+
+
+def test_workspace_sizes(tiles):
+    size = deep_gemm._ffi.lib.dg_fp4_gemm_ragged_workspace_size
+    pieces = {'32 in 2 pieces': 2, '128 in 3 pieces': 3}.get(tiles, 0)
+    if tiles != 'heuristic':
+        assert size(10, 30, 4096, 2) == 10 * 32 * 4 * pieces   # each piece's FP32 sums, rows of whole fours
+    assert size(1 << 29, 1 << 20, 256, 1) == -1                # more threads than a launch counts

@@ -217,3 +217,13 @@ def test_dispatches_of_a_moe_dispatch_that_names_its_launches():
     from deep_gemm.testing import rocprof_summary
     for n in (1, 3):
         assert rocprof_summary.dispatches_per_call(f'moe_dispatch layout=psum experts=4 t=8 k=2 kdim=64 launches={n}') == n
+
+
+def test_tiles_of_the_4_bit_product_that_are_not_there():
+    try:
+        for block, pieces in ((16, 0), (96, 1), (512, 0), (256, 1), (128, 33), (32, -1)):
+            assert lib.dg_set_tile_override(14, block, pieces) != 0, (block, pieces)
+        for block, pieces in ((256, 0), (128, 32), (64, 1), (32, 0)):
+            assert lib.dg_set_tile_override(14, block, pieces) == 0, (block, pieces)
+    finally:
+        lib.dg_set_tile_override(0, 0, 0)
