@@ -20,6 +20,7 @@ from typing import Optional, Tuple
 import ctypes
 
 import torch
+from torch.autograd import forward_ad as _forward_ad
 
 from . import _ffi
 from ._ffi import address as _address, bind as _bind, check as _check, describe as _desc
@@ -450,6 +451,22 @@ def per_token_cast_to_fp8(x: torch.Tensor, use_ue8m0: bool, gran_k: int = 128,
     return q, sf
 
 
+def _takes_kernel(*tensors: torch.Tensor) -> bool:
+    """Whether a kernel may stand for torch ops on these tensors: they are plain ones of one GPU, and torch
+    does not have to follow what becomes of them (tangents, transforms of torch.func)."""
+    return (torch._C._functorch.peek_interpreter_stack() is None and _forward_ad._current_level < 0 and
+            all(type(t) in (torch.Tensor, torch.nn.Parameter) and t.is_cuda and t.device == tensors[0].device for t in tensors))
+
+
+def _cast4_rows(n: int) -> int:
+    """Rows of n columns that a launch of the 4-bit casts takes: below 2^24 blocks of 4 x 1024 values."""
+    return ((1 << 24) - 1) // max((n + 1023) // 1024, 1) * 4
+
+
+def _follows(t: torch.Tensor) -> bool:
+    return t.requires_grad and torch.is_grad_enabled()
+
+
 def per_token_cast_to_fp4(x: torch.Tensor, use_ue8m0: bool, gran_k: int = 128,
                           use_packed_ue8m0: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
     """[m, n] -> (packed e2m1 int8 [m, n / 2], element 2i in the low nibble, float32 SF
@@ -465,18 +482,34 @@ def per_token_cast_to_fp4(x: torch.Tensor, use_ue8m0: bool, gran_k: int = 128,
     return q, sf
 
 
+def _cast_back4_on_device(packed: torch.Tensor, sf: torch.Tensor, gran_k: int, use_packed_ue8m0: bool) -> bool:
+    if not packed.is_cuda or packed.dtype != torch.int8 or packed.dim() != 2 or sf.dim() != 2:
+        return False
+    m, half = packed.shape
+    if gran_k not in (32, 64, 128) or half >= (1 << 26) or (half > 1 and packed.stride(1) != 1):
+        return False
+    groups = (2 * half + gran_k - 1) // gran_k
+    if sf.dtype != (torch.int32 if use_packed_ue8m0 else torch.float32) or _follows(sf):
+        return False
+    return sf.shape == (m, (groups + 3) // 4 if use_packed_ue8m0 else groups) and _takes_kernel(packed, sf)
+
+
 def cast_back_from_fp4(packed: torch.Tensor, sf: torch.Tensor, gran_k: int = 128, use_packed_ue8m0: bool = False,
-                       dtype: torch.dtype = torch.float32) -> torch.Tensor:
-    """The values that per_token_cast_to_fp4's codes and scales stand for, float32 or bfloat16
-    (rounded once; exact for power-of-two scales from 2^-125 on): with it the BF16 products
-    take 4-bit weights, for gradients through them. Device tensors take one HIP kernel;
-    others the torch ops of deep_gemm.utils.math."""
-    if dtype not in (torch.float32, torch.bfloat16):
+                       dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """The values that per_token_cast_to_fp4's codes and scales stand for: float32 (the type of float32
+    times the scales', for scales of other types), or `dtype`, float32 or bfloat16 (rounded once; exact
+    for power-of-two scales from 2^-125 on): with it the BF16 products take 4-bit weights, for
+    gradients through them. Device tensors take one HIP kernel where codes are contiguous within a row
+    and scales are float32 or packed words, one for each group, without a gradient; others the torch ops
+    of deep_gemm.utils.math."""
+    if dtype not in (None, torch.float32, torch.bfloat16):
         raise TypeError('dtype must be torch.float32 or torch.bfloat16')
-    if not packed.is_cuda or packed.dtype != torch.int8 or packed.dim() != 2 or gran_k not in (32, 64, 128):
-        return utils.math.cast_back_from_fp4(packed, sf, gran_k, use_packed_ue8m0).to(dtype)
-    if sf.dtype != (torch.int32 if use_packed_ue8m0 else torch.float32):
-        raise RuntimeError('Assertion error (deep_gemm): sf must be int32 words with use_packed_ue8m0, else float32')
+    if not _cast_back4_on_device(packed, sf, gran_k, use_packed_ue8m0):
+        y = utils.math.cast_back_from_fp4(packed, sf, gran_k, use_packed_ue8m0)
+        return y if dtype is None else y.to(dtype)
+    rows = _cast4_rows(2 * packed.size(1))
+    if packed.size(0) > rows:
+        return torch.cat([cast_back_from_fp4(q, s, gran_k, use_packed_ue8m0, dtype) for q, s in zip(packed.split(rows), sf.split(rows))])
     status, y = _bind.cast_back4(packed, sf, gran_k, int(dtype == torch.bfloat16), _raw_stream_of(packed))
     _check(status)
     return y
