@@ -473,10 +473,15 @@ def per_token_cast_to_fp4(x: torch.Tensor, use_ue8m0: bool, gran_k: int = 128,
     [m, ceil(n / gran_k)] or packed int32 UE8M0 words); gran_k 32 with use_ue8m0 is the microscaled
     format that m_grouped_fp4_gemm_nt_ragged takes. Results of the reference's
     (deep_gemm/utils/math.py) to the bit. BF16 device tensors take the fused HIP kernel (one HBM
-    pass); anything else takes the torch ops of deep_gemm.utils.math."""
-    if not _cast_on_device(x) or gran_k not in (32, 64, 128):
+    pass); anything else takes the torch ops of deep_gemm.utils.math: other granularities and strides,
+    and an x whose gradient the float32 scales carry (the codes and power-of-two scales have none)."""
+    if not (_cast_on_device(x) and x.size(1) % 2 == 0 and gran_k in (32, 64, 128) and _takes_kernel(x)) or \
+            (not use_ue8m0 and _follows(x)):
         return utils.math.per_token_cast_to_fp4(x, use_ue8m0, gran_k, use_packed_ue8m0)
     assert not use_packed_ue8m0 or use_ue8m0
+    if x.size(0) > _cast4_rows(x.size(1)):
+        parts = [per_token_cast_to_fp4(p, use_ue8m0, gran_k, use_packed_ue8m0) for p in x.split(_cast4_rows(x.size(1)))]
+        return torch.cat([q for q, _ in parts]), torch.cat([sf for _, sf in parts])
     status, q, sf = _bind.cast4(x, gran_k, int(bool(use_ue8m0)), int(bool(use_packed_ue8m0)), _raw_stream_of(x))
     _check(status)
     return q, sf

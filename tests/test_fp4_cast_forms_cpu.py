@@ -28,3 +28,10 @@ def test_traced_device_tensors():
         sf = torch.empty((6, 4), device='cuda')
         v = deep_gemm.cast_back_from_fp4(q, sf, 32)
         assert v.shape == (6, 128) and v.dtype == torch.float32 and v.is_cuda
+        q, sf = deep_gemm.per_token_cast_to_fp4(torch.empty((6, 128), dtype=torch.bfloat16, device='cuda'), False, 32)
+        assert q.shape == (6, 64) and q.dtype == torch.int8 and sf.shape == (6, 4) and sf.is_cuda
+
+
+def test_odd_columns_are_refused_alike():
+    with pytest.raises(AssertionError):
+        deep_gemm.per_token_cast_to_fp4(torch.zeros((2, 33), dtype=torch.bfloat16), True, 32)

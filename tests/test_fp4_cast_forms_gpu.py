@@ -63,6 +63,22 @@ def test_gradient_of_the_scales():
         assert deep_gemm.get_last_config().startswith('cast_back_from_fp4')
 
 
+def test_gradient_of_the_float_scales_of_a_cast():
+    """sf = largest magnitude / 6 carries its group's gradient to that element."""
+    x = torch.randn((3, 64), generator=torch.Generator().manual_seed(5)).bfloat16()
+    want = x.clone().requires_grad_()
+    q0, sf0 = plain.per_token_cast_to_fp4(want, False, 32)
+    sf0.sum().backward()
+    got = x.to(DEV).requires_grad_()
+    q, sf = deep_gemm.per_token_cast_to_fp4(got, False, 32)
+    assert torch.equal(q.cpu(), q0) and torch.equal(sf.detach().cpu(), sf0.detach())
+    sf.sum().backward()
+    assert torch.equal(got.grad.cpu(), want.grad) and got.grad.count_nonzero() == 6
+    # power-of-two scales carry none: the kernel
+    q, sf = deep_gemm.per_token_cast_to_fp4(got, True, 32)
+    assert not sf.requires_grad and deep_gemm.get_last_config().startswith('per_token_cast_to_fp4')
+
+
 def test_tangent_of_the_scales():
     q, sf, d = codes(4, 32), scales(4, 2), scales(4, 2, seed=6)
     with forward_ad.dual_level():
@@ -86,3 +102,23 @@ def test_more_rows_than_a_launch_has():
     q[-2:, 0], sf[-2:, 0] = torch.tensor([0x75, -0x46], dtype=torch.int8, device=DEV), torch.tensor([3.0, 0.5], device=DEV)
     v = deep_gemm.cast_back_from_fp4(q, sf, 32)
     assert torch.equal(v[-2:].cpu(), plain.cast_back_from_fp4(q[-2:].cpu(), sf[-2:].cpu(), 32)) and not v[:-2].any()
+
+
+def test_casts_of_more_rows_than_a_launch_has():
+    """Past 2^26 rows of two values."""
+    m = (1 << 26) + 3
+    x = torch.zeros((m, 2), dtype=torch.bfloat16, device=DEV)
+    x[-2:] = torch.tensor([[6.0, -3.0], [0.25, 1.0]], dtype=torch.bfloat16, device=DEV)
+    q, sf = deep_gemm.per_token_cast_to_fp4(x, True, 32, True)
+    rq, rsf = plain.per_token_cast_to_fp4(x[-2:].cpu(), True, 32, True)
+    assert torch.equal(q[-2:].cpu(), rq) and torch.equal(sf[-2:].cpu(), rsf) and not q[:-2].any()
+    v = deep_gemm.cast_back_from_fp4(q, sf, 32, True, torch.bfloat16)
+    assert torch.equal(v[-2:].float().cpu(), plain.cast_back_from_fp4(rq, rsf, 32, True)) and not v[:-2].any()
+
+
+def test_parameters_take_the_kernel():
+    x = torch.nn.Parameter(torch.randn((8, 64), device=DEV).bfloat16())
+    q, sf = deep_gemm.per_token_cast_to_fp4(x, True, 32, True)
+    assert deep_gemm.get_last_config().startswith('per_token_cast_to_fp4')
+    rq, rsf = plain.per_token_cast_to_fp4(x.detach().cpu(), True, 32, True)
+    assert torch.equal(q.cpu(), rq) and torch.equal(sf.cpu(), rsf)
