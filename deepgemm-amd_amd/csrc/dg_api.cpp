@@ -1560,6 +1560,28 @@ ExpertRows expert_rows(const dg_tensor* t_, const char* name, int64_t n) {
             t.dim() == 3 ? (int32_t)t.size(1) : 0};
 }
 
+// Whether expert rows of n elements at `a` and at `b` share memory. Exact where their strides are
+// alike (two ranges of columns of a buffer); others share it where their spans meet.
+bool share_memory(const void* a, const ExpertRows& ra, const void* b, const ExpertRows& rb, int64_t n) {
+    if (ra.rows == 0 || rb.rows == 0 || n == 0) return false;
+    auto per = [](const ExpertRows& r) { return r.max_m ? r.max_m : r.rows; };   // rows of a group
+    auto span = [&](const ExpertRows& r) { return (r.rows / per(r) - 1) * r.gs + (per(r) - 1) * r.ld + n; };
+    const int64_t d = static_cast<int64_t>(reinterpret_cast<intptr_t>(b) - reinterpret_cast<intptr_t>(a)) / 2;   // elements
+    if (d >= span(ra) || -d >= span(rb)) return false;
+    if (ra.ld != rb.ld || ra.gs != rb.gs || ra.max_m != rb.max_m || ra.rows != rb.rows) return true;
+    // Rows lie apart by d + i gs + j ld, i and j below the groups and their rows: the two multiples next to
+    // zero, as a group is no longer than gs and a row than ld.
+    auto near = [](int64_t at, int64_t step, int64_t count, auto&& f) {
+        const int64_t q = step > 0 ? (at >= 0 ? -ceil_div(at, step) : -at / step) : 0;
+        for (int64_t i = q; i <= q + (step > 0); ++i)
+            if (-count < i && i < count && f(at + i * step)) return true;
+        return false;
+    };
+    return near(d, ra.gs, ra.rows / per(ra), [&](int64_t at) {
+        return near(at, ra.ld, per(ra), [&](int64_t x) { return -n < x && x < n; });
+    });
+}
+
 // pos and the token rows of both gradients, and what they share of the arguments.
 MoeGradArgs moe_grad_args(const dg_tensor* tokens_, const char* name, const dg_tensor* pos_) {
     const View x = view(tokens_, name), pos = view(pos_, "pos");
@@ -1619,6 +1641,7 @@ void combine_backward_impl(const dg_tensor* dout_, const dg_tensor* y_, const dg
         const ExpertRows y = expert_rows(y_, "y", p.n);
         DG_CHECK(y_->ndim == dy_->ndim && y.rows == r.rows && y.max_m == r.max_m);
         if (y_->data == dy_->data) DG_CHECK(y.ld == r.ld && y.gs == r.gs);   // in place: the same elements
+        else DG_CHECK(!share_memory(y_->data, y, dy_->data, r, p.n));       // or none: y is read while dy is written
         p.rows_in = static_cast<const uint16_t*>(y_->data), p.ld_in = y.ld, p.gs_in = y.gs;
         p.w = static_cast<const float*>(w.data()), p.w_st = w.stride(0), p.w_sk = w.stride(1);
         p.dw = moe_weight_gradient(dw_, p.t, p.k);

@@ -634,8 +634,8 @@ def moe_combine_backward(dout: torch.Tensor, y: torch.Tensor, pos: torch.Tensor,
     [T, topk] gradient of topk_weights or None without them): dy[pos[t, j]] = w * dout[t], dw =
     the products of dout[t] and y[pos[t, j]] summed. y is read only with topk_weights. Every row
     is named at most once in pos, as moe_dispatch leaves it; rows that it does not name are
-    zeros, or with `out` (a preallocated dy, which may be y itself) left as they were: that
-    saves a pass over dy. N a multiple of 8, topk at most 16."""
+    zeros, or with `out` (a preallocated dy, y itself or memory that neither y nor dout has) left
+    as they were: that saves a pass over dy. N a multiple of 8, topk at most 16."""
     status, dy, dw = _bind.combine_backward(dout, y, pos, topk_weights, out, _raw_stream_of(dout))
     _check(status)
     return dy, dw

@@ -436,7 +436,7 @@ int dg_moe_dispatch_backward(const dg_tensor* drows, const dg_tensor* pos, const
  *   pos             as above; every row is named by at most one entry, as dg_moe_dispatch leaves it
  *   topk_weights    f32 [T, topk], any strides, or NULL (w = 1)
  *   dy              y's shape, bf16, 16-byte rows; rows that no entry names are left as they were;
- *                   may be y itself
+ *                   may be y itself, but must not overlap y otherwise (DG_ERR_INVALID), nor dout
  *   d_topk_weights  f32 [T, topk] contiguous (0 where there is no row); given if and only if
  *                   topk_weights is
  * T < 2^24 where N > 1024. */
