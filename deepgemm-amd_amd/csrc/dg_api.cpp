@@ -2198,6 +2198,7 @@ int dg_moe_dispatch(const dg_tensor* x, const dg_tensor* x_sf, const dg_tensor* 
     return guarded([&] {
         const View ws = view(workspace, "workspace");
         DG_CHECK(ws.dtype() == DG_I32 && ws.on_device() && contiguous_view(ws));
+        one_device({x, workspace});
         int64_t numel = 1;
         for (int i = 0; i < ws.dim(); ++i) numel *= ws.size(i);
         moe_dispatch_impl(x, x_sf, topk_idx, topk_weights, num_experts, layout, alignment, a, sf, grouped_layout, pos,

@@ -227,3 +227,11 @@ def test_tiles_of_the_4_bit_product_that_are_not_there():
             assert lib.dg_set_tile_override(14, block, pieces) == 0, (block, pieces)
     finally:
         lib.dg_set_tile_override(0, 0, 0)
+
+
+@pytest.mark.parametrize('few', [True, False])
+def test_dispatch_refuses_a_workspace_of_another_device(few):
+    t = 8 if few else 4096
+    args = dict(DISPATCH, x=dev(BF16, t, 64), topk=dev(I32, t, 2), a=dev(BF16, 2 * t, 64), pos=dev(I32, t, 2), ws=dev(I32, 1 << 14, device=1))
+    refused('dg_moe_dispatch', args, [('ws', args['ws']), ('ws', dev(I32, 1 << 14, device=-1))])
+    assert call('dg_moe_dispatch', *dict(args, x=None).values()) == _ffi.DG_ERR_INVALID
