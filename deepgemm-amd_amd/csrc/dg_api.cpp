@@ -1388,7 +1388,7 @@ void moe_dispatch_impl(const dg_tensor* x_, const dg_tensor* x_sf_, const dg_ten
     DG_CHECK(x.dim() == 2 && x.stride(-1) == 1 && x.on_device());
     const int64_t size = bf16 ? 2 : 1, t = x.size(0), cols = x.size(1), kdim = cols * size;
     const int64_t sfk = bf16 ? 0 : ceil_div(fp4 ? 2 * cols : cols, (int64_t)128);
-    DG_CHECK(kdim % 16 == 0 && kdim < ((int64_t)1 << 30) && t < ((int64_t)1 << 30));
+    DG_CHECK(kdim % 16 == 0 && kdim <= ((int64_t)1 << 31) - (1 << 14) && t < ((int64_t)1 << 30));   // (32-bit bytes of a row)
     DG_CHECK_GRID((t + 3) / 4 + num_experts + 1, 256);
     check_vector_alignment(x, "x");
     const int sf_dtype = fp4 ? DG_I32 : DG_F32;
@@ -1420,8 +1420,8 @@ void moe_dispatch_impl(const dg_tensor* x_, const dg_tensor* x_sf_, const dg_ten
         DG_CHECK(max_m > 0 && (bf16 || sf_->sizes[1] == max_m) && meta.size(0) == num_experts);
         cap = num_experts * max_m;
     } else {
-        // (the padded products' block heights; the ragged ones take any)
-        DG_CHECK(alignment > 0 && alignment <= (1 << 20) && (alignment % 16 == 0 || x.dtype() != DG_E4M3));
+        // (the padded products' block heights; the ragged ones take any up to 2^20)
+        DG_CHECK(alignment > 0 && (x.dtype() == DG_E4M3 ? alignment % 16 == 0 : alignment <= (1 << 20)));
         DG_CHECK(a.dim() == 2 && (bf16 || sf_->sizes[0] == a.size(0)));
         cap = a.size(0);
         // every routing must fit: the segments take at most T*k + E*(alignment - 1) rows

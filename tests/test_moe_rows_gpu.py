@@ -515,3 +515,28 @@ def test_dispatch_of_many_short_rows(t, h, layout):
     assert torch.equal(got.cpu().long(), pos)
     assert torch.equal(bits(a.reshape(-1, h).cpu()[pos[live]]), bits(x0[live.nonzero()[:, 0]]))
     assert torch.equal(rw.reshape(-1).cpu()[pos[live]], w[live])
+
+
+def test_dispatch_of_8_bit_rows_far_apart():
+    """Segments at multiples of 2^21 rows, and rows of more than 2^30 bytes."""
+    idx = torch.tensor([[1, 0], [1, -1], [-1, 1]], dtype=torch.int32)
+    x = torch.arange(3 * 16, dtype=torch.uint8).view(3, 16)
+    sf = torch.tensor([[1.0], [2.0], [3.0]])
+    a, a_sf, ends, got, _ = deep_gemm.moe_dispatch((x.view(torch.float8_e4m3fn).to(DEV), sf.to(DEV)), idx.to(DEV), 2, layout='psum',
+                                                   alignment=1 << 21)
+    pos, _, want, _ = places(idx, 2, 1 << 21)
+    live = pos >= 0
+    assert torch.equal(got.cpu().long(), pos) and ends.tolist() == want
+    assert torch.equal(a.view(torch.uint8)[pos[live].to(DEV)].cpu(), x[live.nonzero()[:, 0]])
+    assert torch.equal(a_sf[pos[live].to(DEV)].cpu(), sf[live.nonzero()[:, 0]])
+    del a, a_sf
+    k = (1 << 30) + 4096 + 16
+    wide = torch.zeros((1, k), dtype=torch.uint8, device=DEV)
+    at = torch.tensor([0, 1 << 30, k - 1], device=DEV)
+    wide[0, at] = torch.tensor([5, 6, 7], dtype=torch.uint8, device=DEV)
+    scales = torch.zeros((1, -(-k // 128)), device=DEV)
+    scales[0, -1] = 9.0
+    a, a_sf, count, got, _ = deep_gemm.moe_dispatch((wide.view(torch.float8_e4m3fn), scales), torch.tensor([[2]], dtype=torch.int32, device=DEV),
+                                                    3, layout='masked', max_m=1)
+    assert count.tolist() == [0, 0, 1] and got.tolist() == [[2]]
+    assert torch.equal(a.view(torch.uint8)[2], wide) and torch.equal(a_sf[2], scales)
