@@ -569,9 +569,12 @@ void launch_moe_dispatch(const MoeDispatchArgs& a, hipStream_t stream) {
                        stream, a);
     DG_HIP_CHECK(hipGetLastError());
     const int pad_blocks = a.layout == kMoeMasked ? 0 : a.num_experts + 1;
-    // Short rows four tokens a wave: the scan of the totals weighs less. Four / one, us: 32768 x 4 rows of
-    // 512 bytes 27.9/32.6, 20000 x 8 of 128 22.8/30.8; of 1 KB 42.2/38.8, 16384 x 8 of 528 36.1/35.3.
-    const bool several = a.kdim <= kMoeShortRow;
+    // Short rows four tokens a wave, where the fourfold fewer waves still fill the card and a token has little to
+    // store: the scan of the totals weighs less. One / four, us (FP8 rows, alignment 16): 64 experts, 512 bytes
+    // 5000 x 8 18.7/21.2, 8192 x 1 14.5/12.6, 8192 x 4 18.1/16.4, 8192 x 16 34.6/36.7, 16384 x 2 20.8/15.6,
+    // 16384 x 16 47.3/54.3, of 256 bytes 16384 x 8 30.9/26.1; masked 256 bytes 5000 x 8 20.5/25.7, 8192 x 1
+    // 12.7/11.8, 10000 x 4 19.9/20.7, 12000 x 4 21.6/21.0, 16384 x 8 38.3/36.8. 1 KB, 16384 x 8 (BF16) 38.8/42.2.
+    const bool several = a.kdim <= kMoeShortRow && a.k * a.kdim < 4096 && a.t >= (a.layout == kMoeMasked && a.k > 2 ? 12000 : 8192);
     const int per = kThreads / 64 * (several ? 4 : 1);   // tokens of a workgroup
     const dim3 grid((unsigned)(pad_blocks + ((int64_t)a.t + per - 1) / per)), block(kThreads);
     if (several) hipLaunchKernelGGL(moe_scatter_kernel<4>, grid, block, 0, stream, a, pad_blocks);

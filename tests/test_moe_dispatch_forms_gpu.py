@@ -1,0 +1,76 @@
+"""Every form of the dispatch (one launch or several, one or four tokens of a wave, rows and scales in one
+round or more) against counting on the host, bit for bit: rows, scales, weights, and what no token owns."""
+import pytest
+import torch
+
+import deep_gemm
+from ragged import DEV
+from test_moe_rows_gpu import places, routing
+
+pytestmark = pytest.mark.gpu
+
+
+def rows_of(kind, t, cols, seed):
+    """Token rows and scales on the host: bytes as they lie (any bits are allowed: rows are copied)."""
+    gen = torch.Generator().manual_seed(seed)
+    if kind == 'bf16':
+        return torch.randn((t, cols), generator=gen).bfloat16(), None
+    if kind == 'e4m3':
+        return torch.randint(0, 127, (t, cols), generator=gen, dtype=torch.uint8).view(torch.float8_e4m3fn), \
+            torch.rand((t, -(-cols // 128)), generator=gen)
+    return torch.randint(-128, 128, (t, cols // 2), generator=gen, dtype=torch.int8), \
+        torch.randint(-2 ** 31, 2 ** 31, (t, -(-cols // 128)), generator=gen).int()
+
+
+def raw(x):
+    return x.view(torch.int16) if x.dtype == torch.bfloat16 else x.view(torch.int8) if x.element_size() == 1 else x.view(torch.int32)
+
+
+def dispatch(kind, t, k, e, cols, layout, alignment=16, launches=None, lost=0.1, idx=None):
+    print(f'{kind} t={t} k={k} e={e} cols={cols} {layout} alignment={alignment}', flush=True)
+    idx = routing(t, k, e, t + k, lost=lost, again=True) if idx is None else idx
+    x, sf = rows_of(kind, t, cols, t)
+    w = torch.rand((t, k), generator=torch.Generator().manual_seed(1)) + 0.1
+    max_m = max(1, t * k // e)
+    more = dict(max_m=max_m) if layout == 'masked' else dict(alignment=alignment)
+    given = x.to(DEV) if sf is None else (x.to(DEV), sf.to(DEV))
+    a, a_sf, gl, got, rw = deep_gemm.moe_dispatch(given, idx.to(DEV), e, layout=layout, topk_weights=w.to(DEV), **more)
+    config = deep_gemm.get_last_config()
+    assert launches is None or f' launches={launches}' in config, config
+    pos, starts, ends, used = places(idx, e, 1 if layout == 'masked' else alignment)
+    if layout == 'masked':
+        rank = pos - torch.tensor(starts)[idx.clamp(0, e - 1).long()]
+        pos = torch.where((pos >= 0) & (rank < max_m), idx.long() * max_m + rank, -1)
+        assert gl.tolist() == [min(n - s, max_m) for s, n in zip(starts, ends)]
+    elif layout == 'psum':
+        assert gl.tolist() == ends
+    else:
+        want = torch.full((a.shape[0],), -1, dtype=torch.int32)
+        for g, (s, n) in enumerate(zip(starts, ends)):
+            want[s:n] = g
+        assert torch.equal(gl.cpu(), want)
+    live = pos >= 0
+    assert torch.equal(got.cpu().long(), pos)
+    at, token = pos[live], live.nonzero()[:, 0]
+    weights = rw.reshape(-1).cpu()
+    assert torch.equal(weights[at], w[live])
+    for src, dst in ((x, a), (sf, a_sf)):
+        if src is None:
+            assert dst is None
+            continue
+        dst = raw(dst).reshape(-1, dst.shape[-1]).cpu()
+        assert torch.equal(dst[at], raw(src)[token])
+        if layout != 'masked':   # padding rows
+            rest = torch.ones(used, dtype=torch.bool)
+            rest[at] = False
+            assert not dst[:used][rest].any()
+    if layout != 'masked':
+        weights[at] = 0
+        assert not weights.any()
+
+
+@pytest.mark.parametrize('kind,cols', [('bf16', 64), ('e4m3', 256), ('e2m1', 512)])
+@pytest.mark.parametrize('t,k,layout', [(8191, 3, 'psum'), (8192, 3, 'psum'), (8197, 1, 'contiguous'), (11999, 3, 'masked'),
+                                        (12000, 3, 'masked'), (12005, 1, 'masked'), (8192, 2, 'masked'), (9000, 16, 'psum')])
+def test_one_and_four_tokens_of_a_wave(kind, cols, t, k, layout):
+    dispatch(kind, t, k, 40, cols, layout)
