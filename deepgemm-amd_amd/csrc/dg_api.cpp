@@ -1467,7 +1467,8 @@ void moe_dispatch_impl(const dg_tensor* x_, const dg_tensor* x_sf_, const dg_ten
     char buf[160];
     std::snprintf(buf, sizeof(buf), "moe_dispatch%s layout=%s experts=%d t=%lld k=%lld kdim=%lld launches=%d",
                   bf16 ? " x=bf16" : fp4 ? " x=e2m1" : "", layout == kMoeContiguous ? "contiguous" : layout == kMoePsum ? "psum" : "masked", num_experts,
-                  (long long)t, (long long)k, (long long)(fp4 ? 2 * cols : cols), moe_few_tokens(p.t, p.k) ? 1 : 3);
+                  (long long)t, (long long)k, (long long)(fp4 ? 2 * cols : cols),
+                  moe_dispatch_launches(p.t, p.k, p.kdim, num_experts, layout));
     t_last_config = buf;
 }
 

@@ -267,6 +267,17 @@ inline int moe_few_tokens(int64_t t, int64_t k) {
     return t * k * ((t + tokens - 1) / tokens) <= 1 << 23 ? tokens : 0;
 }
 enum MoeLayout : int32_t { kMoeContiguous = 0, kMoePsum = 1, kMoeMasked = 2 };
+// Whether a wave of the scatter has four tokens (rows of `kdim` bytes; the figures: launch_moe_dispatch).
+inline bool moe_four_tokens(int64_t t, int64_t k, int64_t kdim, int32_t layout) {
+    return kdim <= 512 && k * kdim < 4096 && t >= (layout == kMoeMasked && k > 2 ? 12000 : 8192);
+}
+// Launches of a dispatch: count, scan, scatter, and the segment starts between these for many tokens with little
+// to store (figures likewise).
+inline int moe_dispatch_launches(int64_t t, int64_t k, int64_t kdim, int64_t experts, int32_t layout) {
+    if (moe_few_tokens(t, k)) return 1;
+    if (layout == kMoeMasked || t < 8192 || moe_four_tokens(t, k, kdim, layout)) return 3;
+    return k * kdim <= 4096 || k <= 2 || (k <= 4 && experts > 256) ? 4 : 3;
+}
 struct MoeDispatchArgs {
     const uint8_t* x;          // rows of kdim bytes (e4m3, packed e2m1, BF16) [t]
     int64_t ldx;               // bytes

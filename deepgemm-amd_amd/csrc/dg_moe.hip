@@ -7,7 +7,7 @@
 //
 // Dispatch (all integer work, deterministic): each (token t, slot j) routed to
 // expert e gets the next row of e's segment, in token-then-slot order. Few tokens: in one launch
-// (moe_dispatch_few_kernel); others in three:
+// (moe_dispatch_few_kernel); others in three, or four (moe_starts_kernel between the last two):
 //   1. count:   per chunk of 64 tokens, one wave ranks the chunk's entries
 //               among equal experts with ballots (in entry order; the rank goes
 //               to pos) and leaves the chunk's count per expert;
@@ -36,7 +36,6 @@ namespace dgm {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kMoeShortRow = 512;   // bytes
 using dev::i32x4;
 
 __device__ __forceinline__ int align_up(int x, int a) { return (x + a - 1) / a * a; }
@@ -55,9 +54,10 @@ __device__ __forceinline__ int topk_at(const MoeDispatchArgs& p, int t, int j) {
 __device__ __forceinline__ bool routed(const MoeDispatchArgs& p, int e) { return e >= 0 && e < p.num_experts; }
 
 // Workspace: counts [E][chunks] (exclusive prefixes over chunks after the
-// scan), then totals [E].
+// scan), then totals [E], then, where a launch of their own finds them, the segments' first rows [E + 1].
 __device__ __forceinline__ int32_t* ws_counts(const MoeDispatchArgs& p) { return p.ws; }
 __device__ __forceinline__ int32_t* ws_totals(const MoeDispatchArgs& p) { return p.ws + (int64_t)p.chunks * p.num_experts; }
+__device__ __forceinline__ int32_t* ws_starts(const MoeDispatchArgs& p) { return ws_totals(p) + p.num_experts; }
 
 // Inclusive prefix sum over the 64 lanes of a wave.
 __device__ __forceinline__ int wave_inclusive_sum(int v, int lane) {
@@ -143,6 +143,15 @@ __device__ __forceinline__ int segment_starts(const MoeDispatchArgs& p, Total&& 
     return x;
 }
 
+// Contiguous and psum layouts, in four launches: the segments' first rows, once for all, and the psum ends.
+__global__ void __launch_bounds__(kThreads) moe_starts_kernel(const MoeDispatchArgs p) {
+    const int used = segment_starts(p, [&](int e) { return ws_totals(p)[e]; }, [&](int e, int start, int total) {
+        ws_starts(p)[e] = start;
+        if (p.layout == kMoePsum) p.meta[e] = start + total;   // psum[e] = align(psum[e-1]) + count
+    });
+    if (threadIdx.x == kThreads - 1) ws_starts(p)[p.num_experts] = used;
+}
+
 // One wave per expert: the exclusive prefix of its chunk counts (in place, 256
 // chunks per round, 4 consecutive chunks per lane), its total, and for the
 // masked layout masked_m = min(total, max_m).
@@ -206,21 +215,22 @@ __device__ __forceinline__ void pad_past(const MoeDispatchArgs& p, int64_t r0, i
     }
 }
 
-// A wave has TOKENS tokens: 1, or 4 of at most kMoeShortRow bytes. Lane i turns
+// A wave has TOKENS tokens: 1, or 4 short ones. Lane i turns
 // the chunk rank of the wave's entry i into its output row (segment start + the expert's prefix over
 // earlier chunks + the rank; for the masked layout the slot in the group's buffer, -1 past max_m);
 // then the wave stores the tokens' K bytes, read once (8 KB per round of one token, 8 x 16 B per
-// lane in flight), to each routed row, then the SF row. Every workgroup scans the
-// totals into the segment starts for itself (a launch of its own for them: 8192 x 8 rows of 7168 columns
-// 235 us against 230, 4096 x 8 of 512 over 1000 experts 21.9 against 21.3; in the last workgroup of the scan 239 and 41).
+// lane in flight), to each routed row, then the SF row. The segment starts lie in the workspace (STARTS), or
+// every workgroup scans the totals into them for itself (see launch_moe_dispatch; in the last workgroup
+// of the scan, by an atomic count: 8192 x 8 rows of 7168 BF16 columns 239 us, 235 and 230 for these two).
 // The first pad_blocks blocks (E + 1 for the
 // contiguous and psum layouts, else 0) fill an expert's padding rows each, and what is past the
 // segments, beside the copies; the first writes the psum ends.
-template <int TOKENS>
+template <int TOKENS, bool STARTS>
 __global__ void __launch_bounds__(kThreads) moe_scatter_kernel(const MoeDispatchArgs p, int pad_blocks) {
-    __shared__ int s_start[kMoeMaxExperts + 1];
+    __shared__ int s_start[STARTS ? 1 : kMoeMaxExperts + 1];
+    const auto start_of = [&](int x) { return STARTS ? ws_starts(p)[x] : s_start[x]; };
     constexpr int UNITS = TOKENS == 1 ? 8 : 1;   // 16-byte pieces of a token and lane at a time
-    static_assert(TOKENS * kMoeMaxTopk <= 64 && kMoeShortRow <= 64 * 16, "a wave's entries, a piece a lane");
+    static_assert(TOKENS * kMoeMaxTopk <= 64, "a wave's entries");
     const bool padding = (int)blockIdx.x < pad_blocks;
     const int lane = threadIdx.x & 63;
     const int t0 = padding ? p.t : ((int)blockIdx.x - pad_blocks) * (kThreads / 64 * TOKENS) + (int)(threadIdx.x >> 6) * TOKENS;
@@ -241,9 +251,12 @@ __global__ void __launch_bounds__(kThreads) moe_scatter_kernel(const MoeDispatch
     int e = -1, rank = 0;
     if (mine) {
         e = topk_at(p, t0 + own, slot);
-        if (routed(p, e)) rank = ws_counts(p)[(int64_t)e * p.chunks + (t0 + own) / kMoeChunkTokens] + p.pos[entry];
+        if (routed(p, e)) {
+            rank = ws_counts(p)[(int64_t)e * p.chunks + (t0 + own) / kMoeChunkTokens] + p.pos[entry];
+            if constexpr (STARTS) rank += ws_starts(p)[e];   // (a row then)
+        }
     }
-    if (p.layout != kMoeMasked) {
+    if (!STARTS && p.layout != kMoeMasked) {
         const int used = segment_starts(p, [&](int x) { return ws_totals(p)[x]; }, [&](int x, int start, int total) {
             s_start[x] = start;
             if (blockIdx.x == 0 && p.layout == kMoePsum) p.meta[x] = start + total;   // psum[e] = align(psum[e-1]) + count
@@ -253,15 +266,16 @@ __global__ void __launch_bounds__(kThreads) moe_scatter_kernel(const MoeDispatch
     }
     if (padding) {
         const int x = blockIdx.x;
-        if (x == p.num_experts) pad_past(p, (int64_t)s_start[x] + (int)threadIdx.x, kThreads);
-        else pad_rows(p, s_start[x] + ws_totals(p)[x], s_start[x + 1]);
+        if (x == p.num_experts) pad_past(p, (int64_t)start_of(x) + (int)threadIdx.x, kThreads);
+        else pad_rows(p, start_of(x) + ws_totals(p)[x], start_of(x + 1));
         return;
     }
     if (tokens <= 0) return;   // (no barrier follows)
     int flat = -1;
     if (mine) {
         if (routed(p, e)) {
-            flat = p.layout == kMoeMasked ? (rank < p.max_m ? e * p.max_m + rank : -1) : s_start[e] + rank;
+            if constexpr (STARTS) flat = rank;
+            else flat = p.layout == kMoeMasked ? (rank < p.max_m ? e * p.max_m + rank : -1) : s_start[e] + rank;
             if (flat >= 0) {
                 if (p.w_out) p.w_out[flat] = p.topk_w ? p.topk_w[(int64_t)(t0 + own) * p.w_st + (int64_t)slot * p.w_sk] : 1.f;
                 if (p.layout == kMoeContiguous) p.meta[flat] = e;
@@ -541,7 +555,6 @@ int32_t* moe_scratch_device_ptr() {
 int moe_dispatch_chunks(int64_t tokens) { return (int)((tokens + kMoeChunkTokens - 1) / kMoeChunkTokens); }
 
 int64_t moe_dispatch_workspace_ints(int64_t tokens, int num_experts) {
-    // (E + 1 more than counts and totals: the size that callers know)
     return (int64_t)moe_dispatch_chunks(tokens) * num_experts + 2 * (int64_t)num_experts + 1;
 }
 
@@ -568,17 +581,34 @@ void launch_moe_dispatch(const MoeDispatchArgs& a, hipStream_t stream) {
     hipLaunchKernelGGL(moe_scan_kernel, dim3((a.num_experts + kThreads / 64 - 1) / (kThreads / 64)), dim3(kThreads), 0,
                        stream, a);
     DG_HIP_CHECK(hipGetLastError());
+    const int launches = moe_dispatch_launches(a.t, a.k, a.kdim, a.num_experts, a.layout);
+    if (launches == 4) {
+        hipLaunchKernelGGL(moe_starts_kernel, dim3(1), dim3(kThreads), 0, stream, a);
+        DG_HIP_CHECK(hipGetLastError());
+    }
     const int pad_blocks = a.layout == kMoeMasked ? 0 : a.num_experts + 1;
     // Short rows four tokens a wave, where the fourfold fewer waves still fill the card and a token has little to
     // store: the scan of the totals weighs less. One / four, us (FP8 rows, alignment 16): 64 experts, 512 bytes
     // 5000 x 8 18.7/21.2, 8192 x 1 14.5/12.6, 8192 x 4 18.1/16.4, 8192 x 16 34.6/36.7, 16384 x 2 20.8/15.6,
     // 16384 x 16 47.3/54.3, of 256 bytes 16384 x 8 30.9/26.1; masked 256 bytes 5000 x 8 20.5/25.7, 8192 x 1
     // 12.7/11.8, 10000 x 4 19.9/20.7, 12000 x 4 21.6/21.0, 16384 x 8 38.3/36.8. 1 KB, 16384 x 8 (BF16) 38.8/42.2.
-    const bool several = a.kdim <= kMoeShortRow && a.k * a.kdim < 4096 && a.t >= (a.layout == kMoeMasked && a.k > 2 ? 12000 : 8192);
+    const bool several = moe_four_tokens(a.t, a.k, a.kdim, a.layout);
+    // Every workgroup that scans the totals for itself starts some microseconds later, and there are many where
+    // each has little to store: a launch of their own for the starts is then shorter. Three / four launches, us
+    // (FP8 rows, alignment 16): 64 experts 16384 x 8 of 512 bytes 31.9/30.5, 12000 x 2 of 1 KB 17.7/16.9, 32768 x 2
+    // 36.1/32.1, 32768 x 2 of 2 KB 45.2/43.9, 8192 x 8 39.5/41.0; 384 experts 12000 x 2 of 7 KB 55.7/52.6,
+    // 16384 x 4 113.6/108.1, 64 experts 110.0/108.9; 1024 experts 32768 x 2 of 1 KB 45.6/37.5. 256 experts, 8192 x 8
+    // of 7168 BF16 columns 230/235; rows of 128 bytes, four tokens a wave, 16384 x 4 18.5/19.9.
     const int per = kThreads / 64 * (several ? 4 : 1);   // tokens of a workgroup
     const dim3 grid((unsigned)(pad_blocks + ((int64_t)a.t + per - 1) / per)), block(kThreads);
-    if (several) hipLaunchKernelGGL(moe_scatter_kernel<4>, grid, block, 0, stream, a, pad_blocks);
-    else hipLaunchKernelGGL(moe_scatter_kernel<1>, grid, block, 0, stream, a, pad_blocks);
+    if (launches == 4) {
+        if (several) hipLaunchKernelGGL((moe_scatter_kernel<4, true>), grid, block, 0, stream, a, pad_blocks);
+        else hipLaunchKernelGGL((moe_scatter_kernel<1, true>), grid, block, 0, stream, a, pad_blocks);
+    } else if (several) {
+        hipLaunchKernelGGL((moe_scatter_kernel<4, false>), grid, block, 0, stream, a, pad_blocks);
+    } else {
+        hipLaunchKernelGGL((moe_scatter_kernel<1, false>), grid, block, 0, stream, a, pad_blocks);
+    }
     DG_HIP_CHECK(hipGetLastError());
 }
 
