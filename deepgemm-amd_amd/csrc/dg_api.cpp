@@ -1389,7 +1389,7 @@ void moe_dispatch_impl(const dg_tensor* x_, const dg_tensor* x_sf_, const dg_ten
     const int64_t size = bf16 ? 2 : 1, t = x.size(0), cols = x.size(1), kdim = cols * size;
     const int64_t sfk = bf16 ? 0 : ceil_div(fp4 ? 2 * cols : cols, (int64_t)128);
     DG_CHECK(kdim % 16 == 0 && kdim <= ((int64_t)1 << 31) - (1 << 14) && t < ((int64_t)1 << 30));   // (32-bit bytes of a row)
-    DG_CHECK_GRID((t + 3) / 4 + num_experts + 1, 256);
+    DG_CHECK_GRID((t + 3) / 4 + num_experts + 16, 256);
     check_vector_alignment(x, "x");
     const int sf_dtype = fp4 ? DG_I32 : DG_F32;
     if (!bf16) {

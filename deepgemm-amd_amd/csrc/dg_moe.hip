@@ -18,8 +18,8 @@
 //               token's K bytes once and stores them to each routed row, with
 //               the SF row, the weight and m_indices; beside them (contiguous /
 //               psum) a block per expert fills its padding rows (zero A, SF and
-//               weight, m_indices = -1), and one more sets m_indices = -1 past
-//               the segments.
+//               weight, m_indices = -1), and some more set m_indices = -1 and zero weights
+//               past the segments.
 // Bytes: the scatter reads each token row once and writes each routed row once
 // (HBM-bound copy); counts and scans touch 4 bytes per entry and per
 // (chunk, expert). 8192 tokens x 8 of 7168 BF16 columns, 256 experts: 230 us, 4.7 TB/s (the scatter
@@ -36,6 +36,7 @@ namespace dgm {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kPastBlocks = 16;   // workgroups of the scatter for the rows past the segments
 using dev::i32x4;
 
 __device__ __forceinline__ int align_up(int x, int a) { return (x + a - 1) / a * a; }
@@ -222,9 +223,10 @@ __device__ __forceinline__ void pad_past(const MoeDispatchArgs& p, int64_t r0, i
 // lane in flight), to each routed row, then the SF row. The segment starts lie in the workspace (STARTS), or
 // every workgroup scans the totals into them for itself (see launch_moe_dispatch; in the last workgroup
 // of the scan, by an atomic count: 8192 x 8 rows of 7168 BF16 columns 239 us, 235 and 230 for these two).
-// The first pad_blocks blocks (E + 1 for the
+// The first pad_blocks blocks (E + kPastBlocks for the
 // contiguous and psum layouts, else 0) fill an expert's padding rows each, and what is past the
-// segments, beside the copies; the first writes the psum ends.
+// segments, beside the copies (by one block, 8192 x 8 rows of 512 bytes, 1024 experts, alignment 128: 35.0 us, 31.3
+// by sixteen); the first writes the psum ends.
 template <int TOKENS, bool STARTS>
 __global__ void __launch_bounds__(kThreads) moe_scatter_kernel(const MoeDispatchArgs p, int pad_blocks) {
     __shared__ int s_start[STARTS ? 1 : kMoeMaxExperts + 1];
@@ -266,7 +268,8 @@ __global__ void __launch_bounds__(kThreads) moe_scatter_kernel(const MoeDispatch
     }
     if (padding) {
         const int x = blockIdx.x;
-        if (x == p.num_experts) pad_past(p, (int64_t)start_of(x) + (int)threadIdx.x, kThreads);
+        const int past = x - p.num_experts;
+        if (past >= 0) pad_past(p, (int64_t)start_of(p.num_experts) + past * kThreads + (int)threadIdx.x, kPastBlocks * kThreads);
         else pad_rows(p, start_of(x) + ws_totals(p)[x], start_of(x + 1));
         return;
     }
@@ -586,7 +589,7 @@ void launch_moe_dispatch(const MoeDispatchArgs& a, hipStream_t stream) {
         hipLaunchKernelGGL(moe_starts_kernel, dim3(1), dim3(kThreads), 0, stream, a);
         DG_HIP_CHECK(hipGetLastError());
     }
-    const int pad_blocks = a.layout == kMoeMasked ? 0 : a.num_experts + 1;
+    const int pad_blocks = a.layout == kMoeMasked ? 0 : a.num_experts + kPastBlocks;
     // Short rows four tokens a wave, where the fourfold fewer waves still fill the card and a token has little to
     // store: the scan of the totals weighs less. One / four, us (FP8 rows, alignment 16): 64 experts, 512 bytes
     // 5000 x 8 18.7/21.2, 8192 x 1 14.5/12.6, 8192 x 4 18.1/16.4, 8192 x 16 34.6/36.7, 16384 x 2 20.8/15.6,

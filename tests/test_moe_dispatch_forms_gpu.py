@@ -88,3 +88,10 @@ def test_segment_starts_of_a_launch_of_their_own(kind, t, k, e, cols, layout, la
 @pytest.mark.parametrize('layout', ['psum', 'contiguous'])
 def test_no_token_routed_in_four_launches(layout):
     dispatch('e4m3', 8192, 1, 5, 1024, layout, launches=4, lost=1.0)
+
+
+@pytest.mark.parametrize('layout', ['psum', 'contiguous'])
+@pytest.mark.parametrize('t,k,e,alignment', [(8200, 1, 50, 2048), (2100, 8, 200, 512), (3, 1, 30, 4096), (8192, 3, 40, 1), (4100, 4, 1, 16)])
+def test_many_rows_past_the_segments(t, k, e, alignment, layout):
+    """Up to 16 workgroups, and one alone, for the rows that no segment has (and none of them: one expert, all routed)."""
+    dispatch('e4m3', t, k, e, 128, layout, alignment=alignment, lost=0.0 if e == 1 else 0.2)
