@@ -269,7 +269,7 @@ inline int moe_few_tokens(int64_t t, int64_t k) {
 enum MoeLayout : int32_t { kMoeContiguous = 0, kMoePsum = 1, kMoeMasked = 2 };
 // Whether a wave of the scatter has four tokens (rows of `kdim` bytes; the figures: launch_moe_dispatch).
 inline bool moe_four_tokens(int64_t t, int64_t k, int64_t kdim, int32_t layout) {
-    return kdim <= 512 && k * kdim < 4096 && t >= (layout == kMoeMasked && k > 2 ? 12000 : 8192);
+    return kdim <= 512 && k * kdim < 4096 && t >= (layout == kMoeMasked ? 12000 : 8192);
 }
 // Launches of a dispatch: count, scan, scatter, and the segment starts between these for many tokens with little
 // to store (figures likewise).

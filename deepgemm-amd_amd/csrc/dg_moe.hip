@@ -28,6 +28,7 @@
 
 #include <cstdint>
 #include <mutex>
+#include <type_traits>
 
 #include "dg_internal.hpp"
 #include "dg_swiglu.hpp"
@@ -220,17 +221,17 @@ __device__ __forceinline__ void pad_past(const MoeDispatchArgs& p, int64_t r0, i
 // the chunk rank of the wave's entry i into its output row (segment start + the expert's prefix over
 // earlier chunks + the rank; for the masked layout the slot in the group's buffer, -1 past max_m);
 // then the wave stores the tokens' K bytes, read once (8 KB per round of one token, 8 x 16 B per
-// lane in flight), to each routed row, then the SF row. The segment starts lie in the workspace (STARTS), or
-// every workgroup scans the totals into them for itself (see launch_moe_dispatch; in the last workgroup
+// lane in flight), to each routed row, then the SF row. The segment starts lie in the workspace, or
+// every workgroup scans the totals into them for itself (SCAN; see launch_moe_dispatch; in the last workgroup
 // of the scan, by an atomic count: 8192 x 8 rows of 7168 BF16 columns 239 us, 235 and 230 for these two).
 // The first pad_blocks blocks (E + kPastBlocks for the
 // contiguous and psum layouts, else 0) fill an expert's padding rows each, and what is past the
 // segments, beside the copies (by one block, 8192 x 8 rows of 512 bytes, 1024 experts, alignment 128: 35.0 us, 31.3
 // by sixteen); the first writes the psum ends.
-template <int TOKENS, bool STARTS>
+template <int TOKENS, bool SCAN>
 __global__ void __launch_bounds__(kThreads) moe_scatter_kernel(const MoeDispatchArgs p, int pad_blocks) {
-    __shared__ int s_start[STARTS ? 1 : kMoeMaxExperts + 1];
-    const auto start_of = [&](int x) { return STARTS ? ws_starts(p)[x] : s_start[x]; };
+    __shared__ int s_start[SCAN ? kMoeMaxExperts + 1 : 1];
+    const auto start_of = [&](int x) { return SCAN ? s_start[x] : ws_starts(p)[x]; };
     constexpr int UNITS = TOKENS == 1 ? 8 : 1;   // 16-byte pieces of a token and lane at a time
     static_assert(TOKENS * kMoeMaxTopk <= 64, "a wave's entries");
     const bool padding = (int)blockIdx.x < pad_blocks;
@@ -255,10 +256,10 @@ __global__ void __launch_bounds__(kThreads) moe_scatter_kernel(const MoeDispatch
         e = topk_at(p, t0 + own, slot);
         if (routed(p, e)) {
             rank = ws_counts(p)[(int64_t)e * p.chunks + (t0 + own) / kMoeChunkTokens] + p.pos[entry];
-            if constexpr (STARTS) rank += ws_starts(p)[e];   // (a row then)
+            if (!SCAN && p.layout != kMoeMasked) rank += ws_starts(p)[e];   // (a row then)
         }
     }
-    if (!STARTS && p.layout != kMoeMasked) {
+    if constexpr (SCAN) {
         const int used = segment_starts(p, [&](int x) { return ws_totals(p)[x]; }, [&](int x, int start, int total) {
             s_start[x] = start;
             if (blockIdx.x == 0 && p.layout == kMoePsum) p.meta[x] = start + total;   // psum[e] = align(psum[e-1]) + count
@@ -277,8 +278,8 @@ __global__ void __launch_bounds__(kThreads) moe_scatter_kernel(const MoeDispatch
     int flat = -1;
     if (mine) {
         if (routed(p, e)) {
-            if constexpr (STARTS) flat = rank;
-            else flat = p.layout == kMoeMasked ? (rank < p.max_m ? e * p.max_m + rank : -1) : s_start[e] + rank;
+            if constexpr (SCAN) flat = s_start[e] + rank;
+            else flat = p.layout == kMoeMasked ? (rank < p.max_m ? e * p.max_m + rank : -1) : rank;
             if (flat >= 0) {
                 if (p.w_out) p.w_out[flat] = p.topk_w ? p.topk_w[(int64_t)(t0 + own) * p.w_st + (int64_t)slot * p.w_sk] : 1.f;
                 if (p.layout == kMoeContiguous) p.meta[flat] = e;
@@ -593,8 +594,8 @@ void launch_moe_dispatch(const MoeDispatchArgs& a, hipStream_t stream) {
     // Short rows four tokens a wave, where the fourfold fewer waves still fill the card and a token has little to
     // store: the scan of the totals weighs less. One / four, us (FP8 rows, alignment 16): 64 experts, 512 bytes
     // 5000 x 8 18.7/21.2, 8192 x 1 14.5/12.6, 8192 x 4 18.1/16.4, 8192 x 16 34.6/36.7, 16384 x 2 20.8/15.6,
-    // 16384 x 16 47.3/54.3, of 256 bytes 16384 x 8 30.9/26.1; masked 256 bytes 5000 x 8 20.5/25.7, 8192 x 1
-    // 12.7/11.8, 10000 x 4 19.9/20.7, 12000 x 4 21.6/21.0, 16384 x 8 38.3/36.8. 1 KB, 16384 x 8 (BF16) 38.8/42.2.
+    // 16384 x 16 47.3/54.3, of 256 bytes 16384 x 8 30.9/26.1; masked 256 bytes 5000 x 8 20.5/25.7, 10000 x 4
+    // 19.9/20.7, 12000 x 4 21.6/21.0, 16384 x 8 38.3/36.8. 1 KB, 16384 x 8 (BF16) 38.8/42.2.
     const bool several = moe_four_tokens(a.t, a.k, a.kdim, a.layout);
     // Every workgroup that scans the totals for itself starts some microseconds later, and there are many where
     // each has little to store: a launch of their own for the starts is then shorter. Three / four launches, us
@@ -604,14 +605,15 @@ void launch_moe_dispatch(const MoeDispatchArgs& a, hipStream_t stream) {
     // of 7168 BF16 columns 230/235; rows of 128 bytes, four tokens a wave, 16384 x 4 18.5/19.9.
     const int per = kThreads / 64 * (several ? 4 : 1);   // tokens of a workgroup
     const dim3 grid((unsigned)(pad_blocks + ((int64_t)a.t + per - 1) / per)), block(kThreads);
-    if (launches == 4) {
-        if (several) hipLaunchKernelGGL((moe_scatter_kernel<4, true>), grid, block, 0, stream, a, pad_blocks);
-        else hipLaunchKernelGGL((moe_scatter_kernel<1, true>), grid, block, 0, stream, a, pad_blocks);
-    } else if (several) {
-        hipLaunchKernelGGL((moe_scatter_kernel<4, false>), grid, block, 0, stream, a, pad_blocks);
-    } else {
-        hipLaunchKernelGGL((moe_scatter_kernel<1, false>), grid, block, 0, stream, a, pad_blocks);
-    }
+    // (the masked layout has no starts, and without their scan 54 registers instead of 66: eight waves on a SIMD, not seven)
+    const bool scan = launches == 3 && a.layout != kMoeMasked;
+    auto run = [&](auto tokens) {
+        constexpr int T = decltype(tokens)::value;
+        if (scan) hipLaunchKernelGGL((moe_scatter_kernel<T, true>), grid, block, 0, stream, a, pad_blocks);
+        else hipLaunchKernelGGL((moe_scatter_kernel<T, false>), grid, block, 0, stream, a, pad_blocks);
+    };
+    if (several) run(std::integral_constant<int, 4>{});
+    else run(std::integral_constant<int, 1>{});
     DG_HIP_CHECK(hipGetLastError());
 }
 
