@@ -260,13 +260,15 @@ void launch_per_token_cast(const CastArgs& args, hipStream_t stream);
 constexpr int kMoeMaxExperts = 1024;
 constexpr int kMoeMaxTopk = 16;
 constexpr int kMoeChunkTokens = 64;    // tokens per dispatch chunk (count / scatter workgroup)
-// Tokens of a workgroup of the dispatch in one launch, or 0: three launches (the figures: launch_moe_dispatch).
-inline int moe_few_tokens(int64_t t, int64_t k) {
-    if (t > 1 << 15) return 0;   // (the products below stay small)
-    const int tokens = t * k * t <= 1 << 20 ? 1 : 4;
-    return t * k * ((t + tokens - 1) / tokens) <= 1 << 23 ? tokens : 0;
-}
 enum MoeLayout : int32_t { kMoeContiguous = 0, kMoePsum = 1, kMoeMasked = 2 };
+// Tokens of a workgroup of the dispatch in one launch (rows of `kdim` bytes), or 0: several launches (the figures:
+// launch_moe_dispatch).
+inline int moe_few_tokens(int64_t t, int64_t k, int64_t kdim, int64_t experts) {
+    if (t <= 1448) return t * k > 20000 ? 0 : t * t * std::max<int64_t>(k, 2) <= 1 << 20 ? 1 : 4;
+    const bool many = experts > 512 && kdim < 4096;
+    if (t > 1 << 13 || experts < 16 || (many && (t + 3) / 4 + experts > 1536)) return 0;
+    return t * k * ((t + 3) / 4) <= (kdim >= 4096 ? 8 << 20 : many ? 4 << 20 : 5 << 20) ? 4 : 0;
+}
 // Whether a wave of the scatter has four tokens (rows of `kdim` bytes; the figures: launch_moe_dispatch).
 inline bool moe_four_tokens(int64_t t, int64_t k, int64_t kdim, int32_t layout) {
     return kdim <= 512 && k * kdim < 4096 && t >= (layout == kMoeMasked ? 12000 : 8192);
@@ -274,9 +276,10 @@ inline bool moe_four_tokens(int64_t t, int64_t k, int64_t kdim, int32_t layout) 
 // Launches of a dispatch: count, scan, scatter, and the segment starts between these for many tokens with little
 // to store (figures likewise).
 inline int moe_dispatch_launches(int64_t t, int64_t k, int64_t kdim, int64_t experts, int32_t layout) {
-    if (moe_few_tokens(t, k)) return 1;
-    if (layout == kMoeMasked || t < 8192 || moe_four_tokens(t, k, kdim, layout)) return 3;
-    return k * kdim <= 4096 || k <= 2 || (k <= 4 && experts > 256) ? 4 : 3;
+    if (moe_few_tokens(t, k, kdim, experts)) return 1;
+    if (layout == kMoeMasked || moe_four_tokens(t, k, kdim, layout)) return 3;
+    if (k * kdim <= 4096) return t >= (experts > 512 ? 3000 : 8192) ? 4 : 3;
+    return t >= 8192 && (k <= 2 || (k <= 4 && experts > 256)) ? 4 : 3;
 }
 struct MoeDispatchArgs {
     const uint8_t* x;          // rows of kdim bytes (e4m3, packed e2m1, BF16) [t]

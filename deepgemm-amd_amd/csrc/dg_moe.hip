@@ -565,13 +565,20 @@ int64_t moe_dispatch_workspace_ints(int64_t tokens, int num_experts) {
 void launch_moe_dispatch(const MoeDispatchArgs& a, hipStream_t stream) {
     DG_CHECK(a.num_experts > 0 && a.num_experts <= kMoeMaxExperts && a.k > 0 && a.k <= kMoeMaxTopk);
     DG_CHECK(a.chunks == moe_dispatch_chunks(a.t));
-    // One launch or three: every workgroup of the one counts all entries for itself, work that grows
+    // One launch or several: every workgroup of the one counts all entries for itself, work that grows
     // with the square of the tokens, against two launches and a workspace's round trip. BF16 rows, tokens
-    // x slots (columns), one launch / three, us in a graph: 4 x 8 (7168) 6.1/12.9, 256 x 8 (7168) 15.2/22.8,
-    // 777 x 6 (2056) 10.1/14.8, 1024 x 8 (2048) 13.4/17.3, 2048 x 8 (2048) 25.0/24.8, 4096 x 2 (2048)
-    // 17.8/17.3, 3000 x 8 (2048) 38.5/31.9, 8192 x 1 (1024) 37.7/15.5. One token a workgroup or four, us:
-    // 64 x 8 of 7168 10.2/11.9, 512 x 8 of 2048 8.3/8.2, 777 x 6 10.8/9.9.
-    if (const int tokens = moe_few_tokens(a.t, a.k)) {   // of a workgroup
+    // x slots (columns), 64 experts, one launch / three, us in a graph: 4 x 8 (7168) 6.1/12.9, 256 x 8 (7168)
+    // 15.2/22.8, 1024 x 8 (2048) 13.4/17.3, 1449 x 8 (1024) 14.1/15.8, 1700 x 8 16.2/16.6, 2048 x 8 18.7/17.5, 2900 x 4
+    // 14.1/14.0, 4000 x 2 13.0/12.4, 4000 x 1 9.6/11.0. Rows of 4 KB and more hide more of it: 2048 x 8 (4096)
+    // 37.3/37.8, 2048 x 4 20.6/23.0, 4000 x 2 22.9/23.4. The counts are atomics, which take their turns where the entries
+    // go to few experts: FP8 rows of 1 KB to one expert, 1448 x 1 8.4/8.4, 2048 x 1 10.4/8.6, 4096 x 1 27/9.5; to eight,
+    // 1700 x 8 15.5/15.0, 4096 x 1 10.4/9.7; so that from 1449 tokens on there have to be 16 experts. (All tokens to one of
+    // 256 experts 10.5/10.5 at 1448 x 1, 13.1/10.5 at 2048, 32/12 at 4096.) Padding has a workgroup for each
+    // expert, which counts as well, and six workgroups fit a CU at a time: 1024 experts 1448 x 8 18.8/17.9, 2048 x 2
+    // 11.4/14.4, 2900 x 2 16.5/15.0, rows of 8 KB 2048 x 8 50.9/51.9.
+    // One token a workgroup or four, us: 64 x 8 of 7168 10.2/11.9, 512 x 8 of 2048 8.3/8.2, 777 x 6 10.8/9.9, all to
+    // one expert 1000 x 1 9.8/6.5.
+    if (const int tokens = moe_few_tokens(a.t, a.k, a.kdim, a.num_experts)) {   // of a workgroup
         // (without tokens or padding rows: one workgroup for the ends, masked counts and weights)
         const int pad_blocks = a.layout != kMoeMasked ? (a.alignment > 1 ? a.num_experts : 1) : a.t == 0 ? 1 : 0;
         const dim3 grid(pad_blocks + (a.t + tokens - 1) / tokens), block(kThreads);
@@ -601,11 +608,12 @@ void launch_moe_dispatch(const MoeDispatchArgs& a, hipStream_t stream) {
     // each has little to store: a launch of their own for the starts is then shorter. Three / four launches, us
     // (FP8 rows, alignment 16): 64 experts 16384 x 8 of 512 bytes 31.9/30.5, 12000 x 2 of 1 KB 17.7/16.9, 32768 x 2
     // 36.1/32.1, 32768 x 2 of 2 KB 45.2/43.9, 8192 x 8 39.5/41.0; 384 experts 12000 x 2 of 7 KB 55.7/52.6,
-    // 16384 x 4 113.6/108.1, 64 experts 110.0/108.9; 1024 experts 32768 x 2 of 1 KB 45.6/37.5. 256 experts, 8192 x 8
+    // 16384 x 4 113.6/108.1, 64 experts 110.0/108.9; 1024 experts 32768 x 2 of 1 KB 45.6/37.5, 4096 x 1
+    // 16.2/14.4. 256 experts, 8192 x 8
     // of 7168 BF16 columns 230/235; rows of 128 bytes, four tokens a wave, 16384 x 4 18.5/19.9.
     const int per = kThreads / 64 * (several ? 4 : 1);   // tokens of a workgroup
     const dim3 grid((unsigned)(pad_blocks + ((int64_t)a.t + per - 1) / per)), block(kThreads);
-    // (the masked layout has no starts, and without their scan 54 registers instead of 66: eight waves on a SIMD, not seven)
+    // (the masked layout has no starts, and without their scan 56 registers instead of 66: eight waves on a SIMD, not seven)
     const bool scan = launches == 3 && a.layout != kMoeMasked;
     auto run = [&](auto tokens) {
         constexpr int T = decltype(tokens)::value;
