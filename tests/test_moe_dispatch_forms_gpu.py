@@ -110,3 +110,35 @@ def test_sizes_of_one_launch_and_of_several(t, k, e, size, layout, launches):
     dispatch('bf16', t, k, e, size // 2, layout, launches=launches)
     if e > 1:   # all tokens to the same experts
         dispatch('e4m3', t, k, e, size, layout, launches=launches, idx=torch.arange(k, dtype=torch.int32).expand(t, k).contiguous() % e)
+
+
+WIDE = [('e4m3', 8320), ('e4m3', 1024), ('e4m3', 7168), ('e2m1', 2080), ('e2m1', 16640), ('bf16', 7168), ('bf16', 4104), ('bf16', 520)]
+
+
+@pytest.mark.parametrize('layout', ['psum', 'contiguous', 'masked'])
+@pytest.mark.parametrize('kind,cols', WIDE)
+def test_wide_rows_and_scales_of_many_tokens(kind, cols, layout):
+    """Three launches, a token a wave: rows of one and of two rounds of 8 KB, scales of one and of two rounds of 64."""
+    dispatch(kind, 2050, 8, 24, cols, layout, launches=3)
+
+
+@pytest.mark.parametrize('layout', ['psum', 'contiguous'])
+@pytest.mark.parametrize('kind,cols', WIDE)
+def test_wide_rows_and_scales_with_starts_of_their_own(kind, cols, layout):
+    dispatch(kind, 8195, 2, 24, cols, layout, launches=4)
+
+
+@pytest.mark.parametrize('layout', ['psum', 'contiguous', 'masked'])
+@pytest.mark.parametrize('kind,cols', WIDE)
+@pytest.mark.parametrize('t,k', [(800, 4), (1449, 3)])
+def test_wide_rows_and_scales_of_four_tokens_a_workgroup(kind, cols, t, k, layout):
+    """One launch, a token a wave: rounds of 8 KB and 64 scales."""
+    dispatch(kind, t, k, 20, cols, layout, launches=1)
+
+
+@pytest.mark.parametrize('layout', ['psum', 'contiguous', 'masked'])
+@pytest.mark.parametrize('kind,cols', [('e4m3', 33024), ('e4m3', 16384), ('e2m1', 33056), ('e2m1', 66048), ('bf16', 8200)])
+def test_wide_rows_and_scales_of_a_token_a_workgroup(kind, cols, layout):
+    """One launch, the four waves share a token: rounds of 16 KB and 256 scales."""
+    dispatch(kind, 50, 3, 9, cols, layout, launches=1)
+    dispatch(kind, 1, 1, 1, cols, layout, launches=1, lost=0.0)
