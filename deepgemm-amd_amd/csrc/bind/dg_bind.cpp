@@ -14,6 +14,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/GradMode.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
@@ -449,6 +450,48 @@ PyObject* ragged_fp4(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
+// Whether a kernel may stand for torch's operations on a tensor: torch does not have to follow what becomes of it
+// (as a subclass, in a transform of torch.func, with a tangent; with a gradient, where one could pass).
+bool kernel_may_stand(PyObject* o, bool gradient) {
+    const at::Tensor& t = tensor(o);
+    constexpr c10::DispatchKeySet followed{c10::DispatchKey::Python, c10::DispatchKey::Functionalize,
+                                           c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchGradWrapper};
+    return t.is_cuda() && THPVariable_CheckExact(o) && !t.key_set().has_any(followed) && !t._fw_grad(0).defined() &&
+           !(gradient && t.requires_grad() && c10::GradMode::is_enabled());
+}
+// Launches that a 4-bit cast of [m, n] needs: one takes below 2^24 blocks of 4 x 1024 values.
+int32_t cast4_launches(int64_t m, int64_t n) {
+    const int64_t rows = ((int64_t(1) << 24) - 1) / std::max<int64_t>((n + 1023) / 1024, 1) * 4;
+    return m > rows ? 2 : 1;
+}
+
+// cast4_takes(x, gran_k, use_ue8m0) -> 0: a call for the torch operations, 1: for the kernel, 2: for it, in several launches
+PyObject* cast4_takes(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded(n, 3, [&] {
+        const at::Tensor& x = tensor(a[0]);
+        const int32_t gran = integer(a[1]), ue8m0 = integer(a[2]);
+        if (x.dim() != 2 || x.scalar_type() != at::kBFloat16 || (gran != 32 && gran != 64 && gran != 128)) return 0;
+        // (float scales carry a gradient, codes and power-of-two scales none)
+        if (!kernel_may_stand(a[0], !ue8m0) || x.stride(1) != 1 || x.size(1) % 2 != 0 || x.size(1) >= (1 << 27)) return 0;
+        return cast4_launches(x.size(0), x.size(1));
+    });
+}
+
+// cast_back4_takes(q, sf, gran_k, packed) -> as cast4_takes
+PyObject* cast_back4_takes(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded(n, 4, [&] {
+        const at::Tensor &q = tensor(a[0]), &sf = tensor(a[1]);
+        const int32_t gran = integer(a[2]), packed = integer(a[3]);
+        if (q.dim() != 2 || sf.dim() != 2 || q.scalar_type() != at::kChar || (gran != 32 && gran != 64 && gran != 128)) return 0;
+        if (sf.scalar_type() != (packed ? at::kInt : at::kFloat) || sf.device() != q.device()) return 0;
+        if (!kernel_may_stand(a[0], false) || !kernel_may_stand(a[1], true)) return 0;
+        const int64_t m = q.size(0), half = q.size(1), groups = (2 * half + gran - 1) / gran;
+        if (half >= (1 << 26) || (half > 1 && q.stride(1) != 1)) return 0;
+        if (sf.size(0) != m || sf.size(1) != (packed ? (groups + 3) / 4 : groups)) return 0;
+        return cast4_launches(m, 2 * half);
+    });
+}
+
 // cast4(x, gran_k, use_ue8m0, packed, stream) -> (status, q, sf)
 PyObject* cast4(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded_new(n, 5, [&]() -> NewTensors {
@@ -589,7 +632,8 @@ PyMethodDef g_methods[] = {method<init>("init"),     method<gemm_nt>("gemm_nt"),
                            method<swiglu_checkpoint>("swiglu_checkpoint"),
                            method<swiglu_backward>("swiglu_backward"),
                            method<init_rows>("init_rows"), method<ragged_fp4>("ragged_fp4"), method<cast4>("cast4"),
-                           method<cast_back4>("cast_back4"), method<dispatch_rows>("dispatch_rows"),
+                           method<cast_back4>("cast_back4"), method<cast4_takes>("cast4_takes"),
+                           method<cast_back4_takes>("cast_back4_takes"), method<dispatch_rows>("dispatch_rows"),
                            method<dispatch_backward>("dispatch_backward"),
                            method<combine_backward>("combine_backward"),
                            {nullptr, nullptr, 0, nullptr}};

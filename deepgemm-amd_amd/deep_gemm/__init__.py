@@ -20,7 +20,6 @@ from typing import Optional, Tuple
 import ctypes
 
 import torch
-from torch.autograd import forward_ad as _forward_ad
 
 from . import _ffi
 from ._ffi import address as _address, bind as _bind, check as _check, describe as _desc
@@ -451,20 +450,9 @@ def per_token_cast_to_fp8(x: torch.Tensor, use_ue8m0: bool, gran_k: int = 128,
     return q, sf
 
 
-def _takes_kernel(*tensors: torch.Tensor) -> bool:
-    """Whether a kernel may stand for torch ops on these tensors: they are plain ones of one GPU, and torch
-    does not have to follow what becomes of them (tangents, transforms of torch.func)."""
-    return (torch._C._functorch.peek_interpreter_stack() is None and _forward_ad._current_level < 0 and
-            all(type(t) in (torch.Tensor, torch.nn.Parameter) and t.is_cuda and t.device == tensors[0].device for t in tensors))
-
-
 def _cast4_rows(n: int) -> int:
     """Rows of n columns that a launch of the 4-bit casts takes: below 2^24 blocks of 4 x 1024 values."""
     return ((1 << 24) - 1) // max((n + 1023) // 1024, 1) * 4
-
-
-def _follows(t: torch.Tensor) -> bool:
-    return t.requires_grad and torch.is_grad_enabled()
 
 
 def per_token_cast_to_fp4(x: torch.Tensor, use_ue8m0: bool, gran_k: int = 128,
@@ -475,28 +463,17 @@ def per_token_cast_to_fp4(x: torch.Tensor, use_ue8m0: bool, gran_k: int = 128,
     (deep_gemm/utils/math.py) to the bit. BF16 device tensors take the fused HIP kernel (one HBM
     pass); anything else takes the torch ops of deep_gemm.utils.math: other granularities and strides,
     and an x whose gradient the float32 scales carry (the codes and power-of-two scales have none)."""
-    if not (_cast_on_device(x) and x.size(1) % 2 == 0 and gran_k in (32, 64, 128) and _takes_kernel(x)) or \
-            (not use_ue8m0 and _follows(x)):
+    ue8m0, packed = int(bool(use_ue8m0)), int(bool(use_packed_ue8m0))
+    launches = _bind.cast4_takes(x, gran_k, ue8m0)
+    if not launches:
         return utils.math.per_token_cast_to_fp4(x, use_ue8m0, gran_k, use_packed_ue8m0)
-    assert not use_packed_ue8m0 or use_ue8m0
-    if x.size(0) > _cast4_rows(x.size(1)):
+    assert not packed or ue8m0
+    if launches > 1:
         parts = [per_token_cast_to_fp4(p, use_ue8m0, gran_k, use_packed_ue8m0) for p in x.split(_cast4_rows(x.size(1)))]
         return torch.cat([q for q, _ in parts]), torch.cat([sf for _, sf in parts])
-    status, q, sf = _bind.cast4(x, gran_k, int(bool(use_ue8m0)), int(bool(use_packed_ue8m0)), _raw_stream_of(x))
+    status, q, sf = _bind.cast4(x, gran_k, ue8m0, packed, _raw_stream_of(x))
     _check(status)
     return q, sf
-
-
-def _cast_back4_on_device(packed: torch.Tensor, sf: torch.Tensor, gran_k: int, use_packed_ue8m0: bool) -> bool:
-    if not packed.is_cuda or packed.dtype != torch.int8 or packed.dim() != 2 or sf.dim() != 2:
-        return False
-    m, half = packed.shape
-    if gran_k not in (32, 64, 128) or half >= (1 << 26) or (half > 1 and packed.stride(1) != 1):
-        return False
-    groups = (2 * half + gran_k - 1) // gran_k
-    if sf.dtype != (torch.int32 if use_packed_ue8m0 else torch.float32) or _follows(sf):
-        return False
-    return sf.shape == (m, (groups + 3) // 4 if use_packed_ue8m0 else groups) and _takes_kernel(packed, sf)
 
 
 def cast_back_from_fp4(packed: torch.Tensor, sf: torch.Tensor, gran_k: int = 128, use_packed_ue8m0: bool = False,
@@ -507,15 +484,16 @@ def cast_back_from_fp4(packed: torch.Tensor, sf: torch.Tensor, gran_k: int = 128
     gradients through them. Device tensors take one HIP kernel where codes are contiguous within a row
     and scales are float32 or packed words, one for each group, without a gradient; others the torch ops
     of deep_gemm.utils.math."""
-    if dtype not in (None, torch.float32, torch.bfloat16):
+    if dtype is not None and dtype is not torch.float32 and dtype is not torch.bfloat16:
         raise TypeError('dtype must be torch.float32 or torch.bfloat16')
-    if not _cast_back4_on_device(packed, sf, gran_k, use_packed_ue8m0):
+    launches = _bind.cast_back4_takes(packed, sf, gran_k, int(bool(use_packed_ue8m0)))
+    if not launches:
         y = utils.math.cast_back_from_fp4(packed, sf, gran_k, use_packed_ue8m0)
         return y if dtype is None else y.to(dtype)
-    rows = _cast4_rows(2 * packed.size(1))
-    if packed.size(0) > rows:
+    if launches > 1:
+        rows = _cast4_rows(2 * packed.size(1))
         return torch.cat([cast_back_from_fp4(q, s, gran_k, use_packed_ue8m0, dtype) for q, s in zip(packed.split(rows), sf.split(rows))])
-    status, y = _bind.cast_back4(packed, sf, gran_k, int(dtype == torch.bfloat16), _raw_stream_of(packed))
+    status, y = _bind.cast_back4(packed, sf, gran_k, int(dtype is torch.bfloat16), _raw_stream_of(packed))
     _check(status)
     return y
 
