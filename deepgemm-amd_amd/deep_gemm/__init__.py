@@ -532,36 +532,11 @@ def moe_dispatch(x, topk_idx: torch.Tensor, num_experts: int,
     xq, xs = (x, None) if bf16 else _pair(x, 'x')
     if not isinstance(xq, torch.Tensor):
         raise TypeError('x must be a tensor or a (tensor, scaling factor) pair')
-    if bf16 or xq.dtype != torch.float8_e4m3fn or out is not None:
-        o, o_sf = (out, None) if bf16 or out is None else _pair(out, 'out')
-        status, *got = _bind.dispatch_rows(xq, xs, topk_idx, topk_weights, num_experts, _MOE_LAYOUTS[layout], alignment,
-                                           max_m or 0, o, o_sf, _raw_stream_of(xq))
-        _check(status)
-        return tuple(got)
-    t, kdim = xq.shape
-    k = topk_idx.shape[1]
-    dev = xq.device
-    sfk = (kdim + 127) // 128
-    if layout == 'masked':
-        a = torch.empty((num_experts, max_m, kdim), dtype=torch.float8_e4m3fn, device=dev)
-        a_sf = torch.empty((num_experts, max_m, sfk), dtype=torch.float32, device=dev)
-        gl = torch.empty((num_experts,), dtype=torch.int32, device=dev)
-        rows = num_experts * max_m
-    else:
-        rows = int(_lib.dg_moe_dispatch_max_rows(int(t), int(k), int(num_experts), alignment))
-        _check(0 if rows >= 0 else 1)
-        a = torch.empty((rows, kdim), dtype=torch.float8_e4m3fn, device=dev)
-        a_sf = torch.empty((rows, sfk), dtype=torch.float32, device=dev)
-        gl = torch.empty((rows if layout == 'contiguous' else num_experts,), dtype=torch.int32, device=dev)
-    pos = torch.empty((t, k), dtype=torch.int32, device=dev)
-    w = torch.empty((rows,), dtype=torch.float32, device=dev) if topk_weights is not None else None
-    ws_bytes = int(_lib.dg_moe_dispatch_workspace_size(int(t), int(num_experts)))
-    ws = torch.empty((max(ws_bytes, 4) // 4,), dtype=torch.int32, device=dev)
-    _check(_bind.dispatch(xq, xs, topk_idx, topk_weights, int(num_experts), _MOE_LAYOUTS[layout], alignment, a, a_sf, gl,
-                          pos, w, ws, _raw_stream_of(xq)))
-    if w is not None and layout == 'masked':
-        w = w.view(num_experts, max_m)
-    return a, a_sf, gl, pos, w
+    o, o_sf = (out, None) if bf16 or out is None else _pair(out, 'out')
+    status, *got = _bind.dispatch_rows(xq, xs, topk_idx, topk_weights, int(num_experts), _MOE_LAYOUTS[layout], alignment,
+                                       int(max_m or 0), o, o_sf, _raw_stream_of(xq))
+    _check(status)
+    return tuple(got)
 
 
 def moe_swiglu_apply_weight_to_fp8(x: torch.Tensor, row_weights: Optional[torch.Tensor] = None,
