@@ -271,15 +271,15 @@ inline int moe_few_tokens(int64_t t, int64_t k, int64_t kdim, int64_t experts) {
 }
 // Whether a wave of the scatter has four tokens (rows of `kdim` bytes; the figures: launch_moe_dispatch).
 inline bool moe_four_tokens(int64_t t, int64_t k, int64_t kdim, int32_t layout) {
-    return kdim <= 512 && k * kdim < 4096 && t >= (layout == kMoeMasked ? 12000 : 8192);
+    return kdim <= 512 && k * kdim < 4096 && t > (layout == kMoeMasked ? 12000 : 7168);
 }
 // Launches of a dispatch: count, scan, scatter, and the segment starts between these for many tokens with little
 // to store (figures likewise).
 inline int moe_dispatch_launches(int64_t t, int64_t k, int64_t kdim, int64_t experts, int32_t layout) {
     if (moe_few_tokens(t, k, kdim, experts)) return 1;
     if (layout == kMoeMasked || moe_four_tokens(t, k, kdim, layout)) return 3;
-    if (k * kdim <= 4096) return t >= (experts > 512 ? 3000 : 8192) ? 4 : 3;
-    return t >= 8192 && (k <= 2 || (k <= 4 && experts > 256)) ? 4 : 3;
+    if (k * kdim <= 4096) return t > (experts > 512 ? 2999 : k * kdim <= 2048 ? 7168 : 8191) ? 4 : 3;
+    return t > 8191 && (k <= 2 || (k <= 4 && experts > 256)) ? 4 : 3;
 }
 struct MoeDispatchArgs {
     const uint8_t* x;          // rows of kdim bytes (e4m3, packed e2m1, BF16) [t]

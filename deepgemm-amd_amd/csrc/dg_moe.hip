@@ -598,9 +598,9 @@ void launch_moe_dispatch(const MoeDispatchArgs& a, hipStream_t stream) {
         DG_HIP_CHECK(hipGetLastError());
     }
     const int pad_blocks = a.layout == kMoeMasked ? 0 : a.num_experts + kPastBlocks;
-    // Short rows four tokens a wave, where the fourfold fewer waves still fill the card and a token has little to
-    // store: the scan of the totals weighs less. One / four, us (FP8 rows, alignment 16): 64 experts, 512 bytes
-    // 5000 x 8 18.7/21.2, 8192 x 1 14.5/12.6, 8192 x 4 18.1/16.4, 8192 x 16 34.6/36.7, 16384 x 2 20.8/15.6,
+    // Short rows four tokens a wave, where the waves of one each no longer fit the card at a time (1792 workgroups; 2048
+    // without the scan) and a token has little to store: the scan of the totals weighs less. One / four, us (FP8 rows, alignment 16): 64 experts, 512 bytes
+    // 5000 x 8 18.7/21.2, 7200 x 2 15.0/13.8, 8192 x 1 14.5/12.6, 8192 x 4 18.1/16.4, 8192 x 16 34.6/36.7, 16384 x 2 20.8/15.6,
     // 16384 x 16 47.3/54.3, of 256 bytes 16384 x 8 30.9/26.1; masked 256 bytes 5000 x 8 20.5/25.7, 10000 x 4
     // 19.9/20.7, 12000 x 4 21.6/21.0, 16384 x 8 38.3/36.8. 1 KB, 16384 x 8 (BF16) 38.8/42.2.
     const bool several = moe_four_tokens(a.t, a.k, a.kdim, a.layout);

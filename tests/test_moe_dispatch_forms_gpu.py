@@ -70,14 +70,14 @@ def dispatch(kind, t, k, e, cols, layout, alignment=16, launches=None, lost=0.1,
 
 
 @pytest.mark.parametrize('kind,cols', [('bf16', 64), ('e4m3', 256), ('e2m1', 512)])
-@pytest.mark.parametrize('t,k,layout', [(8191, 3, 'psum'), (8192, 3, 'psum'), (8197, 1, 'contiguous'), (11999, 3, 'masked'),
+@pytest.mark.parametrize('t,k,layout', [(7168, 3, 'psum'), (7169, 3, 'psum'), (8191, 3, 'psum'), (8192, 3, 'psum'), (8197, 1, 'contiguous'), (11999, 3, 'masked'),
                                         (12000, 3, 'masked'), (12005, 1, 'masked'), (8192, 2, 'masked'), (9000, 16, 'psum')])
 def test_one_and_four_tokens_of_a_wave(kind, cols, t, k, layout):
     dispatch(kind, t, k, 40, cols, layout)
 
 
 @pytest.mark.parametrize('t,k,e,cols,layout,launches', [
-    (8191, 1, 16, 1024, 'psum', 3), (8192, 1, 16, 1024, 'psum', 4), (8193, 2, 1000, 2304, 'contiguous', 4), (8200, 4, 300, 1152, 'psum', 4),
+    (7168, 1, 16, 1024, 'psum', 3), (7169, 1, 16, 1024, 'psum', 4), (8191, 2, 16, 2048, 'psum', 3), (8192, 2, 16, 2048, 'psum', 4), (8193, 2, 1000, 2304, 'contiguous', 4), (8200, 4, 300, 1152, 'psum', 4),
     (8192, 4, 256, 1152, 'psum', 3), (8192, 5, 300, 1152, 'contiguous', 3), (8195, 8, 24, 512, 'psum', 4), (8195, 1, 24, 1024, 'masked', 3)])
 @pytest.mark.parametrize('kind', ['e4m3', 'bf16'])
 def test_segment_starts_of_a_launch_of_their_own(kind, t, k, e, cols, layout, launches):
