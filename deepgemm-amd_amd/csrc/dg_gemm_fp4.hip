@@ -9,9 +9,10 @@
 // operands is one of the BF16 products' K-major operands, and is loaded, laid out in LDS and
 // read like it. A row has two words of scales a step.
 //
-// 16384 rows over 8 groups, n 4096, k 7168: 275 to 285 us, 3.4 to 3.5 PFLOP/s, bound by the clock that
-// the matrix load leaves (8192 x 4096 x 32768: 4.3 PFLOP/s of random values, 5.6 of zeros); k 2048,
-// n 7168 163 us (a tile's first loads and its stores); 32 rows over 32 groups, 4096 x 7168 90 us, 5.5 TB/s.
+// 16384 rows over 8 groups, n 4096, k 7168: 275 to 285 us, 3.4 to 3.5 PFLOP/s. 8192 x 4096 x 32768 reaches 4.3
+// PFLOP/s of random values and 5.6 of zeros, the clock that the matrix load leaves; what the shorter axis
+// loses to that are a tile's first loads and stores and the last, partial round (36 to 42 us for 6% of the
+// tiles). k 2048, n 7168 163 us; 32 rows over 32 groups, 4096 x 7168 90 us, 5.5 TB/s.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -408,7 +409,11 @@ __global__ void __launch_bounds__(256, 2) fp4_few_rows_kernel(const RaggedFp4Arg
 // Where 128 x 128 tiles fill three quarters of the CUs, smaller ones only read weights again: 128,
 //   64 and 32 rows at 8 x 256, 4096, 7168 30, 48 and 45; 32 x 512, 4096, 7168 97, 107 and 112; 32 x 32, 4096, 7168 90, 95
 //   and 94, 5120 68, 73 and 71. But for up to 8 rows a group and a short reduced axis, where a tile's end
-//   counts: 32 x 32, 4096, 3584 48.9, 49.4 and 48.8, 2048 31.5, 31.0 and 30.5; 8 x 8, 4096, 2048 10.1, 9.5 and 9.2.
+//   counts. 128 and 32 rows, weights from HBM, 32 groups of n 4096: 2, 8, 12, 16 and 24 rows each, 2048 31.9/30.8, 31.9/31.4,
+//   32.0/31.9, 32.3/32.5 and 32.4/33.6; 3584 49.2/49.5, 49.9/51.1, 50.2/51.7, 50.7/53.1 and 51.7/54.7; 1024 21.2/19.5,
+//   21.2/19.5, 21.3/19.9, 21.6/20.4 and 21.8/21.2. 8 groups, 2048: 8 and 16 rows 11.4/10.7 and 11.5/10.9.
+// The rows are the buffer's, padding and what no group has with it, as the ends are on the device: 8 routed rows over 64
+//   groups, 2048, 7168 take 17.2 back to back, 22.0 where they lie 16 apart and 26.0 where they lie 128 apart.
 // Where they do not: 1 x 512, 4096, 7168 22, 19 and 27; 1 x 256, 2112, 7168 22, 18 and 16; 2 x 128, 4096, 4096 14.7, 12.6
 //   and 11.4.
 // Whole, in 2, 4 and 8 pieces, 32 rows: 1 x 64, 2112, 7168 15.4, 13.9, 12.3, 14.3; 1 x 256, 2112, 7168 15.6, 20.2, 22.7, 23.1.

@@ -598,19 +598,20 @@ void launch_moe_dispatch(const MoeDispatchArgs& a, hipStream_t stream) {
         DG_HIP_CHECK(hipGetLastError());
     }
     const int pad_blocks = a.layout == kMoeMasked ? 0 : a.num_experts + kPastBlocks;
-    // Short rows four tokens a wave, where the waves of one each no longer fit the card at a time (1792 workgroups; 2048
-    // without the scan) and a token has little to store: the scan of the totals weighs less. One / four, us (FP8 rows, alignment 16): 64 experts, 512 bytes
-    // 5000 x 8 18.7/21.2, 7200 x 2 15.0/13.8, 8192 x 1 14.5/12.6, 8192 x 4 18.1/16.4, 8192 x 16 34.6/36.7, 16384 x 2 20.8/15.6,
-    // 16384 x 16 47.3/54.3, of 256 bytes 16384 x 8 30.9/26.1; masked 256 bytes 5000 x 8 20.5/25.7, 10000 x 4
-    // 19.9/20.7, 12000 x 4 21.6/21.0, 16384 x 8 38.3/36.8. 1 KB, 16384 x 8 (BF16) 38.8/42.2.
+    // Short rows four tokens a wave, where the workgroups of a token a wave no longer fit the card at a time (1792 of
+    // them; 2048 without the scan) and a token has little to store: the scan of the totals weighs less. One / four, us
+    // in a graph (FP8 rows, alignment 16): 64 experts, 512 bytes 5000 x 8 18.7/21.2, 7200 x 2 15.0/13.8, 8192 x 1
+    // 14.5/12.6, 8192 x 4 18.1/16.4, 8192 x 16 34.6/36.7, 16384 x 2 20.8/15.6, 16384 x 16 47.3/54.3; of 256 bytes
+    // 16384 x 8 30.9/26.1; masked 256 bytes 5000 x 8 20.5/25.7, 10000 x 4 19.9/20.7, 12000 x 4 21.6/21.0, 16384 x 8
+    // 38.3/36.8. Of 1 KB, 16384 x 8 (BF16) 38.8/42.2.
     const bool several = moe_four_tokens(a.t, a.k, a.kdim, a.layout);
     // Every workgroup that scans the totals for itself starts some microseconds later, and there are many where
     // each has little to store: a launch of their own for the starts is then shorter. Three / four launches, us
-    // (FP8 rows, alignment 16): 64 experts 16384 x 8 of 512 bytes 31.9/30.5, 12000 x 2 of 1 KB 17.7/16.9, 32768 x 2
-    // 36.1/32.1, 32768 x 2 of 2 KB 45.2/43.9, 8192 x 8 39.5/41.0; 384 experts 12000 x 2 of 7 KB 55.7/52.6,
-    // 16384 x 4 113.6/108.1, 64 experts 110.0/108.9; 1024 experts 32768 x 2 of 1 KB 45.6/37.5, 4096 x 1
-    // 16.2/14.4. 256 experts, 8192 x 8
-    // of 7168 BF16 columns 230/235; rows of 128 bytes, four tokens a wave, 16384 x 4 18.5/19.9.
+    // in a graph (FP8 rows, alignment 16): 64 experts 16384 x 8 of 512 bytes 31.9/30.5, of 1 KB 7900 x 1 14.7/13.3, 12000 x 2
+    // 17.7/16.9, 32768 x 2 36.1/32.1, of 2 KB 32768 x 2 45.2/43.9, 8192 x 8 39.5/41.0; 384 experts, 7 KB, 12000 x 2
+    // 55.7/52.6, 16384 x 4 113.6/108.1 (64 experts 110.0/108.9); 1024 experts, 1 KB, 32768 x 2 45.6/37.5, 4096 x 1
+    // 16.2/14.4. 256 experts, 8192 x 8 of 7168 BF16 columns 230/235; rows of 128 bytes, four tokens a wave, 16384 x 4
+    // 18.5/19.9.
     const int per = kThreads / 64 * (several ? 4 : 1);   // tokens of a workgroup
     const dim3 grid((unsigned)(pad_blocks + ((int64_t)a.t + per - 1) / per)), block(kThreads);
     // (the masked layout has no starts, and without their scan 56 registers instead of 66: eight waves on a SIMD, not seven)

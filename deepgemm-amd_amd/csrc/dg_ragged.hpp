@@ -379,6 +379,11 @@ __device__ __forceinline__ void store_tile(const RaggedGemmArgs& p, const f32x16
                 // Past the caches' order, in whole lines: it leaves them to the operands. Plain / so, us (4-bit NT, groups x
                 // rows, n, k): 8 x 16384, 7168, 2048 177/163 (FP32 226/196), 4096, 7168 284/282, 32 x 4096, 2048, 2048
                 // 28.0/25.4; BF16 TN 16384 rows to 8 x 4096 x 7168, FP32 + C, 1070/1034, NT 8 x 1000, 4096, 2048 38.4/37.1.
+                // What reads D next finds less of it in the caches, so that a whole forward layer (NT, SwiGLU, NT, combination;
+                // rows in groups, hidden, inner columns) gains little from it, and loses where D is small: BF16 16384 in 8, 7168,
+                // 2048 1305/1295, 2048 in 8, 4096, 2048 152.8/152.0, 4096 in 8, 7168, 2048 353/354, 1001 in 16, 2048, 704 38.6/39.2;
+                // in 4 bits (and a cast) 567/558, 63.6/62.6, 160/162, 30.1/30.8. TN of 4096 rows with a pass over D after it 391/377.
+                // The sums of pieces, which the join reads: even (64 rows, 2112, 7168 17.0/17.0).
                 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
                 __builtin_nontemporal_store(u32x4{w[0], w[1], w[2], w[3]},
                                             reinterpret_cast<u32x4*>(static_cast<uint8_t*>(p.d) + to * SIZE));

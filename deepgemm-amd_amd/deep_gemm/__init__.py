@@ -522,7 +522,8 @@ def moe_dispatch(x, topk_idx: torch.Tensor, num_experts: int,
     e * max_m + r, -1 if none); row_weights: the routing weight of each row (None
     without topk_weights; 0 on rows of no token in the first two layouts). out: optional
     preallocated a (bf16) or (a, a_sf), of R rows or more: rows past the segments are left
-    as they were. Deterministic: an expert's rows follow token order."""
+    as they were. Deterministic: an expert's rows follow token order. The rows of an x that
+    requires a gradient carry none: moe_dispatch_backward gives it."""
     if layout not in _MOE_LAYOUTS:
         raise ValueError(f'layout must be one of {sorted(_MOE_LAYOUTS)}')
     if layout == 'masked' and not max_m:
@@ -570,7 +571,7 @@ def moe_combine(y: torch.Tensor, pos: torch.Tensor, topk_weights: Optional[torch
 
 def moe_dispatch_backward(drows: torch.Tensor, pos: torch.Tensor, drow_weights: Optional[torch.Tensor] = None
                           ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
-    """Gradient of moe_dispatch: drows bf16 ([R, K] or masked [E, max_m, K]) and the gradient of
+    """Gradient of moe_dispatch (autograd does not call it): drows bf16 ([R, K] or masked [E, max_m, K]) and the gradient of
     its row_weights (float32, or None) -> (dx bf16 [T, K], float32 [T, topk] gradient of
     topk_weights or None): dx[t] = sum over the slots of drows[pos[t, j]], in FP32 and their
     order, rounded once. Entries that were not routed count as zeros. K a multiple of 8,
@@ -702,8 +703,8 @@ def m_grouped_fp4_gemm_nt_ragged(a: Tuple[torch.Tensor, torch.Tensor], b: Tuple[
     per_token_cast_to_fp4(x, use_ue8m0=True, gran_k=32, use_packed_ue8m0=True) makes them: a
     power-of-two scale for 32 elements of a row, four to a word. Sums in FP32, d bf16 or float32.
     K a multiple of 32, rows of codes at multiples of 16 bytes; scales with any strides (words of a
-    row side by side are read fastest). Gradients: through the operands' values (cast_back_from_fp4 to
-    bfloat16 is exact) and the BF16 products."""
+    column side by side are read fastest, by up to 4%). Gradients: through the operands' values
+    (cast_back_from_fp4 to bfloat16 is exact, of [G * N, K/2] codes) and the BF16 products."""
     a_t, a_sf = _pair(a, 'a')
     b_t, b_sf = _pair(b, 'b')
     _check(_bind.ragged_fp4(a_t, a_sf, b_t, b_sf, d, group_ends, int(alignment), _raw_stream_of(d)))

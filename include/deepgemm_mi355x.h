@@ -285,7 +285,7 @@ int dg_per_token_cast_to_fp8(const dg_tensor* x, const dg_tensor* q, const dg_te
  *   q   int8 [M, N/2]: element 2i in the low nibble
  *   sf  f32 [M, ceil(N/gran_k)], or int32 [M, ceil(ceil(N/gran_k)/4)] of packed UE8M0 exponents
  *       (needs use_ue8m0; groups past the last as 1.0), any strides
- *   gran_k 32 (microscaled formats), 64 or 128. ceil(M/4) ceil(N/1024) < 2^24. */
+ *   gran_k 32 (microscaled formats), 64 or 128. ceil(M/4) ceil(N/1024) < 2^24 (longer ones in pieces of rows). */
 int dg_per_token_cast_to_fp4(const dg_tensor* x, const dg_tensor* q, const dg_tensor* sf,
                              int32_t gran_k, int32_t use_ue8m0, void* stream);
 

@@ -5,12 +5,17 @@ masked layout for the masked product.
 Bounds: half a step of a result's type plus the FP32 sums' (fp4_ragged.py, ragged.py).
 """
 import ctypes
+import glob
+import os
+import re
+import textwrap
 
 import pytest
 import torch
 
 import deep_gemm
 import ragged
+from conftest import ROOT
 from deep_gemm import _ffi
 from fp4_ragged import operand, sum_error
 from ragged import DEV, bits, check, rounding
@@ -140,3 +145,47 @@ def test_masked_rows_for_the_masked_product(t, k, e, n, cols, max_m):
             ref, off = bound(x64[tok], w64[ex], torch.bfloat16)
             check(d.view(-1, n)[p], ref, off + 65 * 2.0 ** -23 * (x64[tok].abs() @ w64[ex].abs().T), f'expert {ex}')
     assert (d.view(-1, n)[~written] == 7.0).all()
+
+
+def documented(word):
+    """The one documented piece of code with `word` in it."""
+    blocks = []
+    for path in sorted(glob.glob(os.path.join(ROOT, '*.md'))):
+        with open(path) as f:
+            blocks += re.findall(r'^ *```python\n(.*?)^ *```', f.read(), flags=re.S | re.M)
+    blocks = [textwrap.dedent(b) for b in blocks if word in b]
+    assert len(blocks) == 1
+    return blocks[0]
+
+
+def test_documented_gradients():
+    E, hidden, inter, rows = 3, 160, 96, 50
+    ends = torch.tensor([20, 20, 50], dtype=torch.int32, device=DEV)
+    hq, h64 = operand((rows, inter), 1)
+    w2, w64 = operand((E, hidden, inter), 2)
+    dy = torch.randn((rows, hidden), generator=torch.Generator().manual_seed(3)).bfloat16()
+    names = dict(torch=torch, deep_gemm=deep_gemm, E=E, hidden=hidden, inter=inter, ends=ends, hq=hq, w2=w2, dy=dy.to(DEV),
+                 dh=torch.empty((rows, inter), dtype=torch.float32, device=DEV), dw2=torch.zeros((E, hidden, inter), device=DEV))
+    exec(documented('w2_bf16'), names)
+    dy = dy.double()
+    for g, lo, hi in ((0, 0, 20), (2, 20, 50)):
+        ref = dy[lo:hi] @ w64[g]
+        check(names['dh'][lo:hi], ref, rounding(torch.float32, ref) + ragged.sum_error(hidden, dy[lo:hi].abs() @ w64[g].abs()), 'dh')
+        ref = dy[lo:hi].T @ h64[lo:hi]
+        check(names['dw2'][g], ref, rounding(torch.float32, ref) + ragged.sum_error(hi - lo, dy[lo:hi].T.abs() @ h64[lo:hi].abs()), 'dw2')
+    assert not names['dw2'][1].any()
+
+
+def test_documented_masked_rows():
+    t, E, hidden, max_m = 60, 4, 256, 40
+    idx = routing(t, 2, E, 1)
+    xq, _ = operand((t, hidden), 1)
+    names = dict(torch=torch, deep_gemm=deep_gemm, E=E, hidden=hidden, max_m=max_m, xq=xq, topk_idx=idx.to(DEV),
+                 topk_weights=torch.rand((t, 2), device=DEV))
+    exec(documented("layout='masked', max_m=max_m, out=rows"), names)
+    codes, sf = names['rows']
+    assert sf.stride(1) == 1 and sf.stride(2) == max_m
+    pos = names['pos'].cpu().long()
+    at, token = pos[pos >= 0], (pos >= 0).nonzero()[:, 0]
+    assert torch.equal(codes.reshape(-1, hidden // 2).cpu()[at], xq[0].cpu()[token])
+    assert torch.equal(sf.reshape(-1, hidden // 128).cpu()[at], xq[1].cpu()[token])
