@@ -450,12 +450,14 @@ PyObject* ragged_fp4(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
-// Whether a kernel may stand for torch's operations on a tensor: torch does not have to follow what becomes of it
-// (as a subclass, in a transform of torch.func, with a tangent; with a gradient, where one could pass).
+// Whether a kernel may stand for torch's operations on a tensor: its memory holds its values (no negative view, no zeros
+// without memory), and torch does not have to follow what becomes of it (as a subclass, in a transform of torch.func, with
+// a tangent; with a gradient, where one could pass).
 bool kernel_may_stand(PyObject* o, bool gradient) {
     const at::Tensor& t = tensor(o);
-    constexpr c10::DispatchKeySet followed{c10::DispatchKey::Python, c10::DispatchKey::Functionalize,
-                                           c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchGradWrapper};
+    constexpr c10::DispatchKeySet followed{c10::DispatchKey::Python, c10::DispatchKey::Functionalize, c10::DispatchKey::Negative,
+                                           c10::DispatchKey::ZeroTensor, c10::DispatchKey::FuncTorchBatched,
+                                           c10::DispatchKey::FuncTorchGradWrapper};
     return t.is_cuda() && THPVariable_CheckExact(o) && !t.key_set().has_any(followed) && !t._fw_grad(0).defined() &&
            !(gradient && t.requires_grad() && c10::GradMode::is_enabled());
 }

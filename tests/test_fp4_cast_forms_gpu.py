@@ -87,6 +87,17 @@ def test_tangent_of_the_scales():
     assert torch.equal(v.cpu(), plain.cast_back_from_fp4(q, sf, 32)) and torch.equal(tangent.cpu(), plain.cast_back_from_fp4(q, d, 32))
 
 
+def test_negative_views():
+    """Views whose memory holds the negative of their values."""
+    q, sf = codes(4, 32), scales(4, 2)
+    got = deep_gemm.cast_back_from_fp4(q.to(DEV), torch._neg_view(sf.to(DEV)), 32)
+    assert torch.equal(got.cpu(), plain.cast_back_from_fp4(q, -sf, 32))
+    x = torch.randn((4, 64), generator=torch.Generator().manual_seed(7)).bfloat16()
+    got = deep_gemm.per_token_cast_to_fp4(torch._neg_view(x.to(DEV)), True, 32, True)
+    want = plain.per_token_cast_to_fp4(-x, True, 32, True)
+    assert torch.equal(got[0].cpu(), want[0]) and torch.equal(got[1].cpu(), want[1])
+
+
 def test_batches_of_vmap():
     q = torch.stack([codes(4, 32, i) for i in range(3)])
     sf = scales(3, 4, 2)
