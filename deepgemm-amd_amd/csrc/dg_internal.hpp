@@ -263,11 +263,14 @@ constexpr int kMoeChunkTokens = 64;    // tokens per dispatch chunk (count / sca
 enum MoeLayout : int32_t { kMoeContiguous = 0, kMoePsum = 1, kMoeMasked = 2 };
 // Tokens of a workgroup of the dispatch in one launch (rows of `kdim` bytes), or 0: several launches (the figures:
 // launch_moe_dispatch).
-inline int moe_few_tokens(int64_t t, int64_t k, int64_t kdim, int64_t experts) {
+inline int moe_few_tokens(int64_t t, int64_t k, int64_t kdim, int64_t experts, int32_t layout) {
     if (t <= 1448) return t * k > 20000 ? 0 : t * t * std::max<int64_t>(k, 2) <= 1 << 20 ? 1 : 4;
     const bool many = experts > 512 && kdim < 4096;
-    if (t > 1 << 13 || experts < 16 || (many && (t + 3) / 4 + experts > 1536)) return 0;
-    return t * k * ((t + 3) / 4) <= (kdim >= 4096 ? 8 << 20 : many ? 4 << 20 : 5 << 20) ? 4 : 0;
+    if (t > 1 << 13 || (many && k > 1 && (t + 3) / 4 + experts > 1536)) return 0;
+    const int64_t most = kdim >= 4096 ? std::min<int64_t>(8 << 20, experts * 1'000'000)
+                       : many ? 4 << 20
+                              : std::min<int64_t>(layout == kMoeMasked ? 5 << 20 : 6 << 20, experts * 400'000);
+    return t * k * ((t + 3) / 4) <= most ? 4 : 0;
 }
 // Whether a wave of the scatter has four tokens (rows of `kdim` bytes; the figures: launch_moe_dispatch).
 inline bool moe_four_tokens(int64_t t, int64_t k, int64_t kdim, int32_t layout) {
@@ -276,7 +279,7 @@ inline bool moe_four_tokens(int64_t t, int64_t k, int64_t kdim, int32_t layout) 
 // Launches of a dispatch: count, scan, scatter, and the segment starts between these for many tokens with little
 // to store (figures likewise).
 inline int moe_dispatch_launches(int64_t t, int64_t k, int64_t kdim, int64_t experts, int32_t layout) {
-    if (moe_few_tokens(t, k, kdim, experts)) return 1;
+    if (moe_few_tokens(t, k, kdim, experts, layout)) return 1;
     if (layout == kMoeMasked || moe_four_tokens(t, k, kdim, layout)) return 3;
     if (k * kdim <= 4096) return t > (experts > 512 ? 2999 : k * kdim <= 2048 ? 7168 : 8191) ? 4 : 3;
     return t > 8191 && (k <= 2 || (k <= 4 && experts > 256)) ? 4 : 3;

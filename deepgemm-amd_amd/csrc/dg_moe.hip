@@ -569,16 +569,17 @@ void launch_moe_dispatch(const MoeDispatchArgs& a, hipStream_t stream) {
     // with the square of the tokens, against two launches and a workspace's round trip. BF16 rows, tokens
     // x slots (columns), 64 experts, one launch / three, us in a graph: 4 x 8 (7168) 6.1/12.9, 256 x 8 (7168)
     // 15.2/22.8, 1024 x 8 (2048) 13.4/17.3, 1449 x 8 (1024) 14.1/15.8, 1700 x 8 16.2/16.6, 2048 x 8 18.7/17.5, 2900 x 4
-    // 14.1/14.0, 4000 x 2 13.0/12.4, 4000 x 1 9.6/11.0. Rows of 4 KB and more hide more of it: 2048 x 8 (4096)
-    // 37.3/37.8, 2048 x 4 20.6/23.0, 4000 x 2 22.9/23.4. The counts are atomics, which take their turns where the entries
-    // go to few experts: FP8 rows of 1 KB to one expert, 1448 x 1 8.4/8.4, 2048 x 1 10.4/8.6, 4096 x 1 27/9.5; to eight,
-    // 1700 x 8 15.5/15.0, 4096 x 1 10.4/9.7; so that from 1449 tokens on there have to be 16 experts. (All tokens to one of
-    // 256 experts 10.5/10.5 at 1448 x 1, 13.1/10.5 at 2048, 32/12 at 4096.) Padding has a workgroup for each
+    // 14.1/14.0, 4000 x 2 13.0/12.4, 4000 x 1 9.6/11.0; masked 1700 x 8 15.3/15.4, 2900 x 4 13.1/13.1. Rows of 4 KB and more
+    // hide more of it: 2048 x 8 (4096) 37.3/37.8, 2048 x 4 20.6/23.0, 4000 x 2 22.9/23.4. Padding has a workgroup for each
     // expert, which counts as well, and six workgroups fit a CU at a time: 1024 experts 1448 x 8 18.8/17.9, 2048 x 2
-    // 11.4/14.4, 2900 x 2 16.5/15.0, rows of 8 KB 2048 x 8 50.9/51.9.
+    // 11.4/14.4, 2900 x 2 16.5/15.0, 2900 x 1 12.1/13.4, rows of 8 KB 2048 x 8 50.9/51.9. The counts are atomics, which
+    // take their turns where the entries go to few experts: FP8 rows of 1 KB, masked, to one expert 1448 x 1 8.4/8.4, 2048 x 1
+    // 10.4/8.6, 4096 x 1 27/9.5; to two 2048 x 1 8.1/8.7, 2500 x 1 10.3/9.0; to four 2500 x 1 8.5/9.1, 3547 x 1 11.4/9.3,
+    // 2508 x 2 12.1/10.3; to eight 2048 x 2 8.1/10.0, 2900 x 2 11.8/10.8, 4096 x 1 10.4/9.7; hence most by experts. (All
+    // tokens to one of 256 experts: 1448 x 1 10.5/10.5, 2048 x 1 13.1/10.5, 4096 x 1 32/12.)
     // One token a workgroup or four, us: 64 x 8 of 7168 10.2/11.9, 512 x 8 of 2048 8.3/8.2, 777 x 6 10.8/9.9, all to
     // one expert 1000 x 1 9.8/6.5.
-    if (const int tokens = moe_few_tokens(a.t, a.k, a.kdim, a.num_experts)) {   // of a workgroup
+    if (const int tokens = moe_few_tokens(a.t, a.k, a.kdim, a.num_experts, a.layout)) {   // of a workgroup
         // (without tokens or padding rows: one workgroup for the ends, masked counts and weights)
         const int pad_blocks = a.layout != kMoeMasked ? (a.alignment > 1 ? a.num_experts : 1) : a.t == 0 ? 1 : 0;
         const dim3 grid(pad_blocks + (a.t + tokens - 1) / tokens), block(kThreads);

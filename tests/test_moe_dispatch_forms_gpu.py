@@ -100,13 +100,16 @@ def test_many_rows_past_the_segments(t, k, e, alignment, layout):
 
 @pytest.mark.parametrize('t,k,e,size,layout,launches', [
     (724, 1, 1, 256, 'psum', 1), (725, 1, 1, 256, 'masked', 1), (1448, 1, 1, 256, 'contiguous', 1), (1448, 8, 8, 256, 'psum', 1),
-    (1449, 1, 15, 256, 'psum', 3), (1449, 1, 16, 256, 'psum', 1), (1449, 8, 8, 4096, 'masked', 3), (1250, 16, 64, 256, 'psum', 1),
-    (1251, 16, 64, 256, 'psum', 3), (1618, 8, 64, 256, 'contiguous', 1), (1619, 8, 64, 256, 'psum', 3), (2048, 8, 20, 4096, 'psum', 1),
+    (1449, 1, 1, 256, 'psum', 3), (1449, 1, 2, 256, 'psum', 1), (1449, 8, 8, 4096, 'masked', 1), (2048, 2, 8, 256, 'psum', 1),
+    (2900, 2, 8, 256, 'masked', 3), (1250, 16, 64, 256, 'psum', 1), (1251, 16, 64, 256, 'psum', 3), (1772, 8, 64, 256, 'contiguous', 1),
+    (1773, 8, 64, 256, 'psum', 3), (1618, 8, 64, 256, 'masked', 1), (1619, 8, 64, 256, 'masked', 3), (2048, 8, 20, 4096, 'psum', 1),
     (2049, 8, 20, 4096, 'psum', 3), (4578, 1, 32, 256, 'masked', 1), (4579, 1, 32, 256, 'masked', 3), (2048, 2, 1024, 256, 'psum', 1),
-    (2049, 2, 1024, 256, 'psum', 3), (1500, 8, 600, 256, 'psum', 3), (3000, 2, 1024, 256, 'contiguous', 4), (2999, 2, 1024, 256, 'psum', 3)])
+    (2049, 2, 1024, 256, 'psum', 3), (4096, 1, 1024, 256, 'psum', 1), (4097, 1, 1024, 256, 'psum', 4), (1500, 8, 600, 256, 'psum', 3),
+    (3000, 2, 1024, 256, 'contiguous', 4), (2999, 2, 1024, 256, 'psum', 3)])
 def test_sizes_of_one_launch_and_of_several(t, k, e, size, layout, launches):
-    """Around the sizes at which the number of launches changes; `size` bytes a row. (Entries x workgroups of four
-    tokens: 1618 x 8 x 405 and 4578 x 1145 are at most 5 x 2^20, 1619 x 8 x 405 and 4579 x 1145 are more.)"""
+    """Around the sizes at which the number of launches changes; `size` bytes a row. (Entries x workgroups of four tokens:
+    1772 x 8 x 443 is at most 6 x 2^20, 1773 x 8 x 444 more; masked 1618 x 8 x 405 and 4578 x 1145 at most 5 x 2^20, 1619 x 8 x
+    405 and 4579 x 1145 more.)"""
     dispatch('bf16', t, k, e, size // 2, layout, launches=launches)
     if e > 1:   # all tokens to the same experts
         dispatch('e4m3', t, k, e, size, layout, launches=launches, idx=torch.arange(k, dtype=torch.int32).expand(t, k).contiguous() % e)

@@ -116,7 +116,7 @@ def test_noalloc_dispatch_rejects_oversize():
 @pytest.mark.parametrize('layout', ['contiguous', 'psum', 'masked'])
 def test_noalloc_dispatch_reuses_its_scratch(layout):
     """A large call, then a smaller one that needs the scratch as well (in one launch it is not touched)."""
-    for t, k, e, kdim, seed, launches in ((4000, 8, 64, 512, 4, 3), (1500, 3, 8, 256, 5, 3), (2100, 8, 200, 1024, 6, 3), (37, 3, 16, 256, 7, 1),
-                                          (8200, 1, 20, 1024, 8, 3 if layout == 'masked' else 4), (1500, 3, 8, 256, 9, 3)):
+    for t, k, e, kdim, seed, launches in ((4000, 8, 64, 512, 4, 3), (2500, 3, 8, 256, 5, 3), (2100, 8, 200, 1024, 6, 3), (37, 3, 16, 256, 7, 1),
+                                          (8200, 1, 20, 1024, 8, 3 if layout == 'masked' else 4), (2500, 3, 8, 256, 9, 3)):
         _dispatch_both(t, k, e, kdim, layout, seed=seed)
         assert f' launches={launches}' in deep_gemm.get_last_config()
